@@ -724,6 +724,86 @@ int gsx_mesh_raster(int64_t n_faces, const float* tri_xy, const float* tri_z,
                     const int32_t* tile_ranges, int32_t width, int32_t height,
                     float znear, int32_t* pix_to_face, float* zbuf, void* stream);
 
+/* ------------------------------------------- feature field: decoder, loss --
+ * No reference counterpart: the reference renders feature channels
+ * (render_gaussian_features, splatting/render.py:164-220) and leaves what
+ * they train to the caller.  These entry points take rows of features (the
+ * pixels of a render, Gaussians, tokens) into a teacher's space and compare
+ * the result with what the teacher said. */
+
+/* Element types of these tensors; sums are float32 in all of them. */
+enum gsx_dtype { GSX_F32 = 0, GSX_BF16 = 1, GSX_F16 = 2 };
+
+/* The gate's activation: g sigmoid(g), g Phi(g) (with erf), sigmoid(g). */
+enum gsx_activation { GSX_ACT_SILU = 0, GSX_ACT_GELU = 1, GSX_ACT_SIGMOID = 2 };
+
+/* The gated feed-forward block y = (act(x Wg^T) * (x Wu^T)) Wd^T: x (rows,
+ * d_in) with a row stride in elements, w_gate and w_up (hidden, d_in), w_down
+ * (d_out, hidden), y (rows, d_out), the last three contiguous; one type for
+ * all, every pointer aligned to it.  The workspace (16-byte aligned) is
+ * scratch: it may be freed or reused once the call has returned, in stream
+ * order.  GSX_ERR_TOO_LARGE above 2^30 rows or widths of 2^20.  float32 and
+ * 16-bit sums are deterministic. */
+int64_t gsx_ffn_fwd_workspace_bytes(int32_t dtype, int32_t act, int64_t rows, int32_t d_in,
+                                    int32_t hidden, int32_t d_out);
+int gsx_ffn_fwd(int32_t dtype, int32_t act, int64_t rows, int32_t d_in, int32_t hidden,
+                int32_t d_out, const void* x, int64_t x_stride, const void* w_gate,
+                const void* w_up, const void* w_down, void* y, void* workspace,
+                int64_t workspace_bytes, void* stream);
+
+/* Its gradient from g_y (rows, d_out, row stride in elements): g_x (rows,
+ * d_in) and the weights' gradients, contiguous.  g_x, the pair g_w_gate /
+ * g_w_up, and g_w_down may each be NULL.  Needs nothing of the forward call.
+ * rows = 0 clears the weights' gradients. */
+int64_t gsx_ffn_bwd_workspace_bytes(int32_t dtype, int32_t act, int64_t rows, int32_t d_in,
+                                    int32_t hidden, int32_t d_out);
+int gsx_ffn_bwd(int32_t dtype, int32_t act, int64_t rows, int32_t d_in, int32_t hidden,
+                int32_t d_out, const void* x, int64_t x_stride, const void* w_gate,
+                const void* w_up, const void* w_down, const void* g_y, int64_t g_y_stride,
+                void* g_x, void* g_w_gate, void* g_w_up, void* g_w_down, void* workspace,
+                int64_t workspace_bytes, void* stream);
+
+/* What a teacher's values are: logits (softmax over the row's entries at the
+ * temperature), or log-probabilities over the whole vocabulary (the mass that
+ * the entries leave is one more bucket). */
+enum gsx_teacher { GSX_TEACHER_LOGITS = 0, GSX_TEACHER_LOG_PROBS = 1 };
+enum gsx_reduction { GSX_REDUCE_NONE = 0, GSX_REDUCE_SUM = 1, GSX_REDUCE_MEAN = 2 };
+#define GSX_DISTIL_MAX_TOP 256
+
+/* Kullback-Leibler divergence of a student's logits (rows, vocab; a type of
+ * gsx_dtype, row stride in elements) from a teacher's `top` entries a row:
+ * values (rows, top) float32, indices (rows, top) int32 or (index64 = 1)
+ * int64, both contiguous.  With q = softmax(logits / T) and the entries'
+ * probabilities p, the row's loss is T^2 sum p (log p - log q); for
+ * log-probabilities plus T^2 r (log r - log Q), r = max(0, 1 - sum p) and Q
+ * the student's mass outside the entries.  An entry whose index is outside
+ * [0, vocab) or whose value is -inf is absent; two entries of one column both
+ * count.  A row without entries has loss 0 and gradient 0, whatever its logits
+ * hold, and the mean does not count it (no row: 0).  loss: rows floats (none)
+ * or one.  1 <= top <= min(vocab, GSX_DISTIL_MAX_TOP). */
+int64_t gsx_distil_workspace_bytes(int32_t dtype, int64_t rows, int32_t vocab, int32_t top);
+int gsx_distil_fwd(int32_t dtype, int64_t rows, int32_t vocab, int32_t top, const void* logits,
+                   int64_t logits_stride, const float* values, const void* indices,
+                   int32_t index64, float temperature, int32_t teacher, int32_t reduction,
+                   float* loss, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Its gradient g_logits (rows, vocab), contiguous, in the logits' type, from
+ * g_loss (rows floats for none, else one, on the device).  The workspace is
+ * the forward call's, unchanged since. */
+int gsx_distil_bwd(int32_t dtype, int64_t rows, int32_t vocab, int32_t top, const void* logits,
+                   int64_t logits_stride, const float* values, const void* indices,
+                   int32_t index64, float temperature, int32_t teacher, int32_t reduction,
+                   const float* g_loss, void* g_logits, void* workspace, int64_t workspace_bytes,
+                   void* stream);
+
+/* Loss and gradient in one pass over the logits, both times `scale` (the
+ * term's weight in an objective).  Sum or mean. */
+int gsx_distil_fwd_bwd(int32_t dtype, int64_t rows, int32_t vocab, int32_t top, const void* logits,
+                       int64_t logits_stride, const float* values, const void* indices,
+                       int32_t index64, float temperature, int32_t teacher, int32_t reduction,
+                       float scale, float* loss, void* g_logits, void* workspace,
+                       int64_t workspace_bytes, void* stream);
+
 /* ---------------------------------------------------------- diagnostics --
  * Evaluates the device exp used by the rasterizer (the stand-in for
  * metal::exp at rasterize.py:80,171,274) on n inputs; tests check it

@@ -7,5 +7,5 @@ Compute runs in hand-written HIP kernels (``libgsx.so``, C ABI in
 
 __version__ = "0.1.0"
 
-from . import cameras, renderer, splatting  # noqa: F401
+from . import cameras, nn, renderer, splatting  # noqa: F401
 from .cameras import Camera  # noqa: F401

@@ -49,6 +49,9 @@ class GsxCamera(ctypes.Structure):
     ]
 
 
+# gsx_dtype of include/gsx.h
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
 ADAM_MAX_GROUPS = 8  # GSX_ADAM_MAX_GROUPS
 
 
@@ -191,6 +194,19 @@ SIGNATURES = {
     "gsx_geom_loss_bwd": (ctypes.c_int, [_I32, _I32, _P, _P, _P, _P, _F, _F, _F, _P, _P, _P,
                                          _P]),
     "gsx_mesh_raster": (ctypes.c_int, [_I64, _P, _P, _P, _I64, _P, _I32, _I32, _F, _P, _P, _P]),
+    "gsx_ffn_fwd_workspace_bytes": (_I64, [_I32, _I32, _I64, _I32, _I32, _I32]),
+    "gsx_ffn_fwd": (ctypes.c_int, [_I32, _I32, _I64, _I32, _I32, _I32, _P, _I64, _P, _P, _P, _P,
+                                   _P, _I64, _P]),
+    "gsx_ffn_bwd_workspace_bytes": (_I64, [_I32, _I32, _I64, _I32, _I32, _I32]),
+    "gsx_ffn_bwd": (ctypes.c_int, [_I32, _I32, _I64, _I32, _I32, _I32, _P, _I64, _P, _P, _P, _P,
+                                   _I64, _P, _P, _P, _P, _P, _I64, _P]),
+    "gsx_distil_workspace_bytes": (_I64, [_I32, _I64, _I32, _I32]),
+    "gsx_distil_fwd": (ctypes.c_int, [_I32, _I64, _I32, _I32, _P, _I64, _P, _P, _I32, _F, _I32,
+                                      _I32, _P, _P, _I64, _P]),
+    "gsx_distil_bwd": (ctypes.c_int, [_I32, _I64, _I32, _I32, _P, _I64, _P, _P, _I32, _F, _I32,
+                                      _I32, _P, _P, _P, _I64, _P]),
+    "gsx_distil_fwd_bwd": (ctypes.c_int, [_I32, _I64, _I32, _I32, _P, _I64, _P, _P, _I32, _F,
+                                          _I32, _I32, _F, _P, _P, _P, _I64, _P]),
     "gsx_debug_expf": (ctypes.c_int, [_I64, _P, _P, _P]),
     "gsx_debug_atanf": (ctypes.c_int, [_I64, _P, _P, _P]),
 }
@@ -261,6 +277,16 @@ def require_device(*tensors: torch.Tensor | None) -> torch.device:
     if dev is None:
         raise ValueError("no tensor inputs")
     return dev
+
+
+def rows_of(t: torch.Tensor) -> tuple[torch.Tensor, int]:
+    """``t`` (..., C) as (rows, C) with its row stride in elements; copied only
+    if its last dimension is strided or its leading ones do not fold into one."""
+    width = t.shape[-1]
+    t = t.reshape(-1, width)
+    if (t.shape[0] > 1 and t.stride(0) < width) or (width > 1 and t.stride(1) != 1):
+        t = t.contiguous()
+    return t, (t.stride(0) if t.shape[0] > 1 else width)
 
 
 def f32c(t: torch.Tensor) -> torch.Tensor:

@@ -25,7 +25,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 PKG = os.path.dirname(HERE)
 ROOT = os.path.dirname(PKG)
 SOURCES = ["capi.hip", "preprocess.hip", "binning.hip", "raster.hip", "train.hip", "mesh.hip",
-           "density.hip", "geometry.hip"]
+           "density.hip", "geometry.hip", "feedforward.hip", "distil.hip"]
 LIB = os.path.join(PKG, "libgsx.so")
 ARCH = os.environ.get("GSX_OFFLOAD_ARCH", "gfx950")
 

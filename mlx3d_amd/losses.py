@@ -9,6 +9,11 @@ its cotangent (``gsx_photometric_loss_fwd`` / ``_bwd``), the values that
 expression's autograd graph gives.  ``ssim`` is the reference's function on
 top of ``photometric``, and ``l1_loss`` the L1 term alone
 (``gsx_l1_fwd_signs`` / ``gsx_l1_bwd_signs``).
+
+``distillation_loss`` compares a student's logits (a decoded feature render)
+with the largest ones that a teacher kept for each row, and
+``distillation_value_and_grad`` gives loss and gradient in one pass over the
+logits (``gsx_distil_*``; no counterpart in the reference).
 """
 
 from __future__ import annotations
@@ -18,7 +23,7 @@ import torch
 from . import _lib
 from .profiling import stage
 
-__all__ = ["l1_loss", "photometric", "photometric_loss", "psnr", "ssim"]
+__all__ = ["distillation_loss", "distillation_value_and_grad", "l1_loss", "photometric", "photometric_loss", "psnr", "ssim"]
 
 
 class _PhotometricFn(torch.autograd.Function):
@@ -188,3 +193,129 @@ def psnr(pred: torch.Tensor, target: torch.Tensor, max_val: float = 1.0) -> torc
     """Peak signal-to-noise ratio in dB (image_metrics.py:17-20)."""
     mse = ((pred - target) ** 2).mean()
     return 10.0 * torch.log10((max_val * max_val) / torch.clamp(mse, min=1e-12))
+
+
+_TEACHERS = {"logits": 0, "log_probs": 1}
+_REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
+DISTILLATION_MAX_TOP = 256  # GSX_DISTIL_MAX_TOP
+
+
+class _Distillation:
+    """The checked arguments of one distillation call, as the C entry points
+    take them."""
+
+    def __init__(self, logits, values, indices, temperature, teacher, reduction):
+        if logits.ndim < 1 or logits.dtype not in _lib.DTYPES:
+            raise ValueError("logits must be (..., V) in float32, bfloat16 or float16.")
+        if values.shape != indices.shape or values.ndim != logits.ndim or \
+                values.shape[:-1] != logits.shape[:-1]:
+            raise ValueError("teacher_values and teacher_indices must both have shape (..., K), "
+                             "with the logits' leading dimensions.")
+        if not values.is_floating_point():
+            raise ValueError("teacher_values must be floating point.")
+        if indices.dtype not in (torch.int32, torch.int64):
+            raise ValueError("teacher_indices must be int32 or int64.")
+        vocab, top = int(logits.shape[-1]), int(values.shape[-1])
+        if not 1 <= top <= min(vocab, DISTILLATION_MAX_TOP):
+            raise ValueError("a row must have between 1 and "
+                             f"min(V, {DISTILLATION_MAX_TOP}) teacher entries.")
+        if not 0.0 < float(temperature) < 3.0e38:
+            raise ValueError("temperature must be positive and finite.")
+        if teacher not in _TEACHERS:
+            raise ValueError("teacher must be 'logits' or 'log_probs'.")
+        if reduction not in _REDUCTIONS:
+            raise ValueError("reduction must be 'none', 'sum' or 'mean'.")
+        self.device = _lib.require_device(logits, values, indices)
+        self.shape = logits.shape
+        self.reduction = reduction
+        self.values = _lib.f32c(values.detach())
+        self.indices = indices.contiguous()
+        rows = logits.numel() // vocab
+        self.head = (_lib.DTYPES[logits.dtype], rows, vocab, top)
+        self.tail = (_lib.ptr(self.values), _lib.ptr(self.indices),
+                     int(indices.dtype == torch.int64), float(temperature), _TEACHERS[teacher],
+                     _REDUCTIONS[reduction])
+
+    def workspace(self) -> torch.Tensor:
+        n = _lib.check(int(_lib.load().gsx_distil_workspace_bytes(*self.head)),
+                       "gsx_distil_workspace_bytes")
+        return torch.empty((n,), dtype=torch.uint8, device=self.device)
+
+    def loss(self) -> torch.Tensor:
+        shape = self.shape[:-1] if self.reduction == "none" else ()
+        return torch.empty(shape, dtype=torch.float32, device=self.device)
+
+
+class _DistillationFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, call):
+        rows, stride = _lib.rows_of(logits)
+        ws, loss = call.workspace(), call.loss()
+        with stage("distil_fwd"):
+            _lib.check(_lib.load().gsx_distil_fwd(
+                *call.head, _lib.ptr(rows), stride, *call.tail, _lib.ptr(loss), _lib.ptr(ws),
+                ws.numel(), _lib.stream_handle(call.device)), "gsx_distil_fwd")
+        ctx.save_for_backward(logits, ws, call.values, call.indices)
+        ctx.call = call
+        return loss
+
+    @staticmethod
+    def backward(ctx, g_loss):
+        # saved with the rest so that an entry changed in place since is noticed
+        logits, ws, _, _ = ctx.saved_tensors
+        call = ctx.call
+        rows, stride = _lib.rows_of(logits)
+        g = _lib.f32c(g_loss)
+        grad = torch.empty(call.shape, dtype=logits.dtype, device=call.device)
+        with stage("distil_bwd"):
+            _lib.check(_lib.load().gsx_distil_bwd(
+                *call.head, _lib.ptr(rows), stride, *call.tail, _lib.ptr(g), _lib.ptr(grad),
+                _lib.ptr(ws), ws.numel(), _lib.stream_handle(call.device)), "gsx_distil_bwd")
+        return grad, None
+
+
+def distillation_loss(logits: torch.Tensor, teacher_values: torch.Tensor,
+                      teacher_indices: torch.Tensor, temperature: float = 1.0,
+                      teacher: str = "logits", reduction: str = "mean") -> torch.Tensor:
+    """Kullback-Leibler divergence of a student's (..., V) ``logits`` from the
+    (..., K) largest entries that a teacher kept for each row, times
+    temperature^2; differentiable with respect to ``logits``.
+
+    ``teacher="logits"``: the values are logits, p = softmax(values / T) over
+    the row's entries, and the row's loss is T^2 sum p (log p - log q) with
+    q = softmax(logits / T) over all V.  ``teacher="log_probs"``: the values
+    are log-probabilities over the whole vocabulary (taken at the same
+    temperature); the mass that the entries leave, r = 1 - sum p (0 if they
+    exceed 1), is compared as one bucket with the student's mass outside them,
+    or left out where the student has none there.
+
+    An entry whose index lies outside [0, V) or whose value is -inf is absent.
+    A row without entries has loss 0 and gradient 0 whatever its logits hold.
+    ``reduction``: "mean" over the rows that have entries (0 if none has),
+    "sum", or "none" (a loss for each row; weight rows by what multiplies it).
+    At most 256 entries a row; values and indices carry no gradient."""
+    call = _Distillation(logits, teacher_values, teacher_indices, temperature, teacher, reduction)
+    return _DistillationFn.apply(logits, call)
+
+
+def distillation_value_and_grad(logits: torch.Tensor, teacher_values: torch.Tensor,
+                                teacher_indices: torch.Tensor, temperature: float = 1.0,
+                                teacher: str = "logits", reduction: str = "mean",
+                                scale: float = 1.0) -> tuple[torch.Tensor, torch.Tensor]:
+    """(loss, gradient with respect to ``logits``) of
+    :func:`distillation_loss`, both times ``scale``, in one pass over the
+    logits: each is read once and its gradient written once, where autograd
+    reads them a second time.  Feed the gradient on with
+    ``logits.backward(grad)``.  ``reduction``: "mean" or "sum"."""
+    if reduction == "none":
+        raise ValueError("value_and_grad needs a scalar: reduction must be 'sum' or 'mean'.")
+    call = _Distillation(logits, teacher_values, teacher_indices, temperature, teacher, reduction)
+    rows, stride = _lib.rows_of(logits.detach())
+    ws, loss = call.workspace(), call.loss()
+    grad = torch.empty(call.shape, dtype=logits.dtype, device=call.device)
+    with stage("distil_fwd_bwd"):
+        _lib.check(_lib.load().gsx_distil_fwd_bwd(
+            *call.head, _lib.ptr(rows), stride, *call.tail, float(scale), _lib.ptr(loss),
+            _lib.ptr(grad), _lib.ptr(ws), ws.numel(), _lib.stream_handle(call.device)),
+            "gsx_distil_fwd_bwd")
+    return loss, grad

@@ -69,104 +69,216 @@ struct Entry {
     float value;
 };
 
-__device__ __forceinline__ Entry entry(const Distil& q, int64_t row, int k) {
+// An entry as it lies in memory; told apart from its check so that the loads
+// can be in flight for a while.
+struct RawEntry {
+    int lo, hi;
+    float value;
+};
+__device__ __forceinline__ RawEntry raw_entry(const Distil& q, int64_t row, int k) {
     const int64_t at = row * q.top + k;
-    const int64_t i = q.index64 ? ((const int64_t*)q.indices)[at] : ((const int32_t*)q.indices)[at];
-    const float v = q.values[at];
-    return Entry{(i >= 0 && i < q.vocab && v != -INFINITY) ? (int)i : -1, v};
+    RawEntry e;
+    e.value = q.values[at];
+    e.hi = 0;
+    if (q.index64) {
+        const int2 i = ((const int2*)q.indices)[at];
+        e.lo = i.x;
+        e.hi = i.y;
+    } else {
+        e.lo = ((const int*)q.indices)[at];
+    }
+    return e;
+}
+__device__ __forceinline__ Entry checked(const Distil& q, const RawEntry& e) {
+    const bool in = e.hi == 0 && (unsigned)e.lo < (unsigned)q.vocab && e.value != -INFINITY;
+    return Entry{in ? e.lo : -1, e.value};
+}
+__device__ __forceinline__ Entry entry(const Distil& q, int64_t row, int k) {
+    return checked(q, raw_entry(q, row, k));
 }
 
+// Sum or maximum over the G lanes of a group (a power of two, aligned): cross-lane
+// moves inside rows of 16, then swaps of rows and halves.
+template <int CTRL>
+__device__ __forceinline__ float lane_move(float v) {
+    return __uint_as_float(
+        __builtin_amdgcn_update_dpp(0u, __float_as_uint(v), CTRL, 0xF, 0xF, true));
+}
+struct Add {
+    static __device__ __forceinline__ float of(float a, float b) { return a + b; }
+};
+struct Max {
+    static __device__ __forceinline__ float of(float a, float b) { return fmaxf(a, b); }
+};
+template <int G, class Op>
+__device__ __forceinline__ float group_reduce(float v) {
+    if constexpr (G >= 2) v = Op::of(v, lane_move<0xB1>(v));   // quad_perm 1 0 3 2
+    if constexpr (G >= 4) v = Op::of(v, lane_move<0x4E>(v));   // quad_perm 2 3 0 1
+    if constexpr (G >= 8) v = Op::of(v, lane_move<0x141>(v));  // row_half_mirror
+    if constexpr (G >= 16) v = Op::of(v, lane_move<0x140>(v)); // row_mirror
+    if constexpr (G >= 32) {
+        const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v),
+                                                        false, false);
+        v = Op::of(__uint_as_float(p[0]), __uint_as_float(p[1]));
+    }
+    if constexpr (G >= 64) {
+        const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v),
+                                                        false, false);
+        v = Op::of(__uint_as_float(p[0]), __uint_as_float(p[1]));
+    }
+    return v;
+}
 template <int G>
 __device__ __forceinline__ float group_sum(float v) {
-#pragma unroll
-    for (int o = G / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, kWave);
-    return v;
+    return group_reduce<G, Add>(v);
 }
 template <int G>
 __device__ __forceinline__ float group_max(float v) {
-#pragma unroll
-    for (int o = G / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, kWave));
+    return group_reduce<G, Max>(v);
+}
+
+// Keeps the compiler from computing what depends on v ahead of this place (and
+// holding it in registers through a loop).
+__device__ __forceinline__ int here(int v) {
+    asm volatile("" : "+v"(v));
     return v;
 }
 
-// exp((s - m) / T) as a power of two; c = log2(e) / T.  m is the maximum, so
-// the product's rounding matters only where the term itself is small.
-__device__ __forceinline__ float expo(float s, float m, float c) {
-    return __builtin_amdgcn_exp2f((s - m) * c);
+// Orders a wave's own accesses to shared memory (they are executed in order).
+__device__ __forceinline__ void wave_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// exp((s - m) / T) as the power 2^(s c - mc) with c = log2(e) / T and mc = c m
+// rounded once: one multiply-add for a logit.  What mc's rounding moves, up to
+// |mc| 2^-24, it moves in every term of a row alike, so it leaves the quotients;
+// logarithms take the exponents back by the same mc.
+__device__ __forceinline__ float expo(float s, float mc, float c) {
+    return __builtin_amdgcn_exp2f(fmaf(s, c, -mc));
+}
+
+constexpr float kLn2 = 0.69314718055994531f;
+
+// log of a sum that holds an exp(0): the hardware's, to an absolute 2^-22 of a
+// term that is added to logits
+__device__ __forceinline__ float log_of(float v) {
+    return __builtin_amdgcn_logf(v) * kLn2;
+}
+
+// A row's entries on G lanes, KPL in a lane's registers: entry lane + i G.
+template <int KPL>
+struct Entries {
+    int index[KPL];
+    float value[KPL];  // the teacher's, then the probability
+    float s[KPL];      // the student's logit
+    bool again[KPL];   // another entry stands for this column
+};
+template <int G, int KPL>
+__device__ __forceinline__ void read_entries(const Distil& q, int64_t row, int lane,
+                                             Entries<KPL>& e) {
+#pragma unroll
+    for (int i = 0; i < KPL; ++i) {
+        e.index[i] = -1;
+        if (lane + i * G < q.top) {
+            const Entry t = entry(q, row, lane + i * G);
+            e.index[i] = t.index;
+            e.value[i] = t.value;
+        }
+    }
 }
 
 // What the entries and the rest of a row say: the loss, and what the gradient
 // needs.  rest_m, rest_s: maximum logit and sum of exp over the rest (-inf, 0:
-// nothing there).  Runs on G lanes; ei, ep, es: the row's entries in shared
-// memory (index, value then probability, logit).
+// nothing there).  Turns the entries' values into their probabilities.
 struct RowStats {
     float loss;     // without T^2
-    float m, inv;   // maximum over all, S / (sum of exp over all)
+    float mc, inv;  // c times the maximum over all, S / (sum of exp over all)
     float rest;     // the rest's factor on exp((s - rest_m) / T)
     bool active;
 };
 
-template <int G>
-__device__ __forceinline__ RowStats row_stats(const Distil& q, int lane, const int* ei, float* ep,
-                                              const float* es, float rest_m, float rest_s) {
+// (A teacher of logits: rest_m and rest_s run over the whole row, the entries'
+// columns among them.)
+template <int G, int KPL, bool LOG_PROBS>
+__device__ __forceinline__ RowStats row_stats(const Distil& q, Entries<KPL>& e, float rest_m,
+                                              float rest_s) {
     const float c = kLog2e * q.inv_temp;
-    float tm = -INFINITY, m = rest_m;
-    int any = 0;
-    for (int k = lane; k < q.top; k += G)
-        if (ei[k] >= 0) {
-            any = 1;
-            tm = fmaxf(tm, ep[k]);
-            m = fmaxf(m, es[k]);
+    float tm = -INFINITY, m = rest_m, any = 0.f;
+#pragma unroll
+    for (int i = 0; i < KPL; ++i)
+        if (e.index[i] >= 0) {
+            any = 1.f;
+            tm = fmaxf(tm, e.value[i]);
+            m = fmaxf(m, e.s[i]);
         }
     RowStats r;
-    r.active = group_max<G>((float)any) > 0.f;
-    tm = group_max<G>(tm);
-    m = group_max<G>(m);
+    r.active = group_max<G>(any) > 0.f;
     const bool has_rest = rest_m != -INFINITY;
-    float total = 0.f, t_sum = 0.f;
-    for (int k = lane; k < q.top; k += G)
-        if (ei[k] >= 0) {
-            bool again = false;  // a column that two entries name counts once
-            for (int j = 0; j < k; ++j) again |= ei[j] == ei[k];
-            if (!again) total += es[k] == -INFINITY ? 0.f : expo(es[k], m, c);
-            t_sum += q.log_probs ? 0.f : expo(ep[k], tm, c);
-        }
-    const float shift = has_rest ? expo(rest_m, m, c) : 0.f;
-    total = group_sum<G>(total) + (has_rest ? rest_s * shift : 0.f);
-    t_sum = group_sum<G>(t_sum);
-    const float log_total = logf(total), log_t = logf(t_sum);
-    float loss = 0.f, mass = 0.f;
-    for (int k = lane; k < q.top; k += G)
-        if (ei[k] >= 0) {
-            float lp, p;
-            if (q.log_probs) {
-                lp = ep[k];
-                p = expf(lp);
-            } else {
-                lp = (ep[k] - tm) * q.inv_temp - log_t;
-                p = expo(ep[k], tm, c) / t_sum;
+    const float rest_mc = c * rest_m;
+    float total = rest_s, shift = 1.f, mc = rest_mc;
+    if constexpr (LOG_PROBS) {
+        mc = c * group_max<G>(m);
+        shift = has_rest ? __builtin_amdgcn_exp2f(rest_mc - mc) : 0.f;
+        total = 0.f;
+#pragma unroll
+        for (int i = 0; i < KPL; ++i)
+            if (e.index[i] >= 0 && !e.again[i] && e.s[i] != -INFINITY)
+                total += expo(e.s[i], mc, c);
+        total = group_sum<G>(total) + (has_rest ? rest_s * shift : 0.f);
+    }
+    const float log_total = log_of(total);
+    float loss = 0.f, mass = 0.f, t_exp[KPL], inv_t = 1.f, log_t = 0.f, tmc = 0.f;
+    if constexpr (!LOG_PROBS) {
+        tmc = c * group_max<G>(tm);
+        float t_sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < KPL; ++i)
+            if (e.index[i] >= 0) {
+                t_exp[i] = expo(e.value[i], tmc, c);
+                t_sum += t_exp[i];
             }
-            if (p != 0.f) loss += p * (lp - ((es[k] - m) * q.inv_temp - log_total));
+        t_sum = group_sum<G>(t_sum);
+        log_t = log_of(t_sum);
+        inv_t = __builtin_amdgcn_rcpf(t_sum);
+    }
+#pragma unroll
+    for (int i = 0; i < KPL; ++i)
+        if (e.index[i] >= 0) {
+            float lp, p;
+            if constexpr (LOG_PROBS) {
+                lp = e.value[i];
+                p = __builtin_amdgcn_exp2f(lp * kLog2e);
+            } else {
+                lp = fmaf(e.value[i], c, -tmc) * kLn2 - log_t;
+                p = t_exp[i] * inv_t;
+            }
+            if (p != 0.f) loss += p * (lp - (fmaf(e.s[i], c, -mc) * kLn2 - log_total));
             mass += p;
-            ep[k] = p;
+            e.value[i] = p;
         }
     loss = group_sum<G>(loss);
     mass = group_sum<G>(mass);
     float share = 0.f;
-    if (q.log_probs && has_rest) {
+    if (LOG_PROBS && has_rest) {
         const float left = 1.0f - mass;
         if (left > 0.f) {
-            const float log_q = (rest_m - m) * q.inv_temp + logf(rest_s) - log_total;
-            loss += left * (logf(left) - log_q);
+            const float log_q = (rest_mc - mc) * kLn2 + log_of(rest_s) - log_total;
+            loss += left * (log_of(left) - log_q);
             share = left / rest_s;
             mass += left;
         }
     }
     r.loss = loss;
-    r.m = m;
-    r.inv = mass / total;
+    r.mc = mc;
+    r.inv = mass * __builtin_amdgcn_rcpf(total);
     r.rest = r.inv * shift - share;
     return r;
+}
+
+// An entry's gradient without the row's factor; p: the column's probability.
+__device__ __forceinline__ float entry_grad(const RowStats& r, float s, float p, float c) {
+    return (s == -INFINITY ? 0.f : expo(s, r.mc, c)) * r.inv - p;
 }
 
 // The factor on a row's gradient: T, the upstream gradient, 1 / supervised rows.
@@ -193,125 +305,297 @@ __device__ __forceinline__ float inverse_count(const Distil& q, int* scratch) {
 
 // n elements from global to shared memory or back, where both have the same
 // offset from a 16-byte boundary: whole 16-byte pieces between ragged ends.
-template <class T>
-__device__ __forceinline__ void copy_flat(T* dst, const T* src, int64_t n) {
+// By THREADS threads, t the caller's number among them.
+template <int THREADS, class T>
+__device__ __forceinline__ void copy_flat(T* dst, const T* src, int n, int t) {
     constexpr int V = 16 / sizeof(T);
-    int64_t head = (V - ((uintptr_t)src / sizeof(T)) % V) % V;
+    int head = (int)((V - ((uintptr_t)src / sizeof(T)) % V) % V);
     if (head > n) head = n;
-    const int64_t body = (n - head) / V;
-    for (int64_t i = threadIdx.x; i < head; i += kThreads) dst[i] = src[i];
-    for (int64_t i = threadIdx.x; i < body; i += kThreads)
-        *(u32x4*)(dst + head + i * V) = *(const u32x4*)(src + head + i * V);
-    for (int64_t i = head + body * V + threadIdx.x; i < n; i += kThreads) dst[i] = src[i];
+    const int body = (n - head) / V, tail = n - head - body * V;
+    const u32x4* from = (const u32x4*)(src + head);
+    u32x4* to = (u32x4*)(dst + head);
+    for (int i = t; i < body; i += THREADS) to[i] = from[i];
+    if (t < head) dst[t] = src[t];
+    if (t < tail) dst[n - tail + t] = src[n - tail + t];
 }
 
-// Rows in shared memory, G lanes each.  LDS: the rows (with up to a piece of
-// slack so that they lie as in global memory), then the entries.
-template <class E, int G>
-__global__ __launch_bounds__(kThreads) void k_rows(const Distil q) {
+// The 16-byte pieces of a wave's tile on their way to shared memory: the span of `n`
+// elements at `src`, widened to whole pieces.  The few elements of a piece that
+// reaches over an end of the tensor [lo, hi) are copied one by one.
+template <class T, int P>
+struct Ahead {
+    static constexpr int V = 16 / sizeof(T);
+    u32x4 r[P];
+    // the pieces [first, last) that lie in the tensor, counted from src rounded down
+    static __device__ __forceinline__ void span(const T* src, int n, const T* lo, const T* hi,
+                                                unsigned& first, unsigned& count) {
+        const uintptr_t base = (uintptr_t)src & ~(uintptr_t)15;
+        first = base < (uintptr_t)lo ? 1 : 0;
+        const uintptr_t stop = (uintptr_t)(src + n);
+        const unsigned last = (unsigned)((stop - base + (stop > ((uintptr_t)hi & ~(uintptr_t)15)
+                                                             ? 0 : 15)) / 16);
+        count = last > first ? last - first : 0;
+    }
+    __device__ __forceinline__ void load(const T* src, int n, const T* lo, const T* hi, unsigned lane) {
+        unsigned first, count;
+        span(src, n, lo, hi, first, count);
+        const u32x4* p = (const u32x4*)((uintptr_t)src & ~(uintptr_t)15);
+#pragma unroll
+        for (unsigned i = 0; i < P; ++i)
+            if (lane + i * 64 - first < count) r[i] = p[lane + i * 64];
+    }
+    __device__ __forceinline__ void store(u32x4* lds, const T* src, int n, const T* lo, const T* hi,
+                                          unsigned lane) const {
+        unsigned first, count;
+        span(src, n, lo, hi, first, count);
+#pragma unroll
+        for (unsigned i = 0; i < P; ++i)
+            if (lane + i * 64 - first < count)
+                lds[lane + i * 64] = r[i];
+        const T* stop = src + n;
+        const int off = (int)((uintptr_t)src % 16 / sizeof(T));
+        T* at = (T*)lds + off;
+        if (off && src == lo && lane < V - off && (int)lane < n)
+            at[lane] = src[lane];
+        const int tail = (int)((uintptr_t)stop % 16 / sizeof(T));
+        if (tail && stop == hi && lane < tail && (int)lane < n)
+            at[n - 1 - lane] = src[n - 1 - lane];
+    }
+};
+
+// Shared memory of a tile: its rows with up to 15 bytes before them, and as many
+// words behind the last row's beginning as a group reads (the row among them).
+__host__ __device__ inline int64_t tile_room(int rows, int words, int64_t vocab, int size) {
+    return ((int64_t)(rows - 1) * vocab * size + 16 + 4 * (int64_t)words + 15) / 16 * 16;
+}
+
+// Whole rows in shared memory, G lanes each, N 32-bit words and KPL entries of a
+// row in a lane's registers.  Each wave walks tiles of 64 / G rows by itself, with
+// no barrier: the next tile's loads are in flight while one is worked on, and
+// the waves of a unit cover each other's waits.  The logits' exponentials are
+// formed once, for the sum, and kept for the gradient.
+//
+// A row of 16-bit elements may begin inside a word: the elements beside the
+// row are masked on the way in, and written around on the way out.  Entries
+// that name one column find each other through the column itself: each leaves
+// its number there, and one of them reads its own back.  A teacher of logits
+// has no bucket, so there the row's sum runs over all columns at once; with one
+// of log-probabilities the entries' columns are taken out first.
+//
+// FULL: words of a lane that lie in every row that this kernel is launched for.
+template <class E, int G, int N, int KPL, bool LOG_PROBS, int FULL>
+__global__ __launch_bounds__(kThreads, N > 14 ? 2 : KPL > 1 ? 3 : 4) void k_rows(const Distil q,
+                                                                               int64_t tiles) {
     using T = typename E::T;
-    constexpr int R = kThreads / G;
+    constexpr int R = 64 / G;
+    constexpr int W = 4 / sizeof(T);                // elements of a word
+    constexpr int P = (R * G * N * 4 / 16 + 64) / 64;  // pieces of a lane
+    constexpr int kWaves = kThreads / 64;
     extern __shared__ u32x4 smem[];
     __shared__ int scratch[kThreads / 64];
-    __shared__ double sums[R];
-    const int64_t row0 = (int64_t)blockIdx.x * R;
-    const int n_rows = q.rows - row0 < R ? (int)(q.rows - row0) : R;
-    const int64_t n = (int64_t)n_rows * q.vocab;
-    const T* src = (const T*)q.logits + row0 * q.stride;
+    __shared__ double sums[kWaves];
     const bool flat = q.stride == q.vocab;
-    T* tile = (T*)smem + (flat ? ((uintptr_t)src % 16) / sizeof(T) : 0);
-    const int64_t tile_bytes = ((int64_t)R * q.vocab * sizeof(T) + 31) / 16 * 16;
-    int* ei = (int*)((char*)smem + tile_bytes);
-    float* ep = (float*)(ei + R * q.top);
-    float* es = ep + R * q.top;
-    const int sub = threadIdx.x / G, lane = threadIdx.x % G;
-    const int64_t row = row0 + sub;
-    const bool mine = sub < n_rows;
-    T* my = tile + (int64_t)sub * q.vocab;
-    ei += sub * q.top;
-    ep += sub * q.top;
-    es += sub * q.top;
-
-    if (flat)
-        copy_flat(tile, src, n);
-    else if (mine)
-        for (int j = lane; j < q.vocab; j += G) my[j] = src[(int64_t)sub * q.stride + j];
+    const T* logits = (const T*)q.logits;
+    const T* end = logits + q.rows * q.vocab;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int sub = (threadIdx.x & 63) / G, lane = threadIdx.x % G;
+    const unsigned l64 = threadIdx.x & 63;
+    const int64_t room = tile_room(R, G * N, q.vocab, sizeof(T));
+    u32x4* lds = (u32x4*)((char*)smem + wave * room);
+    // index and probability of the row's entries, where some name one column
+    int* ei = (int*)((char*)smem + kWaves * room) + (wave * R + sub) * q.top;
+    float* ep = (float*)ei + kWaves * R * q.top;
     const float inv_count = q.grad ? inverse_count(q, scratch) : 1.f;
-    if (mine)
-        for (int k = lane; k < q.top; k += G) {
-            const Entry e = entry(q, row, k);
-            ei[k] = e.index;
-            ep[k] = e.value;
-        }
-    __syncthreads();
-    if (mine)
-        for (int k = lane; k < q.top; k += G) es[k] = ei[k] >= 0 ? E::up(my[ei[k]]) : 0.f;
-    __syncthreads();
-    if (mine)
-        for (int k = lane; k < q.top; k += G)
-            if (ei[k] >= 0) my[ei[k]] = E::down(-INFINITY);
-    __syncthreads();
     const float c = kLog2e * q.inv_temp;
-    RowStats r{};
-    float rest_m = -INFINITY;
-    if (mine) {
-        for (int j = lane; j < q.vocab; j += G) rest_m = fmaxf(rest_m, E::up(my[j]));
-        rest_m = group_max<G>(rest_m);
-        float rest_s = 0.f;
-        for (int j = lane; j < q.vocab; j += G) {
-            const float s = E::up(my[j]);
-            rest_s += s == -INFINITY ? 0.f : expo(s, rest_m, c);
+    double group_loss = 0.0;
+
+    Ahead<T, P> ahead;
+    RawEntry next[KPL];
+    auto rows_of = [&](int64_t t) {
+        return q.rows - t * R < R ? (int)(q.rows - t * R) : R;
+    };
+    auto fetch = [&](int64_t t) {
+        const int n_rows = rows_of(t);
+        if (flat) ahead.load(logits + t * R * q.vocab, n_rows * q.vocab, logits, end, l64);
+        if (sub < n_rows) {
+#pragma unroll
+            for (int i = 0; i < KPL; ++i)
+                if (lane + i * G < q.top) next[i] = raw_entry(q, t * R + sub, lane + i * G);
         }
-        rest_s = group_sum<G>(rest_s);
-        r = row_stats<G>(q, lane, ei, ep, es, rest_m, rest_s);
-        if (lane == 0) {
-            const float loss = r.active ? q.temp * q.temp * r.loss : 0.f;
-            if (q.loss_rows) q.loss_rows[row] = loss;
-            sums[sub] = loss;
+    };
+    const int64_t first = (int64_t)blockIdx.x * kWaves + wave, step = (int64_t)gridDim.x * kWaves;
+    if (first < tiles) fetch(first);
+    for (int64_t t = first; t < tiles; t += step) {
+        const int64_t row0 = t * R, row = row0 + sub;
+        const int n_rows = rows_of(t);
+        const int n = n_rows * q.vocab;
+        const bool mine = sub < n_rows;
+        const T* src = logits + row0 * q.stride;
+        const int shift = flat ? (int)((uintptr_t)src % 16 / sizeof(T)) : 0;
+        T* tile = (T*)lds + shift;
+        const int e0 = shift + sub * q.vocab;
+        T* my = (T*)lds + e0;
+        if (flat) {
+            ahead.store(lds, src, n, logits, end, l64);
+        } else if (mine) {
+#pragma unroll 1
+            for (int j = lane; j < q.vocab; j += G) my[j] = src[(int64_t)sub * q.stride + j];
         }
-    } else if (lane == 0) {
-        sums[sub] = 0.0;
+        Entries<KPL> e;
+#pragma unroll
+        for (int i = 0; i < KPL; ++i) {
+            const Entry x = checked(q, next[i]);
+            e.index[i] = mine && lane + i * G < q.top ? x.index : -1;
+            e.value[i] = x.value;
+        }
+        wave_fence();
+        if (t + step < tiles) fetch(t + step);
+        if (mine) {
+            bool shared = false;
+            auto mark = [&] {  // each entry's number in its column
+                wave_fence();
+#pragma unroll
+                for (int i = 0; i < KPL; ++i)
+                    if (e.index[i] >= 0) my[e.index[i]] = E::tag(lane + i * G);
+                wave_fence();
+            };
+            auto find = [&] {
+#pragma unroll
+                for (int i = 0; i < KPL; ++i) {
+                    e.again[i] = e.index[i] >= 0 && !E::is_tag(my[e.index[i]], lane + i * G);
+                    shared |= e.again[i];
+                }
+            };
+#pragma unroll
+            for (int i = 0; i < KPL; ++i) e.s[i] = e.index[i] >= 0 ? E::up(my[e.index[i]]) : 0.f;
+            if constexpr (LOG_PROBS) {
+                mark();
+                find();
+                wave_fence();
+#pragma unroll
+                for (int i = 0; i < KPL; ++i)
+                    if (e.index[i] >= 0) my[e.index[i]] = E::down(-INFINITY);
+                wave_fence();
+            }
+            // the row: words into registers, elements beside it at -inf
+            const int skip = W == 2 ? e0 & 1 : 0;
+            uint32_t* words = (uint32_t*)lds + e0 / W;
+            const int l0 = here(lane);
+            float v[N * W];
+            float rest_m = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                // past the row's end: what lies there (the tile has room) is masked
+                const int w = l0 + i * G;
+                const uint32_t raw = words[w];
+#pragma unroll
+                for (int h = 0; h < W; ++h) {
+                    float x = W == 1 ? __uint_as_float(raw) : E::up((T)(raw >> (16 * h)));
+                    if (i >= FULL || i == 0) {
+                        const unsigned j = (unsigned)(W * w - skip + h);
+                        x = j < (unsigned)q.vocab ? x : -INFINITY;
+                    }
+                    v[i * W + h] = x;
+                    rest_m = fmaxf(rest_m, v[i * W + h]);
+                }
+            }
+            if constexpr (!LOG_PROBS) {
+                if (q.grad) mark();
+            }
+            rest_m = group_max<G>(rest_m);
+            const float ref = rest_m == -INFINITY ? 0.f : c * rest_m;
+            float rest_s = 0.f;
+#pragma unroll
+            for (int i = 0; i < N * W; ++i) {
+                v[i] = expo(v[i], ref, c);
+                rest_s += v[i];
+            }
+            rest_s = group_sum<G>(rest_s);
+            const RowStats r = row_stats<G, KPL, LOG_PROBS>(q, e, rest_m, rest_s);
+            if (lane == 0) {
+                const float loss = r.active ? q.temp * q.temp * r.loss : 0.f;
+                if (q.loss_rows) q.loss_rows[row] = loss;
+                group_loss += loss;
+            }
+            if (q.grad) {
+                if constexpr (!LOG_PROBS) find();
+                const float f = r.active ? row_scale(q, row, inv_count) : 0.f;
+                if (!r.active && !(rest_s < INFINITY)) {  // whatever its logits hold
+#pragma unroll
+                    for (int i = 0; i < N * W; ++i) v[i] = 0.f;
+                }
+                const float factor = r.active ? r.rest * f : 0.f;
+                const int l1 = here(lane);
+                wave_fence();
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const int w = l1 + i * G;
+                    const int j = W * w - skip;
+                    if constexpr (W == 1) {
+                        if (i < FULL || j < q.vocab) words[w] = __float_as_uint(v[i] * factor);
+                    } else {
+                        const uint32_t two = E::pair(v[2 * i] * factor, v[2 * i + 1] * factor);
+                        if (i > 0 && i < FULL) {
+                            words[w] = two;
+                            continue;
+                        }
+                        if ((unsigned)j < (unsigned)(q.vocab - 1)) words[w] = two;
+                        if (j == q.vocab - 1) my[j] = (T)two;
+                        if (i == 0 && j < 0) my[0] = (T)(two >> 16);
+                    }
+                }
+                // the entries' columns, over what was written there
+                if (__builtin_expect(__any(shared), 0)) {
+#pragma unroll
+                    for (int i = 0; i < KPL; ++i)
+                        if (lane + i * G < q.top) {
+                            ei[lane + i * G] = e.index[i];
+                            ep[lane + i * G] = e.value[i];
+                        }
+                    wave_fence();
+#pragma unroll
+                    for (int i = 0; i < KPL; ++i)
+                        if (e.index[i] >= 0) {
+                            float p = 0.f;
+#pragma unroll 1
+                            for (int k = 0; k < q.top; ++k)
+                                if (ei[k] == e.index[i]) p += ep[k];
+                            e.value[i] = p;
+                        }
+                }
+                wave_fence();
+#pragma unroll
+                for (int i = 0; i < KPL; ++i)
+                    if (e.index[i] >= 0)
+                        my[e.index[i]] = E::down(f * entry_grad(r, e.s[i], e.value[i], c));
+            }
+        }
+        wave_fence();
+        if (q.grad) {
+            T* dst = (T*)q.grad + row0 * q.vocab;
+            if (flat && ((uintptr_t)dst - (uintptr_t)src) % 16 == 0) {
+                copy_flat<64>(dst, (const T*)tile, n, (int)l64);
+            } else {
+#pragma unroll 1
+                for (int i = (int)l64; i < n; i += 64) dst[i] = tile[i];
+            }
+        }
+        wave_fence();  // the tile is read before the next one is stored
     }
-    __syncthreads();  // the entries' probabilities too
-    if (q.loss_parts && threadIdx.x == 0) {
+    if (!q.loss_parts) return;
+#pragma unroll
+    for (int o = G; o < 64; o *= 2) group_loss += __shfl_xor(group_loss, o, kWave);
+    if (l64 == 0) sums[wave] = group_loss;
+    __syncthreads();
+    if (threadIdx.x == 0) {
         double s = 0.0;
-        for (int i = 0; i < R; ++i) s += sums[i];
+        for (int i = 0; i < kWaves; ++i) s += sums[i];
         q.loss_parts[blockIdx.x] = s;
     }
-    if (!q.grad) return;
-    if (mine) {
-        if (!r.active) {
-            for (int j = lane; j < q.vocab; j += G) my[j] = E::down(0.f);
-        } else {
-            const float f = row_scale(q, row, inv_count);
-            const float rest = r.rest * f;
-            for (int j = lane; j < q.vocab; j += G) {
-                const float s = E::up(my[j]);
-                my[j] = E::down(s == -INFINITY ? 0.f * rest : expo(s, rest_m, c) * rest);
-            }
-        }
-    }
-    __syncthreads();
-    if (mine && r.active) {
-        const float f = row_scale(q, row, inv_count);
-        for (int k = lane; k < q.top; k += G)
-            if (ei[k] >= 0) {
-                float p = 0.f;
-                for (int j = 0; j < q.top; ++j)
-                    if (ei[j] == ei[k]) p += ep[j];
-                const float e = es[k] == -INFINITY ? 0.f : expo(es[k], r.m, c);
-                my[ei[k]] = E::down(f * (e * r.inv - p));
-            }
-    }
-    __syncthreads();
-    T* dst = (T*)q.grad + row0 * q.vocab;
-    if (flat && ((uintptr_t)dst - (uintptr_t)src) % 16 == 0)
-        copy_flat(dst, tile, n);
-    else
-        for (int64_t i = threadIdx.x; i < n; i += kThreads) dst[i] = tile[i];
 }
 
-// A segment of a longer row: maximum and sum of its rest.
+// A segment of a longer row: maximum and sum of its rest (with a teacher of
+// logits, of all of it).
 template <class E>
 __global__ __launch_bounds__(kThreads) void k_seg_sum(const Distil q) {
     using T = typename E::T;
@@ -322,13 +606,15 @@ __global__ __launch_bounds__(kThreads) void k_seg_sum(const Distil q) {
     const int j0 = seg * q.seg, n = q.vocab - j0 < q.seg ? q.vocab - j0 : q.seg;
     const T* src = (const T*)q.logits + row * q.stride + j0;
     T* tile = (T*)smem + ((uintptr_t)src % 16) / sizeof(T);
-    copy_flat(tile, src, n);
+    copy_flat<kThreads>(tile, src, n, threadIdx.x);
     __syncthreads();
-    for (int k = threadIdx.x; k < q.top; k += kThreads) {
-        const int i = entry(q, row, k).index - j0;
-        if (i >= 0 && i < n) tile[i] = E::down(-INFINITY);
+    if (q.log_probs) {
+        for (int k = threadIdx.x; k < q.top; k += kThreads) {
+            const int i = entry(q, row, k).index - j0;
+            if (i >= 0 && i < n) tile[i] = E::down(-INFINITY);
+        }
+        __syncthreads();
     }
-    __syncthreads();
     const float c = kLog2e * q.inv_temp;
     float m = -INFINITY;
     for (int j = threadIdx.x; j < n; j += kThreads) m = fmaxf(m, E::up(tile[j]));
@@ -340,7 +626,7 @@ __global__ __launch_bounds__(kThreads) void k_seg_sum(const Distil q) {
     float s = 0.f;
     for (int j = threadIdx.x; j < n; j += kThreads) {
         const float v = E::up(tile[j]);
-        s += v == -INFINITY ? 0.f : expo(v, m, c);
+        s += v == -INFINITY ? 0.f : expo(v, c * m, c);
     }
     s = group_sum<64>(s);
     __syncthreads();
@@ -362,18 +648,24 @@ __global__ __launch_bounds__(64) void k_seg_join(const Distil q) {
     using T = typename E::T;
     extern __shared__ u32x4 smem[];
     int* ei = (int*)smem;
-    float* ep = (float*)(ei + q.top);
-    float* es = ep + q.top;
     const int64_t row = blockIdx.x;
     const int lane = threadIdx.x;
     const T* src = (const T*)q.logits + row * q.stride;
-    for (int k = lane; k < q.top; k += 64) {
-        const Entry e = entry(q, row, k);
-        ei[k] = e.index;
-        ep[k] = e.value;
-        es[k] = e.index >= 0 ? E::up(src[e.index]) : 0.f;
+    constexpr int KPL = GSX_DISTIL_MAX_TOP / 64;
+    Entries<KPL> e;
+    read_entries<64, KPL>(q, row, lane, e);
+#pragma unroll
+    for (int i = 0; i < KPL; ++i) {
+        if (lane + i * 64 < q.top) ei[lane + i * 64] = e.index[i];
+        e.s[i] = e.index[i] >= 0 ? E::up(src[e.index[i]]) : 0.f;
     }
     __syncthreads();
+#pragma unroll
+    for (int i = 0; i < KPL; ++i) {
+        e.again[i] = false;
+        if (e.index[i] >= 0)
+            for (int k = 0; k < lane + i * 64; ++k) e.again[i] |= ei[k] == e.index[i];
+    }
     const float c = kLog2e * q.inv_temp;
     const float* parts = q.seg_parts + row * q.segs * 2;
     float m = -INFINITY, s = 0.f;
@@ -381,10 +673,11 @@ __global__ __launch_bounds__(64) void k_seg_join(const Distil q) {
     m = group_max<64>(m);
     for (int i = lane; i < q.segs; i += 64) {
         const float pm = parts[2 * i], ps = parts[2 * i + 1];
-        s += pm == -INFINITY ? ps : ps * expo(pm, m, c);  // ps is 0, or NaN
+        s += pm == -INFINITY ? ps : ps * __builtin_amdgcn_exp2f(c * pm - c * m);  // 0, or NaN
     }
     s = group_sum<64>(s);
-    const RowStats r = row_stats<64>(q, lane, ei, ep, es, m, s);
+    const RowStats r = q.log_probs ? row_stats<64, KPL, true>(q, e, m, s)
+                                   : row_stats<64, KPL, false>(q, e, m, s);
     if (lane == 0) {
         const float loss = r.active ? q.temp * q.temp * r.loss : 0.f;
         if (q.loss_rows) q.loss_rows[row] = loss;
@@ -392,13 +685,15 @@ __global__ __launch_bounds__(64) void k_seg_join(const Distil q) {
         float* st = q.stats + row * 8;
         st[0] = m;
         st[1] = r.rest;
-        st[2] = r.m;
+        st[2] = r.mc;
         st[3] = r.inv;
         st[4] = r.active ? 1.f : 0.f;
     }
     // the entries' probabilities, for the gradient
     float* probs = q.stats + q.rows * 8 + row * q.top;
-    for (int k = lane; k < q.top; k += 64) probs[k] = ep[k];
+#pragma unroll
+    for (int i = 0; i < KPL; ++i)
+        if (lane + i * 64 < q.top) probs[lane + i * 64] = e.value[i];
 }
 
 // A segment's gradient.
@@ -418,14 +713,14 @@ __global__ __launch_bounds__(kThreads) void k_seg_grad(const Distil q) {
     const bool active = st[4] != 0.f;
     const float f = row_scale(q, row, inv_count);
     const float c = kLog2e * q.inv_temp;
-    const float rest_m = st[0], rest = st[1] * f;
-    if (active) copy_flat(tile, src, n);
+    const float rest_mc = c * st[0], rest = st[1] * f;
+    if (active) copy_flat<kThreads>(tile, src, n, threadIdx.x);
     __syncthreads();
     for (int j = threadIdx.x; j < n; j += kThreads) {
         float g = 0.f;
         if (active) {
             const float s = E::up(tile[j]);
-            g = s == -INFINITY ? 0.f * rest : expo(s, rest_m, c) * rest;
+            g = s == -INFINITY ? 0.f * rest : expo(s, rest_mc, c) * rest;
         }
         tile[j] = E::down(g);
     }
@@ -445,20 +740,28 @@ __global__ __launch_bounds__(kThreads) void k_seg_grad(const Distil q) {
     }
     __syncthreads();
     if (((uintptr_t)dst - (uintptr_t)src) % 16 == 0)
-        copy_flat(dst, tile, n);
+        copy_flat<kThreads>(dst, (const T*)tile, n, threadIdx.x);
     else
         for (int i = threadIdx.x; i < n; i += kThreads) dst[i] = tile[i];
 }
 
-// Rows that have an entry, a count for each of kCountParts workgroups.
-__global__ __launch_bounds__(kThreads) void k_count(const Distil q, int* counts) {
-    __shared__ int red[kThreads / 64];
+// Rows that have an entry, a count for each of kCountParts workgroups.  Most
+// rows show one in their first entry: four rows' are in flight at a time.
+__global__ __launch_bounds__(1024) void k_count(const Distil q, int* counts) {
+    __shared__ int red[1024 / 64];
+    constexpr int64_t step = (int64_t)kCountParts * 1024;
     int n = 0;
-    for (int64_t row = (int64_t)blockIdx.x * kThreads + threadIdx.x; row < q.rows;
-         row += (int64_t)kCountParts * kThreads) {
-        int any = 0;
-        for (int k = 0; k < q.top && !any; ++k) any = entry(q, row, k).index >= 0;
-        n += any;
+    for (int64_t row = (int64_t)blockIdx.x * 1024 + threadIdx.x; row < q.rows; row += 4 * step) {
+        int found[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            found[i] = row + i * step < q.rows && entry(q, row + i * step, 0).index >= 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            for (int k = 1; k < q.top && !found[i] && row + i * step < q.rows; ++k)
+                found[i] = entry(q, row + i * step, k).index >= 0;
+            n += found[i];
+        }
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o, kWave);
@@ -467,7 +770,7 @@ __global__ __launch_bounds__(kThreads) void k_count(const Distil q, int* counts)
     if (threadIdx.x == 0) {
         n = 0;
 #pragma unroll
-        for (int w = 0; w < kThreads / 64; ++w) n += red[w];
+        for (int w = 0; w < 1024 / 64; ++w) n += red[w];
         counts[blockIdx.x] = n;
     }
 }
@@ -478,7 +781,15 @@ __global__ __launch_bounds__(kThreads) void k_total(const double* parts, int64_t
     __shared__ double red[kThreads];
     __shared__ int cnt[kThreads];
     double s = 0.0;
-    for (int64_t i = threadIdx.x; i < n; i += kThreads) s += parts[i];
+    int64_t i = threadIdx.x;
+    for (; i + 7 * kThreads < n; i += 8 * kThreads) {  // eight loads in flight
+        double v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = parts[i + j * kThreads];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s += v[j];
+    }
+    for (; i < n; i += kThreads) s += parts[i];
     red[threadIdx.x] = s;
     cnt[threadIdx.x] = counts && threadIdx.x < kCountParts ? counts[threadIdx.x] : 0;
     __syncthreads();
@@ -511,12 +822,19 @@ int check_shape(int dtype, int64_t rows, int64_t vocab, int64_t top) {
 int elem(int dtype) { return dtype == GSX_F32 ? 4 : 2; }
 bool short_rows(int dtype, int64_t vocab) { return vocab * elem(dtype) <= kRowBytes; }
 
-// Lanes for a row: about eight logits each, 4 to 64.
-int lanes_for(int64_t vocab) {
+// 32-bit words that a row may touch (a 16-bit row may begin inside one), and
+// the lanes that hold them: up to kHeld words each, 4 to 64 lanes.
+// Four entries at most on a lane.
+int words_of(int dtype, int64_t vocab) {
+    return (int)(dtype == GSX_F32 ? vocab : (vocab + 1) / 2 + 1);
+}
+constexpr int kHeld = 14;
+int lanes_for(int dtype, int64_t vocab, int64_t top) {
     int g = 4;
-    while (g < 64 && g * 8 < vocab) g *= 2;
+    while (g < 64 && (g * kHeld < words_of(dtype, vocab) || g * 4 < top)) g *= 2;
     return g;
 }
+constexpr int64_t kRowGroups = 2048;  // workgroups that walk the tiles: eight for a unit
 
 // The workspace: the count's parts, the workgroups' losses, then for longer
 // rows the segments' sums, the rows' statistics and the entries' probabilities.
@@ -529,8 +847,9 @@ Layout layout(int dtype, int64_t rows, int64_t vocab, int64_t top) {
     Layout l{};
     l.parts = kCountParts * 4;
     if (short_rows(dtype, vocab)) {
-        const int r = kThreads / lanes_for(vocab);
+        const int r = kThreads / lanes_for(dtype, vocab, top);
         l.n_parts = (rows + r - 1) / r;
+        if (l.n_parts > kRowGroups) l.n_parts = kRowGroups;
         l.segs = l.stats = l.total = up_to(l.parts + l.n_parts * 8, 256);
         return l;
     }
@@ -543,27 +862,64 @@ Layout layout(int dtype, int64_t rows, int64_t vocab, int64_t top) {
     return l;
 }
 
-template <class E, int G>
+template <class E, int G, int N, int KPL, bool LOG_PROBS, int FULL>
 int launch_rows(const Distil& q, hipStream_t st) {
-    constexpr int R = kThreads / G;
-    const int64_t blocks = (q.rows + R - 1) / R;
-    const int64_t tile = ((int64_t)R * q.vocab * sizeof(typename E::T) + 31) / 16 * 16;
-    const int64_t lds = tile + (int64_t)R * q.top * 12;
-    if (blocks >= (1LL << 31) || lds > 160 * 1024 - 4096) return GSX_ERR_TOO_LARGE;
-    hipLaunchKernelGGL((k_rows<E, G>), dim3((unsigned)blocks), dim3(kThreads), (unsigned)lds, st,
-                       q);
+    constexpr int R = 64 / G, kWaves = kThreads / 64;
+    const int64_t tiles = (q.rows + R - 1) / R, groups = (tiles + kWaves - 1) / kWaves;
+    const int64_t lds = kWaves * (tile_room(R, G * N, q.vocab, sizeof(typename E::T)) +
+                                  (int64_t)R * q.top * 8);
+    if (lds > 64 * 1024) return GSX_ERR_TOO_LARGE;
+    hipLaunchKernelGGL((k_rows<E, G, N, KPL, LOG_PROBS, FULL>),
+                       dim3((unsigned)(groups < kRowGroups ? groups : kRowGroups)), dim3(kThreads),
+                       (unsigned)lds, st, q, tiles);
     GSX_LAUNCH_CHECK();
     return GSX_OK;
 }
 
+// For rows of MORE to N words a lane: of 16-bit rows, which may begin inside a
+// word, all but the first and the last MORE - 2 are whole words of the row.
+template <class E, int G, int N, int KPL, int MORE>
+int launch_rows(const Distil& q, hipStream_t st) {
+    constexpr int FULL = MORE > 2 ? MORE - 2 : 0;
+    return q.log_probs ? launch_rows<E, G, N, KPL, true, FULL>(q, st)
+                       : launch_rows<E, G, N, KPL, false, FULL>(q, st);
+}
+
+// The kernel whose lanes hold the row's words with the least room to spare
+// (fewer to choose from where a lane has several entries).
+template <class E, int G>
+int launch_rows(const Distil& q, int words, hipStream_t st) {
+    const int n = (words + G - 1) / G;
+    if (q.top > G) {
+        if (n <= 6) return launch_rows<E, G, 6, 4, 0>(q, st);
+        if constexpr (G == 64) {
+            if (n > 14) return launch_rows<E, G, 33, 4, 15>(q, st);
+        }
+        return launch_rows<E, G, 14, 4, 7>(q, st);
+    }
+    if constexpr (G == 4) {
+        if (n <= 3) return launch_rows<E, G, 3, 1, 0>(q, st);
+    }
+    if (n <= 6) return launch_rows<E, G, 6, 1, 0>(q, st);
+    if (n <= 8) return launch_rows<E, G, 8, 1, 7>(q, st);
+    if (n <= 10) return launch_rows<E, G, 10, 1, 9>(q, st);
+    if constexpr (G == 64) {
+        if (n > 20) return launch_rows<E, G, 33, 1, 21>(q, st);
+        if (n > 14) return launch_rows<E, G, 20, 1, 15>(q, st);
+    }
+    return launch_rows<E, G, 14, 1, 11>(q, st);
+}
+
 template <class E>
 int run_rows(const Distil& q, hipStream_t st) {
-    switch (lanes_for(q.vocab)) {
-        case 4: return launch_rows<E, 4>(q, st);
-        case 8: return launch_rows<E, 8>(q, st);
-        case 16: return launch_rows<E, 16>(q, st);
-        case 32: return launch_rows<E, 32>(q, st);
-        default: return launch_rows<E, 64>(q, st);
+    constexpr int dtype = sizeof(typename E::T) == 4 ? GSX_F32 : GSX_BF16;
+    const int words = words_of(dtype, q.vocab);
+    switch (lanes_for(dtype, q.vocab, q.top)) {
+        case 4: return launch_rows<E, 4>(q, words, st);
+        case 8: return launch_rows<E, 8>(q, words, st);
+        case 16: return launch_rows<E, 16>(q, words, st);
+        case 32: return launch_rows<E, 32>(q, words, st);
+        default: return launch_rows<E, 64>(q, words, st);
     }
 }
 
@@ -578,7 +934,7 @@ int run(const Distil& q, bool sums, hipStream_t st) {
         hipLaunchKernelGGL((k_seg_sum<E>), dim3((unsigned)blocks), dim3(kThreads), 0, st, q);
         GSX_LAUNCH_CHECK();
         hipLaunchKernelGGL((k_seg_join<E>), dim3((unsigned)q.rows), dim3(64),
-                           (unsigned)(q.top * 12), st, q);
+                           (unsigned)(q.top * 4), st, q);
         GSX_LAUNCH_CHECK();
     }
     if (q.grad) {
@@ -667,7 +1023,7 @@ int forward(const Args& a, float scale, float* loss, void* grad, void* stream) {
     else
         q.loss_parts = parts;
     if (a.reduction == GSX_REDUCE_MEAN) {
-        hipLaunchKernelGGL(k_count, dim3(kCountParts), dim3(kThreads), 0, st, q,
+        hipLaunchKernelGGL(k_count, dim3(kCountParts), dim3(1024), 0, st, q,
                            (int*)a.workspace);
         GSX_LAUNCH_CHECK();
     }

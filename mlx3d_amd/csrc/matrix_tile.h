@@ -37,7 +37,15 @@ struct F32 {
     }
     static __device__ __forceinline__ float up(T v) { return v; }
     static __device__ __forceinline__ T down(float v) { return v; }
+    // a small whole number in an element's place, told apart by its bits
+    static __device__ __forceinline__ T tag(int k) { return __uint_as_float((uint32_t)k); }
+    static __device__ __forceinline__ bool is_tag(T v, int k) {
+        return __float_as_uint(v) == (uint32_t)k;
+    }
 };
+using f32x2 = __attribute__((ext_vector_type(2))) float;
+using bf16x2 = __attribute__((ext_vector_type(2))) __bf16;
+
 struct BF16 {
     using T = uint16_t;
     static constexpr int VEC = 8;
@@ -49,6 +57,11 @@ struct BF16 {
     static __device__ __forceinline__ T down(float v) {
         return __builtin_bit_cast(uint16_t, (__bf16)v);
     }
+    static __device__ __forceinline__ uint32_t pair(float lo, float hi) {
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{lo, hi}, bf16x2));
+    }
+    static __device__ __forceinline__ T tag(int k) { return (T)k; }
+    static __device__ __forceinline__ bool is_tag(T v, int k) { return v == (T)k; }
 };
 struct F16 {
     using T = uint16_t;
@@ -63,6 +76,11 @@ struct F16 {
     static __device__ __forceinline__ T down(float v) {
         return __builtin_bit_cast(uint16_t, (_Float16)v);
     }
+    static __device__ __forceinline__ uint32_t pair(float lo, float hi) {
+        return (uint32_t)down(lo) | (uint32_t)down(hi) << 16;
+    }
+    static __device__ __forceinline__ T tag(int k) { return (T)k; }
+    static __device__ __forceinline__ bool is_tag(T v, int k) { return v == (T)k; }
 };
 
 }  // namespace gsx

@@ -33,21 +33,42 @@ constexpr int kBN = 64;   // rows of the second
 
 // ---------------------------------------------------------- activations --
 
+// exp(-g).  float32 tensors: 2^t with what rounding t = -g log2(e) left out put
+// back (a relative error of some 2^-23 for any g, where 2^t alone loses |t| 2^-24);
+// 16-bit ones 2^t.  Beyond +-126 the result is past 0 or infinity for 1 + e.
+template <bool EXACT>
+__device__ __forceinline__ float exp_neg(float g) {
+    constexpr float L = -1.44269504088896341f, L2 = -1.92596299e-8f;  // -log2(e), its rest
+    if constexpr (EXACT) {
+        const float x = __builtin_amdgcn_fmed3f(g, -126.f, 126.f);
+        const float t = x * L;
+        const float rest = fmaf(x, L2, fmaf(x, L, -t));
+        const float e = __builtin_amdgcn_exp2f(t);
+        return fmaf(e, rest * 0.69314718055994531f, e);
+    } else {
+        return __builtin_amdgcn_exp2f(g * L);
+    }
+}
+
 // act(g) and act'(g); NaN and infinities as the formulas give them.
+template <bool EXACT>
 __device__ __forceinline__ float activate(int act, float g, float& slope) {
     if (act == GSX_ACT_GELU) {
         const float cdf = 0.5f * (1.0f + erff(g * 0.70710678118654752f));
         slope = cdf + g * 0.39894228040143268f * __expf(-0.5f * g * g);
         return g * cdf;
     }
-    const float s = 1.0f / (1.0f + __expf(-g));
+    const float s = __builtin_amdgcn_rcpf(1.0f + exp_neg<EXACT>(g));
     if (act == GSX_ACT_SIGMOID) {
         slope = s * (1.0f - s);
-        return s;
+        return g != g ? g : s;
     }
     slope = s * (1.0f + g * (1.0f - s));
     return g * s;
 }
+
+template <class E>
+constexpr bool kExact = sizeof(typename E::T) == 4;
 
 // ---------------------------------------------------------------- tiles --
 
@@ -296,7 +317,7 @@ __global__ __launch_bounds__(kThreads) void k_tile(const Tile q) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     float slope;
-                    h[e] = activate(q.act, c0[i][j][e], slope) * c1[i][j][e];
+                    h[e] = activate<kExact<E>>(q.act, c0[i][j][e], slope) * c1[i][j][e];
                 }
                 put<E>((T*)q.out[0], q.ldo, row, col, q.m, q.n, q.vec_out, h);
             } else if constexpr (MODE == BWD_HIDDEN) {
@@ -304,7 +325,7 @@ __global__ __launch_bounds__(kThreads) void k_tile(const Tile q) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     float slope;
-                    const float a = activate(q.act, c0[i][j][e], slope);
+                    const float a = activate<kExact<E>>(q.act, c0[i][j][e], slope);
                     const float u = c1[i][j][e], dh = c2[i][j][e];
                     h[e] = a * u;
                     du[e] = dh * a;
@@ -333,6 +354,170 @@ __global__ __launch_bounds__(kThreads) void k_join(const float* parts, int64_t n
 __global__ __launch_bounds__(kThreads) void k_zero_bytes(uint8_t* p, int64_t n) {
     const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
     if (i < n) p[i] = 0;
+}
+
+// --------------------------------------------------------------- narrow --
+
+// The whole block in one kernel, for narrow widths and many rows: h stays in
+// registers, so x is read and y written once and nothing else moves.  Each wave
+// takes 32 rows through all of it.
+//
+// Products run with the weights first, so that a lane holds one row (its column
+// of the product) and consecutive channels: g^T and u^T come out with channels
+// 4 (l / 16) .. + 3 of 16 on a lane, and two such blocks are the eight channels
+// that the next product's operand wants there, if the blocks' rows are taken in
+// the order 8 (r / 4) + r % 4 (+ 4 in the second).  h never crosses lanes.
+//
+// The weights lie in shared memory in operand order, cut into chunks of 32
+// hidden channels; as many chunks at a time as fit (all of them: staged once).
+constexpr int kNarrowThreads = 512;
+constexpr int kNarrowRows = 32;                   // rows of a wave
+constexpr int64_t kNarrowLds = 144 * 1024;
+
+template <class E>
+struct Narrow {
+    const typename E::T *x, *wg, *wu, *wd;
+    typename E::T* y;
+    int64_t ldx, rows;
+    int d_in, hidden, d_out, act;
+    int chunks, resident;  // chunks of 32 hidden channels, how many are staged at a time
+};
+
+// Stages `count` chunks from number c0 on: for each chunk, fragments of Wg (two
+// blocks of 16 channels times KD), of Wu, then OB of Wd, each with its pieces.
+template <class E, int KD, int OB>
+__device__ __forceinline__ void stage_weights(const Narrow<E>& q, u32x4* lds, int c0, int count) {
+    using Wd = Wide<E>;
+    constexpr int PC = Wd::PIECES, FRAGS = 4 * KD + OB;
+    const int64_t in = (int64_t)q.hidden * q.d_in, out = (int64_t)q.d_out * q.hidden;
+    for (int i = threadIdx.x; i < count * FRAGS * 64; i += kNarrowThreads) {
+        const int lane = i & 63, frag = (i >> 6) % FRAGS, c = (i >> 6) / FRAGS;
+        const int r = lane & 15, k8 = (lane >> 4) * 8;
+        typename Wd::Raw raw{};
+        if (frag < 4 * KD) {
+            const int kd = frag % KD, which = frag / KD;  // Wg a, Wg b, Wu a, Wu b
+            const int f = (c0 + c) * 32 + 8 * (r >> 2) + (r & 3) + 4 * (which & 1);
+            const int k = kd * 32 + k8;
+            if (f < q.hidden && k < q.d_in)
+                raw = load8<E>((which < 2 ? q.wg : q.wu) + (int64_t)f * q.d_in, k, q.d_in,
+                               in - (int64_t)f * q.d_in);
+        } else {
+            const int o = (frag - 4 * KD) * 16 + r, k = (c0 + c) * 32 + k8;
+            if (o < q.d_out && k < q.hidden)
+                raw = load8<E>(q.wd + (int64_t)o * q.hidden, k, q.hidden,
+                               out - (int64_t)o * q.hidden);
+        }
+        const typename Wd::Frag w = Wd::frag(raw);
+#pragma unroll
+        for (int p = 0; p < PC; ++p) lds[((c * FRAGS + frag) * PC + p) * 64 + lane] = w.p[p];
+    }
+}
+
+template <class E, int KD, int OB>
+__global__ __launch_bounds__(kNarrowThreads) void k_narrow_fwd(const Narrow<E> q) {
+    using T = typename E::T;
+    using W = Wide<E>;
+    constexpr int PC = W::PIECES, FRAGS = 4 * KD + OB;
+    constexpr int kWaves = kNarrowThreads / 64, R = kNarrowRows / 16;
+    extern __shared__ u32x4 smem[];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int col = lane & 15, k8 = (lane >> 4) * 8;
+    const bool once = q.resident >= q.chunks;
+    auto weights = [&](int c, int frag) {
+        typename W::Frag w;
+#pragma unroll
+        for (int p = 0; p < PC; ++p) w.p[p] = smem[((c * FRAGS + frag) * PC + p) * 64 + lane];
+        return w;
+    };
+    if (once) {
+        stage_weights<E, KD, OB>(q, smem, 0, q.chunks);
+        __syncthreads();
+    }
+    const int64_t tile_rows = kWaves * kNarrowRows;
+    for (int64_t base = blockIdx.x * tile_rows; base < q.rows; base += gridDim.x * tile_rows) {
+        const int64_t row0 = base + wave * kNarrowRows + col;
+        typename W::Frag x[R][KD];
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int kd = 0; kd < KD; ++kd) {
+                const int64_t row = row0 + 16 * r;
+                const int k = kd * 32 + k8;
+                typename W::Raw raw{};
+                if (row < q.rows && k < q.d_in)
+                    raw = load8<E>(q.x + row * q.ldx, k, q.d_in,
+                                   (q.rows - 1 - row) * q.ldx + q.d_in);
+                x[r][kd] = W::frag(raw);
+            }
+        f32x4 y[OB][R];
+#pragma unroll
+        for (int o = 0; o < OB; ++o)
+#pragma unroll
+            for (int r = 0; r < R; ++r) y[o][r] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int c0 = 0; c0 < q.chunks; c0 += q.resident) {
+            const int count = q.chunks - c0 < q.resident ? q.chunks - c0 : q.resident;
+            if (!once) {
+                __syncthreads();  // the last chunks are read
+                stage_weights<E, KD, OB>(q, smem, c0, count);
+                __syncthreads();
+            }
+            for (int c = 0; c < count; ++c) {
+                f32x4 g[2][R], u[2][R];
+#pragma unroll
+                for (int b = 0; b < 2; ++b)
+#pragma unroll
+                    for (int r = 0; r < R; ++r) g[b][r] = u[b][r] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int kd = 0; kd < KD; ++kd)
+#pragma unroll
+                    for (int b = 0; b < 2; ++b) {
+                        const auto wg = weights(c, b * KD + kd), wu = weights(c, (2 + b) * KD + kd);
+#pragma unroll
+                        for (int r = 0; r < R; ++r) {
+                            g[b][r] = W::mma(wg, x[r][kd], g[b][r]);
+                            u[b][r] = W::mma(wu, x[r][kd], u[b][r]);
+                        }
+                    }
+                typename W::Frag h[R];
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    float v[8], slope;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        v[i] = activate<kExact<E>>(q.act, g[i >> 2][r][i & 3], slope) *
+                               u[i >> 2][r][i & 3];
+                    h[r] = W::frag(v);
+                }
+#pragma unroll
+                for (int o = 0; o < OB; ++o)
+                    if (o * 16 < q.d_out) {
+                        const auto wd = weights(c, 4 * KD + o);
+#pragma unroll
+                        for (int r = 0; r < R; ++r) y[o][r] = W::mma(wd, h[r], y[o][r]);
+                    }
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const int64_t row = row0 + 16 * r;
+            if (row >= q.rows) continue;
+#pragma unroll
+            for (int o = 0; o < OB; ++o) {
+                const int at = o * 16 + (lane >> 4) * 4;
+                T w[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[i] = E::down(y[o][r][i]);
+                T* out = q.y + row * q.d_out + at;
+                if (at + 4 <= q.d_out) {
+                    __builtin_memcpy(out, w, sizeof(w));
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (at + i < q.d_out) out[i] = w[i];
+                }
+            }
+        }
+    }
 }
 
 // ----------------------------------------------------------------- host --
@@ -411,7 +596,68 @@ int launch_tile(const Tile& q, int splits, hipStream_t st) {
 int64_t pitch(const Shape& s) { return up_to(s.hidden, 8); }
 int64_t hidden_bytes(const Shape& s) { return up_to(s.rows * pitch(s) * s.size(), 256); }
 
-int64_t fwd_bytes(const Shape& s) { return s.rows == 0 ? 0 : hidden_bytes(s); }
+// Whether the narrow kernel holds a row's operands and sums in its registers:
+// 8 (KD pieces + OB) of them, beside some 100 others.
+constexpr bool narrow_fits(int pieces, int kd, int ob) { return 8 * (kd * pieces + ob) <= 152; }
+int64_t narrow_chunk_bytes(const Shape& s, int kd, int ob) {
+    return (s.dtype == GSX_F32 ? 3 : 1) * (int64_t)(4 * kd + ob) * 1024;
+}
+int narrow_kd(const Shape& s) { return s.d_in <= 32 ? 1 : s.d_in <= 64 ? 2 : 4; }
+int narrow_ob(const Shape& s) {
+    return s.d_out <= 16 ? 1 : s.d_out <= 32 ? 2 : s.d_out <= 64 ? 4 : s.d_out <= 128 ? 8 : 16;
+}
+bool narrow_fwd(const Shape& s) {
+    return s.d_in <= 128 && s.d_out <= 256 &&
+           narrow_fits(s.dtype == GSX_F32 ? 3 : 1, narrow_kd(s), narrow_ob(s));
+}
+
+int64_t fwd_bytes(const Shape& s) {
+    return s.rows == 0 || narrow_fwd(s) ? 0 : hidden_bytes(s);
+}
+
+template <class E, int KD, int OB>
+int launch_narrow_fwd(const Shape& s, const void* x, int64_t ldx, const void* wg, const void* wu,
+                      const void* wd, void* y, hipStream_t st) {
+    using T = typename E::T;
+    Narrow<E> q{(const T*)x, (const T*)wg, (const T*)wu, (const T*)wd, (T*)y, ldx,
+                s.rows,      s.d_in,       s.hidden,     s.d_out,      s.act, 0, 0};
+    const int64_t chunk = narrow_chunk_bytes(s, KD, OB);
+    q.chunks = (s.hidden + 31) / 32;
+    q.resident = (int)(kNarrowLds / chunk);
+    if (q.resident > q.chunks) q.resident = q.chunks;
+    const int64_t lds = q.resident * chunk;
+    const int64_t tiles = (s.rows + kNarrowThreads / 64 * kNarrowRows - 1) /
+                          (kNarrowThreads / 64 * kNarrowRows);
+    int64_t per_cu = 160 * 1024 / lds;
+    if (per_cu > 2) per_cu = 2;
+    const int64_t grid = tiles < 256 * per_cu ? tiles : 256 * per_cu;
+    const hipError_t e = hipFuncSetAttribute((const void*)&k_narrow_fwd<E, KD, OB>,
+                                             hipFuncAttributeMaxDynamicSharedMemorySize,
+                                             (int)kNarrowLds);
+    if (e != hipSuccess) return GSX_ERR_HIP;
+    hipLaunchKernelGGL((k_narrow_fwd<E, KD, OB>), dim3((unsigned)grid), dim3(kNarrowThreads),
+                       (unsigned)lds, st, q);
+    GSX_LAUNCH_CHECK();
+    return GSX_OK;
+}
+
+template <class E, int KD, int OB, class... A>
+int narrow_if(const Shape& s, A... a) {
+    if constexpr (narrow_fits(Wide<E>::PIECES, KD, OB))
+        return launch_narrow_fwd<E, KD, OB>(s, a...);
+    else
+        return GSX_ERR_INVALID;  // narrow_fwd() keeps these out
+}
+template <class E, int KD, class... A>
+int narrow_forward(const Shape& s, A... a) {
+    switch (narrow_ob(s)) {
+        case 1: return narrow_if<E, KD, 1>(s, a...);
+        case 2: return narrow_if<E, KD, 2>(s, a...);
+        case 4: return narrow_if<E, KD, 4>(s, a...);
+        case 8: return narrow_if<E, KD, 8>(s, a...);
+        default: return narrow_if<E, KD, 16>(s, a...);
+    }
+}
 
 int64_t parts_bytes(const Shape& s) {
     const Splits a = splits_of(s.rows, s.d_in, s.hidden), b = splits_of(s.rows, s.hidden, s.d_out);
@@ -425,6 +671,13 @@ int64_t bwd_bytes(const Shape& s) { return s.rows == 0 ? 0 : 3 * hidden_bytes(s)
 template <class E>
 int forward(const Shape& s, const void* x, int64_t ldx, const void* wg, const void* wu,
             const void* wd, void* y, int64_t ldy, void* ws, hipStream_t st) {
+    if (narrow_fwd(s)) {
+        switch (narrow_kd(s)) {
+            case 1: return narrow_forward<E, 1>(s, x, ldx, wg, wu, wd, y, st);
+            case 2: return narrow_forward<E, 2>(s, x, ldx, wg, wu, wd, y, st);
+            default: return narrow_forward<E, 4>(s, x, ldx, wg, wu, wd, y, st);
+        }
+    }
     const int64_t ph = pitch(s);
     Tile q{};
     q.a = first<E>(x, ldx, s.rows, true);
@@ -568,7 +821,7 @@ int gsx_ffn_fwd(int32_t dtype, int32_t act, int64_t rows, int32_t d_in, int32_t 
     if (!x || !w_gate || !w_up || !w_down || !y || x_stride < d_in) return GSX_ERR_INVALID;
     for (const void* p : {x, w_gate, w_up, w_down, (const void*)y})
         if (misaligned(p, s.size())) return GSX_ERR_INVALID;
-    if (workspace_bytes < fwd_bytes(s) || !workspace) return GSX_ERR_WORKSPACE;
+    if (workspace_bytes < fwd_bytes(s) || (fwd_bytes(s) && !workspace)) return GSX_ERR_WORKSPACE;
     if (misaligned(workspace, 16)) return GSX_ERR_INVALID;
     hipStream_t st = (hipStream_t)stream;
     if (dtype == GSX_F32)

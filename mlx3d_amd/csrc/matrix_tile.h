@@ -83,4 +83,102 @@ struct F16 {
     static __device__ __forceinline__ bool is_tag(T v, int k) { return v == (T)k; }
 };
 
+// What the narrow kernels multiply: a float32 operand as three bf16 pieces
+// (rounded to nearest: 8 + 8 + 8 bits hold the 24 exactly, the pieces falling by
+// 2^-8 each) and six of their nine products, the rest below 2^-23 of a product;
+// 16-bit operands as they are.  The matrix units take 16 bits at eight times
+// the float32 rate (1248 against 154 TFLOP/s in large products), so six products
+// cost less than half of one in float32.
+struct Split3 {
+    u32x4 p[3];
+};
+__device__ __forceinline__ Split3 split(const float* x) {
+    Split3 s;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        float a = x[2 * i], b = x[2 * i + 1];
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+            const uint32_t two = BF16::pair(a, b);
+            s.p[k][i] = two;
+            if (k < 2) {
+                a -= __uint_as_float(two << 16);
+                b -= __uint_as_float(two & 0xffff0000u);
+            }
+        }
+    }
+    return s;
+}
+
+// An element type with its operand form: eight elements of a row on a lane.
+template <class E>
+struct Wide {
+    static constexpr int PIECES = 1;
+    using Raw = u32x4;
+    struct Frag {
+        u32x4 p[1];
+    };
+    static __device__ __forceinline__ Frag frag(const Raw& r) { return Frag{{r}}; }
+    static __device__ __forceinline__ Frag frag(const float* x) {
+        Frag f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f.p[0][i] = E::pair(x[2 * i], x[2 * i + 1]);
+        return f;
+    }
+    static __device__ __forceinline__ f32x4 mma(const Frag& a, const Frag& b, f32x4 c) {
+        return E::mma(a.p[0], b.p[0], c);
+    }
+    // zero elements from number n on
+    static __device__ __forceinline__ void cut(Raw& r, int n) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (2 * i + 1 >= n) r[i] &= 0xffffu;
+            if (2 * i >= n) r[i] = 0;
+        }
+    }
+};
+template <>
+struct Wide<F32> {
+    static constexpr int PIECES = 3;
+    struct Raw {
+        float v[8];
+    };
+    using Frag = Split3;
+    static __device__ __forceinline__ Frag frag(const Raw& r) { return split(r.v); }
+    static __device__ __forceinline__ Frag frag(const float* x) { return split(x); }
+    static __device__ __forceinline__ f32x4 mma(const Frag& a, const Frag& b, f32x4 c) {
+        c = BF16::mma(a.p[2], b.p[0], c);
+        c = BF16::mma(a.p[0], b.p[2], c);
+        c = BF16::mma(a.p[1], b.p[1], c);
+        c = BF16::mma(a.p[1], b.p[0], c);
+        c = BF16::mma(a.p[0], b.p[1], c);
+        return BF16::mma(a.p[0], b.p[0], c);
+    }
+    static __device__ __forceinline__ void cut(Raw& r, int n) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i >= n) r.v[i] = 0.f;
+    }
+};
+
+// Elements k .. k + 7 of the row at p, which has n; zeros behind its end.  A
+// piece that reaches over the row's end may read what follows (and drop it)
+// where `room`, the elements of the tensor from the row's first on, holds it.
+template <class E>
+__device__ __forceinline__ typename Wide<E>::Raw load8(const typename E::T* p, int k, int n,
+                                                       int64_t room) {
+    using T = typename E::T;
+    typename Wide<E>::Raw r;
+    if (k + 8 <= room) {
+        __builtin_memcpy(&r, p + k, sizeof(r));
+        if (k + 8 > n) Wide<E>::cut(r, n - k);
+    } else {
+        T v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = k + i < n ? p[k + i] : (T)0;
+        __builtin_memcpy(&r, v, sizeof(r));
+    }
+    return r;
+}
+
 }  // namespace gsx

@@ -520,6 +520,393 @@ __global__ __launch_bounds__(kNarrowThreads) void k_narrow_fwd(const Narrow<E> q
     }
 }
 
+// The whole backward pass in one kernel for narrow widths and many rows.  Each
+// wave of a workgroup owns 32 hidden channels and keeps everything of theirs in
+// registers: their rows of Wg and Wu and columns of Wd in both orders, and the
+// running sums of their weight gradients.  The workgroup walks tiles of 32 rows:
+// x and dy are staged once for its waves, g, u and dh are formed again, dx is
+// summed over the waves through shared memory, and dg, du and h pass through a
+// wave's own piece of it to be read along the rows, the summed index of the
+// weight gradients (a transposing read: 16 lanes turn 4 x 16 elements).  One
+// barrier a tile: what the tiles share is there twice.
+//
+// More than 4 x 32 hidden channels run as groups, each with its part of dx;
+// the workgroups' weight gradients and the groups' dx are added up in a fixed
+// order afterwards.
+constexpr int kBwdWaves = 4;
+constexpr int kBwdRows = 32;
+
+template <class E>
+struct NarrowBwd {
+    using T = typename E::T;
+    const T *x, *wg, *wu, *wd, *dy;
+    T* dx;            // one group's result, or NULL
+    float* dx_parts;  // (groups, rows, d_in), or NULL
+    float* parts;     // (workgroups, groups, waves, sums, 64)
+    int64_t ldx, lddy, rows;
+    int d_in, hidden, d_out, act;
+};
+
+// A tile of 32 rows in shared memory, SLOTS 16-byte slots a row, the slots turned
+// by the row so that lanes of consecutive rows meet different banks.
+template <int SLOTS>
+__device__ __forceinline__ int tile_slot(int row, int slot) {
+    constexpr int shift = SLOTS == 4 ? 2 : 0;
+    return row * SLOTS + (slot ^ ((row >> shift) & (SLOTS - 1)));
+}
+
+// The operand whose rows are a tile's columns c0 .. c0 + 15 and whose summed
+// index are the tile's 32 rows.
+template <int SLOTS>
+__device__ __forceinline__ u32x4 read_turned(const u32x4* tile, int c0, int lane) {
+    using v4 = __attribute__((ext_vector_type(4))) short;
+    typedef __attribute__((address_space(3))) v4* lds_v4;
+    const int s = lane & 15, row = 8 * (lane >> 4) + (s >> 2), col = c0 + 4 * (s & 3);
+    union {
+        v4 h[2];
+        u32x4 v;
+    } r;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        char* at = (char*)(tile + tile_slot<SLOTS>(row + 4 * i, col >> 3)) + 8 * ((col >> 2) & 1);
+        r.h[i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4)at);
+    }
+    return r.v;
+}
+
+template <class E, int KD, int KO>
+struct BwdShape {
+    static constexpr int PC = Wide<E>::PIECES;
+    static constexpr int XS = 4 * KD, YS = 4 * KO;      // slots of a row of x, of dy
+    static constexpr int TILE = kBwdRows * (XS + YS) * PC;  // 16-byte slots of a staged tile
+    static constexpr int GATE = kBwdRows * 4 * PC;      // of a wave's turning piece
+    static constexpr int SUM = kBwdRows * 8 * KD;       // of a wave's part of dx
+    static constexpr int SUMS = 32 * KD + 16 * KO;      // weight gradient registers
+    static int64_t lds(int waves) { return 16 * (2 * TILE + (int64_t)waves * (GATE + 2 * SUM)); }
+};
+
+template <class E, int KD, int KO>
+__global__ __launch_bounds__(64 * kBwdWaves, 1) void k_narrow_bwd(const NarrowBwd<E> q) {
+    using T = typename E::T;
+    using W = Wide<E>;
+    using S = BwdShape<E, KD, KO>;
+    using Frag = typename W::Frag;
+    constexpr int PC = S::PC, R = kBwdRows / 16;
+    extern __shared__ u32x4 smem[];
+    const int waves = blockDim.x >> 6, threads = blockDim.x;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int col = lane & 15, quad = lane >> 4, k8 = quad * 8;
+    u32x4* tiles = smem;
+    u32x4* gate = smem + 2 * S::TILE + wave * S::GATE;
+    u32x4* sums = smem + 2 * S::TILE + waves * S::GATE;
+    const int f0 = (blockIdx.y * kBwdWaves + wave) * 32;
+
+    // the wave's weights: operands with rows f (of x and dy), with rows d (of dg, du)
+    Frag wg[2][KD], wu[2][KD], wd[2][KO], wgt[2 * KD], wut[2 * KD];
+    {
+        const int64_t in = (int64_t)q.hidden * q.d_in;
+        auto gather = [&](const T* w, int64_t first, int64_t step, int n) {
+            typename W::Raw raw;
+            T v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = i < n ? w[first + i * step] : (T)0;
+            __builtin_memcpy(&raw, v, sizeof(raw));
+            return W::frag(raw);
+        };
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            const int f = f0 + 8 * (col >> 2) + (col & 3) + 4 * b;
+            const bool there = f < q.hidden;
+#pragma unroll
+            for (int kd = 0; kd < KD; ++kd) {
+                const int k = kd * 32 + k8;
+                typename W::Raw a{}, c{};
+                if (there && k < q.d_in) {
+                    a = load8<E>(q.wg + (int64_t)f * q.d_in, k, q.d_in, in - (int64_t)f * q.d_in);
+                    c = load8<E>(q.wu + (int64_t)f * q.d_in, k, q.d_in, in - (int64_t)f * q.d_in);
+                }
+                wg[b][kd] = W::frag(a);
+                wu[b][kd] = W::frag(c);
+            }
+#pragma unroll
+            for (int ko = 0; ko < KO; ++ko) {
+                const int o = ko * 32 + k8;
+                wd[b][ko] = gather(q.wd, (int64_t)o * q.hidden + f, q.hidden,
+                                   there ? q.d_out - o : 0);
+            }
+        }
+#pragma unroll
+        for (int db = 0; db < 2 * KD; ++db) {
+            const int d = 16 * db + col, f = f0 + k8;
+            const int n = d < q.d_in ? q.hidden - f : 0;
+            wgt[db] = gather(q.wg, (int64_t)f * q.d_in + d, q.d_in, n);
+            wut[db] = gather(q.wu, (int64_t)f * q.d_in + d, q.d_in, n);
+        }
+    }
+
+    // staging: pieces of eight elements of x's and dy's rows
+    constexpr int PIECES = kBwdRows * (S::XS + S::YS);
+    auto fetch = [&](int64_t row0, int n, typename W::Raw& raw) {
+        const bool of_x = n < kBwdRows * S::XS;
+        const int i = of_x ? n : n - kBwdRows * S::XS;
+        const int slots = of_x ? S::XS : S::YS, row = i / slots, k = i % slots * 8;
+        const int width = of_x ? q.d_in : q.d_out;
+        const int64_t ld = of_x ? q.ldx : q.lddy, at = row0 + row;
+        raw = typename W::Raw{};
+        if (at < q.rows && k < width)
+            raw = load8<E>((of_x ? q.x : q.dy) + at * ld, k, width, (q.rows - 1 - at) * ld + width);
+    };
+    auto settle = [&](u32x4* tile, int n, const typename W::Raw& raw) {
+        const bool of_x = n < kBwdRows * S::XS;
+        const int i = of_x ? n : n - kBwdRows * S::XS;
+        const Frag f = W::frag(raw);
+#pragma unroll
+        for (int p = 0; p < PC; ++p) {
+            if (of_x)
+                tile[p * kBwdRows * S::XS + tile_slot<S::XS>(i / S::XS, i % S::XS)] = f.p[p];
+            else
+                tile[PC * kBwdRows * S::XS + p * kBwdRows * S::YS +
+                     tile_slot<S::YS>(i / S::YS, i % S::YS)] = f.p[p];
+        }
+    };
+
+    f32x4 sg[2][2 * KD], su[2][2 * KD], sd[2][2 * KO];  // the weight gradients' sums
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+#pragma unroll
+        for (int d = 0; d < 2 * KD; ++d) sg[b][d] = su[b][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int o = 0; o < 2 * KO; ++o) sd[b][o] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+
+    constexpr int HELD = (PIECES + 255) / 256;  // a thread's pieces of the next tile, four waves
+    const bool ahead = threads == 256;
+    typename W::Raw next[HELD];
+    auto fetch_all = [&](int64_t row0) {
+#pragma unroll
+        for (int i = 0; i < HELD; ++i)
+            if (threadIdx.x + i * 256 < PIECES) fetch(row0, threadIdx.x + i * 256, next[i]);
+    };
+    auto settle_all = [&](u32x4* tile) {
+#pragma unroll
+        for (int i = 0; i < HELD; ++i)
+            if (threadIdx.x + i * 256 < PIECES) settle(tile, threadIdx.x + i * 256, next[i]);
+    };
+    auto stage_all = [&](u32x4* tile, int64_t row0) {  // fewer waves: no registers ahead
+        for (int n = threadIdx.x; n < PIECES; n += threads) {
+            typename W::Raw raw;
+            fetch(row0, n, raw);
+            settle(tile, n, raw);
+        }
+    };
+
+    const int64_t step = (int64_t)gridDim.x * kBwdRows;
+    int64_t row0 = (int64_t)blockIdx.x * kBwdRows;
+    if (ahead) {
+        fetch_all(row0);
+        settle_all(tiles);
+        fetch_all(row0 + step);
+    } else {
+        stage_all(tiles, row0);
+    }
+    __syncthreads();
+    for (int turn = 0; row0 < q.rows; row0 += step, turn ^= 1) {
+        const u32x4* xt = tiles + turn * S::TILE;
+        const u32x4* yt = xt + PC * kBwdRows * S::XS;
+        u32x4* sum = sums + turn * waves * S::SUM;
+        Frag dg[R], du[R], h[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const int row = 16 * r + col;
+            f32x4 g[2], u[2], dh[2];
+#pragma unroll
+            for (int b = 0; b < 2; ++b) g[b] = u[b] = dh[b] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int kd = 0; kd < KD; ++kd) {
+                Frag x;
+#pragma unroll
+                for (int p = 0; p < PC; ++p)
+                    x.p[p] = xt[p * kBwdRows * S::XS + tile_slot<S::XS>(row, kd * 4 + quad)];
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                    g[b] = W::mma(wg[b][kd], x, g[b]);
+                    u[b] = W::mma(wu[b][kd], x, u[b]);
+                }
+            }
+#pragma unroll
+            for (int ko = 0; ko < KO; ++ko) {
+                Frag y;
+#pragma unroll
+                for (int p = 0; p < PC; ++p)
+                    y.p[p] = yt[p * kBwdRows * S::YS + tile_slot<S::YS>(row, ko * 4 + quad)];
+#pragma unroll
+                for (int b = 0; b < 2; ++b) dh[b] = W::mma(wd[b][ko], y, dh[b]);
+            }
+            float vg[8], vu[8], vh[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                float slope;
+                const float a = activate<kExact<E>>(q.act, g[i >> 2][i & 3], slope);
+                const float uu = u[i >> 2][i & 3], d = dh[i >> 2][i & 3];
+                vh[i] = a * uu;
+                vu[i] = d * a;
+                vg[i] = d * uu * slope;
+            }
+            dg[r] = W::frag(vg);
+            du[r] = W::frag(vu);
+            h[r] = W::frag(vh);
+            // this wave's part of dx
+#pragma unroll
+            for (int db = 0; db < 2 * KD; ++db) {
+                f32x4 d{0.f, 0.f, 0.f, 0.f};
+                d = W::mma(wgt[db], dg[r], d);
+                d = W::mma(wut[db], du[r], d);
+                sum[wave * S::SUM + tile_slot<8 * KD>(row, db * 4 + quad)] =
+                    __builtin_bit_cast(u32x4, d);
+            }
+        }
+        // weight gradients: operands along the rows
+        auto turn_piece = [&](const Frag* v, Frag out[2]) {
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+#pragma unroll
+                for (int p = 0; p < PC; ++p)
+                    gate[p * kBwdRows * 4 + tile_slot<4>(16 * r + col, quad)] = v[r].p[p];
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int p = 0; p < PC; ++p)
+                    out[b].p[p] = read_turned<4>(gate + p * kBwdRows * 4, 16 * b, lane);
+        };
+        Frag tg[2], tu[2], th[2];
+        turn_piece(dg, tg);
+        turn_piece(du, tu);
+#pragma unroll
+        for (int db = 0; db < 2 * KD; ++db) {
+            Frag x;
+#pragma unroll
+            for (int p = 0; p < PC; ++p)
+                x.p[p] = read_turned<S::XS>(xt + p * kBwdRows * S::XS, 16 * db, lane);
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                sg[b][db] = W::mma(x, tg[b], sg[b][db]);
+                su[b][db] = W::mma(x, tu[b], su[b][db]);
+            }
+        }
+        turn_piece(h, th);
+#pragma unroll
+        for (int ob = 0; ob < 2 * KO; ++ob) {
+            Frag y;
+#pragma unroll
+            for (int p = 0; p < PC; ++p)
+                y.p[p] = read_turned<S::YS>(yt + p * kBwdRows * S::YS, 16 * ob, lane);
+#pragma unroll
+            for (int b = 0; b < 2; ++b) sd[b][ob] = W::mma(y, th[b], sd[b][ob]);
+        }
+        // the next tile into the other place, then everybody's parts of dx
+        u32x4* other = tiles + (turn ^ 1) * S::TILE;
+        if (ahead) {
+            settle_all(other);
+            fetch_all(row0 + 2 * step);
+        } else {
+            stage_all(other, row0 + step);
+        }
+        __syncthreads();
+        if (q.dx || q.dx_parts)
+            for (int n = threadIdx.x; n < kBwdRows * 8 * KD; n += threads) {
+                const int row = n / (8 * KD), slot = n % (8 * KD), d = 4 * slot;
+                const int64_t at = row0 + row;
+                if (at >= q.rows || d >= q.d_in) continue;
+                f32x4 v{0.f, 0.f, 0.f, 0.f};
+                for (int w = 0; w < waves; ++w)
+                    v += __builtin_bit_cast(f32x4,
+                                            sum[w * S::SUM + tile_slot<8 * KD>(row, slot)]);
+                if (q.dx_parts) {
+                    float* out = q.dx_parts + ((int64_t)blockIdx.y * q.rows + at) * q.d_in + d;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (d + i < q.d_in) out[i] = v[i];
+                } else {
+                    T w[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) w[i] = E::down(v[i]);
+                    T* out = q.dx + at * q.d_in + d;
+                    if (d + 4 <= q.d_in) {
+                        __builtin_memcpy(out, w, sizeof(w));
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (d + i < q.d_in) out[i] = w[i];
+                    }
+                }
+            }
+    }
+    float* out = q.parts +
+                 (((int64_t)blockIdx.x * gridDim.y + blockIdx.y) * kBwdWaves + wave) * S::SUMS * 64 +
+                 lane;
+    int n = 0;
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+#pragma unroll
+        for (int d = 0; d < 2 * KD; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                out[64 * n++] = sg[b][d][i];
+                out[64 * n++] = su[b][d][i];
+            }
+#pragma unroll
+        for (int o = 0; o < 2 * KO; ++o)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) out[64 * n++] = sd[b][o][i];
+    }
+}
+
+// Adds up the workgroups' weight gradients in their order: 64 sums of one wave
+// on the lanes, a quarter of the workgroups on each of four waves.
+template <class E, int KD, int KO>
+__global__ __launch_bounds__(kThreads) void k_narrow_join(const float* parts, int blocks,
+                                                          int groups, int d_in, int hidden,
+                                                          int d_out, typename E::T* dwg,
+                                                          typename E::T* dwu, typename E::T* dwd) {
+    constexpr int SUMS = 32 * KD + 16 * KO, HALF = SUMS / 2;
+    __shared__ float red[kThreads];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int unit = blockIdx.x;  // (group, wave, sum)
+    const int n = unit % SUMS, chunk = unit / SUMS;
+    const int64_t pitch = (int64_t)groups * kBwdWaves * SUMS * 64;
+    const float* p = parts + (int64_t)unit * 64 + lane;
+    const int per = (blocks + 3) / 4, b0 = wave * per, b1 = b0 + per < blocks ? b0 + per : blocks;
+    float s = 0.f;
+    int b = b0;
+    for (; b + 8 <= b1; b += 8) {
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = p[(b + i) * pitch];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s += v[i];
+    }
+    for (; b < b1; ++b) s += p[b * pitch];
+    red[threadIdx.x] = s;
+    __syncthreads();
+    if (wave) return;
+    s = red[lane] + red[lane + 64] + red[lane + 128] + red[lane + 192];
+    const int half = n / HALF, in = n % HALF;  // as the kernel above lays them down
+    const int f = chunk * 32 + 16 * half + (lane & 15), quad = lane >> 4;
+    if (f >= hidden) return;
+    if (in < 16 * KD) {
+        const int d = 16 * (in / 8) + 4 * quad + in % 8 / 2;
+        typename E::T* out = in & 1 ? dwu : dwg;
+        if (d < d_in && out) out[(int64_t)f * d_in + d] = E::down(s);
+    } else {
+        const int o = 16 * ((in - 16 * KD) / 4) + 4 * quad + in % 4;
+        if (o < d_out && dwd) dwd[(int64_t)o * hidden + f] = E::down(s);
+    }
+}
+
 // ----------------------------------------------------------------- host --
 
 struct Shape {
@@ -666,7 +1053,100 @@ int64_t parts_bytes(const Shape& s) {
     return up_to((in > out ? in : out) * 4, 256);
 }
 
-int64_t bwd_bytes(const Shape& s) { return s.rows == 0 ? 0 : 3 * hidden_bytes(s) + parts_bytes(s); }
+// The narrow backward: which widths fit its registers (weights in both orders
+// and their gradients' sums), its workgroups and its workspace.
+constexpr int bwd_registers(int pieces, int kd, int ko) {
+    return pieces * (32 * kd + 8 * ko) + 32 * kd + 16 * ko;
+}
+constexpr bool narrow_bwd_fits(int pieces, int kd, int ko) {
+    return bwd_registers(pieces, kd, ko) <= (pieces == 3 ? 250 : 340);
+}
+int narrow_ko(const Shape& s) { return s.d_out <= 32 ? 1 : s.d_out <= 64 ? 2 : 4; }
+bool narrow_bwd(const Shape& s) {
+    return s.d_in <= 128 && s.d_out <= 128 && s.hidden <= 512 &&
+           narrow_bwd_fits(s.dtype == GSX_F32 ? 3 : 1, narrow_kd(s), narrow_ko(s));
+}
+struct BwdPlan {
+    int waves, groups, blocks;
+    int64_t parts, dx_parts, bytes;
+};
+BwdPlan bwd_plan(const Shape& s) {
+    BwdPlan p{};
+    const int kd = narrow_kd(s), ko = narrow_ko(s), chunks = (s.hidden + 31) / 32;
+    p.groups = (chunks + kBwdWaves - 1) / kBwdWaves;
+    p.waves = chunks < kBwdWaves ? chunks : kBwdWaves;
+    const int64_t tiles = (s.rows + kBwdRows - 1) / kBwdRows;
+    int64_t want = 512 / (p.groups * p.waves) * 2;
+    if (want > tiles) want = tiles;
+    p.blocks = (int)(want < 1 ? 1 : want);
+    p.parts = up_to((int64_t)p.blocks * p.groups * kBwdWaves * (32 * kd + 16 * ko) * 256, 256);
+    p.dx_parts = p.groups > 1 ? up_to(p.groups * s.rows * s.d_in * 4, 256) : 0;
+    p.bytes = p.parts + p.dx_parts;
+    return p;
+}
+
+int64_t bwd_bytes(const Shape& s) {
+    if (s.rows == 0) return 0;
+    return narrow_bwd(s) ? bwd_plan(s).bytes : 3 * hidden_bytes(s) + parts_bytes(s);
+}
+
+struct BwdArgs {
+    const void* x;
+    int64_t ldx;
+    const void *wg, *wu, *wd, *dy;
+    int64_t lddy;
+    void *dx, *dwg, *dwu, *dwd, *ws;
+    hipStream_t st;
+};
+
+template <class E, int KD, int KO>
+int launch_narrow_bwd(const Shape& s, const BwdArgs& a) {
+    if constexpr (!narrow_bwd_fits(Wide<E>::PIECES, KD, KO)) {
+        return GSX_ERR_INVALID;  // narrow_bwd() keeps these out
+    } else {
+        using T = typename E::T;
+        using S = BwdShape<E, KD, KO>;
+        const BwdPlan p = bwd_plan(s);
+        float* parts = (float*)a.ws;
+        float* dx_parts = p.groups > 1 ? (float*)((char*)a.ws + p.parts) : nullptr;
+        if (!a.dx) dx_parts = nullptr;
+        const NarrowBwd<E> q{(const T*)a.x, (const T*)a.wg, (const T*)a.wu, (const T*)a.wd,
+                             (const T*)a.dy, p.groups > 1 ? nullptr : (T*)a.dx, dx_parts, parts,
+                             a.ldx, a.lddy, s.rows, s.d_in, s.hidden, s.d_out, s.act};
+        const int64_t lds = S::lds(p.waves);
+        if (hipFuncSetAttribute((const void*)&k_narrow_bwd<E, KD, KO>,
+                                hipFuncAttributeMaxDynamicSharedMemorySize,
+                                160 * 1024) != hipSuccess)
+            return GSX_ERR_HIP;
+        hipLaunchKernelGGL((k_narrow_bwd<E, KD, KO>), dim3(p.blocks, p.groups), dim3(64 * p.waves),
+                           (unsigned)lds, a.st, q);
+        GSX_LAUNCH_CHECK();
+        if (a.dwg || a.dwd) {
+            const int chunks = p.groups * kBwdWaves;
+            hipLaunchKernelGGL((k_narrow_join<E, KD, KO>), dim3(chunks * S::SUMS), dim3(kThreads),
+                               0, a.st, parts, p.blocks, p.groups, s.d_in, s.hidden, s.d_out,
+                               (T*)a.dwg, (T*)a.dwu, (T*)a.dwd);
+            GSX_LAUNCH_CHECK();
+        }
+        if (dx_parts) {
+            const int64_t n = s.rows * s.d_in;
+            const int64_t blocks = (n + kThreads - 1) / kThreads;
+            if (blocks >= (1LL << 31)) return GSX_ERR_TOO_LARGE;
+            hipLaunchKernelGGL((k_join<E>), dim3((unsigned)blocks), dim3(kThreads), 0, a.st,
+                               dx_parts, n, p.groups, (T*)a.dx);
+            GSX_LAUNCH_CHECK();
+        }
+        return GSX_OK;
+    }
+}
+template <class E, int KD>
+int launch_narrow_bwd(const Shape& s, const BwdArgs& a) {
+    switch (narrow_ko(s)) {
+        case 1: return launch_narrow_bwd<E, KD, 1>(s, a);
+        case 2: return launch_narrow_bwd<E, KD, 2>(s, a);
+        default: return launch_narrow_bwd<E, KD, 4>(s, a);
+    }
+}
 
 template <class E>
 int forward(const Shape& s, const void* x, int64_t ldx, const void* wg, const void* wu,
@@ -732,6 +1212,14 @@ template <class E>
 int backward(const Shape& s, const void* x, int64_t ldx, const void* wg, const void* wu,
              const void* wd, const void* dy, int64_t lddy, void* dx, void* dwg, void* dwu,
              void* dwd, void* ws, hipStream_t st) {
+    if (narrow_bwd(s)) {
+        const BwdArgs a{x, ldx, wg, wu, wd, dy, lddy, dx, dwg, dwu, dwd, ws, st};
+        switch (narrow_kd(s)) {
+            case 1: return launch_narrow_bwd<E, 1>(s, a);
+            case 2: return launch_narrow_bwd<E, 2>(s, a);
+            default: return launch_narrow_bwd<E, 4>(s, a);
+        }
+    }
     const int64_t ph = pitch(s), hb = hidden_bytes(s);
     void* dg = ws;
     void* du = (char*)ws + hb;

@@ -63,8 +63,9 @@ __device__ __forceinline__ float activate(int act, float g, float& slope) {
         slope = s * (1.0f - s);
         return g != g ? g : s;
     }
-    slope = s * (1.0f + g * (1.0f - s));
-    return g * s;
+    const float a = g * s;
+    slope = fmaf(a, 1.0f - s, s);
+    return a;
 }
 
 template <class E>
@@ -520,20 +521,20 @@ __global__ __launch_bounds__(kNarrowThreads) void k_narrow_fwd(const Narrow<E> q
     }
 }
 
-// The whole backward pass in one kernel for narrow widths and many rows.  Each
-// wave of a workgroup owns 32 hidden channels and keeps everything of theirs in
-// registers: their rows of Wg and Wu and columns of Wd in both orders, and the
-// running sums of their weight gradients.  The workgroup walks tiles of 32 rows:
-// x and dy are staged once for its waves, g, u and dh are formed again, dx is
-// summed over the waves through shared memory, and dg, du and h pass through a
-// wave's own piece of it to be read along the rows, the summed index of the
-// weight gradients (a transposing read: 16 lanes turn 4 x 16 elements).  One
-// barrier a tile: what the tiles share is there twice.
+// The whole backward pass in one kernel for narrow widths and many rows.  A pair
+// of waves owns 32 hidden channels, 16 each: their rows of Wg and Wu, their
+// columns of Wd and the running sums of their weight gradients stay in its
+// registers while the workgroup walks tiles of 32 rows.  x and dy are staged
+// once for all pairs, g, u and dh are formed again, and dg, du and h go through
+// shared memory once: read as they lie they are dx's operand (the pair shares
+// dx's channels), read along the rows (a transposing read: 16 lanes turn 4 x 16
+// elements) the weight gradients'.  The pairs' parts of dx are added up there
+// too.  Two barriers a tile; the next tile's loads are in flight meanwhile.
 //
 // More than 4 x 32 hidden channels run as groups, each with its part of dx;
 // the workgroups' weight gradients and the groups' dx are added up in a fixed
 // order afterwards.
-constexpr int kBwdWaves = 4;
+constexpr int kBwdPairs = 4;
 constexpr int kBwdRows = 32;
 
 template <class E>
@@ -542,7 +543,7 @@ struct NarrowBwd {
     const T *x, *wg, *wu, *wd, *dy;
     T* dx;            // one group's result, or NULL
     float* dx_parts;  // (groups, rows, d_in), or NULL
-    float* parts;     // (workgroups, groups, waves, sums, 64)
+    float* parts;     // (workgroups, groups, pairs, halves, sums, 64)
     int64_t ldx, lddy, rows;
     int d_in, hidden, d_out, act;
 };
@@ -577,32 +578,41 @@ __device__ __forceinline__ u32x4 read_turned(const u32x4* tile, int c0, int lane
 template <class E, int KD, int KO>
 struct BwdShape {
     static constexpr int PC = Wide<E>::PIECES;
-    static constexpr int XS = 4 * KD, YS = 4 * KO;      // slots of a row of x, of dy
+    static constexpr int XS = 4 * KD, YS = 4 * KO;          // slots of a row of x, of dy
     static constexpr int TILE = kBwdRows * (XS + YS) * PC;  // 16-byte slots of a staged tile
-    static constexpr int GATE = kBwdRows * 4 * PC;      // of a wave's turning piece
-    static constexpr int SUM = kBwdRows * 8 * KD;       // of a wave's part of dx
-    static constexpr int SUMS = 32 * KD + 16 * KO;      // weight gradient registers
-    static int64_t lds(int waves) { return 16 * (2 * TILE + (int64_t)waves * (GATE + 2 * SUM)); }
+    static constexpr int GATE = kBwdRows * 4 * PC;          // of a pair's dg, du or h
+    static constexpr int SUM = kBwdRows * 8 * KD;           // of a pair's part of dx
+    static constexpr int SUMS = 16 * KD + 8 * KO;           // weight gradient registers
+    static int64_t lds(int pairs) { return 16 * (2 * TILE + (int64_t)pairs * (3 * GATE + SUM)); }
 };
 
+// Waves for a SIMD that the registers leave room for.
 template <class E, int KD, int KO>
-__global__ __launch_bounds__(64 * kBwdWaves, 1) void k_narrow_bwd(const NarrowBwd<E> q) {
+constexpr int bwd_waves() {
+    return sizeof(typename E::T) == 4 || KD + KO > 4 ? 2 : KD == 2 ? 3 : 4;
+}
+
+template <class E, int KD, int KO>
+__global__ __launch_bounds__(128 * kBwdPairs, (bwd_waves<E, KD, KO>()))
+void k_narrow_bwd(const NarrowBwd<E> q) {
     using T = typename E::T;
     using W = Wide<E>;
     using S = BwdShape<E, KD, KO>;
     using Frag = typename W::Frag;
     constexpr int PC = S::PC, R = kBwdRows / 16;
     extern __shared__ u32x4 smem[];
-    const int waves = blockDim.x >> 6, threads = blockDim.x;
+    const int threads = blockDim.x, pairs = threads >> 7;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int pair = wave >> 1, half = wave & 1;
     const int col = lane & 15, quad = lane >> 4, k8 = quad * 8;
     u32x4* tiles = smem;
-    u32x4* gate = smem + 2 * S::TILE + wave * S::GATE;
-    u32x4* sums = smem + 2 * S::TILE + waves * S::GATE;
-    const int f0 = (blockIdx.y * kBwdWaves + wave) * 32;
+    u32x4* gates = smem + 2 * S::TILE + pair * 3 * S::GATE;
+    u32x4* sums = smem + 2 * S::TILE + pairs * 3 * S::GATE;
+    const int f0 = (blockIdx.y * kBwdPairs + pair) * 32;
 
-    // the wave's weights: operands with rows f (of x and dy), with rows d (of dg, du)
-    Frag wg[2][KD], wu[2][KD], wd[2][KO], wgt[2 * KD], wut[2 * KD];
+    // the wave's weights: its 16 channels' rows (operands of x and of dy), and the
+    // pair's 32 channels for every other 16 of dx's
+    Frag wg[KD], wu[KD], wd[KO], wgt[KD], wut[KD];
     {
         const int64_t in = (int64_t)q.hidden * q.d_in;
         auto gather = [&](const T* w, int64_t first, int64_t step, int n) {
@@ -613,39 +623,37 @@ __global__ __launch_bounds__(64 * kBwdWaves, 1) void k_narrow_bwd(const NarrowBw
             __builtin_memcpy(&raw, v, sizeof(raw));
             return W::frag(raw);
         };
+        const int f = f0 + 16 * half + col;
+        const bool there = f < q.hidden;
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
-            const int f = f0 + 8 * (col >> 2) + (col & 3) + 4 * b;
-            const bool there = f < q.hidden;
-#pragma unroll
-            for (int kd = 0; kd < KD; ++kd) {
-                const int k = kd * 32 + k8;
-                typename W::Raw a{}, c{};
-                if (there && k < q.d_in) {
-                    a = load8<E>(q.wg + (int64_t)f * q.d_in, k, q.d_in, in - (int64_t)f * q.d_in);
-                    c = load8<E>(q.wu + (int64_t)f * q.d_in, k, q.d_in, in - (int64_t)f * q.d_in);
-                }
-                wg[b][kd] = W::frag(a);
-                wu[b][kd] = W::frag(c);
+        for (int kd = 0; kd < KD; ++kd) {
+            const int k = kd * 32 + k8;
+            typename W::Raw a{}, c{};
+            if (there && k < q.d_in) {
+                a = load8<E>(q.wg + (int64_t)f * q.d_in, k, q.d_in, in - (int64_t)f * q.d_in);
+                c = load8<E>(q.wu + (int64_t)f * q.d_in, k, q.d_in, in - (int64_t)f * q.d_in);
             }
-#pragma unroll
-            for (int ko = 0; ko < KO; ++ko) {
-                const int o = ko * 32 + k8;
-                wd[b][ko] = gather(q.wd, (int64_t)o * q.hidden + f, q.hidden,
-                                   there ? q.d_out - o : 0);
-            }
+            wg[kd] = W::frag(a);
+            wu[kd] = W::frag(c);
         }
 #pragma unroll
-        for (int db = 0; db < 2 * KD; ++db) {
-            const int d = 16 * db + col, f = f0 + k8;
-            const int n = d < q.d_in ? q.hidden - f : 0;
-            wgt[db] = gather(q.wg, (int64_t)f * q.d_in + d, q.d_in, n);
-            wut[db] = gather(q.wu, (int64_t)f * q.d_in + d, q.d_in, n);
+        for (int ko = 0; ko < KO; ++ko) {
+            const int o = ko * 32 + k8;
+            wd[ko] = gather(q.wd, (int64_t)o * q.hidden + f, q.hidden, there ? q.d_out - o : 0);
+        }
+#pragma unroll
+        for (int j = 0; j < KD; ++j) {
+            const int d = 16 * (2 * j + half) + col, f8 = f0 + k8;
+            const int n = d < q.d_in ? q.hidden - f8 : 0;
+            wgt[j] = gather(q.wg, (int64_t)f8 * q.d_in + d, q.d_in, n);
+            wut[j] = gather(q.wu, (int64_t)f8 * q.d_in + d, q.d_in, n);
         }
     }
 
-    // staging: pieces of eight elements of x's and dy's rows
+    // staging: pieces of eight elements of x's and dy's rows, HELD of them in a
+    // thread's registers one tile ahead
     constexpr int PIECES = kBwdRows * (S::XS + S::YS);
+    constexpr int HELD = (PIECES + 128 * kBwdPairs - 1) / (128 * kBwdPairs);
     auto fetch = [&](int64_t row0, int n, typename W::Raw& raw) {
         const bool of_x = n < kBwdRows * S::XS;
         const int i = of_x ? n : n - kBwdRows * S::XS;
@@ -669,69 +677,54 @@ __global__ __launch_bounds__(64 * kBwdWaves, 1) void k_narrow_bwd(const NarrowBw
                      tile_slot<S::YS>(i / S::YS, i % S::YS)] = f.p[p];
         }
     };
-
-    f32x4 sg[2][2 * KD], su[2][2 * KD], sd[2][2 * KO];  // the weight gradients' sums
-#pragma unroll
-    for (int b = 0; b < 2; ++b) {
-#pragma unroll
-        for (int d = 0; d < 2 * KD; ++d) sg[b][d] = su[b][d] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int o = 0; o < 2 * KO; ++o) sd[b][o] = f32x4{0.f, 0.f, 0.f, 0.f};
-    }
-
-    constexpr int HELD = (PIECES + 255) / 256;  // a thread's pieces of the next tile, four waves
-    const bool ahead = threads == 256;
     typename W::Raw next[HELD];
     auto fetch_all = [&](int64_t row0) {
 #pragma unroll
-        for (int i = 0; i < HELD; ++i)
-            if (threadIdx.x + i * 256 < PIECES) fetch(row0, threadIdx.x + i * 256, next[i]);
+        for (int i = 0; i < HELD; ++i) {
+            const int n = threadIdx.x + i * threads;
+            if (n < PIECES) fetch(row0, n, next[i]);
+        }
     };
-    auto settle_all = [&](u32x4* tile) {
+    auto settle_all = [&](u32x4* tile, int64_t row0) {
 #pragma unroll
-        for (int i = 0; i < HELD; ++i)
-            if (threadIdx.x + i * 256 < PIECES) settle(tile, threadIdx.x + i * 256, next[i]);
-    };
-    auto stage_all = [&](u32x4* tile, int64_t row0) {  // fewer waves: no registers ahead
-        for (int n = threadIdx.x; n < PIECES; n += threads) {
+        for (int i = 0; i < HELD; ++i) {
+            const int n = threadIdx.x + i * threads;
+            if (n < PIECES) settle(tile, n, next[i]);
+        }
+        for (int n = threadIdx.x + HELD * threads; n < PIECES; n += threads) {  // fewer pairs
             typename W::Raw raw;
             fetch(row0, n, raw);
             settle(tile, n, raw);
         }
     };
 
+    f32x4 sg[2 * KD], su[2 * KD], sd[2 * KO];  // the weight gradients' sums
+#pragma unroll
+    for (int d = 0; d < 2 * KD; ++d) sg[d] = su[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int o = 0; o < 2 * KO; ++o) sd[o] = f32x4{0.f, 0.f, 0.f, 0.f};
+
     const int64_t step = (int64_t)gridDim.x * kBwdRows;
     int64_t row0 = (int64_t)blockIdx.x * kBwdRows;
-    if (ahead) {
-        fetch_all(row0);
-        settle_all(tiles);
-        fetch_all(row0 + step);
-    } else {
-        stage_all(tiles, row0);
-    }
+    fetch_all(row0);
+    settle_all(tiles, row0);
+    fetch_all(row0 + step);
     __syncthreads();
     for (int turn = 0; row0 < q.rows; row0 += step, turn ^= 1) {
         const u32x4* xt = tiles + turn * S::TILE;
         const u32x4* yt = xt + PC * kBwdRows * S::XS;
-        u32x4* sum = sums + turn * waves * S::SUM;
-        Frag dg[R], du[R], h[R];
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             const int row = 16 * r + col;
-            f32x4 g[2], u[2], dh[2];
-#pragma unroll
-            for (int b = 0; b < 2; ++b) g[b] = u[b] = dh[b] = f32x4{0.f, 0.f, 0.f, 0.f};
+            f32x4 g{0.f, 0.f, 0.f, 0.f}, u = g, dh = g;
 #pragma unroll
             for (int kd = 0; kd < KD; ++kd) {
                 Frag x;
 #pragma unroll
                 for (int p = 0; p < PC; ++p)
                     x.p[p] = xt[p * kBwdRows * S::XS + tile_slot<S::XS>(row, kd * 4 + quad)];
-#pragma unroll
-                for (int b = 0; b < 2; ++b) {
-                    g[b] = W::mma(wg[b][kd], x, g[b]);
-                    u[b] = W::mma(wu[b][kd], x, u[b]);
-                }
+                g = W::mma(wg[kd], x, g);
+                u = W::mma(wu[kd], x, u);
             }
 #pragma unroll
             for (int ko = 0; ko < KO; ++ko) {
@@ -739,82 +732,74 @@ __global__ __launch_bounds__(64 * kBwdWaves, 1) void k_narrow_bwd(const NarrowBw
 #pragma unroll
                 for (int p = 0; p < PC; ++p)
                     y.p[p] = yt[p * kBwdRows * S::YS + tile_slot<S::YS>(row, ko * 4 + quad)];
-#pragma unroll
-                for (int b = 0; b < 2; ++b) dh[b] = W::mma(wd[b][ko], y, dh[b]);
+                dh = W::mma(wd[ko], y, dh);
             }
-            float vg[8], vu[8], vh[8];
+            float v[3][4];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
+            for (int i = 0; i < 4; ++i) {
                 float slope;
-                const float a = activate<kExact<E>>(q.act, g[i >> 2][i & 3], slope);
-                const float uu = u[i >> 2][i & 3], d = dh[i >> 2][i & 3];
-                vh[i] = a * uu;
-                vu[i] = d * a;
-                vg[i] = d * uu * slope;
+                const float a = activate<kExact<E>>(q.act, g[i], slope);
+                v[0][i] = dh[i] * u[i] * slope;
+                v[1][i] = dh[i] * a;
+                v[2][i] = a * u[i];
             }
-            dg[r] = W::frag(vg);
-            du[r] = W::frag(vu);
-            h[r] = W::frag(vh);
-            // this wave's part of dx
 #pragma unroll
-            for (int db = 0; db < 2 * KD; ++db) {
+            for (int j = 0; j < 3; ++j) {
+                uint2 w[PC];
+                W::four(v[j], w);
+#pragma unroll
+                for (int p = 0; p < PC; ++p)
+                    ((uint2*)(gates + j * S::GATE + p * kBwdRows * 4 +
+                              tile_slot<4>(row, 2 * half + (quad >> 1))))[quad & 1] = w[p];
+            }
+        }
+        __syncthreads();
+        // the pair's part of dx, every other 16 of its channels
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const int row = 16 * r + col;
+            Frag dg, du;
+#pragma unroll
+            for (int p = 0; p < PC; ++p) {
+                dg.p[p] = gates[p * kBwdRows * 4 + tile_slot<4>(row, quad)];
+                du.p[p] = gates[S::GATE + p * kBwdRows * 4 + tile_slot<4>(row, quad)];
+            }
+#pragma unroll
+            for (int j = 0; j < KD; ++j) {
                 f32x4 d{0.f, 0.f, 0.f, 0.f};
-                d = W::mma(wgt[db], dg[r], d);
-                d = W::mma(wut[db], du[r], d);
-                sum[wave * S::SUM + tile_slot<8 * KD>(row, db * 4 + quad)] =
+                d = W::mma(wgt[j], dg, d);
+                d = W::mma(wut[j], du, d);
+                sums[pair * S::SUM + tile_slot<8 * KD>(row, (2 * j + half) * 4 + quad)] =
                     __builtin_bit_cast(u32x4, d);
             }
         }
         // weight gradients: operands along the rows
-        auto turn_piece = [&](const Frag* v, Frag out[2]) {
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
+        Frag t[3];
 #pragma unroll
-            for (int r = 0; r < R; ++r)
+        for (int j = 0; j < 3; ++j)
 #pragma unroll
-                for (int p = 0; p < PC; ++p)
-                    gate[p * kBwdRows * 4 + tile_slot<4>(16 * r + col, quad)] = v[r].p[p];
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
-#pragma unroll
-            for (int b = 0; b < 2; ++b)
-#pragma unroll
-                for (int p = 0; p < PC; ++p)
-                    out[b].p[p] = read_turned<4>(gate + p * kBwdRows * 4, 16 * b, lane);
-        };
-        Frag tg[2], tu[2], th[2];
-        turn_piece(dg, tg);
-        turn_piece(du, tu);
+            for (int p = 0; p < PC; ++p)
+                t[j].p[p] = read_turned<4>(gates + j * S::GATE + p * kBwdRows * 4, 16 * half, lane);
 #pragma unroll
         for (int db = 0; db < 2 * KD; ++db) {
             Frag x;
 #pragma unroll
             for (int p = 0; p < PC; ++p)
                 x.p[p] = read_turned<S::XS>(xt + p * kBwdRows * S::XS, 16 * db, lane);
-#pragma unroll
-            for (int b = 0; b < 2; ++b) {
-                sg[b][db] = W::mma(x, tg[b], sg[b][db]);
-                su[b][db] = W::mma(x, tu[b], su[b][db]);
-            }
+            sg[db] = W::mma(x, t[0], sg[db]);
+            su[db] = W::mma(x, t[1], su[db]);
         }
-        turn_piece(h, th);
 #pragma unroll
         for (int ob = 0; ob < 2 * KO; ++ob) {
             Frag y;
 #pragma unroll
             for (int p = 0; p < PC; ++p)
                 y.p[p] = read_turned<S::YS>(yt + p * kBwdRows * S::YS, 16 * ob, lane);
-#pragma unroll
-            for (int b = 0; b < 2; ++b) sd[b][ob] = W::mma(y, th[b], sd[b][ob]);
+            sd[ob] = W::mma(y, t[2], sd[ob]);
         }
-        // the next tile into the other place, then everybody's parts of dx
-        u32x4* other = tiles + (turn ^ 1) * S::TILE;
-        if (ahead) {
-            settle_all(other);
-            fetch_all(row0 + 2 * step);
-        } else {
-            stage_all(other, row0 + step);
-        }
+        // the next tile into the other place, then the pairs' parts of dx
+        settle_all(tiles + (turn ^ 1) * S::TILE, row0 + step);
+        fetch_all(row0 + 2 * step);
         __syncthreads();
         if (q.dx || q.dx_parts)
             for (int n = threadIdx.x; n < kBwdRows * 8 * KD; n += threads) {
@@ -822,9 +807,9 @@ __global__ __launch_bounds__(64 * kBwdWaves, 1) void k_narrow_bwd(const NarrowBw
                 const int64_t at = row0 + row;
                 if (at >= q.rows || d >= q.d_in) continue;
                 f32x4 v{0.f, 0.f, 0.f, 0.f};
-                for (int w = 0; w < waves; ++w)
+                for (int w = 0; w < pairs; ++w)
                     v += __builtin_bit_cast(f32x4,
-                                            sum[w * S::SUM + tile_slot<8 * KD>(row, slot)]);
+                                            sums[w * S::SUM + tile_slot<8 * KD>(row, slot)]);
                 if (q.dx_parts) {
                     float* out = q.dx_parts + ((int64_t)blockIdx.y * q.rows + at) * q.d_in + d;
 #pragma unroll
@@ -846,23 +831,20 @@ __global__ __launch_bounds__(64 * kBwdWaves, 1) void k_narrow_bwd(const NarrowBw
             }
     }
     float* out = q.parts +
-                 (((int64_t)blockIdx.x * gridDim.y + blockIdx.y) * kBwdWaves + wave) * S::SUMS * 64 +
-                 lane;
+                 (((int64_t)blockIdx.x * gridDim.y + blockIdx.y) * 2 * kBwdPairs + wave) * S::SUMS *
+                     64 + lane;
     int n = 0;
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
+    for (int d = 0; d < 2 * KD; ++d)
 #pragma unroll
-        for (int d = 0; d < 2 * KD; ++d)
+        for (int i = 0; i < 4; ++i) {
+            out[64 * n++] = sg[d][i];
+            out[64 * n++] = su[d][i];
+        }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                out[64 * n++] = sg[b][d][i];
-                out[64 * n++] = su[b][d][i];
-            }
+    for (int o = 0; o < 2 * KO; ++o)
 #pragma unroll
-        for (int o = 0; o < 2 * KO; ++o)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) out[64 * n++] = sd[b][o][i];
-    }
+        for (int i = 0; i < 4; ++i) out[64 * n++] = sd[o][i];
 }
 
 // Adds up the workgroups' weight gradients in their order: 64 sums of one wave
@@ -872,12 +854,12 @@ __global__ __launch_bounds__(kThreads) void k_narrow_join(const float* parts, in
                                                           int groups, int d_in, int hidden,
                                                           int d_out, typename E::T* dwg,
                                                           typename E::T* dwu, typename E::T* dwd) {
-    constexpr int SUMS = 32 * KD + 16 * KO, HALF = SUMS / 2;
+    constexpr int SUMS = 16 * KD + 8 * KO;
     __shared__ float red[kThreads];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int unit = blockIdx.x;  // (group, wave, sum)
-    const int n = unit % SUMS, chunk = unit / SUMS;
-    const int64_t pitch = (int64_t)groups * kBwdWaves * SUMS * 64;
+    const int unit = blockIdx.x;  // (group, pair, half, sum)
+    const int in = unit % SUMS, chunk = unit / SUMS;
+    const int64_t pitch = (int64_t)groups * 2 * kBwdPairs * SUMS * 64;
     const float* p = parts + (int64_t)unit * 64 + lane;
     const int per = (blocks + 3) / 4, b0 = wave * per, b1 = b0 + per < blocks ? b0 + per : blocks;
     float s = 0.f;
@@ -894,8 +876,7 @@ __global__ __launch_bounds__(kThreads) void k_narrow_join(const float* parts, in
     __syncthreads();
     if (wave) return;
     s = red[lane] + red[lane + 64] + red[lane + 128] + red[lane + 192];
-    const int half = n / HALF, in = n % HALF;  // as the kernel above lays them down
-    const int f = chunk * 32 + 16 * half + (lane & 15), quad = lane >> 4;
+    const int f = chunk * 16 + (lane & 15), quad = lane >> 4;
     if (f >= hidden) return;
     if (in < 16 * KD) {
         const int d = 16 * (in / 8) + 4 * quad + in % 8 / 2;
@@ -1055,11 +1036,8 @@ int64_t parts_bytes(const Shape& s) {
 
 // The narrow backward: which widths fit its registers (weights in both orders
 // and their gradients' sums), its workgroups and its workspace.
-constexpr int bwd_registers(int pieces, int kd, int ko) {
-    return pieces * (32 * kd + 8 * ko) + 32 * kd + 16 * ko;
-}
 constexpr bool narrow_bwd_fits(int pieces, int kd, int ko) {
-    return bwd_registers(pieces, kd, ko) <= (pieces == 3 ? 250 : 340);
+    return pieces == 3 ? kd + ko <= 3 : kd < 4 || ko == 1;
 }
 int narrow_ko(const Shape& s) { return s.d_out <= 32 ? 1 : s.d_out <= 64 ? 2 : 4; }
 bool narrow_bwd(const Shape& s) {
@@ -1067,19 +1045,20 @@ bool narrow_bwd(const Shape& s) {
            narrow_bwd_fits(s.dtype == GSX_F32 ? 3 : 1, narrow_kd(s), narrow_ko(s));
 }
 struct BwdPlan {
-    int waves, groups, blocks;
+    int pairs, groups, blocks;
     int64_t parts, dx_parts, bytes;
 };
 BwdPlan bwd_plan(const Shape& s) {
     BwdPlan p{};
     const int kd = narrow_kd(s), ko = narrow_ko(s), chunks = (s.hidden + 31) / 32;
-    p.groups = (chunks + kBwdWaves - 1) / kBwdWaves;
-    p.waves = chunks < kBwdWaves ? chunks : kBwdWaves;
+    p.groups = (chunks + kBwdPairs - 1) / kBwdPairs;
+    p.pairs = chunks < kBwdPairs ? chunks : kBwdPairs;
     const int64_t tiles = (s.rows + kBwdRows - 1) / kBwdRows;
-    int64_t want = 512 / (p.groups * p.waves) * 2;
+    const int per_unit = (s.dtype == GSX_F32 ? 1 : 2) * kBwdPairs / p.pairs;
+    int64_t want = 256 * per_unit / p.groups;
     if (want > tiles) want = tiles;
     p.blocks = (int)(want < 1 ? 1 : want);
-    p.parts = up_to((int64_t)p.blocks * p.groups * kBwdWaves * (32 * kd + 16 * ko) * 256, 256);
+    p.parts = up_to((int64_t)p.blocks * p.groups * 2 * kBwdPairs * (16 * kd + 8 * ko) * 256, 256);
     p.dx_parts = p.groups > 1 ? up_to(p.groups * s.rows * s.d_in * 4, 256) : 0;
     p.bytes = p.parts + p.dx_parts;
     return p;
@@ -1113,17 +1092,17 @@ int launch_narrow_bwd(const Shape& s, const BwdArgs& a) {
         const NarrowBwd<E> q{(const T*)a.x, (const T*)a.wg, (const T*)a.wu, (const T*)a.wd,
                              (const T*)a.dy, p.groups > 1 ? nullptr : (T*)a.dx, dx_parts, parts,
                              a.ldx, a.lddy, s.rows, s.d_in, s.hidden, s.d_out, s.act};
-        const int64_t lds = S::lds(p.waves);
+        const int64_t lds = S::lds(p.pairs);
         if (hipFuncSetAttribute((const void*)&k_narrow_bwd<E, KD, KO>,
                                 hipFuncAttributeMaxDynamicSharedMemorySize,
                                 160 * 1024) != hipSuccess)
             return GSX_ERR_HIP;
-        hipLaunchKernelGGL((k_narrow_bwd<E, KD, KO>), dim3(p.blocks, p.groups), dim3(64 * p.waves),
+        hipLaunchKernelGGL((k_narrow_bwd<E, KD, KO>), dim3(p.blocks, p.groups), dim3(128 * p.pairs),
                            (unsigned)lds, a.st, q);
         GSX_LAUNCH_CHECK();
         if (a.dwg || a.dwd) {
-            const int chunks = p.groups * kBwdWaves;
-            hipLaunchKernelGGL((k_narrow_join<E, KD, KO>), dim3(chunks * S::SUMS), dim3(kThreads),
+            const int halves = p.groups * 2 * kBwdPairs;
+            hipLaunchKernelGGL((k_narrow_join<E, KD, KO>), dim3(halves * S::SUMS), dim3(kThreads),
                                0, a.st, parts, p.blocks, p.groups, s.d_in, s.hidden, s.d_out,
                                (T*)a.dwg, (T*)a.dwu, (T*)a.dwd);
             GSX_LAUNCH_CHECK();

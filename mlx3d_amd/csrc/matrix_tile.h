@@ -92,20 +92,24 @@ struct F16 {
 struct Split3 {
     u32x4 p[3];
 };
+__device__ __forceinline__ void split_pair(float a, float b, uint32_t* p0, uint32_t* p1,
+                                           uint32_t* p2) {
+    *p0 = BF16::pair(a, b);
+    a -= __uint_as_float(*p0 << 16);
+    b -= __uint_as_float(*p0 & 0xffff0000u);
+    *p1 = BF16::pair(a, b);
+    a -= __uint_as_float(*p1 << 16);
+    b -= __uint_as_float(*p1 & 0xffff0000u);
+    *p2 = BF16::pair(a, b);
+}
 __device__ __forceinline__ Split3 split(const float* x) {
     Split3 s;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        float a = x[2 * i], b = x[2 * i + 1];
+        uint32_t w[3];
+        split_pair(x[2 * i], x[2 * i + 1], &w[0], &w[1], &w[2]);
 #pragma unroll
-        for (int k = 0; k < 3; ++k) {
-            const uint32_t two = BF16::pair(a, b);
-            s.p[k][i] = two;
-            if (k < 2) {
-                a -= __uint_as_float(two << 16);
-                b -= __uint_as_float(two & 0xffff0000u);
-            }
-        }
+        for (int k = 0; k < 3; ++k) s.p[k][i] = w[k];
     }
     return s;
 }
@@ -124,6 +128,10 @@ struct Wide {
 #pragma unroll
         for (int i = 0; i < 4; ++i) f.p[0][i] = E::pair(x[2 * i], x[2 * i + 1]);
         return f;
+    }
+    // four elements of each piece
+    static __device__ __forceinline__ void four(const float* x, uint2* w) {
+        w[0] = uint2{E::pair(x[0], x[1]), E::pair(x[2], x[3])};
     }
     static __device__ __forceinline__ f32x4 mma(const Frag& a, const Frag& b, f32x4 c) {
         return E::mma(a.p[0], b.p[0], c);
@@ -146,6 +154,10 @@ struct Wide<F32> {
     using Frag = Split3;
     static __device__ __forceinline__ Frag frag(const Raw& r) { return split(r.v); }
     static __device__ __forceinline__ Frag frag(const float* x) { return split(x); }
+    static __device__ __forceinline__ void four(const float* x, uint2* w) {
+        split_pair(x[0], x[1], &w[0].x, &w[1].x, &w[2].x);
+        split_pair(x[2], x[3], &w[0].y, &w[1].y, &w[2].y);
+    }
     static __device__ __forceinline__ f32x4 mma(const Frag& a, const Frag& b, f32x4 c) {
         c = BF16::mma(a.p[2], b.p[0], c);
         c = BF16::mma(a.p[0], b.p[2], c);

@@ -137,13 +137,6 @@ __device__ __forceinline__ float group_max(float v) {
     return group_reduce<G, Max>(v);
 }
 
-// Keeps the compiler from computing what depends on v ahead of this place (and
-// holding it in registers through a loop).
-__device__ __forceinline__ int here(int v) {
-    asm volatile("" : "+v"(v));
-    return v;
-}
-
 // Orders a wave's own accesses to shared memory (they are executed in order).
 __device__ __forceinline__ void wave_fence() {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");

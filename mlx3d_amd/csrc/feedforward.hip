@@ -33,43 +33,47 @@ constexpr int kBN = 64;   // rows of the second
 
 // ---------------------------------------------------------- activations --
 
-// exp(-g).  float32 tensors: 2^t with what rounding t = -g log2(e) left out put
-// back (a relative error of some 2^-23 for any g, where 2^t alone loses |t| 2^-24);
-// 16-bit ones 2^t.  Beyond +-126 the result is past 0 or infinity for 1 + e.
-template <bool EXACT>
-__device__ __forceinline__ float exp_neg(float g) {
-    constexpr float L = -1.44269504088896341f, L2 = -1.92596299e-8f;  // -log2(e), its rest
-    if constexpr (EXACT) {
-        const float x = __builtin_amdgcn_fmed3f(g, -126.f, 126.f);
-        const float t = x * L;
-        const float rest = fmaf(x, L2, fmaf(x, L, -t));
-        const float e = __builtin_amdgcn_exp2f(t);
-        return fmaf(e, rest * 0.69314718055994531f, e);
-    } else {
-        return __builtin_amdgcn_exp2f(g * L);
-    }
-}
-
 // act(g) and act'(g); NaN and infinities as the formulas give them.
-template <bool EXACT>
-__device__ __forceinline__ float activate(int act, float g, float& slope) {
-    if (act == GSX_ACT_GELU) {
-        const float cdf = 0.5f * (1.0f + erff(g * 0.70710678118654752f));
-        slope = cdf + g * 0.39894228040143268f * __expf(-0.5f * g * g);
-        return g * cdf;
-    }
-    const float s = __builtin_amdgcn_rcpf(1.0f + exp_neg<EXACT>(g));
-    if (act == GSX_ACT_SIGMOID) {
-        slope = s * (1.0f - s);
-        return g != g ? g : s;
-    }
-    const float a = g * s;
-    slope = fmaf(a, 1.0f - s, s);
-    return a;
-}
-
+//
+// sigmoid from the hardware's power of two and reciprocal: exp(-g)'s relative
+// error, |g| 2^-24 and one unit, comes into s times 1 - s, so act(g) is within
+// two units of max(|g|, 1) 2^-24 for every g.  Phi(g): in 16 bits by Abramowitz
+// and Stegun 7.1.26 (|error| <= 0.75e-7, its exp(-g^2 / 2) the slope's too), in
+// float32, where that is too coarse for a slope near zero, from erff.
 template <class E>
 constexpr bool kExact = sizeof(typename E::T) == 4;
+
+template <bool GELU, bool EXACT>
+__device__ __forceinline__ float activate(bool silu, float g, float& slope) {
+    if constexpr (GELU) {
+        const float e = __builtin_amdgcn_exp2f(g * g * -0.72134752044448170f);
+        float cdf;
+        if constexpr (EXACT) {
+            cdf = 0.5f * (1.0f + erff(g * 0.70710678118654752f));
+        } else {
+            const float t = __builtin_amdgcn_rcpf(fmaf(fabsf(g), 0.23164189f, 1.0f));
+            float p = fmaf(t, 0.5307027145f, -0.7265760135f);
+            p = fmaf(t, p, 0.7107068705f);
+            p = fmaf(t, p, -0.142248368f);
+            p = fmaf(t, p, 0.127414796f);
+            const float tail = p * t * e;  // Phi(-|g|)
+            cdf = g < 0.f ? tail : 1.0f - tail;
+        }
+        slope = fmaf(g * 0.39894228040143268f, e, cdf);
+        return g * cdf;
+    } else {
+        const float e = __builtin_amdgcn_exp2f(g * -1.4426950408889634f);
+        const float s = __builtin_amdgcn_rcpf(1.0f + e);
+        const float a = s * (silu ? g : 1.0f);
+        slope = fmaf(a, 1.0f - s, silu ? s : 0.0f);
+        return a;
+    }
+}
+template <bool EXACT>
+__device__ __forceinline__ float activate_any(int act, float g, float& slope) {
+    return act == GSX_ACT_GELU ? activate<true, EXACT>(false, g, slope)
+                               : activate<false, EXACT>(act == GSX_ACT_SILU, g, slope);
+}
 
 // ---------------------------------------------------------------- tiles --
 
@@ -318,7 +322,7 @@ __global__ __launch_bounds__(kThreads) void k_tile(const Tile q) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     float slope;
-                    h[e] = activate<kExact<E>>(q.act, c0[i][j][e], slope) * c1[i][j][e];
+                    h[e] = activate_any<kExact<E>>(q.act, c0[i][j][e], slope) * c1[i][j][e];
                 }
                 put<E>((T*)q.out[0], q.ldo, row, col, q.m, q.n, q.vec_out, h);
             } else if constexpr (MODE == BWD_HIDDEN) {
@@ -326,7 +330,7 @@ __global__ __launch_bounds__(kThreads) void k_tile(const Tile q) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     float slope;
-                    const float a = activate<kExact<E>>(q.act, c0[i][j][e], slope);
+                    const float a = activate_any<kExact<E>>(q.act, c0[i][j][e], slope);
                     const float u = c1[i][j][e], dh = c2[i][j][e];
                     h[e] = a * u;
                     du[e] = dh * a;
@@ -390,7 +394,6 @@ template <class E, int KD, int OB>
 __device__ __forceinline__ void stage_weights(const Narrow<E>& q, u32x4* lds, int c0, int count) {
     using Wd = Wide<E>;
     constexpr int PC = Wd::PIECES, FRAGS = 4 * KD + OB;
-    const int64_t in = (int64_t)q.hidden * q.d_in, out = (int64_t)q.d_out * q.hidden;
     for (int i = threadIdx.x; i < count * FRAGS * 64; i += kNarrowThreads) {
         const int lane = i & 63, frag = (i >> 6) % FRAGS, c = (i >> 6) / FRAGS;
         const int r = lane & 15, k8 = (lane >> 4) * 8;
@@ -400,13 +403,12 @@ __device__ __forceinline__ void stage_weights(const Narrow<E>& q, u32x4* lds, in
             const int f = (c0 + c) * 32 + 8 * (r >> 2) + (r & 3) + 4 * (which & 1);
             const int k = kd * 32 + k8;
             if (f < q.hidden && k < q.d_in)
-                raw = load8<E>((which < 2 ? q.wg : q.wu) + (int64_t)f * q.d_in, k, q.d_in,
-                               in - (int64_t)f * q.d_in);
+                raw = load8<E>((which < 2 ? q.wg : q.wu) + (int64_t)f * q.d_in + k, q.d_in - k,
+                               q.hidden - 1 - f);
         } else {
             const int o = (frag - 4 * KD) * 16 + r, k = (c0 + c) * 32 + k8;
             if (o < q.d_out && k < q.hidden)
-                raw = load8<E>(q.wd + (int64_t)o * q.hidden, k, q.hidden,
-                               out - (int64_t)o * q.hidden);
+                raw = load8<E>(q.wd + (int64_t)o * q.hidden + k, q.hidden - k, q.d_out - 1 - o);
         }
         const typename Wd::Frag w = Wd::frag(raw);
 #pragma unroll
@@ -414,7 +416,7 @@ __device__ __forceinline__ void stage_weights(const Narrow<E>& q, u32x4* lds, in
     }
 }
 
-template <class E, int KD, int OB>
+template <class E, int KD, int OB, bool GELU>
 __global__ __launch_bounds__(kNarrowThreads) void k_narrow_fwd(const Narrow<E> q) {
     using T = typename E::T;
     using W = Wide<E>;
@@ -423,7 +425,7 @@ __global__ __launch_bounds__(kNarrowThreads) void k_narrow_fwd(const Narrow<E> q
     extern __shared__ u32x4 smem[];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const int col = lane & 15, k8 = (lane >> 4) * 8;
-    const bool once = q.resident >= q.chunks;
+    const bool once = q.resident >= q.chunks, silu = q.act == GSX_ACT_SILU;
     auto weights = [&](int c, int frag) {
         typename W::Frag w;
 #pragma unroll
@@ -446,8 +448,7 @@ __global__ __launch_bounds__(kNarrowThreads) void k_narrow_fwd(const Narrow<E> q
                 const int k = kd * 32 + k8;
                 typename W::Raw raw{};
                 if (row < q.rows && k < q.d_in)
-                    raw = load8<E>(q.x + row * q.ldx, k, q.d_in,
-                                   (q.rows - 1 - row) * q.ldx + q.d_in);
+                    raw = load8<E>(q.x + row * q.ldx + k, q.d_in - k, (int)(q.rows - 1 - row));
                 x[r][kd] = W::frag(raw);
             }
         f32x4 y[OB][R];
@@ -485,7 +486,7 @@ __global__ __launch_bounds__(kNarrowThreads) void k_narrow_fwd(const Narrow<E> q
                     float v[8], slope;
 #pragma unroll
                     for (int i = 0; i < 8; ++i)
-                        v[i] = activate<kExact<E>>(q.act, g[i >> 2][r][i & 3], slope) *
+                        v[i] = activate<GELU, kExact<E>>(silu, g[i >> 2][r][i & 3], slope) *
                                u[i >> 2][r][i & 3];
                     h[r] = W::frag(v);
                 }
@@ -549,11 +550,23 @@ struct NarrowBwd {
 };
 
 // A tile of 32 rows in shared memory, SLOTS 16-byte slots a row, the slots turned
-// by the row so that lanes of consecutive rows meet different banks.
+// by the row so that no access meets a bank twice.  What the accesses ask for
+// (measured with a counter of conflicts): a 16-byte read serves lanes 0-3, 12-15,
+// 20-27 of a half wave in one clock, then the others, so rows 0-3 and 12-15 of
+// one slot with rows 4-11 of the next; a transposing read 32 lanes, rows r .. r + 3
+// and r + 8 .. r + 11 of two slots; a 16-byte write eight lanes, over half the
+// banks.
 template <int SLOTS>
 __device__ __forceinline__ int tile_slot(int row, int slot) {
-    constexpr int shift = SLOTS == 4 ? 2 : 0;
-    return row * SLOTS + (slot ^ ((row >> shift) & (SLOTS - 1)));
+    const int b0 = row & 1, b1 = row >> 1 & 1, b2 = row >> 2 & 1, b3 = row >> 3 & 1;
+    if constexpr (SLOTS == 4) return row * 4 + (slot ^ ((b2 ^ b3) << 1 | (b3 ^ b1)));
+    if constexpr (SLOTS == 8) return row * 8 + (slot ^ (b1 << 1 | b3 << 2));
+    return row * SLOTS + (slot ^ (b0 << 1 | b1 << 2 | b3 << 3));
+}
+// Rows of float32 sums, written and read along the slots only.
+template <int SLOTS>
+__device__ __forceinline__ int sum_slot(int row, int slot) {
+    return row * SLOTS + (slot ^ (row & (SLOTS - 1)));
 }
 
 // The operand whose rows are a tile's columns c0 .. c0 + 15 and whose summed
@@ -586,13 +599,13 @@ struct BwdShape {
     static int64_t lds(int pairs) { return 16 * (2 * TILE + (int64_t)pairs * (3 * GATE + SUM)); }
 };
 
-// Waves for a SIMD that the registers leave room for.
+// Waves for a SIMD that the registers leave room for: one workgroup or two.
 template <class E, int KD, int KO>
 constexpr int bwd_waves() {
-    return sizeof(typename E::T) == 4 || KD + KO > 4 ? 2 : KD == 2 ? 3 : 4;
+    return sizeof(typename E::T) == 4 || KD > 1 || KO > 2 ? 2 : 4;
 }
 
-template <class E, int KD, int KO>
+template <class E, int KD, int KO, bool GELU>
 __global__ __launch_bounds__(128 * kBwdPairs, (bwd_waves<E, KD, KO>()))
 void k_narrow_bwd(const NarrowBwd<E> q) {
     using T = typename E::T;
@@ -602,9 +615,10 @@ void k_narrow_bwd(const NarrowBwd<E> q) {
     constexpr int PC = S::PC, R = kBwdRows / 16;
     extern __shared__ u32x4 smem[];
     const int threads = blockDim.x, pairs = threads >> 7;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane0 = threadIdx.x & 63;
     const int pair = wave >> 1, half = wave & 1;
-    const int col = lane & 15, quad = lane >> 4, k8 = quad * 8;
+    const bool silu = q.act == GSX_ACT_SILU;
+    const int col = lane0 & 15, quad = lane0 >> 4, k8 = quad * 8;
     u32x4* tiles = smem;
     u32x4* gates = smem + 2 * S::TILE + pair * 3 * S::GATE;
     u32x4* sums = smem + 2 * S::TILE + pairs * 3 * S::GATE;
@@ -614,7 +628,6 @@ void k_narrow_bwd(const NarrowBwd<E> q) {
     // pair's 32 channels for every other 16 of dx's
     Frag wg[KD], wu[KD], wd[KO], wgt[KD], wut[KD];
     {
-        const int64_t in = (int64_t)q.hidden * q.d_in;
         auto gather = [&](const T* w, int64_t first, int64_t step, int n) {
             typename W::Raw raw;
             T v[8];
@@ -630,8 +643,9 @@ void k_narrow_bwd(const NarrowBwd<E> q) {
             const int k = kd * 32 + k8;
             typename W::Raw a{}, c{};
             if (there && k < q.d_in) {
-                a = load8<E>(q.wg + (int64_t)f * q.d_in, k, q.d_in, in - (int64_t)f * q.d_in);
-                c = load8<E>(q.wu + (int64_t)f * q.d_in, k, q.d_in, in - (int64_t)f * q.d_in);
+                const int64_t at = (int64_t)f * q.d_in + k;
+                a = load8<E>(q.wg + at, q.d_in - k, q.hidden - 1 - f);
+                c = load8<E>(q.wu + at, q.d_in - k, q.hidden - 1 - f);
             }
             wg[kd] = W::frag(a);
             wu[kd] = W::frag(c);
@@ -654,48 +668,65 @@ void k_narrow_bwd(const NarrowBwd<E> q) {
     // thread's registers one tile ahead
     constexpr int PIECES = kBwdRows * (S::XS + S::YS);
     constexpr int HELD = (PIECES + 128 * kBwdPairs - 1) / (128 * kBwdPairs);
-    auto fetch = [&](int64_t row0, int n, typename W::Raw& raw) {
+    const int rows = (int)q.rows, step = (int)gridDim.x * kBwdRows;
+    struct Piece {
+        const T* p;    // in the next tile to be read
+        int64_t hop;   // from a tile to the next
+        int row, n;    // its row; how many elements the row has from here on
+        int slot;      // its place in the staged tile
+    };
+    auto piece_of = [&](int n, int row0) {
         const bool of_x = n < kBwdRows * S::XS;
         const int i = of_x ? n : n - kBwdRows * S::XS;
         const int slots = of_x ? S::XS : S::YS, row = i / slots, k = i % slots * 8;
-        const int width = of_x ? q.d_in : q.d_out;
-        const int64_t ld = of_x ? q.ldx : q.lddy, at = row0 + row;
-        raw = typename W::Raw{};
-        if (at < q.rows && k < width)
-            raw = load8<E>((of_x ? q.x : q.dy) + at * ld, k, width, (q.rows - 1 - at) * ld + width);
+        const int64_t ld = of_x ? q.ldx : q.lddy;
+        Piece m;
+        m.row = row0 + row;
+        m.p = (of_x ? q.x : q.dy) + (int64_t)m.row * ld + k;
+        m.hop = step * ld;
+        m.n = (of_x ? q.d_in : q.d_out) - k;
+        m.slot = of_x ? tile_slot<S::XS>(row, i % S::XS)
+                      : PC * kBwdRows * S::XS + tile_slot<S::YS>(row, i % S::YS);
+        return m;
     };
-    auto settle = [&](u32x4* tile, int n, const typename W::Raw& raw) {
-        const bool of_x = n < kBwdRows * S::XS;
-        const int i = of_x ? n : n - kBwdRows * S::XS;
+    auto fetch = [&](const Piece& m) {
+        typename W::Raw raw{};
+        if (m.row < rows && m.n > 0) raw = load8<E>(m.p, m.n, rows - 1 - m.row);
+        return raw;
+    };
+    auto settle = [&](u32x4* tile, const Piece& m, bool of_x, const typename W::Raw& raw) {
         const Frag f = W::frag(raw);
+        const int pitch = kBwdRows * (of_x ? S::XS : S::YS);
 #pragma unroll
-        for (int p = 0; p < PC; ++p) {
-            if (of_x)
-                tile[p * kBwdRows * S::XS + tile_slot<S::XS>(i / S::XS, i % S::XS)] = f.p[p];
-            else
-                tile[PC * kBwdRows * S::XS + p * kBwdRows * S::YS +
-                     tile_slot<S::YS>(i / S::YS, i % S::YS)] = f.p[p];
-        }
+        for (int p = 0; p < PC; ++p) tile[m.slot + p * pitch] = f.p[p];
     };
+    Piece mine[HELD];
     typename W::Raw next[HELD];
-    auto fetch_all = [&](int64_t row0) {
+    auto fetch_all = [&] {
 #pragma unroll
-        for (int i = 0; i < HELD; ++i) {
-            const int n = threadIdx.x + i * threads;
-            if (n < PIECES) fetch(row0, n, next[i]);
-        }
+        for (int i = 0; i < HELD; ++i)
+            if (threadIdx.x + i * threads < PIECES) {
+                next[i] = fetch(mine[i]);
+                mine[i].p += mine[i].hop;
+                mine[i].row += step;
+            }
     };
-    auto settle_all = [&](u32x4* tile, int64_t row0) {
+    auto settle_all = [&](u32x4* tile, int row0) {
 #pragma unroll
         for (int i = 0; i < HELD; ++i) {
             const int n = threadIdx.x + i * threads;
-            if (n < PIECES) settle(tile, n, next[i]);
+            if (n < PIECES) settle(tile, mine[i], n < kBwdRows * S::XS, next[i]);
         }
         for (int n = threadIdx.x + HELD * threads; n < PIECES; n += threads) {  // fewer pairs
-            typename W::Raw raw;
-            fetch(row0, n, raw);
-            settle(tile, n, raw);
+            const Piece m = piece_of(n, row0);
+            settle(tile, m, n < kBwdRows * S::XS, fetch(m));
         }
+    };
+
+    // 16 bits: no work is moved over these places (two workgroups to a unit hide
+    // the waits, and what is in flight takes their registers)
+    auto pause = [] {
+        if constexpr (PC == 1) __builtin_amdgcn_sched_barrier(0);
     };
 
     f32x4 sg[2 * KD], su[2 * KD], sd[2 * KO];  // the weight gradients' sums
@@ -704,15 +735,18 @@ void k_narrow_bwd(const NarrowBwd<E> q) {
 #pragma unroll
     for (int o = 0; o < 2 * KO; ++o) sd[o] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-    const int64_t step = (int64_t)gridDim.x * kBwdRows;
-    int64_t row0 = (int64_t)blockIdx.x * kBwdRows;
-    fetch_all(row0);
+    int row0 = (int)blockIdx.x * kBwdRows;
+#pragma unroll
+    for (int i = 0; i < HELD; ++i)
+        if (threadIdx.x + i * threads < PIECES) mine[i] = piece_of(threadIdx.x + i * threads, row0);
+    fetch_all();
     settle_all(tiles, row0);
-    fetch_all(row0 + step);
+    fetch_all();
     __syncthreads();
-    for (int turn = 0; row0 < q.rows; row0 += step, turn ^= 1) {
+    for (int turn = 0; row0 < rows; row0 += step, turn ^= 1) {
         const u32x4* xt = tiles + turn * S::TILE;
         const u32x4* yt = xt + PC * kBwdRows * S::XS;
+        uint2 gate[R][3][PC];
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             const int row = 16 * r + col;
@@ -738,21 +772,29 @@ void k_narrow_bwd(const NarrowBwd<E> q) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 float slope;
-                const float a = activate<kExact<E>>(q.act, g[i], slope);
+                const float a = activate<GELU, kExact<E>>(silu, g[i], slope);
                 v[0][i] = dh[i] * u[i] * slope;
                 v[1][i] = dh[i] * a;
                 v[2][i] = a * u[i];
             }
 #pragma unroll
-            for (int j = 0; j < 3; ++j) {
-                uint2 w[PC];
-                W::four(v[j], w);
-#pragma unroll
-                for (int p = 0; p < PC; ++p)
-                    ((uint2*)(gates + j * S::GATE + p * kBwdRows * 4 +
-                              tile_slot<4>(row, 2 * half + (quad >> 1))))[quad & 1] = w[p];
-            }
+            for (int j = 0; j < 3; ++j) W::four(v[j], gate[r][j]);
+            pause();
         }
+        // lanes of neighbouring quads hold channels 0-3 and 4-7 of the same two
+        // rows: they swap, and each stores eight of one row
+#pragma unroll
+        for (int j = 0; j < 3; ++j)
+#pragma unroll
+            for (int p = 0; p < PC; ++p) {
+                const auto lo = __builtin_amdgcn_permlane16_swap(gate[0][j][p].x, gate[1][j][p].x,
+                                                                 false, false);
+                const auto hi = __builtin_amdgcn_permlane16_swap(gate[0][j][p].y, gate[1][j][p].y,
+                                                                 false, false);
+                gates[j * S::GATE + p * kBwdRows * 4 +
+                      tile_slot<4>(16 * (quad & 1) + col, 2 * half + (quad >> 1))] =
+                    u32x4{lo[0], hi[0], lo[1], hi[1]};
+            }
         __syncthreads();
         // the pair's part of dx, every other 16 of its channels
 #pragma unroll
@@ -769,11 +811,13 @@ void k_narrow_bwd(const NarrowBwd<E> q) {
                 f32x4 d{0.f, 0.f, 0.f, 0.f};
                 d = W::mma(wgt[j], dg, d);
                 d = W::mma(wut[j], du, d);
-                sums[pair * S::SUM + tile_slot<8 * KD>(row, (2 * j + half) * 4 + quad)] =
+                sums[pair * S::SUM + sum_slot<8 * KD>(row, (2 * j + half) * 4 + quad)] =
                     __builtin_bit_cast(u32x4, d);
             }
         }
+        pause();
         // weight gradients: operands along the rows
+        const int lane = lane0;
         Frag t[3];
 #pragma unroll
         for (int j = 0; j < 3; ++j)
@@ -789,6 +833,7 @@ void k_narrow_bwd(const NarrowBwd<E> q) {
             sg[db] = W::mma(x, t[0], sg[db]);
             su[db] = W::mma(x, t[1], su[db]);
         }
+        pause();
 #pragma unroll
         for (int ob = 0; ob < 2 * KO; ++ob) {
             Frag y;
@@ -799,17 +844,18 @@ void k_narrow_bwd(const NarrowBwd<E> q) {
         }
         // the next tile into the other place, then the pairs' parts of dx
         settle_all(tiles + (turn ^ 1) * S::TILE, row0 + step);
-        fetch_all(row0 + 2 * step);
+        fetch_all();
         __syncthreads();
         if (q.dx || q.dx_parts)
             for (int n = threadIdx.x; n < kBwdRows * 8 * KD; n += threads) {
                 const int row = n / (8 * KD), slot = n % (8 * KD), d = 4 * slot;
                 const int64_t at = row0 + row;
-                if (at >= q.rows || d >= q.d_in) continue;
+                if (at >= rows || d >= q.d_in) continue;
                 f32x4 v{0.f, 0.f, 0.f, 0.f};
-                for (int w = 0; w < pairs; ++w)
-                    v += __builtin_bit_cast(f32x4,
-                                            sums[w * S::SUM + tile_slot<8 * KD>(row, slot)]);
+                const u32x4* part = sums + sum_slot<8 * KD>(row, slot);
+#pragma unroll
+                for (int w = 0; w < kBwdPairs; ++w)
+                    if (w < pairs) v += __builtin_bit_cast(f32x4, part[w * S::SUM]);
                 if (q.dx_parts) {
                     float* out = q.dx_parts + ((int64_t)blockIdx.y * q.rows + at) * q.d_in + d;
 #pragma unroll
@@ -832,7 +878,7 @@ void k_narrow_bwd(const NarrowBwd<E> q) {
     }
     float* out = q.parts +
                  (((int64_t)blockIdx.x * gridDim.y + blockIdx.y) * 2 * kBwdPairs + wave) * S::SUMS *
-                     64 + lane;
+                     64 + lane0;
     int n = 0;
 #pragma unroll
     for (int d = 0; d < 2 * KD; ++d)
@@ -999,12 +1045,12 @@ int launch_narrow_fwd(const Shape& s, const void* x, int64_t ldx, const void* wg
     int64_t per_cu = 160 * 1024 / lds;
     if (per_cu > 2) per_cu = 2;
     const int64_t grid = tiles < 256 * per_cu ? tiles : 256 * per_cu;
-    const hipError_t e = hipFuncSetAttribute((const void*)&k_narrow_fwd<E, KD, OB>,
-                                             hipFuncAttributeMaxDynamicSharedMemorySize,
-                                             (int)kNarrowLds);
-    if (e != hipSuccess) return GSX_ERR_HIP;
-    hipLaunchKernelGGL((k_narrow_fwd<E, KD, OB>), dim3((unsigned)grid), dim3(kNarrowThreads),
-                       (unsigned)lds, st, q);
+    const auto kernel = s.act == GSX_ACT_GELU ? k_narrow_fwd<E, KD, OB, true>
+                                              : k_narrow_fwd<E, KD, OB, false>;
+    if (hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize,
+                            (int)kNarrowLds) != hipSuccess)
+        return GSX_ERR_HIP;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(kNarrowThreads), (unsigned)lds, st, q);
     GSX_LAUNCH_CHECK();
     return GSX_OK;
 }
@@ -1093,12 +1139,13 @@ int launch_narrow_bwd(const Shape& s, const BwdArgs& a) {
                              (const T*)a.dy, p.groups > 1 ? nullptr : (T*)a.dx, dx_parts, parts,
                              a.ldx, a.lddy, s.rows, s.d_in, s.hidden, s.d_out, s.act};
         const int64_t lds = S::lds(p.pairs);
-        if (hipFuncSetAttribute((const void*)&k_narrow_bwd<E, KD, KO>,
-                                hipFuncAttributeMaxDynamicSharedMemorySize,
+        const auto kernel = s.act == GSX_ACT_GELU ? k_narrow_bwd<E, KD, KO, true>
+                                                  : k_narrow_bwd<E, KD, KO, false>;
+        if (hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize,
                                 160 * 1024) != hipSuccess)
             return GSX_ERR_HIP;
-        hipLaunchKernelGGL((k_narrow_bwd<E, KD, KO>), dim3(p.blocks, p.groups), dim3(128 * p.pairs),
-                           (unsigned)lds, a.st, q);
+        hipLaunchKernelGGL(kernel, dim3(p.blocks, p.groups), dim3(128 * p.pairs), (unsigned)lds,
+                           a.st, q);
         GSX_LAUNCH_CHECK();
         if (a.dwg || a.dwd) {
             const int halves = p.groups * 2 * kBwdPairs;

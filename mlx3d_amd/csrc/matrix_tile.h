@@ -18,6 +18,13 @@
 
 namespace gsx {
 
+// Keeps the compiler from computing what depends on v ahead of this place (and
+// holding it in registers through a loop).
+__device__ __forceinline__ int here(int v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
+
 using f32x4 = __attribute__((ext_vector_type(4))) float;
 using f16x8 = __attribute__((ext_vector_type(8))) _Float16;
 using bf16x8 = __attribute__((ext_vector_type(8))) __bf16;
@@ -173,21 +180,21 @@ struct Wide<F32> {
     }
 };
 
-// Elements k .. k + 7 of the row at p, which has n; zeros behind its end.  A
-// piece that reaches over the row's end may read what follows (and drop it)
-// where `room`, the elements of the tensor from the row's first on, holds it.
+// Eight elements from p on, of which the first n (at least one) belong to the
+// row; zeros for the others.  With `after` rows behind this one, eight or more,
+// what follows the row's end is the tensor's too (a row takes an element at
+// least) and may be read and dropped.
 template <class E>
-__device__ __forceinline__ typename Wide<E>::Raw load8(const typename E::T* p, int k, int n,
-                                                       int64_t room) {
+__device__ __forceinline__ typename Wide<E>::Raw load8(const typename E::T* p, int n, int after) {
     using T = typename E::T;
     typename Wide<E>::Raw r;
-    if (k + 8 <= room) {
-        __builtin_memcpy(&r, p + k, sizeof(r));
-        if (k + 8 > n) Wide<E>::cut(r, n - k);
+    if (n >= 8 || after >= 8) {
+        __builtin_memcpy(&r, p, sizeof(r));
+        if (n < 8) Wide<E>::cut(r, n);
     } else {
         T v[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = k + i < n ? p[k + i] : (T)0;
+        for (int i = 0; i < 8; ++i) v[i] = i < n ? p[i] : (T)0;
         __builtin_memcpy(&r, v, sizeof(r));
     }
     return r;

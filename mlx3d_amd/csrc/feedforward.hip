@@ -615,10 +615,10 @@ void k_narrow_bwd(const NarrowBwd<E> q) {
     constexpr int PC = S::PC, R = kBwdRows / 16;
     extern __shared__ u32x4 smem[];
     const int threads = blockDim.x, pairs = threads >> 7;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane0 = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int pair = wave >> 1, half = wave & 1;
     const bool silu = q.act == GSX_ACT_SILU;
-    const int col = lane0 & 15, quad = lane0 >> 4, k8 = quad * 8;
+    const int col = lane & 15, quad = lane >> 4, k8 = quad * 8;
     u32x4* tiles = smem;
     u32x4* gates = smem + 2 * S::TILE + pair * 3 * S::GATE;
     u32x4* sums = smem + 2 * S::TILE + pairs * 3 * S::GATE;
@@ -723,10 +723,15 @@ void k_narrow_bwd(const NarrowBwd<E> q) {
         }
     };
 
-    // 16 bits: no work is moved over these places (two workgroups to a unit hide
-    // the waits, and what is in flight takes their registers)
+    // no work is moved over these places where the registers hold what is asked for
+    constexpr bool EARLY = PC == 3 && KD == 1;
+    auto asked = [] {
+        if constexpr (EARLY) __builtin_amdgcn_sched_barrier(0);
+    };
+    // elsewhere over these: what is in flight would take too many (or, in 16 bits,
+    // the registers of the second workgroup that hides the waits)
     auto pause = [] {
-        if constexpr (PC == 1) __builtin_amdgcn_sched_barrier(0);
+        if constexpr (!EARLY) __builtin_amdgcn_sched_barrier(0);
     };
 
     f32x4 sg[2 * KD], su[2 * KD], sd[2 * KO];  // the weight gradients' sums
@@ -746,28 +751,39 @@ void k_narrow_bwd(const NarrowBwd<E> q) {
     for (int turn = 0; row0 < rows; row0 += step, turn ^= 1) {
         const u32x4* xt = tiles + turn * S::TILE;
         const u32x4* yt = xt + PC * kBwdRows * S::XS;
+        // where the registers allow it, a phase asks shared memory for all that it
+        // needs first, and its products begin with the first answer
+        Frag fx[R][KD], fy[R][KO];
+        auto ask = [&](int r) {
+            const int row = 16 * r + col;
+#pragma unroll
+            for (int kd = 0; kd < KD; ++kd)
+#pragma unroll
+                for (int p = 0; p < PC; ++p)
+                    fx[r][kd].p[p] = xt[p * kBwdRows * S::XS + tile_slot<S::XS>(row, kd * 4 + quad)];
+#pragma unroll
+            for (int ko = 0; ko < KO; ++ko)
+#pragma unroll
+                for (int p = 0; p < PC; ++p)
+                    fy[r][ko].p[p] = yt[p * kBwdRows * S::YS + tile_slot<S::YS>(row, ko * 4 + quad)];
+        };
+        if constexpr (EARLY) {
+#pragma unroll
+            for (int r = 0; r < R; ++r) ask(r);
+            asked();
+        }
         uint2 gate[R][3][PC];
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            const int row = 16 * r + col;
+            if constexpr (!EARLY) ask(r);
             f32x4 g{0.f, 0.f, 0.f, 0.f}, u = g, dh = g;
 #pragma unroll
             for (int kd = 0; kd < KD; ++kd) {
-                Frag x;
-#pragma unroll
-                for (int p = 0; p < PC; ++p)
-                    x.p[p] = xt[p * kBwdRows * S::XS + tile_slot<S::XS>(row, kd * 4 + quad)];
-                g = W::mma(wg[kd], x, g);
-                u = W::mma(wu[kd], x, u);
+                g = W::mma(wg[kd], fx[r][kd], g);
+                u = W::mma(wu[kd], fx[r][kd], u);
             }
 #pragma unroll
-            for (int ko = 0; ko < KO; ++ko) {
-                Frag y;
-#pragma unroll
-                for (int p = 0; p < PC; ++p)
-                    y.p[p] = yt[p * kBwdRows * S::YS + tile_slot<S::YS>(row, ko * 4 + quad)];
-                dh = W::mma(wd[ko], y, dh);
-            }
+            for (int ko = 0; ko < KO; ++ko) dh = W::mma(wd[ko], fy[r][ko], dh);
             float v[3][4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -796,50 +812,89 @@ void k_narrow_bwd(const NarrowBwd<E> q) {
                     u32x4{lo[0], hi[0], lo[1], hi[1]};
             }
         __syncthreads();
-        // the pair's part of dx, every other 16 of its channels
+        // the pair's part of dx, every other 16 of its channels, and the weight
+        // gradients, whose operands lie along the rows
+        Frag fg[R], fu[R], t[3];
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             const int row = 16 * r + col;
-            Frag dg, du;
 #pragma unroll
             for (int p = 0; p < PC; ++p) {
-                dg.p[p] = gates[p * kBwdRows * 4 + tile_slot<4>(row, quad)];
-                du.p[p] = gates[S::GATE + p * kBwdRows * 4 + tile_slot<4>(row, quad)];
+                fg[r].p[p] = gates[p * kBwdRows * 4 + tile_slot<4>(row, quad)];
+                fu[r].p[p] = gates[S::GATE + p * kBwdRows * 4 + tile_slot<4>(row, quad)];
             }
+        }
+        auto turn_gate = [&](int j) {
+#pragma unroll
+            for (int p = 0; p < PC; ++p)
+                t[j].p[p] = read_turned<4>(gates + j * S::GATE + p * kBwdRows * 4, 16 * half, lane);
+        };
+        if constexpr (EARLY) {
+            turn_gate(0);
+            turn_gate(1);
+            turn_gate(2);
+        }
+        asked();
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const int row = 16 * r + col;
 #pragma unroll
             for (int j = 0; j < KD; ++j) {
                 f32x4 d{0.f, 0.f, 0.f, 0.f};
-                d = W::mma(wgt[j], dg, d);
-                d = W::mma(wut[j], du, d);
+                d = W::mma(wgt[j], fg[r], d);
+                d = W::mma(wut[j], fu[r], d);
                 sums[pair * S::SUM + sum_slot<8 * KD>(row, (2 * j + half) * 4 + quad)] =
                     __builtin_bit_cast(u32x4, d);
             }
         }
         pause();
-        // weight gradients: operands along the rows
-        const int lane = lane0;
-        Frag t[3];
-#pragma unroll
-        for (int j = 0; j < 3; ++j)
-#pragma unroll
-            for (int p = 0; p < PC; ++p)
-                t[j].p[p] = read_turned<4>(gates + j * S::GATE + p * kBwdRows * 4, 16 * half, lane);
-#pragma unroll
-        for (int db = 0; db < 2 * KD; ++db) {
+        auto turned_x = [&](int db) {
             Frag x;
 #pragma unroll
             for (int p = 0; p < PC; ++p)
                 x.p[p] = read_turned<S::XS>(xt + p * kBwdRows * S::XS, 16 * db, lane);
-            sg[db] = W::mma(x, t[0], sg[db]);
-            su[db] = W::mma(x, t[1], su[db]);
-        }
-        pause();
-#pragma unroll
-        for (int ob = 0; ob < 2 * KO; ++ob) {
+            return x;
+        };
+        auto turned_y = [&](int ob) {
             Frag y;
 #pragma unroll
             for (int p = 0; p < PC; ++p)
                 y.p[p] = read_turned<S::YS>(yt + p * kBwdRows * S::YS, 16 * ob, lane);
+            return y;
+        };
+        Frag ahead;  // the next block's operand
+        if constexpr (EARLY) {
+            ahead = turned_x(0);
+        } else {
+            turn_gate(0);
+            turn_gate(1);
+        }
+        asked();
+#pragma unroll
+        for (int db = 0; db < 2 * KD; ++db) {
+            Frag x;
+            if constexpr (EARLY) {
+                x = ahead;
+                ahead = db + 1 < 2 * KD ? turned_x(db + 1) : turned_y(0);
+                asked();
+            } else {
+                x = turned_x(db);
+            }
+            sg[db] = W::mma(x, t[0], sg[db]);
+            su[db] = W::mma(x, t[1], su[db]);
+        }
+        pause();
+        if constexpr (!EARLY) turn_gate(2);
+#pragma unroll
+        for (int ob = 0; ob < 2 * KO; ++ob) {
+            Frag y;
+            if constexpr (EARLY) {
+                y = ahead;
+                if (ob + 1 < 2 * KO) ahead = turned_y(ob + 1);
+                asked();
+            } else {
+                y = turned_y(ob);
+            }
             sd[ob] = W::mma(y, t[2], sd[ob]);
         }
         // the next tile into the other place, then the pairs' parts of dx
@@ -878,7 +933,7 @@ void k_narrow_bwd(const NarrowBwd<E> q) {
     }
     float* out = q.parts +
                  (((int64_t)blockIdx.x * gridDim.y + blockIdx.y) * 2 * kBwdPairs + wave) * S::SUMS *
-                     64 + lane0;
+                     64 + lane;
     int n = 0;
 #pragma unroll
     for (int d = 0; d < 2 * KD; ++d)

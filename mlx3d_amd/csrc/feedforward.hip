@@ -78,17 +78,21 @@ __device__ __forceinline__ float activate_any(int act, float g, float& slope) {
 // ---------------------------------------------------------------- tiles --
 
 // One operand: element (row, k) is p[row * ld + k] where KC (the summed index
-// is contiguous), else p[k * ld + row].  `vec`: its 16-byte pieces (KC) or its
-// pieces of a few rows are aligned.
+// is contiguous), else p[k * ld + row].
 struct Operand {
     const void* p;
     int64_t ld;
     int rows;
-    int vec;
 };
 
 // ROWS rows times two fragments' depth of one operand, kept in fragment order
-// (row block, fragment, lane): reads and writes are whole 16-byte lanes.
+// (row block, fragment, lane), a lane's 16 bytes at a time.  Rows of odd length
+// are read unaligned, which global memory allows at the price of a sector.
+//
+// The lanes of a fragment lie so that what a wave reads, and eight lanes of what
+// it stores, meet each bank once: where the summed index is contiguous a wave
+// stores whole fragments; else its lanes are a few rows apart, and the four low
+// bits of the row are turned (bits 2, 3, 0, 1), odd row blocks half a turn on.
 template <class E, int ROWS, bool KC>
 struct Stage {
     using T = typename E::T;
@@ -97,21 +101,30 @@ struct Stage {
     static constexpr int N = ROWS / 32;   // 16-byte pieces of a thread
     u32x4 r[N];
 
+    static __device__ __forceinline__ int place(int row, int quad) {
+        const int in = row & 15;
+        return KC ? quad * 16 + in
+                  : quad * 16 + (((in & 3) << 2 | in >> 2) ^ (row >> 4 & 1) << 2);
+    }
     static __device__ __forceinline__ int slot(int row, int piece) {
-        return ((row >> 4) * 2 + (piece >> 2)) * 64 + (piece & 3) * 16 + (row & 15);
+        return ((row >> 4) * 2 + (piece >> 2)) * 64 + place(row, piece & 3);
+    }
+    // the fragment f of row block b, on this lane
+    static __device__ __forceinline__ u32x4 read(const u32x4* lds, int b, int f, int lane) {
+        return lds[(b * 2 + f) * 64 + place(b * 16 + (lane & 15), lane >> 4)];
     }
 
     __device__ __forceinline__ void load(const Operand& o, int row0, int64_t k0, int64_t k1) {
         const T* p = (const T*)o.p;
         const int t = threadIdx.x;
         if constexpr (KC) {
+            const int64_t k = k0 + (t >> 4 & 7) * VEC;
 #pragma unroll
             for (int n = 0; n < N; ++n) {
-                const int row = row0 + (t >> 3) + 32 * n;
-                const int64_t k = k0 + (t & 7) * VEC;
+                const int row = row0 + (t >> 7) * 16 + (t & 15) + 32 * n;
                 const T* at = p + (int64_t)row * o.ld + k;
-                if (row < o.rows && k + VEC <= k1 && o.vec) {
-                    r[n] = *(const u32x4*)at;
+                if (row < o.rows && k + VEC <= k1) {
+                    __builtin_memcpy(&r[n], at, 16);
                 } else {
                     T v[VEC];
 #pragma unroll
@@ -128,9 +141,8 @@ struct Stage {
 #pragma unroll
             for (int i = 0; i < VEC; ++i) {
                 const T* at = p + (k + i) * o.ld + row;
-                if (k + i < k1 && row + N <= o.rows && o.vec) {
-                    __builtin_memcpy(v[i], __builtin_assume_aligned(at, N * sizeof(T)),
-                                     N * sizeof(T));
+                if (k + i < k1 && row + N <= o.rows) {
+                    __builtin_memcpy(v[i], at, N * sizeof(T));
                 } else {
 #pragma unroll
                     for (int n = 0; n < N; ++n)
@@ -152,7 +164,7 @@ struct Stage {
 #pragma unroll
         for (int n = 0; n < N; ++n) {
             if constexpr (KC)
-                lds[slot((t >> 3) + 32 * n, t & 7)] = r[n];
+                lds[slot((t >> 7) * 16 + (t & 15) + 32 * n, t >> 4 & 7)] = r[n];
             else
                 lds[slot((t & 31) * N + n, t >> 5)] = r[n];
         }
@@ -205,16 +217,16 @@ __device__ __forceinline__ void multiply(u32x4* lds, const Operand& A, const Ope
         for (int f = 0; f < 2; ++f) {
             u32x4 fa[4], fb[2];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) fa[i] = la[((wm + i) * 2 + f) * 64 + lane];
+            for (int i = 0; i < 4; ++i) fa[i] = SA::read(la, wm + i, f, lane);
 #pragma unroll
-            for (int j = 0; j < 2; ++j) fb[j] = lb0[((wn + j) * 2 + f) * 64 + lane];
+            for (int j = 0; j < 2; ++j) fb[j] = SB::read(lb0, wn + j, f, lane);
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
                 for (int j = 0; j < 2; ++j) c0[i][j] = E::mma(fb[j], fa[i], c0[i][j]);
             if constexpr (NB == 2) {
 #pragma unroll
-                for (int j = 0; j < 2; ++j) fb[j] = lb1[((wn + j) * 2 + f) * 64 + lane];
+                for (int j = 0; j < 2; ++j) fb[j] = SB::read(lb1, wn + j, f, lane);
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -227,15 +239,15 @@ __device__ __forceinline__ void multiply(u32x4* lds, const Operand& A, const Ope
 // Four consecutive columns of one row; the row's end cuts them short.
 template <class E>
 __device__ __forceinline__ void put(typename E::T* p, int64_t ld, int row, int col, int rows,
-                                    int cols, bool vec, f32x4 v) {
+                                    int cols, f32x4 v) {
     using T = typename E::T;
     if (row >= rows || col >= cols) return;
     T w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) w[i] = E::down(v[i]);
     T* at = p + (int64_t)row * ld + col;
-    if (vec && col + 4 <= cols) {
-        __builtin_memcpy(__builtin_assume_aligned(at, 4 * sizeof(T)), w, 4 * sizeof(T));
+    if (col + 4 <= cols) {
+        __builtin_memcpy(at, w, 4 * sizeof(T));
     } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -258,7 +270,6 @@ struct Tile {
     int m, n;             // rows of A, rows of B
     void* out[3];
     int64_t ldo;
-    int vec_out;
     int act;
     int64_t split_k;      // depth of a split (WGRAD*)
     int64_t split_out;    // floats of a split's partial sums; 0: out itself, in E
@@ -324,7 +335,7 @@ __global__ __launch_bounds__(kThreads) void k_tile(const Tile q) {
                     float slope;
                     h[e] = activate_any<kExact<E>>(q.act, c0[i][j][e], slope) * c1[i][j][e];
                 }
-                put<E>((T*)q.out[0], q.ldo, row, col, q.m, q.n, q.vec_out, h);
+                put<E>((T*)q.out[0], q.ldo, row, col, q.m, q.n, h);
             } else if constexpr (MODE == BWD_HIDDEN) {
                 f32x4 dg, du, h;
 #pragma unroll
@@ -336,11 +347,11 @@ __global__ __launch_bounds__(kThreads) void k_tile(const Tile q) {
                     du[e] = dh * a;
                     dg[e] = dh * u * slope;
                 }
-                put<E>((T*)q.out[0], q.ldo, row, col, q.m, q.n, q.vec_out, dg);
-                put<E>((T*)q.out[1], q.ldo, row, col, q.m, q.n, q.vec_out, du);
-                put<E>((T*)q.out[2], q.ldo, row, col, q.m, q.n, q.vec_out, h);
+                put<E>((T*)q.out[0], q.ldo, row, col, q.m, q.n, dg);
+                put<E>((T*)q.out[1], q.ldo, row, col, q.m, q.n, du);
+                put<E>((T*)q.out[2], q.ldo, row, col, q.m, q.n, h);
             } else {
-                put<E>((T*)q.out[0], q.ldo, row, col, q.m, q.n, q.vec_out, c0[i][j]);
+                put<E>((T*)q.out[0], q.ldo, row, col, q.m, q.n, c0[i][j]);
             }
         }
 }
@@ -1029,28 +1040,6 @@ Splits splits_of(int64_t rows, int64_t m, int64_t n) {
     return Splits{(int)((rows + depth - 1) / depth), depth};
 }
 
-template <class E>
-Operand operand(const void* p, int64_t ld, int64_t rows, bool kc, int n_rc) {
-    const int64_t a = kc ? 16 : n_rc * (int64_t)sizeof(typename E::T);
-    const bool vec = (uintptr_t)p % a == 0 && ld * (int64_t)sizeof(typename E::T) % a == 0;
-    return Operand{p, ld, (int)rows, vec ? 1 : 0};
-}
-// the first operand's patches are four rows wide, the second's two
-template <class E>
-Operand first(const void* p, int64_t ld, int64_t rows, bool kc) {
-    return operand<E>(p, ld, rows, kc, kBM / 32);
-}
-template <class E>
-Operand second(const void* p, int64_t ld, int64_t rows, bool kc) {
-    return operand<E>(p, ld, rows, kc, kBN / 32);
-}
-
-template <class E>
-bool out_vec(const void* p, int64_t ld) {
-    const int64_t a = 4 * sizeof(typename E::T);
-    return (uintptr_t)p % a == 0 && ld * (int64_t)sizeof(typename E::T) % a == 0;
-}
-
 template <class E, Mode MODE>
 int launch_tile(const Tile& q, int splits, hipStream_t st) {
     const int64_t n = tiles(q.m, q.n);
@@ -1241,26 +1230,24 @@ int forward(const Shape& s, const void* x, int64_t ldx, const void* wg, const vo
     }
     const int64_t ph = pitch(s);
     Tile q{};
-    q.a = first<E>(x, ldx, s.rows, true);
-    q.b0 = second<E>(wg, s.d_in, s.hidden, true);
-    q.b1 = second<E>(wu, s.d_in, s.hidden, true);
+    q.a = Operand{x, ldx, (int)s.rows};
+    q.b0 = Operand{wg, s.d_in, s.hidden};
+    q.b1 = Operand{wu, s.d_in, s.hidden};
     q.k = s.d_in;
     q.m = (int)s.rows;
     q.n = s.hidden;
     q.out[0] = ws;
     q.ldo = ph;
-    q.vec_out = 1;
     q.act = s.act;
     if (int e = launch_tile<E, HIDDEN>(q, 1, st)) return e;
     Tile r{};
-    r.a = first<E>(ws, ph, s.rows, true);
-    r.b0 = second<E>(wd, s.hidden, s.d_out, true);
+    r.a = Operand{ws, ph, (int)s.rows};
+    r.b0 = Operand{wd, s.hidden, s.d_out};
     r.k = s.hidden;
     r.m = (int)s.rows;
     r.n = s.d_out;
     r.out[0] = y;
     r.ldo = ldy;
-    r.vec_out = out_vec<E>(y, ldy);
     return launch_tile<E, PLAIN>(r, 1, st);
 }
 
@@ -1307,12 +1294,12 @@ int backward(const Shape& s, const void* x, int64_t ldx, const void* wg, const v
     void* h = (char*)ws + 2 * hb;
     float* parts = (float*)((char*)ws + 3 * hb);
     Tile q{};
-    q.a = first<E>(x, ldx, s.rows, true);
-    q.b0 = second<E>(wg, s.d_in, s.hidden, true);
-    q.b1 = second<E>(wu, s.d_in, s.hidden, true);
+    q.a = Operand{x, ldx, (int)s.rows};
+    q.b0 = Operand{wg, s.d_in, s.hidden};
+    q.b1 = Operand{wu, s.d_in, s.hidden};
     q.k = s.d_in;
-    q.a2 = first<E>(dy, lddy, s.rows, true);
-    q.b2 = second<E>(wd, s.hidden, s.hidden, false);
+    q.a2 = Operand{dy, lddy, (int)s.rows};
+    q.b2 = Operand{wd, s.hidden, s.hidden};
     q.k2 = s.d_out;
     q.m = (int)s.rows;
     q.n = s.hidden;
@@ -1320,28 +1307,26 @@ int backward(const Shape& s, const void* x, int64_t ldx, const void* wg, const v
     q.out[1] = du;
     q.out[2] = h;
     q.ldo = ph;
-    q.vec_out = 1;
     q.act = s.act;
     if (int e = launch_tile<E, BWD_HIDDEN>(q, 1, st)) return e;
     if (dx) {
         Tile r{};
-        r.a = first<E>(dg, ph, s.rows, true);
-        r.b0 = second<E>(wg, s.d_in, s.d_in, false);
-        r.a2 = first<E>(du, ph, s.rows, true);
-        r.b2 = second<E>(wu, s.d_in, s.d_in, false);
+        r.a = Operand{dg, ph, (int)s.rows};
+        r.b0 = Operand{wg, s.d_in, s.d_in};
+        r.a2 = Operand{du, ph, (int)s.rows};
+        r.b2 = Operand{wu, s.d_in, s.d_in};
         r.k = s.hidden;
         r.m = (int)s.rows;
         r.n = s.d_in;
         r.out[0] = dx;
         r.ldo = s.d_in;
-        r.vec_out = out_vec<E>(dx, s.d_in);
         if (int e = launch_tile<E, SUM2>(r, 1, st)) return e;
     }
     if (dwg) {
         Tile r{};
-        r.a = first<E>(x, ldx, s.d_in, false);
-        r.b0 = second<E>(dg, ph, s.hidden, false);
-        r.b1 = second<E>(du, ph, s.hidden, false);
+        r.a = Operand{x, ldx, s.d_in};
+        r.b0 = Operand{dg, ph, s.hidden};
+        r.b1 = Operand{du, ph, s.hidden};
         r.m = s.d_in;
         r.n = s.hidden;
         void* outs[2] = {dwg, dwu};
@@ -1349,8 +1334,8 @@ int backward(const Shape& s, const void* x, int64_t ldx, const void* wg, const v
     }
     if (dwd) {
         Tile r{};
-        r.a = first<E>(h, ph, s.hidden, false);
-        r.b0 = second<E>(dy, lddy, s.d_out, false);
+        r.a = Operand{h, ph, s.hidden};
+        r.b0 = Operand{dy, lddy, s.d_out};
         r.m = s.hidden;
         r.n = s.d_out;
         void* outs[1] = {dwd};

@@ -85,9 +85,45 @@ struct Operand {
     int rows;
 };
 
+// Rows in shared memory, SLOTS 16-byte slots a row, the slots turned
+// by the row so that no access meets a bank twice.  What the accesses ask for
+// (measured with a counter of conflicts): a 16-byte read serves lanes 0-3, 12-15,
+// 20-27 of a half wave in one clock, then the others, so rows 0-3 and 12-15 of
+// one slot with rows 4-11 of the next; a transposing read 32 lanes, rows r .. r + 3
+// and r + 8 .. r + 11 of two slots; a 16-byte write eight lanes, over half the
+// banks.
+template <int SLOTS>
+__device__ __forceinline__ int tile_slot(int row, int slot) {
+    const int b0 = row & 1, b1 = row >> 1 & 1, b2 = row >> 2 & 1, b3 = row >> 3 & 1;
+    if constexpr (SLOTS == 4) return row * 4 + (slot ^ ((b2 ^ b3) << 1 | (b3 ^ b1)));
+    if constexpr (SLOTS == 8) return row * 8 + (slot ^ (b1 << 1 | b3 << 2));
+    return row * SLOTS + (slot ^ (b0 << 1 | b1 << 2 | b3 << 3));
+}
+// The operand whose rows are a tile's columns c0 .. c0 + 15 and whose summed
+// index are 32 of the tile's rows (16-bit elements).
+template <int SLOTS>
+__device__ __forceinline__ u32x4 read_turned(const u32x4* tile, int c0, int lane) {
+    using v4 = __attribute__((ext_vector_type(4))) short;
+    typedef __attribute__((address_space(3))) v4* lds_v4;
+    const int s = lane & 15, row = 8 * (lane >> 4) + (s >> 2), col = c0 + 4 * (s & 3);
+    union {
+        v4 h[2];
+        u32x4 v;
+    } r;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        char* at = (char*)(tile + tile_slot<SLOTS>(row + 4 * i, col >> 3)) + 8 * ((col >> 2) & 1);
+        r.h[i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4)at);
+    }
+    return r.v;
+}
+
 // ROWS rows times two fragments' depth of one operand, kept in fragment order
 // (row block, fragment, lane), a lane's 16 bytes at a time.  Rows of odd length
 // are read unaligned, which global memory allows at the price of a sector.
+//
+// Where the rows are contiguous instead, 16-bit operands are staged as they lie
+// and turned by the reads; float32 ones are turned in registers by patches.
 //
 // The lanes of a fragment lie so that what a wave reads, and eight lanes of what
 // it stores, meet each bank once: where the summed index is contiguous a wave
@@ -95,6 +131,8 @@ struct Operand {
 // bits of the row are turned (bits 2, 3, 0, 1), odd row blocks half a turn on.
 template <class E, int ROWS, bool KC>
 struct Stage {
+    static constexpr bool TURNED = !KC && E::VEC == 8;
+    static constexpr int SLOTS = ROWS / 8;  // of one summed index, TURNED
     using T = typename E::T;
     static constexpr int VEC = E::VEC;
     static constexpr int STEP = 8 * VEC;  // depth of a stage
@@ -111,6 +149,7 @@ struct Stage {
     }
     // the fragment f of row block b, on this lane
     static __device__ __forceinline__ u32x4 read(const u32x4* lds, int b, int f, int lane) {
+        if constexpr (TURNED) return read_turned<SLOTS>(lds + f * 32 * SLOTS, 16 * b, lane);
         return lds[(b * 2 + f) * 64 + place(b * 16 + (lane & 15), lane >> 4)];
     }
 
@@ -130,6 +169,21 @@ struct Stage {
 #pragma unroll
                     for (int i = 0; i < VEC; ++i)
                         v[i] = (row < o.rows && k + i < k1) ? at[i] : (T)0;
+                    __builtin_memcpy(&r[n], v, 16);
+                }
+            }
+        } else if constexpr (TURNED) {
+            const int row = row0 + t % SLOTS * 8;
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                const int64_t k = k0 + t / SLOTS + n * (kThreads / SLOTS);
+                const T* at = p + k * o.ld + row;
+                if (k < k1 && row + 8 <= o.rows) {
+                    __builtin_memcpy(&r[n], at, 16);
+                } else {
+                    T v[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) v[i] = (k < k1 && row + i < o.rows) ? at[i] : (T)0;
                     __builtin_memcpy(&r[n], v, 16);
                 }
             }
@@ -165,6 +219,8 @@ struct Stage {
         for (int n = 0; n < N; ++n) {
             if constexpr (KC)
                 lds[slot((t >> 7) * 16 + (t & 15) + 32 * n, t >> 4 & 7)] = r[n];
+            else if constexpr (TURNED)
+                lds[tile_slot<SLOTS>(t / SLOTS + n * (kThreads / SLOTS), t % SLOTS)] = r[n];
             else
                 lds[slot((t & 31) * N + n, t >> 5)] = r[n];
         }
@@ -560,43 +616,10 @@ struct NarrowBwd {
     int d_in, hidden, d_out, act;
 };
 
-// A tile of 32 rows in shared memory, SLOTS 16-byte slots a row, the slots turned
-// by the row so that no access meets a bank twice.  What the accesses ask for
-// (measured with a counter of conflicts): a 16-byte read serves lanes 0-3, 12-15,
-// 20-27 of a half wave in one clock, then the others, so rows 0-3 and 12-15 of
-// one slot with rows 4-11 of the next; a transposing read 32 lanes, rows r .. r + 3
-// and r + 8 .. r + 11 of two slots; a 16-byte write eight lanes, over half the
-// banks.
-template <int SLOTS>
-__device__ __forceinline__ int tile_slot(int row, int slot) {
-    const int b0 = row & 1, b1 = row >> 1 & 1, b2 = row >> 2 & 1, b3 = row >> 3 & 1;
-    if constexpr (SLOTS == 4) return row * 4 + (slot ^ ((b2 ^ b3) << 1 | (b3 ^ b1)));
-    if constexpr (SLOTS == 8) return row * 8 + (slot ^ (b1 << 1 | b3 << 2));
-    return row * SLOTS + (slot ^ (b0 << 1 | b1 << 2 | b3 << 3));
-}
 // Rows of float32 sums, written and read along the slots only.
 template <int SLOTS>
 __device__ __forceinline__ int sum_slot(int row, int slot) {
     return row * SLOTS + (slot ^ (row & (SLOTS - 1)));
-}
-
-// The operand whose rows are a tile's columns c0 .. c0 + 15 and whose summed
-// index are the tile's 32 rows.
-template <int SLOTS>
-__device__ __forceinline__ u32x4 read_turned(const u32x4* tile, int c0, int lane) {
-    using v4 = __attribute__((ext_vector_type(4))) short;
-    typedef __attribute__((address_space(3))) v4* lds_v4;
-    const int s = lane & 15, row = 8 * (lane >> 4) + (s >> 2), col = c0 + 4 * (s & 3);
-    union {
-        v4 h[2];
-        u32x4 v;
-    } r;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        char* at = (char*)(tile + tile_slot<SLOTS>(row + 4 * i, col >> 3)) + 8 * ((col >> 2) & 1);
-        r.h[i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4)at);
-    }
-    return r.v;
 }
 
 template <class E, int KD, int KO>

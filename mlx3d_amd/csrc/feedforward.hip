@@ -126,9 +126,10 @@ __device__ __forceinline__ u32x4 read_turned(const u32x4* tile, int c0, int lane
 // and turned by the reads; float32 ones are turned in registers by patches.
 //
 // The lanes of a fragment lie so that what a wave reads, and eight lanes of what
-// it stores, meet each bank once: where the summed index is contiguous a wave
-// stores whole fragments; else its lanes are a few rows apart, and the four low
-// bits of the row are turned (bits 2, 3, 0, 1), odd row blocks half a turn on.
+// it stores, meet each bank once: where the summed index is contiguous eight lanes
+// load and store one row's 128 bytes, and the row's low bits are turned by the
+// piece; else its lanes are a few rows apart, and the four low bits of the row
+// change places (bits 2, 3, 0, 1), odd row blocks half a turn on.
 template <class E, int ROWS, bool KC>
 struct Stage {
     static constexpr bool TURNED = !KC && E::VEC == 8;
@@ -139,28 +140,53 @@ struct Stage {
     static constexpr int N = ROWS / 32;   // 16-byte pieces of a thread
     u32x4 r[N];
 
-    static __device__ __forceinline__ int place(int row, int quad) {
-        const int in = row & 15;
-        return KC ? quad * 16 + in
-                  : quad * 16 + (((in & 3) << 2 | in >> 2) ^ (row >> 4 & 1) << 2);
-    }
     static __device__ __forceinline__ int slot(int row, int piece) {
-        return ((row >> 4) * 2 + (piece >> 2)) * 64 + place(row, piece & 3);
+        const int in = row & 15;
+        const int turned = KC ? in ^ piece : ((in & 3) << 2 | in >> 2) ^ (row >> 4 & 1) << 2;
+        return ((row >> 4) * 2 + (piece >> 2)) * 64 + (piece & 3) * 16 + turned;
     }
     // the fragment f of row block b, on this lane
     static __device__ __forceinline__ u32x4 read(const u32x4* lds, int b, int f, int lane) {
         if constexpr (TURNED) return read_turned<SLOTS>(lds + f * 32 * SLOTS, 16 * b, lane);
-        return lds[(b * 2 + f) * 64 + place(b * 16 + (lane & 15), lane >> 4)];
+        return lds[slot(b * 16 + (lane & 15), f * 4 + (lane >> 4))];
+    }
+
+    // A stage of the summed index [k0, k1).  Not the last one: no bounds, so that
+    // the loads of several stages can be in flight and each waited for alone.
+    // Rows past the operand's then repeat its last one, or hold what follows it:
+    // they only reach outputs that are not stored.
+    __device__ __forceinline__ void load_inner(const Operand& o, int row0, int64_t k0) {
+        const T* p = (const T*)o.p;
+        const int t = threadIdx.x;
+        if constexpr (KC) {
+            const int64_t k = k0 + (t & 7) * VEC;
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                int row = row0 + (t >> 3) + 32 * n;
+                row = row < o.rows ? row : o.rows - 1;
+                __builtin_memcpy(&r[n], p + (int64_t)row * o.ld + k, 16);
+            }
+        } else if constexpr (TURNED) {
+            int row = row0 + t % SLOTS * 8;
+            row = row < o.rows ? row : o.rows - 1;
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                const int64_t k = k0 + t / SLOTS + n * (kThreads / SLOTS);
+                __builtin_memcpy(&r[n], p + k * o.ld + row, 16);
+            }
+        } else {
+            load(o, row0, k0, k0 + STEP);
+        }
     }
 
     __device__ __forceinline__ void load(const Operand& o, int row0, int64_t k0, int64_t k1) {
         const T* p = (const T*)o.p;
         const int t = threadIdx.x;
         if constexpr (KC) {
-            const int64_t k = k0 + (t >> 4 & 7) * VEC;
+            const int64_t k = k0 + (t & 7) * VEC;
 #pragma unroll
             for (int n = 0; n < N; ++n) {
-                const int row = row0 + (t >> 7) * 16 + (t & 15) + 32 * n;
+                const int row = row0 + (t >> 3) + 32 * n;
                 const T* at = p + (int64_t)row * o.ld + k;
                 if (row < o.rows && k + VEC <= k1) {
                     __builtin_memcpy(&r[n], at, 16);
@@ -218,7 +244,7 @@ struct Stage {
 #pragma unroll
         for (int n = 0; n < N; ++n) {
             if constexpr (KC)
-                lds[slot((t >> 7) * 16 + (t & 15) + 32 * n, t >> 4 & 7)] = r[n];
+                lds[slot((t >> 3) + 32 * n, t & 7)] = r[n];
             else if constexpr (TURNED)
                 lds[tile_slot<SLOTS>(t / SLOTS + n * (kThreads / SLOTS), t % SLOTS)] = r[n];
             else
@@ -239,36 +265,48 @@ __device__ __forceinline__ void clear(Acc& c) {
 }
 
 // c0 += A B0^T and (NB == 2) c1 += A B1^T over the summed index [k0, k1).  The
-// next stage's loads are in flight while the present one is multiplied.
+// next two stages' loads are in flight while one is multiplied, and shared memory
+// holds two stages, so one barrier each.
+//
+// Every stage but the last runs without bounds.  A transposed operand's may read
+// up to seven elements past its rows, which the next of the summed index holds if
+// the pitch is eight or more; below, every stage is bounded.
 template <class E, bool AKC, bool BKC, int NB>
 __device__ __forceinline__ void multiply(u32x4* lds, const Operand& A, const Operand& B0,
                                          const Operand& B1, int m0, int n0, int64_t k0, int64_t k1,
                                          Acc& c0, Acc& c1) {
     using SA = Stage<E, kBM, AKC>;
     using SB = Stage<E, kBN, BKC>;
-    u32x4* la = lds;
-    u32x4* lb0 = lds + kBM * 8;
-    u32x4* lb1 = lb0 + kBN * 8;
-    SA a;
-    SB b0, b1;
+    constexpr int STAGE = (kBM + NB * kBN) * 8;
+    SA a[2];
+    SB b0[2], b1[2];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const int wm = (wave >> 1) * 4, wn = (wave & 1) * 2;  // in blocks of 16
-    if (k0 < k1) {
-        a.load(A, m0, k0, k1);
-        b0.load(B0, n0, k0, k1);
-        if constexpr (NB == 2) b1.load(B1, n0, k0, k1);
-    }
-    for (int64_t k = k0; k < k1; k += SA::STEP) {
-        __syncthreads();  // the last stage's reads
-        a.store(la);
-        b0.store(lb0);
-        if constexpr (NB == 2) b1.store(lb1);
-        __syncthreads();
-        if (k + SA::STEP < k1) {
-            a.load(A, m0, k + SA::STEP, k1);
-            b0.load(B0, n0, k + SA::STEP, k1);
-            if constexpr (NB == 2) b1.load(B1, n0, k + SA::STEP, k1);
+    const int steps = (int)((k1 - k0 + SA::STEP - 1) / SA::STEP);
+    const bool inner = (AKC || A.ld >= 8) && (BKC || (B0.ld >= 8 && B1.ld >= 8));
+    auto load = [&](int step, int i) {
+        if (step >= steps) return;
+        const int64_t k = k0 + (int64_t)step * SA::STEP;
+        if (step + 1 < steps && inner) {
+            a[i].load_inner(A, m0, k);
+            b0[i].load_inner(B0, n0, k);
+            if constexpr (NB == 2) b1[i].load_inner(B1, n0, k);
+        } else {
+            const int64_t stop = k + SA::STEP < k1 ? k + SA::STEP : k1;
+            a[i].load(A, m0, k, stop);
+            b0[i].load(B0, n0, k, stop);
+            if constexpr (NB == 2) b1[i].load(B1, n0, k, stop);
         }
+    };
+    auto step = [&](int s, int i) {
+        u32x4* la = lds + i * STAGE;
+        u32x4* lb0 = la + kBM * 8;
+        u32x4* lb1 = lb0 + kBN * 8;
+        a[i].store(la);
+        b0[i].store(lb0);
+        if constexpr (NB == 2) b1[i].store(lb1);
+        __syncthreads();
+        load(s + 2, i);
 #pragma unroll
         for (int f = 0; f < 2; ++f) {
             u32x4 fa[4], fb[2];
@@ -289,6 +327,13 @@ __device__ __forceinline__ void multiply(u32x4* lds, const Operand& A, const Ope
                     for (int j = 0; j < 2; ++j) c1[i][j] = E::mma(fb[j], fa[i], c1[i][j]);
             }
         }
+    };
+    __syncthreads();  // an earlier product's reads
+    load(0, 0);
+    load(1, 1);
+    for (int s = 0; s < steps; s += 2) {
+        step(s, 0);
+        if (s + 1 < steps) step(s + 1, 1);
     }
 }
 
@@ -332,10 +377,11 @@ struct Tile {
 };
 
 template <class E, Mode MODE>
-__global__ __launch_bounds__(kThreads) void k_tile(const Tile q) {
+__global__ __launch_bounds__(kThreads, 2) void k_tile(const Tile q) {
     using T = typename E::T;
-    __shared__ u32x4 lds[(kBM + 2 * kBN) * 8];
     constexpr bool wgrad = MODE == WGRAD || MODE == WGRAD2;
+    constexpr bool dual = MODE == HIDDEN || MODE == BWD_HIDDEN || MODE == WGRAD2;
+    __shared__ u32x4 lds[2 * (kBM + (dual ? 2 : 1) * kBN) * 8];
     const int tiles_n = (q.n + kBN - 1) / kBN;
     const uint32_t id = xcd_remap(blockIdx.x, gridDim.x);
     const int m0 = (int)(id / tiles_n) * kBM, n0 = (int)(id % tiles_n) * kBN;
@@ -1048,14 +1094,15 @@ int check_shape(const Shape& s) {
 // Workgroups of one product; the grid's x holds all of them.
 int64_t tiles(int64_t m, int64_t n) { return up_to(m, kBM) / kBM * (up_to(n, kBN) / kBN); }
 
-// Splits of the rows for a weight gradient of m x n: enough workgroups for
-// twice the 256 compute units, no split under eight stages of 64 rows.
+// Splits of the rows for a weight gradient of m x n: workgroups for twice the 256
+// compute units, which hold two each (a few more would run as a second round),
+// no split under eight stages of 64 rows.
 struct Splits {
     int count;
     int64_t depth;
 };
 Splits splits_of(int64_t rows, int64_t m, int64_t n) {
-    int64_t want = (512 + tiles(m, n) - 1) / tiles(m, n);
+    int64_t want = 512 / tiles(m, n);
     const int64_t most = (rows + 511) / 512;
     if (want > most) want = most;
     if (want < 1) want = 1;

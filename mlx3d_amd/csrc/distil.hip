@@ -653,12 +653,15 @@ __global__ __launch_bounds__(64) void k_seg_join(const Distil q) {
         e.s[i] = e.index[i] >= 0 ? E::up(src[e.index[i]]) : 0.f;
     }
     __syncthreads();
+    bool shared = false;
 #pragma unroll
     for (int i = 0; i < KPL; ++i) {
         e.again[i] = false;
         if (e.index[i] >= 0)
             for (int k = 0; k < lane + i * 64; ++k) e.again[i] |= ei[k] == e.index[i];
+        shared |= e.again[i];
     }
+    shared = __any(shared);
     const float c = kLog2e * q.inv_temp;
     const float* parts = q.seg_parts + row * q.segs * 2;
     float m = -INFINITY, s = 0.f;
@@ -681,6 +684,7 @@ __global__ __launch_bounds__(64) void k_seg_join(const Distil q) {
         st[2] = r.mc;
         st[3] = r.inv;
         st[4] = r.active ? 1.f : 0.f;
+        st[5] = shared ? 1.f : 0.f;
     }
     // the entries' probabilities, for the gradient
     float* probs = q.stats + q.rows * 8 + row * q.top;
@@ -695,19 +699,46 @@ __global__ __launch_bounds__(kThreads) void k_seg_grad(const Distil q) {
     using T = typename E::T;
     __shared__ u32x4 smem[kSegBytes / 16 + 1];
     __shared__ int scratch[kThreads / 64];
+    __shared__ int ei[GSX_DISTIL_MAX_TOP];
+    __shared__ float ep[GSX_DISTIL_MAX_TOP];
     const int64_t row = blockIdx.x / q.segs;
     const int seg = (int)(blockIdx.x % q.segs);
     const int j0 = seg * q.seg, n = q.vocab - j0 < q.seg ? q.vocab - j0 : q.seg;
     const T* src = (const T*)q.logits + row * q.stride + j0;
     T* dst = (T*)q.grad + row * q.vocab + j0;
     T* tile = (T*)smem + ((uintptr_t)src % 16) / sizeof(T);
-    const float inv_count = inverse_count(q, scratch);
     const float* st = q.stats + row * 8;
-    const bool active = st[4] != 0.f;
+    const bool active = st[4] != 0.f, shared = st[5] != 0.f;
+    if (active) {
+        copy_flat<kThreads>(tile, src, n, threadIdx.x);
+        const float* probs = q.stats + q.rows * 8 + row * q.top;
+        for (int k = threadIdx.x; k < q.top; k += kThreads) {
+            ei[k] = entry(q, row, k).index;
+            ep[k] = probs[k];
+        }
+    }
+    const float inv_count = inverse_count(q, scratch);
     const float f = row_scale(q, row, inv_count);
     const float c = kLog2e * q.inv_temp;
     const float rest_mc = c * st[0], rest = st[1] * f;
-    if (active) copy_flat<kThreads>(tile, src, n, threadIdx.x);
+    __syncthreads();
+    // this thread's entry of this segment (there are no more entries than threads)
+    float own = 0.f;
+    int at = -1;
+    if (active && threadIdx.x < q.top) {
+        const int i = ei[threadIdx.x] - j0;
+        if (ei[threadIdx.x] >= 0 && i >= 0 && i < n) {
+            at = i;
+            float p = ep[threadIdx.x];
+            if (shared) {
+                p = 0.f;
+                for (int j = 0; j < q.top; ++j)
+                    if (ei[j] == i + j0) p += ep[j];
+            }
+            const float s = E::up(tile[i]);
+            own = f * ((s == -INFINITY ? 0.f : expo(s, st[2], c)) * st[3] - p);
+        }
+    }
     __syncthreads();
     for (int j = threadIdx.x; j < n; j += kThreads) {
         float g = 0.f;
@@ -718,25 +749,14 @@ __global__ __launch_bounds__(kThreads) void k_seg_grad(const Distil q) {
         tile[j] = E::down(g);
     }
     __syncthreads();
-    if (active) {
-        const float* probs = q.stats + q.rows * 8 + row * q.top;
-        for (int k = threadIdx.x; k < q.top; k += kThreads) {
-            const int i = entry(q, row, k).index;
-            if (i < j0 || i >= j0 + n) continue;
-            float p = 0.f;
-            for (int j = 0; j < q.top; ++j)
-                if (entry(q, row, j).index == i) p += probs[j];
-            const float s = E::up(src[i - j0]);
-            const float e = s == -INFINITY ? 0.f : expo(s, st[2], c);
-            tile[i - j0] = E::down(f * (e * st[3] - p));
-        }
-    }
+    if (at >= 0) tile[at] = E::down(own);
     __syncthreads();
     if (((uintptr_t)dst - (uintptr_t)src) % 16 == 0)
         copy_flat<kThreads>(dst, (const T*)tile, n, threadIdx.x);
     else
         for (int i = threadIdx.x; i < n; i += kThreads) dst[i] = tile[i];
 }
+static_assert(GSX_DISTIL_MAX_TOP <= kThreads, "an entry for each thread");
 
 // Rows that have an entry, a count for each of kCountParts workgroups.  Most
 // rows show one in their first entry: four rows' are in flight at a time.
@@ -751,8 +771,15 @@ __global__ __launch_bounds__(1024) void k_count(const Distil q, int* counts) {
             found[i] = row + i * step < q.rows && entry(q, row + i * step, 0).index >= 0;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            for (int k = 1; k < q.top && !found[i] && row + i * step < q.rows; ++k)
-                found[i] = entry(q, row + i * step, k).index >= 0;
+            // otherwise eight entries at a time
+            for (int k = 1; k < q.top && !found[i] && row + i * step < q.rows; k += 8) {
+                RawEntry e[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    e[j] = raw_entry(q, row + i * step, k + j < q.top ? k + j : 0);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) found[i] |= checked(q, e[j]).index >= 0;
+            }
             n += found[i];
         }
     }

@@ -362,7 +362,7 @@ enum Mode {
     BWD_HIDDEN,  // g, u as in HIDDEN, dh = A2 B2^T: out0 = dg, out1 = du, out2 = h
     SUM2,        // out0 = A B0^T + A2 B2^T
     WGRAD2,      // out0^T = A B0^T, out1^T = A B1^T over a split of the summed index
-    WGRAD        // out0^T = A B0^T over a split
+    WGRAD        // out0 = A B0^T over a split
 };
 
 struct Tile {
@@ -379,7 +379,6 @@ struct Tile {
 template <class E, Mode MODE>
 __global__ __launch_bounds__(kThreads, 2) void k_tile(const Tile q) {
     using T = typename E::T;
-    constexpr bool wgrad = MODE == WGRAD || MODE == WGRAD2;
     constexpr bool dual = MODE == HIDDEN || MODE == BWD_HIDDEN || MODE == WGRAD2;
     __shared__ u32x4 lds[2 * (kBM + (dual ? 2 : 1) * kBN) * 8];
     const int tiles_n = (q.n + kBN - 1) / kBN;
@@ -414,8 +413,8 @@ __global__ __launch_bounds__(kThreads, 2) void k_tile(const Tile q) {
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             const int row = row0 + 16 * i, col = col0 + 16 * j;
-            if constexpr (wgrad) {
-                // the gradients lie (B row, A row): lanes run along A's
+            if constexpr (MODE == WGRAD2) {
+                // these gradients lie (B row, A row): lanes run along A's
                 if (row >= q.m) continue;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
@@ -424,12 +423,18 @@ __global__ __launch_bounds__(kThreads, 2) void k_tile(const Tile q) {
                     if (q.split_out) {
                         const int64_t s = blockIdx.y * q.split_out;
                         ((float*)q.out[0])[s + at] = c0[i][j][e];
-                        if constexpr (MODE == WGRAD2) ((float*)q.out[1])[s + at] = c1[i][j][e];
+                        ((float*)q.out[1])[s + at] = c1[i][j][e];
                     } else {
                         ((T*)q.out[0])[at] = E::down(c0[i][j][e]);
-                        if constexpr (MODE == WGRAD2) ((T*)q.out[1])[at] = E::down(c1[i][j][e]);
+                        ((T*)q.out[1])[at] = E::down(c1[i][j][e]);
                     }
                 }
+            } else if constexpr (MODE == WGRAD) {
+                if (q.split_out)
+                    put<F32>((float*)q.out[0] + blockIdx.y * q.split_out, q.ldo, row, col, q.m,
+                             q.n, c0[i][j]);
+                else
+                    put<E>((T*)q.out[0], q.ldo, row, col, q.m, q.n, c0[i][j]);
             } else if constexpr (MODE == HIDDEN) {
                 f32x4 h;
 #pragma unroll
@@ -1188,7 +1193,7 @@ int narrow_forward(const Shape& s, A... a) {
 }
 
 int64_t parts_bytes(const Shape& s) {
-    const Splits a = splits_of(s.rows, s.d_in, s.hidden), b = splits_of(s.rows, s.hidden, s.d_out);
+    const Splits a = splits_of(s.rows, s.d_in, s.hidden), b = splits_of(s.rows, s.d_out, s.hidden);
     const int64_t in = 2 * a.count * (int64_t)s.hidden * s.d_in;
     const int64_t out = b.count * (int64_t)s.d_out * s.hidden;
     return up_to((in > out ? in : out) * 4, 256);
@@ -1330,7 +1335,7 @@ int weight_grad(const Tile& base, int64_t rows, void* const* outs, int count, fl
     q.k = rows;
     q.split_k = sp.depth;
     q.split_out = sp.count > 1 ? n : 0;
-    q.ldo = base.m;
+    q.ldo = count == 2 ? base.m : base.n;
     for (int i = 0; i < count; ++i)
         q.out[i] = sp.count > 1 ? (void*)(parts + i * sp.count * n) : outs[i];
     const int e = count == 2 ? launch_tile<E, WGRAD2>(q, sp.count, st)
@@ -1404,10 +1409,10 @@ int backward(const Shape& s, const void* x, int64_t ldx, const void* wg, const v
     }
     if (dwd) {
         Tile r{};
-        r.a = Operand{h, ph, s.hidden};
-        r.b0 = Operand{dy, lddy, s.d_out};
-        r.m = s.hidden;
-        r.n = s.d_out;
+        r.a = Operand{dy, lddy, s.d_out};
+        r.b0 = Operand{h, ph, s.hidden};
+        r.m = s.d_out;
+        r.n = s.hidden;
         void* outs[1] = {dwd};
         if (int e = weight_grad<E>(r, s.rows, outs, 1, parts, st)) return e;
     }

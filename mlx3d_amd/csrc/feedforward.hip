@@ -18,6 +18,7 @@
 #include <hip/hip_runtime.h>
 
 #include <cmath>
+#include <type_traits>
 
 #include "gsx.h"
 #include "gsx_device.h"
@@ -284,21 +285,21 @@ __device__ __forceinline__ void multiply(u32x4* lds, const Operand& A, const Ope
     const int wm = (wave >> 1) * 4, wn = (wave & 1) * 2;  // in blocks of 16
     const int steps = (int)((k1 - k0 + SA::STEP - 1) / SA::STEP);
     const bool inner = (AKC || A.ld >= 8) && (BKC || (B0.ld >= 8 && B1.ld >= 8));
+    auto load_inner = [&](int step, int i) {
+        const int64_t k = k0 + (int64_t)step * SA::STEP;
+        a[i].load_inner(A, m0, k);
+        b0[i].load_inner(B0, n0, k);
+        if constexpr (NB == 2) b1[i].load_inner(B1, n0, k);
+    };
     auto load = [&](int step, int i) {
         if (step >= steps) return;
         const int64_t k = k0 + (int64_t)step * SA::STEP;
-        if (step + 1 < steps && inner) {
-            a[i].load_inner(A, m0, k);
-            b0[i].load_inner(B0, n0, k);
-            if constexpr (NB == 2) b1[i].load_inner(B1, n0, k);
-        } else {
-            const int64_t stop = k + SA::STEP < k1 ? k + SA::STEP : k1;
-            a[i].load(A, m0, k, stop);
-            b0[i].load(B0, n0, k, stop);
-            if constexpr (NB == 2) b1[i].load(B1, n0, k, stop);
-        }
+        const int64_t stop = k + SA::STEP < k1 ? k + SA::STEP : k1;
+        a[i].load(A, m0, k, stop);
+        b0[i].load(B0, n0, k, stop);
+        if constexpr (NB == 2) b1[i].load(B1, n0, k, stop);
     };
-    auto step = [&](int s, int i) {
+    auto step = [&](int s, int i, auto is_inner) {
         u32x4* la = lds + i * STAGE;
         u32x4* lb0 = la + kBM * 8;
         u32x4* lb1 = lb0 + kBN * 8;
@@ -306,7 +307,10 @@ __device__ __forceinline__ void multiply(u32x4* lds, const Operand& A, const Ope
         b0[i].store(lb0);
         if constexpr (NB == 2) b1[i].store(lb1);
         __syncthreads();
-        load(s + 2, i);
+        if constexpr (is_inner)
+            load_inner(s + 2, i);
+        else
+            load(s + 2, i);
 #pragma unroll
         for (int f = 0; f < 2; ++f) {
             u32x4 fa[4], fb[2];
@@ -329,11 +333,22 @@ __device__ __forceinline__ void multiply(u32x4* lds, const Operand& A, const Ope
         }
     };
     __syncthreads();  // an earlier product's reads
-    load(0, 0);
-    load(1, 1);
-    for (int s = 0; s < steps; s += 2) {
-        step(s, 0);
-        if (s + 1 < steps) step(s + 1, 1);
+    int s = 0;
+    if (inner && steps > 4) {
+        // a loop of its own, so that its waits count on every load being there
+        load_inner(0, 0);
+        load_inner(1, 1);
+        for (; s + 4 < steps; s += 2) {
+            step(s, 0, std::true_type{});
+            step(s + 1, 1, std::true_type{});
+        }
+    } else {
+        load(0, 0);
+        load(1, 1);
+    }
+    for (; s < steps; s += 2) {
+        step(s, 0, std::false_type{});
+        if (s + 1 < steps) step(s + 1, 1, std::false_type{});
     }
 }
 
@@ -377,7 +392,7 @@ struct Tile {
 };
 
 template <class E, Mode MODE>
-__global__ __launch_bounds__(kThreads, 2) void k_tile(const Tile q) {
+__global__ __launch_bounds__(kThreads, kExact<E> ? 1 : 2) void k_tile(const Tile q) {
     using T = typename E::T;
     constexpr bool dual = MODE == HIDDEN || MODE == BWD_HIDDEN || MODE == WGRAD2;
     __shared__ u32x4 lds[2 * (kBM + (dual ? 2 : 1) * kBN) * 8];

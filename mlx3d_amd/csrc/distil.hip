@@ -57,8 +57,11 @@ struct Distil {
     void* grad;              // or NULL
     const float* upstream;   // one for each row, or one, or NULL (scale alone)
     int upstream_rows;
-    const int* counts;       // kCountParts counts of supervised rows (mean), or NULL
+    const int* counts;       // kCountParts counts of supervised rows
     float scale;
+    int mean;
+    int alone;               // one workgroup walks all rows, and counts them itself
+    float* total;            // ... and their sum or mean goes here, or NULL
     float* seg_parts;        // longer rows: (rows, segments, 2) maximum and sum
     float* stats;            // longer rows: (rows, 8)
     int seg, segs;
@@ -281,10 +284,30 @@ __device__ __forceinline__ float row_scale(const Distil& q, int64_t row, float i
     return s;
 }
 
-// 1 / supervised rows (1 where nothing asks for the mean), from the count's parts.
+// Whether a row has an entry: most rows show one in their first, otherwise eight
+// are in flight at a time.
+__device__ __forceinline__ int supervised(const Distil& q, int64_t row) {
+    int found = entry(q, row, 0).index >= 0;
+    for (int k = 1; k < q.top && !found; k += 8) {
+        RawEntry e[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) e[j] = raw_entry(q, row, k + j < q.top ? k + j : 0);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) found |= checked(q, e[j]).index >= 0;
+    }
+    return found;
+}
+
+// 1 / supervised rows (1 where nothing asks for the mean), from the count's parts,
+// or by the one workgroup that there is.
 __device__ __forceinline__ float inverse_count(const Distil& q, int* scratch) {
-    if (!q.counts) return 1.f;
-    int v = threadIdx.x < kCountParts ? q.counts[threadIdx.x] : 0;
+    if (!q.mean) return 1.f;
+    int v = 0;
+    if (q.alone) {
+        for (int64_t row = threadIdx.x; row < q.rows; row += kThreads) v += supervised(q, row);
+    } else {
+        v = threadIdx.x < kCountParts ? q.counts[threadIdx.x] : 0;
+    }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, kWave);
     if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = v;
@@ -398,7 +421,7 @@ __global__ __launch_bounds__(kThreads, N > 14 ? 2 : KPL > 1 ? 3 : 4) void k_rows
     // index and probability of the row's entries, where some name one column
     int* ei = (int*)((char*)smem + kWaves * room) + (wave * R + sub) * q.top;
     float* ep = (float*)ei + kWaves * R * q.top;
-    const float inv_count = q.grad ? inverse_count(q, scratch) : 1.f;
+    const float inv_count = q.grad || q.total ? inverse_count(q, scratch) : 1.f;
     const float c = kLog2e * q.inv_temp;
     double group_loss = 0.0;
 
@@ -575,7 +598,7 @@ __global__ __launch_bounds__(kThreads, N > 14 ? 2 : KPL > 1 ? 3 : 4) void k_rows
         }
         wave_fence();  // the tile is read before the next one is stored
     }
-    if (!q.loss_parts) return;
+    if (!q.loss_parts && !q.total) return;
 #pragma unroll
     for (int o = G; o < 64; o *= 2) group_loss += __shfl_xor(group_loss, o, kWave);
     if (l64 == 0) sums[wave] = group_loss;
@@ -583,7 +606,10 @@ __global__ __launch_bounds__(kThreads, N > 14 ? 2 : KPL > 1 ? 3 : 4) void k_rows
     if (threadIdx.x == 0) {
         double s = 0.0;
         for (int i = 0; i < kWaves; ++i) s += sums[i];
-        q.loss_parts[blockIdx.x] = s;
+        if (q.total)
+            *q.total = (float)(s * (double)q.scale * (double)inv_count);
+        else
+            q.loss_parts[blockIdx.x] = s;
     }
 }
 
@@ -758,8 +784,8 @@ __global__ __launch_bounds__(kThreads) void k_seg_grad(const Distil q) {
 }
 static_assert(GSX_DISTIL_MAX_TOP <= kThreads, "an entry for each thread");
 
-// Rows that have an entry, a count for each of kCountParts workgroups.  Most
-// rows show one in their first entry: four rows' are in flight at a time.
+// Rows that have an entry, a count for each of kCountParts workgroups; four rows
+// of a thread are in flight at a time.
 __global__ __launch_bounds__(1024) void k_count(const Distil q, int* counts) {
     __shared__ int red[1024 / 64];
     constexpr int64_t step = (int64_t)kCountParts * 1024;
@@ -770,18 +796,8 @@ __global__ __launch_bounds__(1024) void k_count(const Distil q, int* counts) {
         for (int i = 0; i < 4; ++i)
             found[i] = row + i * step < q.rows && entry(q, row + i * step, 0).index >= 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            // otherwise eight entries at a time
-            for (int k = 1; k < q.top && !found[i] && row + i * step < q.rows; k += 8) {
-                RawEntry e[8];
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    e[j] = raw_entry(q, row + i * step, k + j < q.top ? k + j : 0);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) found[i] |= checked(q, e[j]).index >= 0;
-            }
-            n += found[i];
-        }
+        for (int i = 0; i < 4; ++i)
+            n += found[i] || (row + i * step < q.rows && supervised(q, row + i * step));
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o, kWave);
@@ -854,6 +870,10 @@ int lanes_for(int dtype, int64_t vocab, int64_t top) {
     while (g < 64 && (g * kHeld < words_of(dtype, vocab) || g * 4 < top)) g *= 2;
     return g;
 }
+// Workgroups' worth of tiles that one walks alone, with the count and the sum in
+// its one launch: a patch of 64 rows takes 18 us a call instead of 23, whose three
+// launches take longer than their work.
+constexpr int64_t kAlone = 4;
 constexpr int64_t kRowGroups = 2048;  // workgroups that walk the tiles: eight for a unit
 
 // The workspace: the count's parts, the workgroups' losses, then for longer
@@ -890,7 +910,10 @@ int launch_rows(const Distil& q, hipStream_t st) {
                                   (int64_t)R * q.top * 8);
     if (lds > 64 * 1024) return GSX_ERR_TOO_LARGE;
     hipLaunchKernelGGL((k_rows<E, G, N, KPL, LOG_PROBS, FULL>),
-                       dim3((unsigned)(groups < kRowGroups ? groups : kRowGroups)), dim3(kThreads),
+                       dim3(q.alone                ? 1u
+                            : groups < kRowGroups ? (unsigned)groups
+                                                  : (unsigned)kRowGroups),
+                       dim3(kThreads),
                        (unsigned)lds, st, q, tiles);
     GSX_LAUNCH_CHECK();
     return GSX_OK;
@@ -1020,7 +1043,9 @@ Distil problem(const Args& a, const Layout& l) {
     q.log_probs = a.teacher == GSX_TEACHER_LOG_PROBS;
     q.scale = 1.0f;
     char* ws = (char*)a.workspace;
-    q.counts = a.reduction == GSX_REDUCE_MEAN ? (const int*)ws : nullptr;
+    q.counts = (const int*)ws;
+    q.mean = a.reduction == GSX_REDUCE_MEAN;
+    q.alone = a.rows > 0 && l.n_segs == 0 && l.n_parts <= kAlone;
     q.seg_parts = (float*)(ws + l.segs);
     q.stats = (float*)(ws + l.stats);
     q.seg = l.seg;
@@ -1038,6 +1063,10 @@ int forward(const Args& a, float scale, float* loss, void* grad, void* stream) {
     q.scale = scale;
     q.grad = grad;
     double* parts = (double*)((char*)a.workspace + l.parts);
+    if (q.alone && a.reduction != GSX_REDUCE_NONE) {
+        q.total = loss;
+        return run_any(a.dtype, q, true, st);
+    }
     if (a.reduction == GSX_REDUCE_NONE)
         q.loss_rows = loss;
     else
@@ -1051,7 +1080,7 @@ int forward(const Args& a, float scale, float* loss, void* grad, void* stream) {
         if (int e = run_any(a.dtype, q, true, st)) return e;
     if (a.reduction != GSX_REDUCE_NONE) {
         hipLaunchKernelGGL(k_total, dim3(1), dim3(kThreads), 0, st, parts,
-                           a.rows > 0 ? l.n_parts : 0, q.counts, scale, loss);
+                           a.rows > 0 ? l.n_parts : 0, q.mean ? q.counts : nullptr, scale, loss);
         GSX_LAUNCH_CHECK();
     }
     return GSX_OK;

@@ -1154,9 +1154,19 @@ int narrow_kd(const Shape& s) { return s.d_in <= 32 ? 1 : s.d_in <= 64 ? 2 : 4; 
 int narrow_ob(const Shape& s) {
     return s.d_out <= 16 ? 1 : s.d_out <= 32 ? 2 : s.d_out <= 64 ? 4 : s.d_out <= 128 ? 8 : 16;
 }
+// Weights that shared memory holds whole are staged once; others by every
+// workgroup for every 256 rows, which many rows have to pay for.  Against the
+// tiled path, us a call (131 072, 16 384, 64 rows): 32 -> 128 -> 64 float32, held
+// whole, 32 / 85, 19 / 22, 19 / 22; 128 -> 1024 -> 64 float32 419 / 904, 202 / 144,
+// 191 / 58; 128 -> 512 -> 64 bf16 74 / 113, 34 / 23, 30 / 22.
+constexpr int64_t kStreamRows = 32768;
+
 bool narrow_fwd(const Shape& s) {
-    return s.d_in <= 128 && s.d_out <= 256 &&
-           narrow_fits(s.dtype == GSX_F32 ? 3 : 1, narrow_kd(s), narrow_ob(s));
+    if (s.d_in > 128 || s.d_out > 256) return false;
+    const int kd = narrow_kd(s), ob = narrow_ob(s);
+    if (!narrow_fits(s.dtype == GSX_F32 ? 3 : 1, kd, ob)) return false;
+    return (s.hidden + 31) / 32 * narrow_chunk_bytes(s, kd, ob) <= kNarrowLds ||
+           s.rows >= kStreamRows;
 }
 
 int64_t fwd_bytes(const Shape& s) {
@@ -1217,11 +1227,16 @@ int64_t parts_bytes(const Shape& s) {
 // The narrow backward: which widths fit its registers (weights in both orders
 // and their gradients' sums), its workgroups and its workspace.
 constexpr bool narrow_bwd_fits(int pieces, int kd, int ko) {
-    return pieces == 3 ? kd + ko <= 3 : kd < 4 || ko == 1;
+    return pieces == 3 ? kd + ko <= 3 : kd < 4 || ko <= 2;
 }
+// Faster than the tiled path wherever its registers hold the widths, us a call
+// (131 072 and 64 rows): 32 -> 128 -> 64 float32 81 / 586 and 57 / 102 (the host's
+// time), 32 -> 512 -> 64, four groups, 264 / 1592, bf16 108 / 465; hidden widths
+// are bounded by the groups' parts of dx, a float32 array of x's size each.
+constexpr int kNarrowHidden = 2048;
 int narrow_ko(const Shape& s) { return s.d_out <= 32 ? 1 : s.d_out <= 64 ? 2 : 4; }
 bool narrow_bwd(const Shape& s) {
-    return s.d_in <= 128 && s.d_out <= 128 && s.hidden <= 512 &&
+    return s.d_in <= 128 && s.d_out <= 128 && s.hidden <= kNarrowHidden &&
            narrow_bwd_fits(s.dtype == GSX_F32 ? 3 : 1, narrow_kd(s), narrow_ko(s));
 }
 struct BwdPlan {

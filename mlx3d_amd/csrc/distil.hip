@@ -408,7 +408,7 @@ __host__ __device__ inline int64_t tile_room(int rows, int words, int64_t vocab,
 // follow each other in a wave, and four waves of a SIMD do not cover all of it; six
 // spill.  Stores held back behind the next tile's loads took 7 us more.
 template <class E, int G, int N, int KPL, bool LOG_PROBS, int FULL>
-__global__ __launch_bounds__(kThreads, N > 14 ? 2 : KPL > 1 ? 3 : 4) void k_rows(const Distil q,
+__global__ __launch_bounds__(kThreads, N > 14 ? 2 : KPL > 2 ? 3 : 4) void k_rows(const Distil q,
                                                                                int64_t tiles) {
     using T = typename E::T;
     constexpr int R = 64 / G;
@@ -942,11 +942,23 @@ int launch_rows(const Distil& q, hipStream_t st) {
                        : launch_rows<E, G, N, KPL, false, FULL>(q, st);
 }
 
-// The kernel whose lanes hold the row's words with the least room to spare
-// (fewer to choose from where a lane has several entries).
+// The kernel whose lanes hold the row's words and entries with the least room to
+// spare (fewer to choose from where a lane has several entries).  307 039 rows of
+// 21 float16 logits and 5 entries, loss or gradient alone: 20 us with room for two
+// entries and three words, 24 with four and six.
 template <class E, int G>
 int launch_rows(const Distil& q, int words, hipStream_t st) {
     const int n = (words + G - 1) / G;
+    if (q.top > G && q.top <= 2 * G) {
+        if constexpr (G == 4) {
+            if (n <= 3) return launch_rows<E, G, 3, 2, 0>(q, st);
+        }
+        if (n <= 6) return launch_rows<E, G, 6, 2, 0>(q, st);
+        if constexpr (G == 64) {
+            if (n > 14) return launch_rows<E, G, 33, 2, 15>(q, st);
+        }
+        return launch_rows<E, G, 14, 2, 7>(q, st);
+    }
     if (q.top > G) {
         if (n <= 6) return launch_rows<E, G, 6, 4, 0>(q, st);
         if constexpr (G == 64) {

@@ -137,6 +137,14 @@ def test_against_64_bits(size, teacher, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("teacher", TEACHERS)
+@pytest.mark.parametrize("size", [(33, 11, 5), (50, 23, 8), (7, 41, 6), (70, 110, 13), (9, 300, 30),
+                                  (5, 800, 70), (3, 2037, 128)], ids=str)
+def test_two_entries_a_lane(size, teacher, dtype):
+    test_against_64_bits(size, teacher, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
 @pytest.mark.parametrize("vocab", [30, 5000])
 @pytest.mark.parametrize("teacher", TEACHERS)
 def test_masked_columns_and_rows(vocab, dtype, teacher):

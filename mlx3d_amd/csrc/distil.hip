@@ -859,17 +859,25 @@ __global__ __launch_bounds__(kThreads) void k_total(const double* parts, int64_t
 
 int64_t up_to(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
 
+int elem(int dtype) { return dtype == GSX_F32 ? 4 : 2; }
+bool short_rows(int dtype, int64_t vocab) { return vocab * elem(dtype) <= kRowBytes; }
+int segments(int dtype, int64_t vocab) {
+    const int64_t seg = kSegBytes / elem(dtype);
+    return (int)((vocab + seg - 1) / seg);
+}
+
 int check_shape(int dtype, int64_t rows, int64_t vocab, int64_t top) {
     if (dtype != GSX_F32 && dtype != GSX_BF16 && dtype != GSX_F16) return GSX_ERR_INVALID;
     if (rows < 0 || vocab <= 0 || top <= 0) return GSX_ERR_INVALID;
     if (top > vocab) return GSX_ERR_INVALID;
     if (rows >= (1LL << 30) || vocab >= (1LL << 30) || top > GSX_DISTIL_MAX_TOP)
         return GSX_ERR_TOO_LARGE;
+    // a launch holds fewer than 2^32 threads in all, a workgroup for each segment
+    if (!short_rows(dtype, vocab) &&
+        rows * segments(dtype, vocab) >= (1LL << 32) / kThreads)
+        return GSX_ERR_TOO_LARGE;
     return GSX_OK;
 }
-
-int elem(int dtype) { return dtype == GSX_F32 ? 4 : 2; }
-bool short_rows(int dtype, int64_t vocab) { return vocab * elem(dtype) <= kRowBytes; }
 
 // 32-bit words that a row may touch (a 16-bit row may begin inside one), and
 // the lanes that hold them: up to kHeld words each (more leave a SIMD two waves
@@ -908,7 +916,7 @@ Layout layout(int dtype, int64_t rows, int64_t vocab, int64_t top) {
         return l;
     }
     l.seg = kSegBytes / elem(dtype);
-    l.n_segs = (int)((vocab + l.seg - 1) / l.seg);
+    l.n_segs = segments(dtype, vocab);
     l.n_parts = rows;
     l.segs = up_to(l.parts + l.n_parts * 8, 256);
     l.stats = up_to(l.segs + rows * l.n_segs * 8, 256);
@@ -998,7 +1006,6 @@ template <class E>
 int run(const Distil& q, bool sums, hipStream_t st) {
     if (q.segs == 0) return run_rows<E>(q, st);
     const int64_t blocks = q.rows * q.segs;
-    if (blocks >= (1LL << 31)) return GSX_ERR_TOO_LARGE;
     if (sums) {
         hipLaunchKernelGGL((k_seg_sum<E>), dim3((unsigned)blocks), dim3(kThreads), 0, st, q);
         GSX_LAUNCH_CHECK();

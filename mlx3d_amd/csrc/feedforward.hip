@@ -489,16 +489,17 @@ __global__ __launch_bounds__(kThreads, kExact<E> ? 1 : 2) void k_tile(const Tile
 template <class E>
 __global__ __launch_bounds__(kThreads) void k_join(const float* parts, int64_t n, int splits,
                                                    typename E::T* out) {
-    const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-    if (i >= n) return;
-    float s = 0.f;
-    for (int k = 0; k < splits; ++k) s += parts[k * n + i];
-    out[i] = E::down(s);
+    const int64_t step = (int64_t)gridDim.x * kThreads;
+    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < n; i += step) {
+        float s = 0.f;
+        for (int k = 0; k < splits; ++k) s += parts[k * n + i];
+        out[i] = E::down(s);
+    }
 }
 
 __global__ __launch_bounds__(kThreads) void k_zero_bytes(uint8_t* p, int64_t n) {
-    const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-    if (i < n) p[i] = 0;
+    const int64_t step = (int64_t)gridDim.x * kThreads;
+    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < n; i += step) p[i] = 0;
 }
 
 // --------------------------------------------------------------- narrow --
@@ -1130,6 +1131,14 @@ int check_shape(const Shape& s) {
     return GSX_OK;
 }
 
+// A launch holds fewer than 2^32 threads in all, workgroups times their size.
+constexpr int64_t kMostGroups = (1LL << 32) / kThreads - 1;
+// Workgroups for n elements that threads walk by the grid's size.
+dim3 groups_for(int64_t n) {
+    const int64_t groups = (n + kThreads - 1) / kThreads;
+    return dim3((unsigned)(groups < kMostGroups ? groups : kMostGroups));
+}
+
 // Workgroups of one product; the grid's x holds all of them.
 int64_t tiles(int64_t m, int64_t n) { return up_to(m, kBM) / kBM * (up_to(n, kBN) / kBN); }
 
@@ -1152,7 +1161,7 @@ Splits splits_of(int64_t rows, int64_t m, int64_t n) {
 template <class E, Mode MODE>
 int launch_tile(const Tile& q, int splits, hipStream_t st) {
     const int64_t n = tiles(q.m, q.n);
-    if (n >= (1LL << 31)) return GSX_ERR_TOO_LARGE;
+    if (n * splits > kMostGroups) return GSX_ERR_TOO_LARGE;
     hipLaunchKernelGGL((k_tile<E, MODE>), dim3((unsigned)n, (unsigned)splits), dim3(kThreads), 0,
                        st, q);
     GSX_LAUNCH_CHECK();
@@ -1324,10 +1333,8 @@ int launch_narrow_bwd(const Shape& s, const BwdArgs& a) {
         }
         if (dx_parts) {
             const int64_t n = s.rows * s.d_in;
-            const int64_t blocks = (n + kThreads - 1) / kThreads;
-            if (blocks >= (1LL << 31)) return GSX_ERR_TOO_LARGE;
-            hipLaunchKernelGGL((k_join<E>), dim3((unsigned)blocks), dim3(kThreads), 0, a.st,
-                               dx_parts, n, p.groups, (T*)a.dx);
+            hipLaunchKernelGGL((k_join<E>), groups_for(n), dim3(kThreads), 0, a.st, dx_parts, n,
+                               p.groups, (T*)a.dx);
             GSX_LAUNCH_CHECK();
         }
         return GSX_OK;
@@ -1392,9 +1399,8 @@ int weight_grad(const Tile& base, int64_t rows, void* const* outs, int count, fl
     if (e) return e;
     if (sp.count > 1)
         for (int i = 0; i < count; ++i) {
-            hipLaunchKernelGGL((k_join<E>), dim3((unsigned)((n + kThreads - 1) / kThreads)),
-                               dim3(kThreads), 0, st, parts + i * sp.count * n, n, sp.count,
-                               (typename E::T*)outs[i]);
+            hipLaunchKernelGGL((k_join<E>), groups_for(n), dim3(kThreads), 0, st,
+                               parts + i * sp.count * n, n, sp.count, (typename E::T*)outs[i]);
             GSX_LAUNCH_CHECK();
         }
     return GSX_OK;
@@ -1470,8 +1476,7 @@ int backward(const Shape& s, const void* x, int64_t ldx, const void* wg, const v
 
 int zero(void* p, int64_t bytes, hipStream_t st) {
     if (!p) return GSX_OK;
-    hipLaunchKernelGGL(k_zero_bytes, dim3((unsigned)((bytes + kThreads - 1) / kThreads)),
-                       dim3(kThreads), 0, st, (uint8_t*)p, bytes);
+    hipLaunchKernelGGL(k_zero_bytes, groups_for(bytes), dim3(kThreads), 0, st, (uint8_t*)p, bytes);
     GSX_LAUNCH_CHECK();
     return GSX_OK;
 }

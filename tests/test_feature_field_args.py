@@ -70,7 +70,8 @@ def told(logits=(4, 9), values=(4, 2), index=None, dtype=torch.float32, vtype=to
     (dict(reduction="batch"), "reduction"),
     (dict(call=distillation_value_and_grad, reduction="none"), "scalar"),
     (dict(), "GPU only"),
-], ids=str)
+], ids=lambda v: str({k: getattr(w, "__name__", w) for k, w in v.items()})
+    if isinstance(v, dict) else v)
 def test_distillation_refuses(wrong, words):
     with pytest.raises(ValueError, match=words):
         told(**wrong)
@@ -119,3 +120,13 @@ def test_c_entries_refuse_before_a_launch():
     assert L.gsx_distil_fwd(*head, *good, None, p, big, None) == -1
     assert L.gsx_distil_bwd(*head, *good, None, p, p, big, None) == -1
     assert L.gsx_distil_fwd_bwd(*head, *good[:7], 0, 1.0, p, p, p, big, None) == -1
+
+
+def test_more_segments_than_a_launch_holds_are_refused():
+    """Rows over 8192 bytes take a workgroup of 256 threads for each 16 KB."""
+    L = _lib.load()
+    for dtype, rows, vocab, rc in ((1, 1 << 24, 4097, -4), (0, 1 << 24, 2049, -4),
+                                   (1, (1 << 24) // 3 + 1, 16385, -4), (1, 1 << 24, 4096, 0),
+                                   (1, (1 << 24) - 1, 4097, 0), (1, (1 << 24) // 3, 16385, 0)):
+        need = L.gsx_distil_workspace_bytes(dtype, rows, vocab, 2)
+        assert need == rc if rc else need > 0

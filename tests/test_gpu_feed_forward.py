@@ -262,3 +262,27 @@ def test_module_trains():
     assert y.shape == (256, 3) and set(block.params) == {"w_gate", "w_up", "w_down"}
     y.square().mean().backward()
     assert all(p.grad is not None and bool(p.grad.isfinite().all()) for p in block.params.values())
+
+
+def test_more_elements_than_32_bits_count():
+    """x and its gradient of more than 2^32 elements, the hidden channels in two
+    groups whose parts of dx are added up: rows at both ends and on both sides of
+    the 2^31st and the 2^32nd element against the formulas."""
+    if torch.cuda.mem_get_info()[0] < 100 << 30:
+        pytest.skip("takes 100 GB of device memory")
+    d_in, hidden = 128, 160
+    rows = (1 << 32) // d_in + 3
+    g = torch.Generator(device=DEV).manual_seed(6)
+    x = torch.empty((rows, d_in), dtype=torch.bfloat16, device=DEV)
+    for part in x.split(1 << 22):
+        part.copy_(torch.randn(part.shape, generator=g, device=DEV))
+    _, wg, wu, wd, _ = inputs(1, d_in, hidden, 1, torch.bfloat16, seed=6)
+    dy = torch.ones((rows, 1), dtype=torch.bfloat16, device=DEV)
+    x.requires_grad_(True)
+    y = gated_feed_forward(x, wg, wu, wd)
+    (dx,) = torch.autograd.grad(y, x, dy)
+    picks = torch.tensor([0, 1, rows // 2 - 1, rows // 2, rows // 2 + 1, rows - 4, rows - 3,
+                          rows - 2, rows - 1], device=DEV)
+    val, err = formulas(x.detach()[picks], wg, wu, wd, dy[picks], "silu")
+    got = {"y": y.detach()[picks], "dx": dx[picks]}
+    check(got, {k: val[k] for k in got}, err, torch.bfloat16)

@@ -376,8 +376,9 @@ struct Ahead {
         T* at = (T*)lds + off;
         if (off && src == lo && lane < V - off && (int)lane < n)
             at[lane] = src[lane];
-        const int tail = (int)((uintptr_t)stop % 16 / sizeof(T));
-        if (tail && stop == hi && lane < tail && (int)lane < n)
+        // also before a last tile of so few elements that this one ends in the last piece
+        const unsigned tail = (unsigned)((uintptr_t)stop % 16 / sizeof(T));
+        if ((uintptr_t)stop > ((uintptr_t)hi & ~(uintptr_t)15) && lane < tail && (int)lane < n)
             at[n - 1 - lane] = src[n - 1 - lane];
     }
 };

@@ -323,3 +323,33 @@ def test_more_logits_than_32_bits_count():
     assert abs(float(loss) - sum(want) / 2) < 1e-5
     assert abs(float(g[-2, 3]) - (1 / vocab - 1) / 2) < 2e-3
     assert float(g[:-2].float().abs().max()) == 0.0
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("teacher", TEACHERS)
+@pytest.mark.parametrize("vocab", (1, 2, 3, 5, 7))
+def test_rows_that_begin_and_end_between_pieces(vocab, teacher, dtype):
+    """Short rows in a buffer at every offset from a 16-byte boundary, with last
+    tiles of a row or two that share their 16 bytes with the tile before.  By
+    whole words off, the bits of the same rows at a boundary; else rows begin
+    inside other words and their sums take another order: the definition."""
+    top = min(vocab, 2)
+    size = torch.empty((), dtype=dtype).element_size()
+    for rows in (1, 2, 15, 16, 17, 18, 33, 49, 1025):
+        logits, values, index = inputs(rows, vocab, top, dtype, teacher, seed=rows)
+        want = distillation_value_and_grad(logits.clone(), values, index, teacher=teacher,
+                                           reduction="sum")
+        if rows < 50:
+            loss, grad, loss_tol, grad_tol, _ = definition(logits, values, index, 1.0, teacher)
+        for offset in range(1, 16 // size):
+            buf = torch.full((offset + rows * vocab + 16,), float("nan"), dtype=dtype, device=DEV)
+            view = buf[offset:offset + rows * vocab].view(rows, vocab)
+            view.copy_(logits)
+            got = distillation_value_and_grad(view, values, index, teacher=teacher,
+                                              reduction="sum")
+            if offset * size % 4 == 0:
+                for a, b in zip(got, want):
+                    assert torch.equal(a, b), (rows, offset)
+            elif rows < 50:
+                near_rows(got[0], loss.sum(), loss_tol.sum())
+                near_rows(got[1], grad, grad_tol, dtype)

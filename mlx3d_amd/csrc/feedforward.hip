@@ -7,9 +7,11 @@
 //
 // x (rows, d_in), Wg and Wu (hidden, d_in), Wd (d_out, hidden), row-major.
 // Products and their sums are float32 on the matrix units: 16-bit operands as
-// they are, float32 ones as three bf16 pieces each (matrix_tile.h).  h, dg and
+// they are, float32 ones as three bf16 pieces each in the narrow kernels
+// (matrix_tile.h) and by the float32 instructions in the tiled ones.  h, dg and
 // du are rounded once to the tensors' type where they become operands, which in
-// 16 bits the matrix units need anyway.
+// 16 bits the matrix units need anyway: against 64 bits that makes 1.4 times the
+// error of one rounding at the end.
 //
 // Two paths.  Narrow widths (a decoder over pixels) run the whole block in one
 // kernel, forward and backward: h, dg and du never leave the chip.  Any other

@@ -283,6 +283,8 @@ def rows_of(t: torch.Tensor) -> tuple[torch.Tensor, int]:
     """``t`` (..., C) as (rows, C) with its row stride in elements; copied only
     if its last dimension is strided or its leading ones do not fold into one."""
     width = t.shape[-1]
+    if t.is_contiguous():  # 0.5 us a call, what follows takes 4
+        return (t if t.ndim == 2 else t.reshape(-1, width)), width
     t = t.reshape(-1, width)
     if (t.shape[0] > 1 and t.stride(0) < width) or (width > 1 and t.stride(1) != 1):
         t = t.contiguous()

@@ -34,7 +34,7 @@ class _GatedFeedForward(torch.autograd.Function):
                 w_down.shape[0])
         y = torch.empty((*x.shape[:-1], w_down.shape[0]), dtype=x.dtype, device=x.device)
         n = _lib.check(int(L.gsx_ffn_fwd_workspace_bytes(*head)), "gsx_ffn_fwd_workspace_bytes")
-        ws = torch.empty((n,), dtype=torch.uint8, device=x.device)
+        ws = torch.empty((n,), dtype=torch.uint8, device=x.device) if n else None
         with stage("ffn_fwd"):
             _lib.check(L.gsx_ffn_fwd(*head, _lib.ptr(rows), stride, *map(_lib.ptr, weights),
                                      _lib.ptr(y), _lib.ptr(ws), n, _lib.stream_handle(x.device)),

@@ -149,12 +149,13 @@ __device__ __forceinline__ void wave_fence() {
     __builtin_amdgcn_wave_barrier();
 }
 
-// exp((s - m) / T) as the power 2^(s c - mc) with c = log2(e) / T and mc = c m
-// rounded once: one multiply-add for a logit.  What mc's rounding moves, up to
-// |mc| 2^-24, it moves in every term of a row alike, so it leaves the quotients;
-// logarithms take the exponents back by the same mc.
-__device__ __forceinline__ float expo(float s, float mc, float c) {
-    return __builtin_amdgcn_exp2f(fmaf(s, c, -mc));
+// exp((s - m) / T) as the power 2^((s - m) c) with c = log2(e) / T.  The difference
+// comes first: it is 0 at the maximum whatever its size, so a row, a rest or a
+// segment that only holds a mask's finite lowest value has equal parts, where
+// s c - m c would round m c by many powers of two (from |m| of 1e9 on) or
+// overflow.  m is finite; s may be -inf (0).
+__device__ __forceinline__ float expo(float s, float m, float c) {
+    return __builtin_amdgcn_exp2f((s - m) * c);
 }
 
 constexpr float kLn2 = 0.69314718055994531f;
@@ -190,9 +191,13 @@ __device__ __forceinline__ void read_entries(const Distil& q, int64_t row, int l
 // What the entries and the rest of a row say: the loss, and what the gradient
 // needs.  rest_m, rest_s: maximum logit and sum of exp over the rest (-inf, 0:
 // nothing there).  Turns the entries' values into their probabilities.
+//
+// The loss is summed times T^2, T log q and the like: T^2 p (log p - log q) is
+// p T (T (log p + log total) - (s - m)), which needs no quotient by T that could
+// overflow next to a mask.
 struct RowStats {
-    float loss;     // without T^2
-    float mc, inv;  // c times the maximum over all, S / (sum of exp over all)
+    float loss;
+    float m, inv;   // the maximum over all, S / (sum of exp over all)
     float rest;     // the rest's factor on exp((s - rest_m) / T)
     bool active;
 };
@@ -202,7 +207,7 @@ struct RowStats {
 template <int G, int KPL, bool LOG_PROBS>
 __device__ __forceinline__ RowStats row_stats(const Distil& q, Entries<KPL>& e, float rest_m,
                                               float rest_s) {
-    const float c = kLog2e * q.inv_temp;
+    const float c = kLog2e * q.inv_temp, temp = q.temp;
     float tm = -INFINITY, m = rest_m, any = 0.f;
 #pragma unroll
     for (int i = 0; i < KPL; ++i)
@@ -214,27 +219,28 @@ __device__ __forceinline__ RowStats row_stats(const Distil& q, Entries<KPL>& e, 
     RowStats r;
     r.active = group_max<G>(any) > 0.f;
     const bool has_rest = rest_m != -INFINITY;
-    const float rest_mc = c * rest_m;
-    float total = rest_s, shift = 1.f, mc = rest_mc;
+    float total = rest_s, shift = 1.f;
     if constexpr (LOG_PROBS) {
-        mc = c * group_max<G>(m);
-        shift = has_rest ? __builtin_amdgcn_exp2f(rest_mc - mc) : 0.f;
+        m = group_max<G>(m);
+        shift = has_rest ? expo(rest_m, m, c) : 0.f;
         total = 0.f;
 #pragma unroll
         for (int i = 0; i < KPL; ++i)
             if (e.index[i] >= 0 && !e.again[i] && e.s[i] != -INFINITY)
-                total += expo(e.s[i], mc, c);
+                total += expo(e.s[i], m, c);
         total = group_sum<G>(total) + (has_rest ? rest_s * shift : 0.f);
+    } else {
+        m = rest_m;
     }
     const float log_total = log_of(total);
-    float loss = 0.f, mass = 0.f, t_exp[KPL], inv_t = 1.f, log_t = 0.f, tmc = 0.f;
+    float loss = 0.f, mass = 0.f, t_exp[KPL], inv_t = 1.f, log_t = 0.f;
     if constexpr (!LOG_PROBS) {
-        tmc = c * group_max<G>(tm);
+        tm = group_max<G>(tm);
         float t_sum = 0.f;
 #pragma unroll
         for (int i = 0; i < KPL; ++i)
             if (e.index[i] >= 0) {
-                t_exp[i] = expo(e.value[i], tmc, c);
+                t_exp[i] = expo(e.value[i], tm, c);
                 t_sum += t_exp[i];
             }
         t_sum = group_sum<G>(t_sum);
@@ -244,15 +250,15 @@ __device__ __forceinline__ RowStats row_stats(const Distil& q, Entries<KPL>& e, 
 #pragma unroll
     for (int i = 0; i < KPL; ++i)
         if (e.index[i] >= 0) {
-            float lp, p;
+            float lp, p;  // T log p
             if constexpr (LOG_PROBS) {
-                lp = e.value[i];
-                p = __builtin_amdgcn_exp2f(lp * kLog2e);
+                lp = temp * e.value[i];
+                p = __builtin_amdgcn_exp2f(e.value[i] * kLog2e);
             } else {
-                lp = fmaf(e.value[i], c, -tmc) * kLn2 - log_t;
+                lp = (e.value[i] - tm) - temp * log_t;
                 p = t_exp[i] * inv_t;
             }
-            if (p != 0.f) loss += p * (lp - (fmaf(e.s[i], c, -mc) * kLn2 - log_total));
+            if (p != 0.f) loss += (p * temp) * (fmaf(temp, log_total, lp) - (e.s[i] - m));
             mass += p;
             e.value[i] = p;
         }
@@ -262,14 +268,14 @@ __device__ __forceinline__ RowStats row_stats(const Distil& q, Entries<KPL>& e, 
     if (LOG_PROBS && has_rest) {
         const float left = 1.0f - mass;
         if (left > 0.f) {
-            const float log_q = (rest_mc - mc) * kLn2 + log_of(rest_s) - log_total;
-            loss += left * (log_of(left) - log_q);
+            const float logs = log_of(left) - log_of(rest_s) + log_total;
+            loss += (left * temp) * (temp * logs - (rest_m - m));
             share = left / rest_s;
             mass += left;
         }
     }
     r.loss = loss;
-    r.mc = mc;
+    r.m = m;
     r.inv = mass * __builtin_amdgcn_rcpf(total);
     r.rest = r.inv * shift - share;
     return r;
@@ -277,7 +283,7 @@ __device__ __forceinline__ RowStats row_stats(const Distil& q, Entries<KPL>& e, 
 
 // An entry's gradient without the row's factor; p: the column's probability.
 __device__ __forceinline__ float entry_grad(const RowStats& r, float s, float p, float c) {
-    return (s == -INFINITY ? 0.f : expo(s, r.mc, c)) * r.inv - p;
+    return (s == -INFINITY ? 0.f : expo(s, r.m, c)) * r.inv - p;
 }
 
 // The factor on a row's gradient: T, the upstream gradient, 1 / supervised rows.
@@ -528,7 +534,7 @@ __global__ __launch_bounds__(kThreads, N > 14 ? 2 : KPL > 2 ? 3 : 4) void k_rows
                 if (q.grad) mark();
             }
             rest_m = group_max<G>(rest_m);
-            const float ref = rest_m == -INFINITY ? 0.f : c * rest_m;
+            const float ref = rest_m == -INFINITY ? 0.f : rest_m;
             float rest_s = 0.f;
 #pragma unroll
             for (int i = 0; i < N * W; ++i) {
@@ -538,7 +544,7 @@ __global__ __launch_bounds__(kThreads, N > 14 ? 2 : KPL > 2 ? 3 : 4) void k_rows
             rest_s = group_sum<G>(rest_s);
             const RowStats r = row_stats<G, KPL, LOG_PROBS>(q, e, rest_m, rest_s);
             if (lane == 0) {
-                const float loss = r.active ? q.temp * q.temp * r.loss : 0.f;
+                const float loss = r.active ? r.loss : 0.f;
                 if (q.loss_rows) q.loss_rows[row] = loss;
                 group_loss += loss;
             }
@@ -655,7 +661,7 @@ __global__ __launch_bounds__(kThreads) void k_seg_sum(const Distil q) {
     float s = 0.f;
     for (int j = threadIdx.x; j < n; j += kThreads) {
         const float v = E::up(tile[j]);
-        s += v == -INFINITY ? 0.f : expo(v, c * m, c);
+        s += v == -INFINITY ? 0.f : expo(v, m, c);
     }
     s = group_sum<64>(s);
     __syncthreads();
@@ -705,19 +711,19 @@ __global__ __launch_bounds__(64) void k_seg_join(const Distil q) {
     m = group_max<64>(m);
     for (int i = lane; i < q.segs; i += 64) {
         const float pm = parts[2 * i], ps = parts[2 * i + 1];
-        s += pm == -INFINITY ? ps : ps * __builtin_amdgcn_exp2f(c * pm - c * m);  // 0, or NaN
+        s += pm == -INFINITY ? ps : ps * expo(pm, m, c);  // 0, or NaN
     }
     s = group_sum<64>(s);
     const RowStats r = q.log_probs ? row_stats<64, KPL, true>(q, e, m, s)
                                    : row_stats<64, KPL, false>(q, e, m, s);
     if (lane == 0) {
-        const float loss = r.active ? q.temp * q.temp * r.loss : 0.f;
+        const float loss = r.active ? r.loss : 0.f;
         if (q.loss_rows) q.loss_rows[row] = loss;
         if (q.loss_parts) q.loss_parts[row] = loss;
         float* st = q.stats + row * 8;
         st[0] = m;
         st[1] = r.rest;
-        st[2] = r.mc;
+        st[2] = r.m;
         st[3] = r.inv;
         st[4] = r.active ? 1.f : 0.f;
         st[5] = shared ? 1.f : 0.f;
@@ -758,7 +764,7 @@ __global__ __launch_bounds__(kThreads) void k_seg_grad(const Distil q) {
     const float inv_count = inverse_count(q, scratch);
     const float f = row_scale(q, row, inv_count);
     const float c = kLog2e * q.inv_temp;
-    const float rest_mc = c * st[0], rest = st[1] * f;
+    const float rest_m = st[0], rest = st[1] * f;
     __syncthreads();
     // this thread's entry of this segment (there are no more entries than threads)
     float own = 0.f;
@@ -782,7 +788,7 @@ __global__ __launch_bounds__(kThreads) void k_seg_grad(const Distil q) {
         float g = 0.f;
         if (active) {
             const float s = E::up(tile[j]);
-            g = s == -INFINITY ? 0.f * rest : expo(s, rest_mc, c) * rest;
+            g = s == -INFINITY ? 0.f * rest : expo(s, rest_m, c) * rest;
         }
         tile[j] = E::down(g);
     }

@@ -218,7 +218,8 @@ __device__ __forceinline__ RowStats row_stats(const Distil& q, Entries<KPL>& e, 
         }
     RowStats r;
     r.active = group_max<G>(any) > 0.f;
-    const bool has_rest = rest_m != -INFINITY;
+    // NaN leaves no maximum; a sum over anything else than -inf is 1 or more
+    const bool has_rest = rest_s != 0.f;
     float total = rest_s, shift = 1.f;
     if constexpr (LOG_PROBS) {
         m = group_max<G>(m);

@@ -8,6 +8,7 @@ device, the call raises instead of silently computing something else.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 import threading
 
@@ -277,6 +278,38 @@ def require_device(*tensors: torch.Tensor | None) -> torch.device:
     if dev is None:
         raise ValueError("no tensor inputs")
     return dev
+
+
+class _NoSecondDerivative(torch.autograd.Function):
+    """Hands a gradient on; differentiating it raises."""
+
+    @staticmethod
+    def forward(ctx, what, grad, *sources):
+        ctx.what = what
+        return grad.view_as(grad)
+
+    @staticmethod
+    def backward(ctx, _):
+        raise RuntimeError(f"{ctx.what} has no second derivatives (once_differentiable).")
+
+
+def once_differentiable(what: str):
+    """For a Function's ``backward``: with ``create_graph=True`` its gradients
+    depend on the saved tensors and raise when they are differentiated.  torch's
+    decorator looks at the incoming gradient alone, and hands out constants where
+    that one needs none."""
+    def wrap(backward):
+        @functools.wraps(backward)
+        def run(ctx, *grads):
+            if not torch.is_grad_enabled():
+                return backward(ctx, *grads)
+            with torch.no_grad():
+                out = backward(ctx, *grads)
+            return tuple(g if g is None else
+                         _NoSecondDerivative.apply(what, g, *grads, *ctx.saved_tensors)
+                         for g in out)
+        return run
+    return wrap
 
 
 def rows_of(t: torch.Tensor) -> tuple[torch.Tensor, int]:

@@ -260,6 +260,7 @@ class _DistillationFn(torch.autograd.Function):
         return loss
 
     @staticmethod
+    @_lib.once_differentiable("distillation_loss")
     def backward(ctx, g_loss):
         # saved with the rest so that an entry changed in place since is noticed
         logits, ws, _, _ = ctx.saved_tensors
@@ -293,7 +294,8 @@ def distillation_loss(logits: torch.Tensor, teacher_values: torch.Tensor,
     A row without entries has loss 0 and gradient 0 whatever its logits hold.
     ``reduction``: "mean" over the rows that have entries (0 if none has),
     "sum", or "none" (a loss for each row; weight rows by what multiplies it).
-    At most 256 entries a row; values and indices carry no gradient."""
+    At most 256 entries a row; values and indices carry no gradient, and the
+    gradient none of its own (differentiating it raises an error)."""
     call = _Distillation(logits, teacher_values, teacher_indices, temperature, teacher, reduction)
     return _DistillationFn.apply(logits, call)
 

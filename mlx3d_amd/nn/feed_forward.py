@@ -44,6 +44,7 @@ class _GatedFeedForward(torch.autograd.Function):
         return y
 
     @staticmethod
+    @_lib.once_differentiable("gated_feed_forward")
     def backward(ctx, g_y):
         x, *weights = ctx.saved_tensors
         L = _lib.load()
@@ -73,7 +74,8 @@ def gated_feed_forward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor
     """(..., d_out) = (act(x w_gate^T) * (x w_up^T)) w_down^T of x (..., d_in)
     with w_gate, w_up (hidden, d_in) and w_down (d_out, hidden), all of one
     type (float32, bfloat16, float16); differentiable with respect to all
-    four.  ``activation``: "silu", "gelu" (with erf) or "sigmoid".
+    four, once (its gradient has none and says so).  ``activation``: "silu",
+    "gelu" (with erf) or "sigmoid".
 
     Products are summed in float32.  In 16 bits the hidden channels and their
     gradients are rounded to the type once before they are multiplied again."""

@@ -90,20 +90,26 @@ struct F16 {
     static __device__ __forceinline__ bool is_tag(T v, int k) { return v == (T)k; }
 };
 
-// What the narrow kernels multiply: a float32 operand as three bf16 pieces
-// (rounded to nearest: 8 + 8 + 8 bits hold the 24 exactly, the pieces falling by
-// 2^-8 each) and six of their nine products, the rest below 2^-23 of a product;
-// 16-bit operands as they are.  The matrix units take 16 bits at eight times
-// the float32 rate (1248 against 154 TFLOP/s in large products), so six products
-// cost less than half of one in float32.
+// What the narrow kernels multiply: a float32 operand as three bf16 pieces (the
+// first cut off, the others rounded to nearest: 8 + 8 + 8 bits hold the 24
+// exactly) and six of their nine products; the rest is below 2^-22 of a product.
+// 16-bit operands are taken as they are.  The matrix units take 16 bits at eight
+// times the float32 rate (1248 against 154 TFLOP/s in large products), so six
+// products cost less than half of one in float32.
+//
+// Cutting holds every finite number, where rounding would make infinities of those
+// next to the largest; it takes as many instructions.  Pieces end at bf16's
+// smallest number, so of an operand below 2^-110 up to 2^-126 is lost.  An
+// infinity has no second piece: it gives NaN.
 struct Split3 {
     u32x4 p[3];
 };
 __device__ __forceinline__ void split_pair(float a, float b, uint32_t* p0, uint32_t* p1,
                                            uint32_t* p2) {
-    *p0 = BF16::pair(a, b);
-    a -= __uint_as_float(*p0 << 16);
-    b -= __uint_as_float(*p0 & 0xffff0000u);
+    const uint32_t ha = __float_as_uint(a) & 0xffff0000u, hb = __float_as_uint(b) & 0xffff0000u;
+    *p0 = ha >> 16 | hb;
+    a -= __uint_as_float(ha);
+    b -= __uint_as_float(hb);
     *p1 = BF16::pair(a, b);
     a -= __uint_as_float(*p1 << 16);
     b -= __uint_as_float(*p1 & 0xffff0000u);

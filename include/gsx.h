@@ -780,8 +780,9 @@ enum gsx_reduction { GSX_REDUCE_NONE = 0, GSX_REDUCE_SUM = 1, GSX_REDUCE_MEAN = 
  * [0, vocab) or whose value is -inf is absent; two entries of one column both
  * count.  A row without entries has loss 0 and gradient 0, whatever its logits
  * hold, and the mean does not count it (no row: 0).  loss: rows floats (none)
- * or one.  1 <= top <= min(vocab, GSX_DISTIL_MAX_TOP).  GSX_ERR_TOO_LARGE from
- * 2^30 rows, and from 2^24 pieces of 16 KB where rows are over 8 KB. */
+ * or one.  1e-38 <= T <= 3e38; 1 <= top <= min(vocab, GSX_DISTIL_MAX_TOP).
+ * GSX_ERR_TOO_LARGE from 2^30 rows, and from 2^24 pieces of 16 KB where rows
+ * are over 8 KB. */
 int64_t gsx_distil_workspace_bytes(int32_t dtype, int64_t rows, int32_t vocab, int32_t top);
 int gsx_distil_fwd(int32_t dtype, int64_t rows, int32_t vocab, int32_t top, const void* logits,
                    int64_t logits_stride, const float* values, const void* indices,

@@ -1045,7 +1045,8 @@ struct Args {
 
 int check_args(const Args& a) {
     if (int e = check_shape(a.dtype, a.rows, a.vocab, a.top)) return e;
-    if (!(a.temperature > 0.f) || a.temperature > 3.0e38f) return GSX_ERR_INVALID;
+    // 1 / T is a float32, too
+    if (!(a.temperature >= 1e-38f) || a.temperature > 3.0e38f) return GSX_ERR_INVALID;
     if (a.teacher != GSX_TEACHER_LOGITS && a.teacher != GSX_TEACHER_LOG_PROBS)
         return GSX_ERR_INVALID;
     if (a.reduction != GSX_REDUCE_NONE && a.reduction != GSX_REDUCE_SUM &&

@@ -219,8 +219,9 @@ class _Distillation:
         if not 1 <= top <= min(vocab, DISTILLATION_MAX_TOP):
             raise ValueError("a row must have between 1 and "
                              f"min(V, {DISTILLATION_MAX_TOP}) teacher entries.")
-        if not 0.0 < float(temperature) < 3.0e38:
-            raise ValueError("temperature must be positive and finite.")
+        if not 1e-38 <= float(temperature) < 3.0e38:
+            raise ValueError("temperature must be positive and finite, with a reciprocal that "
+                             "float32 holds (from 1e-38 on).")
         if teacher not in _TEACHERS:
             raise ValueError("teacher must be 'logits' or 'log_probs'.")
         if reduction not in _REDUCTIONS:

@@ -398,6 +398,7 @@ struct Tile {
     int act;
     int64_t split_k;      // depth of a split (WGRAD*)
     int64_t split_out;    // floats of a split's partial sums; 0: out itself, in E
+    bool add;             // to the partial sums that an earlier stretch of rows left
 };
 
 template <class E, Mode MODE>
@@ -446,18 +447,26 @@ __global__ __launch_bounds__(kThreads, kExact<E> ? 1 : 2) void k_tile(const Tile
                     const int64_t at = (int64_t)(col + e) * q.ldo + row;
                     if (q.split_out) {
                         const int64_t s = blockIdx.y * q.split_out;
-                        ((float*)q.out[0])[s + at] = c0[i][j][e];
-                        ((float*)q.out[1])[s + at] = c1[i][j][e];
+                        float* o0 = (float*)q.out[0] + s + at;
+                        float* o1 = (float*)q.out[1] + s + at;
+                        *o0 = q.add ? *o0 + c0[i][j][e] : c0[i][j][e];
+                        *o1 = q.add ? *o1 + c1[i][j][e] : c1[i][j][e];
                     } else {
                         ((T*)q.out[0])[at] = E::down(c0[i][j][e]);
                         ((T*)q.out[1])[at] = E::down(c1[i][j][e]);
                     }
                 }
             } else if constexpr (MODE == WGRAD) {
-                if (q.split_out)
-                    put<F32>((float*)q.out[0] + blockIdx.y * q.split_out, q.ldo, row, col, q.m,
-                             q.n, c0[i][j]);
-                else
+                if (q.split_out) {
+                    float* parts = (float*)q.out[0] + blockIdx.y * q.split_out;
+                    f32x4 v = c0[i][j];
+                    if (q.add && row < q.m) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (col + e < q.n) v[e] += parts[(int64_t)row * q.ldo + col + e];
+                    }
+                    put<F32>(parts, q.ldo, row, col, q.m, q.n, v);
+                } else
                     put<E>((T*)q.out[0], q.ldo, row, col, q.m, q.n, c0[i][j]);
             } else if constexpr (MODE == HIDDEN) {
                 f32x4 h;
@@ -702,6 +711,7 @@ struct NarrowBwd {
     float* parts;     // (workgroups, groups, pairs, halves, sums, 64)
     int64_t ldx, lddy, rows;
     int d_in, hidden, d_out, act;
+    bool add;         // to the parts that an earlier stretch of rows left
 };
 
 // Rows of float32 sums, written and read along the slots only.
@@ -1056,18 +1066,21 @@ void k_narrow_bwd(const NarrowBwd<E> q) {
     float* out = q.parts +
                  (((int64_t)blockIdx.x * gridDim.y + blockIdx.y) * 2 * kBwdPairs + wave) * S::SUMS *
                      64 + lane;
-    int n = 0;
+    auto leave = [&](float v) {
+        *out = q.add ? *out + v : v;
+        out += 64;
+    };
 #pragma unroll
     for (int d = 0; d < 2 * KD; ++d)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            out[64 * n++] = sg[d][i];
-            out[64 * n++] = su[d][i];
+            leave(sg[d][i]);
+            leave(su[d][i]);
         }
 #pragma unroll
     for (int o = 0; o < 2 * KO; ++o)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) out[64 * n++] = sd[o][i];
+        for (int i = 0; i < 4; ++i) leave(sd[o][i]);
 }
 
 // Adds up the workgroups' weight gradients in their order: 64 sums of one wave
@@ -1170,9 +1183,36 @@ int launch_tile(const Tile& q, int splits, hipStream_t st) {
     return GSX_OK;
 }
 
+// The rows are walked in stretches, so that what stands between two kernels
+// (arrays of hidden width, the groups' parts of dx) is bounded: kStretchBytes an
+// array, and no more workgroups than a launch holds.  Stretches of equal length:
+// a power of two (131 072 rows of 512 float32) cost 8 %, its splits begin on the
+// same memory channels.  Gradient, us in one stretch / in stretches of 1 GB / of
+// 256 MB, 921 600 rows: 200 -> 512 -> 256 bf16 5200 / 5190 / 5250; 128 -> 1024 -> 32
+// bf16, whose workgroups take up 100 MB of sums in each, 4220 / 4550 / 5370.
+constexpr int64_t kStretchBytes = 1 << 30;
+
+// Rows of a stretch that holds at most `most`, in whole tiles.
+int64_t even_stretch(int64_t rows, int64_t most, int tile) {
+    most = most / tile * tile;
+    if (most < tile) most = tile;
+    if (rows <= most) return rows;
+    const int64_t count = (rows + most - 1) / most;
+    return up_to((rows + count - 1) / count, tile);
+}
+
 // hidden's row pitch in the workspace: whole 16-byte pieces
 int64_t pitch(const Shape& s) { return up_to(s.hidden, 8); }
-int64_t hidden_bytes(const Shape& s) { return up_to(s.rows * pitch(s) * s.size(), 256); }
+int64_t tiled_stretch(const Shape& s) {
+    const int wide = s.hidden > s.d_out ? (s.hidden > s.d_in ? s.hidden : s.d_in)
+                                        : (s.d_out > s.d_in ? s.d_out : s.d_in);
+    const int64_t fit = kStretchBytes / (pitch(s) * s.size());
+    const int64_t most = kMostGroups / (up_to(wide, kBN) / kBN) * kBM;
+    return even_stretch(s.rows, fit < most ? fit : most, kBM);
+}
+int64_t hidden_bytes(const Shape& s) {
+    return up_to(tiled_stretch(s) * pitch(s) * s.size(), 256);
+}
 
 // Whether the narrow kernel holds a row's operands and sums in its registers:
 // 8 (KD pieces + OB) of them, beside some 100 others.
@@ -1247,11 +1287,20 @@ int narrow_forward(const Shape& s, A... a) {
     }
 }
 
+// One split of one stretch leaves the gradient itself; else each leaves partial
+// sums, kept over the stretches.
+bool direct_grad(const Shape& s, int m) {
+    const int64_t rows = tiled_stretch(s);
+    return rows == s.rows && splits_of(rows, m, s.hidden).count == 1;
+}
+// of one weight matrix with m columns or rows beside the hidden ones
+int64_t sums_bytes(const Shape& s, int m) {
+    if (direct_grad(s, m)) return 0;
+    return splits_of(tiled_stretch(s), m, s.hidden).count * (int64_t)s.hidden * m * 4;
+}
+int64_t pair_parts_bytes(const Shape& s) { return up_to(2 * sums_bytes(s, s.d_in), 256); }
 int64_t parts_bytes(const Shape& s) {
-    const Splits a = splits_of(s.rows, s.d_in, s.hidden), b = splits_of(s.rows, s.d_out, s.hidden);
-    const int64_t in = 2 * a.count * (int64_t)s.hidden * s.d_in;
-    const int64_t out = b.count * (int64_t)s.d_out * s.hidden;
-    return up_to((in > out ? in : out) * 4, 256);
+    return pair_parts_bytes(s) + up_to(sums_bytes(s, s.d_out), 256);
 }
 
 // The narrow backward: which widths fit its registers (weights in both orders
@@ -1271,6 +1320,7 @@ bool narrow_bwd(const Shape& s) {
 }
 struct BwdPlan {
     int pairs, groups, blocks;
+    int64_t stretch;  // rows of one launch
     int64_t parts, dx_parts, bytes;
 };
 BwdPlan bwd_plan(const Shape& s) {
@@ -1278,13 +1328,16 @@ BwdPlan bwd_plan(const Shape& s) {
     const int kd = narrow_kd(s), ko = narrow_ko(s), chunks = (s.hidden + 31) / 32;
     p.groups = (chunks + kBwdPairs - 1) / kBwdPairs;
     p.pairs = chunks < kBwdPairs ? chunks : kBwdPairs;
-    const int64_t tiles = (s.rows + kBwdRows - 1) / kBwdRows;
+    p.stretch = p.groups == 1 ? s.rows
+                              : even_stretch(s.rows, kStretchBytes / (p.groups * s.d_in * 4),
+                                             kBwdRows);
+    const int64_t tiles = (p.stretch + kBwdRows - 1) / kBwdRows;
     const int per_unit = (s.dtype == GSX_F32 ? 1 : 2) * kBwdPairs / p.pairs;
     int64_t want = 256 * per_unit / p.groups;
     if (want > tiles) want = tiles;
     p.blocks = (int)(want < 1 ? 1 : want);
     p.parts = up_to((int64_t)p.blocks * p.groups * 2 * kBwdPairs * (16 * kd + 8 * ko) * 256, 256);
-    p.dx_parts = p.groups > 1 ? up_to(p.groups * s.rows * s.d_in * 4, 256) : 0;
+    p.dx_parts = p.groups > 1 ? up_to(p.groups * p.stretch * s.d_in * 4, 256) : 0;
     p.bytes = p.parts + p.dx_parts;
     return p;
 }
@@ -1314,29 +1367,34 @@ int launch_narrow_bwd(const Shape& s, const BwdArgs& a) {
         float* parts = (float*)a.ws;
         float* dx_parts = p.groups > 1 ? (float*)((char*)a.ws + p.parts) : nullptr;
         if (!a.dx) dx_parts = nullptr;
-        const NarrowBwd<E> q{(const T*)a.x, (const T*)a.wg, (const T*)a.wu, (const T*)a.wd,
-                             (const T*)a.dy, p.groups > 1 ? nullptr : (T*)a.dx, dx_parts, parts,
-                             a.ldx, a.lddy, s.rows, s.d_in, s.hidden, s.d_out, s.act};
         const int64_t lds = S::lds(p.pairs);
         const auto kernel = s.act == GSX_ACT_GELU ? k_narrow_bwd<E, KD, KO, true>
                                                   : k_narrow_bwd<E, KD, KO, false>;
         if (hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize,
                                 160 * 1024) != hipSuccess)
             return GSX_ERR_HIP;
-        hipLaunchKernelGGL(kernel, dim3(p.blocks, p.groups), dim3(128 * p.pairs), (unsigned)lds,
-                           a.st, q);
-        GSX_LAUNCH_CHECK();
+        for (int64_t row0 = 0; row0 < s.rows; row0 += p.stretch) {
+            const int64_t rows = s.rows - row0 < p.stretch ? s.rows - row0 : p.stretch;
+            T* dx = a.dx ? (T*)a.dx + row0 * s.d_in : nullptr;
+            const NarrowBwd<E> q{(const T*)a.x + row0 * a.ldx, (const T*)a.wg, (const T*)a.wu,
+                                 (const T*)a.wd, (const T*)a.dy + row0 * a.lddy,
+                                 p.groups > 1 ? nullptr : dx, dx_parts, parts, a.ldx, a.lddy, rows,
+                                 s.d_in, s.hidden, s.d_out, s.act, row0 > 0};
+            hipLaunchKernelGGL(kernel, dim3(p.blocks, p.groups), dim3(128 * p.pairs),
+                               (unsigned)lds, a.st, q);
+            GSX_LAUNCH_CHECK();
+            if (dx_parts) {
+                const int64_t n = rows * s.d_in;
+                hipLaunchKernelGGL((k_join<E>), groups_for(n), dim3(kThreads), 0, a.st, dx_parts,
+                                   n, p.groups, dx);
+                GSX_LAUNCH_CHECK();
+            }
+        }
         if (a.dwg || a.dwd) {
             const int halves = p.groups * 2 * kBwdPairs;
             hipLaunchKernelGGL((k_narrow_join<E, KD, KO>), dim3(halves * S::SUMS), dim3(kThreads),
                                0, a.st, parts, p.blocks, p.groups, s.d_in, s.hidden, s.d_out,
                                (T*)a.dwg, (T*)a.dwu, (T*)a.dwd);
-            GSX_LAUNCH_CHECK();
-        }
-        if (dx_parts) {
-            const int64_t n = s.rows * s.d_in;
-            hipLaunchKernelGGL((k_join<E>), groups_for(n), dim3(kThreads), 0, a.st, dx_parts, n,
-                               p.groups, (T*)a.dx);
             GSX_LAUNCH_CHECK();
         }
         return GSX_OK;
@@ -1353,7 +1411,7 @@ int launch_narrow_bwd(const Shape& s, const BwdArgs& a) {
 
 template <class E>
 int forward(const Shape& s, const void* x, int64_t ldx, const void* wg, const void* wu,
-            const void* wd, void* y, int64_t ldy, void* ws, hipStream_t st) {
+            const void* wd, void* y, void* ws, hipStream_t st) {
     if (narrow_fwd(s)) {
         switch (narrow_kd(s)) {
             case 1: return narrow_forward<E, 1>(s, x, ldx, wg, wu, wd, y, st);
@@ -1361,45 +1419,55 @@ int forward(const Shape& s, const void* x, int64_t ldx, const void* wg, const vo
             default: return narrow_forward<E, 4>(s, x, ldx, wg, wu, wd, y, st);
         }
     }
-    const int64_t ph = pitch(s);
-    Tile q{};
-    q.a = Operand{x, ldx, (int)s.rows};
-    q.b0 = Operand{wg, s.d_in, s.hidden};
-    q.b1 = Operand{wu, s.d_in, s.hidden};
-    q.k = s.d_in;
-    q.m = (int)s.rows;
-    q.n = s.hidden;
-    q.out[0] = ws;
-    q.ldo = ph;
-    q.act = s.act;
-    if (int e = launch_tile<E, HIDDEN>(q, 1, st)) return e;
-    Tile r{};
-    r.a = Operand{ws, ph, (int)s.rows};
-    r.b0 = Operand{wd, s.hidden, s.d_out};
-    r.k = s.hidden;
-    r.m = (int)s.rows;
-    r.n = s.d_out;
-    r.out[0] = y;
-    r.ldo = ldy;
-    return launch_tile<E, PLAIN>(r, 1, st);
+    using T = typename E::T;
+    const int64_t ph = pitch(s), stretch = tiled_stretch(s);
+    for (int64_t row0 = 0; row0 < s.rows; row0 += stretch) {
+        const int rows = (int)(s.rows - row0 < stretch ? s.rows - row0 : stretch);
+        Tile q{};
+        q.a = Operand{(const T*)x + row0 * ldx, ldx, rows};
+        q.b0 = Operand{wg, s.d_in, s.hidden};
+        q.b1 = Operand{wu, s.d_in, s.hidden};
+        q.k = s.d_in;
+        q.m = rows;
+        q.n = s.hidden;
+        q.out[0] = ws;
+        q.ldo = ph;
+        q.act = s.act;
+        if (int e = launch_tile<E, HIDDEN>(q, 1, st)) return e;
+        Tile r{};
+        r.a = Operand{ws, ph, rows};
+        r.b0 = Operand{wd, s.hidden, s.d_out};
+        r.k = s.hidden;
+        r.m = rows;
+        r.n = s.d_out;
+        r.out[0] = (T*)y + row0 * s.d_out;
+        r.ldo = s.d_out;
+        if (int e = launch_tile<E, PLAIN>(r, 1, st)) return e;
+    }
+    return GSX_OK;
 }
 
+// A weight gradient's sums over the stretch of rows that begins at row0, in splits
+// that each add to their own part; the last stretch adds the parts up.
 template <class E>
-int weight_grad(const Tile& base, int64_t rows, void* const* outs, int count, float* parts,
-                hipStream_t st) {
-    const Splits sp = splits_of(rows, base.m, base.n);
+int weight_grad(const Tile& base, const Shape& s, int64_t row0, int64_t stretch,
+                void* const* outs, int count, float* parts, hipStream_t st) {
+    const Splits sp = splits_of(stretch, base.m, base.n);
     const int64_t n = (int64_t)base.m * base.n;
+    const bool direct = direct_grad(s, base.m), last = row0 + stretch >= s.rows;
     Tile q = base;
-    q.k = rows;
+    q.k = last ? s.rows - row0 : stretch;
     q.split_k = sp.depth;
-    q.split_out = sp.count > 1 ? n : 0;
+    q.split_out = direct ? 0 : n;
+    q.add = row0 > 0;
     q.ldo = count == 2 ? base.m : base.n;
     for (int i = 0; i < count; ++i)
-        q.out[i] = sp.count > 1 ? (void*)(parts + i * sp.count * n) : outs[i];
-    const int e = count == 2 ? launch_tile<E, WGRAD2>(q, sp.count, st)
-                             : launch_tile<E, WGRAD>(q, sp.count, st);
+        q.out[i] = direct ? outs[i] : (void*)(parts + i * sp.count * n);
+    const int splits = (int)((q.k + sp.depth - 1) / sp.depth);
+    const int e = count == 2 ? launch_tile<E, WGRAD2>(q, splits, st)
+                             : launch_tile<E, WGRAD>(q, splits, st);
     if (e) return e;
-    if (sp.count > 1)
+    if (!direct && last)
         for (int i = 0; i < count; ++i) {
             hipLaunchKernelGGL((k_join<E>), groups_for(n), dim3(kThreads), 0, st,
                                parts + i * sp.count * n, n, sp.count, (typename E::T*)outs[i]);
@@ -1420,58 +1488,66 @@ int backward(const Shape& s, const void* x, int64_t ldx, const void* wg, const v
             default: return launch_narrow_bwd<E, 4>(s, a);
         }
     }
-    const int64_t ph = pitch(s), hb = hidden_bytes(s);
+    using T = typename E::T;
+    const int64_t ph = pitch(s), hb = hidden_bytes(s), stretch = tiled_stretch(s);
     void* dg = ws;
     void* du = (char*)ws + hb;
     void* h = (char*)ws + 2 * hb;
-    float* parts = (float*)((char*)ws + 3 * hb);
-    Tile q{};
-    q.a = Operand{x, ldx, (int)s.rows};
-    q.b0 = Operand{wg, s.d_in, s.hidden};
-    q.b1 = Operand{wu, s.d_in, s.hidden};
-    q.k = s.d_in;
-    q.a2 = Operand{dy, lddy, (int)s.rows};
-    q.b2 = Operand{wd, s.hidden, s.hidden};
-    q.k2 = s.d_out;
-    q.m = (int)s.rows;
-    q.n = s.hidden;
-    q.out[0] = dg;
-    q.out[1] = du;
-    q.out[2] = h;
-    q.ldo = ph;
-    q.act = s.act;
-    if (int e = launch_tile<E, BWD_HIDDEN>(q, 1, st)) return e;
-    if (dx) {
-        Tile r{};
-        r.a = Operand{dg, ph, (int)s.rows};
-        r.b0 = Operand{wg, s.d_in, s.d_in};
-        r.a2 = Operand{du, ph, (int)s.rows};
-        r.b2 = Operand{wu, s.d_in, s.d_in};
-        r.k = s.hidden;
-        r.m = (int)s.rows;
-        r.n = s.d_in;
-        r.out[0] = dx;
-        r.ldo = s.d_in;
-        if (int e = launch_tile<E, SUM2>(r, 1, st)) return e;
-    }
-    if (dwg) {
-        Tile r{};
-        r.a = Operand{x, ldx, s.d_in};
-        r.b0 = Operand{dg, ph, s.hidden};
-        r.b1 = Operand{du, ph, s.hidden};
-        r.m = s.d_in;
-        r.n = s.hidden;
-        void* outs[2] = {dwg, dwu};
-        if (int e = weight_grad<E>(r, s.rows, outs, 2, parts, st)) return e;
-    }
-    if (dwd) {
-        Tile r{};
-        r.a = Operand{dy, lddy, s.d_out};
-        r.b0 = Operand{h, ph, s.hidden};
-        r.m = s.d_out;
-        r.n = s.hidden;
-        void* outs[1] = {dwd};
-        if (int e = weight_grad<E>(r, s.rows, outs, 1, parts, st)) return e;
+    // the pair's parts, then the down weights'
+    float* pair_parts = (float*)((char*)ws + 3 * hb);
+    float* down_parts = (float*)((char*)ws + 3 * hb + pair_parts_bytes(s));
+    for (int64_t row0 = 0; row0 < s.rows; row0 += stretch) {
+        const int rows = (int)(s.rows - row0 < stretch ? s.rows - row0 : stretch);
+        const T* xs = (const T*)x + row0 * ldx;
+        const T* dys = (const T*)dy + row0 * lddy;
+        Tile q{};
+        q.a = Operand{xs, ldx, rows};
+        q.b0 = Operand{wg, s.d_in, s.hidden};
+        q.b1 = Operand{wu, s.d_in, s.hidden};
+        q.k = s.d_in;
+        q.a2 = Operand{dys, lddy, rows};
+        q.b2 = Operand{wd, s.hidden, s.hidden};
+        q.k2 = s.d_out;
+        q.m = rows;
+        q.n = s.hidden;
+        q.out[0] = dg;
+        q.out[1] = du;
+        q.out[2] = h;
+        q.ldo = ph;
+        q.act = s.act;
+        if (int e = launch_tile<E, BWD_HIDDEN>(q, 1, st)) return e;
+        if (dx) {
+            Tile r{};
+            r.a = Operand{dg, ph, rows};
+            r.b0 = Operand{wg, s.d_in, s.d_in};
+            r.a2 = Operand{du, ph, rows};
+            r.b2 = Operand{wu, s.d_in, s.d_in};
+            r.k = s.hidden;
+            r.m = rows;
+            r.n = s.d_in;
+            r.out[0] = (T*)dx + row0 * s.d_in;
+            r.ldo = s.d_in;
+            if (int e = launch_tile<E, SUM2>(r, 1, st)) return e;
+        }
+        if (dwg) {
+            Tile r{};
+            r.a = Operand{xs, ldx, s.d_in};
+            r.b0 = Operand{dg, ph, s.hidden};
+            r.b1 = Operand{du, ph, s.hidden};
+            r.m = s.d_in;
+            r.n = s.hidden;
+            void* outs[2] = {dwg, dwu};
+            if (int e = weight_grad<E>(r, s, row0, stretch, outs, 2, pair_parts, st)) return e;
+        }
+        if (dwd) {
+            Tile r{};
+            r.a = Operand{dys, lddy, s.d_out};
+            r.b0 = Operand{h, ph, s.hidden};
+            r.m = s.d_out;
+            r.n = s.hidden;
+            void* outs[1] = {dwd};
+            if (int e = weight_grad<E>(r, s, row0, stretch, outs, 1, down_parts, st)) return e;
+        }
     }
     return GSX_OK;
 }
@@ -1510,10 +1586,10 @@ int gsx_ffn_fwd(int32_t dtype, int32_t act, int64_t rows, int32_t d_in, int32_t 
     if (misaligned(workspace, 16)) return GSX_ERR_INVALID;
     hipStream_t st = (hipStream_t)stream;
     if (dtype == GSX_F32)
-        return forward<F32>(s, x, x_stride, w_gate, w_up, w_down, y, d_out, workspace, st);
+        return forward<F32>(s, x, x_stride, w_gate, w_up, w_down, y, workspace, st);
     if (dtype == GSX_BF16)
-        return forward<BF16>(s, x, x_stride, w_gate, w_up, w_down, y, d_out, workspace, st);
-    return forward<F16>(s, x, x_stride, w_gate, w_up, w_down, y, d_out, workspace, st);
+        return forward<BF16>(s, x, x_stride, w_gate, w_up, w_down, y, workspace, st);
+    return forward<F16>(s, x, x_stride, w_gate, w_up, w_down, y, workspace, st);
 }
 
 int64_t gsx_ffn_bwd_workspace_bytes(int32_t dtype, int32_t act, int64_t rows, int32_t d_in,

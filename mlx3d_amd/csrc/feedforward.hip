@@ -44,9 +44,11 @@ constexpr int kBN = 64;   // rows of the second
 //
 // sigmoid from the hardware's power of two and reciprocal: exp(-g)'s relative
 // error, |g| 2^-24 and one unit, comes into s times 1 - s, so act(g) is within
-// two units of max(|g|, 1) 2^-24 for every g.  Phi(g): in 16 bits by Abramowitz
-// and Stegun 7.1.26 (|error| <= 0.75e-7, its exp(-g^2 / 2) the slope's too), in
-// float32, where that is too coarse for a slope near zero, from erff.
+// two units of max(|g|, 1) 2^-24 for every g.  Phi(g): in 16 bits Phi(-a) is
+// exp(-a^2 / 2) t P(t) with t = 1 / (1 + 0.3 a), P of degree seven fitted to the
+// scaled complementary error function for the least relative error (2^-21 as
+// evaluated), so the far tail keeps the type's bits, and the power serves the slope
+// too; in float32, where that is too coarse for a slope near zero, from erff.
 template <class E>
 constexpr bool kExact = sizeof(typename E::T) == 4;
 
@@ -58,11 +60,14 @@ __device__ __forceinline__ float activate(bool silu, float g, float& slope) {
         if constexpr (EXACT) {
             cdf = 0.5f * (1.0f + erff(g * 0.70710678118654752f));
         } else {
-            const float t = __builtin_amdgcn_rcpf(fmaf(fabsf(g), 0.23164189f, 1.0f));
-            float p = fmaf(t, 0.5307027145f, -0.7265760135f);
-            p = fmaf(t, p, 0.7107068705f);
-            p = fmaf(t, p, -0.142248368f);
-            p = fmaf(t, p, 0.127414796f);
+            const float t = __builtin_amdgcn_rcpf(fmaf(fabsf(g), 0.3f, 1.0f));
+            float p = fmaf(t, 0.03567432f, -0.15720116f);
+            p = fmaf(t, p, 0.20635013f);
+            p = fmaf(t, p, -0.05368054f);
+            p = fmaf(t, p, 0.12855998f);
+            p = fmaf(t, p, 0.099914f);
+            p = fmaf(t, p, 0.12075388f);
+            p = fmaf(t, p, 0.11962931f);
             const float tail = p * t * e;  // Phi(-|g|)
             cdf = g < 0.f ? tail : 1.0f - tail;
         }
@@ -1188,8 +1193,8 @@ int launch_tile(const Tile& q, int splits, hipStream_t st) {
 // array, and no more workgroups than a launch holds.  Stretches of equal length:
 // a power of two (131 072 rows of 512 float32) cost 8 %, its splits begin on the
 // same memory channels.  Gradient, us in one stretch / in stretches of 1 GB / of
-// 256 MB, 921 600 rows: 200 -> 512 -> 256 bf16 5200 / 5190 / 5250; 128 -> 1024 -> 32
-// bf16, whose workgroups take up 100 MB of sums in each, 4220 / 4550 / 5370.
+// 256 MB, 921 600 rows: 64 -> 512 -> 64 float32 11 470 / 11 670 / 12 430; 128 ->
+// 1024 -> 32 bf16, whose workgroups take up 100 MB of sums in each, 4220 / 4520 / 5370.
 constexpr int64_t kStretchBytes = 1 << 30;
 
 // Rows of a stretch that holds at most `most`, in whole tiles.

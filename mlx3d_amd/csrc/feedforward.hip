@@ -6,12 +6,11 @@
 //   dx = dg Wg + du Wu,  dWg = dg^T x,  dWu = du^T x,  dWd = dy^T h
 //
 // x (rows, d_in), Wg and Wu (hidden, d_in), Wd (d_out, hidden), row-major.
-// Products and their sums are float32 on the matrix units: 16-bit operands as
-// they are, float32 ones as three bf16 pieces each in the narrow kernels
-// (matrix_tile.h) and by the float32 instructions in the tiled ones.  h, dg and
-// du are rounded once to the tensors' type where they become operands, which in
-// 16 bits the matrix units need anyway: against 64 bits that makes 1.4 times the
-// error of one rounding at the end.
+// Products and their sums are float32 on the matrix units.  What they multiply is
+// held to float32 where the tensors are float32 (three bf16 pieces in the narrow
+// kernels, the float32 instructions in the tiled ones) and to sixteen bits, two bf16
+// pieces, for h, dg and du of 16-bit tensors (matrix_tile.h), so that 16-bit outputs
+// are rounded once, at the end, and h may be what float16 cannot hold.
 //
 // Two paths.  Narrow widths (a decoder over pixels) run the whole block in one
 // kernel, forward and backward: h, dg and du never leave the chip.  Any other
@@ -95,6 +94,7 @@ struct Operand {
     const void* p;
     int64_t ld;
     int rows;
+    const void* lo = nullptr;  // a second piece of every element, where there is one
 };
 
 // Rows in shared memory, SLOTS 16-byte slots a row, the slots turned
@@ -111,20 +111,27 @@ __device__ __forceinline__ int tile_slot(int row, int slot) {
     if constexpr (SLOTS == 8) return row * 8 + (slot ^ (b1 << 1 | b3 << 2));
     return row * SLOTS + (slot ^ (b0 << 1 | b1 << 2 | b3 << 3));
 }
-// The operand whose rows are a tile's columns c0 .. c0 + 15 and whose summed
-// index are 32 of the tile's rows (16-bit elements).
+// The operand whose rows are 16 of a tile's columns, block `block` of them, and whose
+// summed index are 32 of the tile's rows (16-bit elements).  A lane's two places
+// differ from the ones that turned_base() gives for block 0 by what the turned slots
+// change: bits of the address, flipped.
 template <int SLOTS>
-__device__ __forceinline__ u32x4 read_turned(const u32x4* tile, int c0, int lane) {
+__device__ __forceinline__ int turned_base(int lane) {
+    const int s = lane & 15, row = 8 * (lane >> 4) + (s >> 2), col = 4 * (s & 3);
+    return tile_slot<SLOTS>(row, col >> 3) * 16 + 8 * ((col >> 2) & 1);
+}
+template <int SLOTS>
+__device__ __forceinline__ u32x4 read_turned(const u32x4* tile, int block, int base) {
     using v4 = __attribute__((ext_vector_type(4))) short;
     typedef __attribute__((address_space(3))) v4* lds_v4;
-    const int s = lane & 15, row = 8 * (lane >> 4) + (s >> 2), col = c0 + 4 * (s & 3);
     union {
         v4 h[2];
         u32x4 v;
     } r;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        char* at = (char*)(tile + tile_slot<SLOTS>(row + 4 * i, col >> 3)) + 8 * ((col >> 2) & 1);
+    for (int i = 0; i < 2; ++i) {  // four rows on: with four slots a row they turn by two
+        const int flip = SLOTS == 4 ? (block ^ i) * 32 : block * 32;
+        char* at = (char*)tile + (base ^ flip) + i * 64 * SLOTS;
         r.h[i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4)at);
     }
     return r.v;
@@ -159,7 +166,8 @@ struct Stage {
     }
     // the fragment f of row block b, on this lane
     static __device__ __forceinline__ u32x4 read(const u32x4* lds, int b, int f, int lane) {
-        if constexpr (TURNED) return read_turned<SLOTS>(lds + f * 32 * SLOTS, 16 * b, lane);
+        if constexpr (TURNED)
+            return read_turned<SLOTS>(lds + f * 32 * SLOTS, b, turned_base<SLOTS>(lane));
         return lds[slot(b * 16 + (lane & 15), f * 4 + (lane >> 4))];
     }
 
@@ -276,50 +284,77 @@ __device__ __forceinline__ void clear(Acc& c) {
         for (int b = 0; b < 2; ++b) c[a][b] = f32x4{0.f, 0.f, 0.f, 0.f};
 }
 
-// c0 += A B0^T and (NB == 2) c1 += A B1^T over the summed index [k0, k1).  The
+// 16-byte slots of shared memory for a workgroup: half of a unit's, so that two
+// run on it (y of 8205 x 1365 x 512 f16 81 us, with two stages for one 107), but all
+// of it where the registers of two second operands of pieces fill a SIMD with one
+// wave (the pair of weight gradients 123, with two workgroups' registers 165).
+template <int NB, int PA, int PB>
+constexpr bool kAlone = NB == 2 && PA + PB > 2;
+template <int NB, int PA, int PB>
+constexpr int kTileSlots = (kAlone<NB, PA, PB> ? 160 : 80) * 1024 / 16;
+
+// c0 += A B0^T and (NB == 2) c1 += A B1^T over the summed index [k0, k1), of
+// operands of PA and PB pieces whose product of second pieces is left out.  The
 // next two stages' loads are in flight while one is multiplied, and shared memory
-// holds two stages, so one barrier each.  What bounds it is the time that a stage's
-// loads take to arrive (8205 x 512 x 1365 f16: 330 to 500 TFLOP/s against 1200 of
-// an 8192-wide square product): one stage ahead and two barriers took 473 us for
-// the training step instead of 343.  Tiles of 128 columns were no faster.
+// holds two stages where two workgroups a unit leave room for them, so one barrier
+// each, else one.  What bounds it is the time that a stage's
+// loads take to arrive (8205 x 512 x 1365 f16: 420 to 500 TFLOP/s, its second
+// products' three counted, against 1200 of an 8192-wide square product): one stage
+// ahead and two barriers took 473 us for the training step of one piece instead of
+// 343.  Tiles of 128 columns were no faster.
 //
 // Every stage but the last runs without bounds.  A transposed operand's may read
 // up to seven elements past its rows, which the next of the summed index holds if
 // the pitch is eight or more; below, every stage is bounded.
-template <class E, bool AKC, bool BKC, int NB>
+template <class E, bool AKC, bool BKC, int NB, int PA = 1, int PB = 1>
 __device__ __forceinline__ void multiply(u32x4* lds, const Operand& A, const Operand& B0,
                                          const Operand& B1, int m0, int n0, int64_t k0, int64_t k1,
                                          Acc& c0, Acc& c1) {
     using SA = Stage<E, kBM, AKC>;
     using SB = Stage<E, kBN, BKC>;
-    constexpr int STAGE = (kBM + NB * kBN) * 8;
-    SA a[2];
-    SB b0[2], b1[2];
+    constexpr int STAGE = (PA * kBM + NB * PB * kBN) * 8;
+    constexpr bool BOTH = 2 * STAGE <= kTileSlots<NB, PA, PB>;  // stages in shared memory
+    SA a[2][PA];
+    SB b0[2][PB], b1[2][PB];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const int wm = (wave >> 1) * 4, wn = (wave & 1) * 2;  // in blocks of 16
     const int steps = (int)((k1 - k0 + SA::STEP - 1) / SA::STEP);
     const bool inner = (AKC || A.ld >= 8) && (BKC || (B0.ld >= 8 && B1.ld >= 8));
+    auto piece = [](const Operand& o, int p) { return p ? Operand{o.lo, o.ld, o.rows} : o; };
     auto load_inner = [&](int step, int i) {
         const int64_t k = k0 + (int64_t)step * SA::STEP;
-        a[i].load_inner(A, m0, k);
-        b0[i].load_inner(B0, n0, k);
-        if constexpr (NB == 2) b1[i].load_inner(B1, n0, k);
+#pragma unroll
+        for (int p = 0; p < PA; ++p) a[i][p].load_inner(piece(A, p), m0, k);
+#pragma unroll
+        for (int p = 0; p < PB; ++p) {
+            b0[i][p].load_inner(piece(B0, p), n0, k);
+            if constexpr (NB == 2) b1[i][p].load_inner(piece(B1, p), n0, k);
+        }
     };
     auto load = [&](int step, int i) {
         if (step >= steps) return;
         const int64_t k = k0 + (int64_t)step * SA::STEP;
         const int64_t stop = k + SA::STEP < k1 ? k + SA::STEP : k1;
-        a[i].load(A, m0, k, stop);
-        b0[i].load(B0, n0, k, stop);
-        if constexpr (NB == 2) b1[i].load(B1, n0, k, stop);
+#pragma unroll
+        for (int p = 0; p < PA; ++p) a[i][p].load(piece(A, p), m0, k, stop);
+#pragma unroll
+        for (int p = 0; p < PB; ++p) {
+            b0[i][p].load(piece(B0, p), n0, k, stop);
+            if constexpr (NB == 2) b1[i][p].load(piece(B1, p), n0, k, stop);
+        }
     };
     auto step = [&](int s, int i, auto is_inner) {
-        u32x4* la = lds + i * STAGE;
-        u32x4* lb0 = la + kBM * 8;
-        u32x4* lb1 = lb0 + kBN * 8;
-        a[i].store(la);
-        b0[i].store(lb0);
-        if constexpr (NB == 2) b1[i].store(lb1);
+        u32x4* la = lds + (BOTH ? i * STAGE : 0);
+        u32x4* lb0 = la + PA * kBM * 8;
+        if constexpr (!BOTH) __syncthreads();  // the last stage's reads
+        u32x4* lb1 = lb0 + PB * kBN * 8;
+#pragma unroll
+        for (int p = 0; p < PA; ++p) a[i][p].store(la + p * kBM * 8);
+#pragma unroll
+        for (int p = 0; p < PB; ++p) {
+            b0[i][p].store(lb0 + p * kBN * 8);
+            if constexpr (NB == 2) b1[i][p].store(lb1 + p * kBN * 8);
+        }
         __syncthreads();
         if constexpr (is_inner)
             load_inner(s + 2, i);
@@ -327,23 +362,28 @@ __device__ __forceinline__ void multiply(u32x4* lds, const Operand& A, const Ope
             load(s + 2, i);
 #pragma unroll
         for (int f = 0; f < 2; ++f) {
-            u32x4 fa[4], fb[2];
+            u32x4 fa[PA][4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) fa[i] = SA::read(la, wm + i, f, lane);
+            for (int p = 0; p < PA; ++p)
 #pragma unroll
-            for (int j = 0; j < 2; ++j) fb[j] = SB::read(lb0, wn + j, f, lane);
+                for (int i = 0; i < 4; ++i) fa[p][i] = SA::read(la + p * kBM * 8, wm + i, f, lane);
+            auto with = [&](const u32x4* lb, Acc& c) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+                for (int p = PB - 1; p >= 0; --p) {
+                    u32x4 fb[2];
 #pragma unroll
-                for (int j = 0; j < 2; ++j) c0[i][j] = E::mma(fb[j], fa[i], c0[i][j]);
-            if constexpr (NB == 2) {
+                    for (int j = 0; j < 2; ++j) fb[j] = SB::read(lb + p * kBN * 8, wn + j, f, lane);
 #pragma unroll
-                for (int j = 0; j < 2; ++j) fb[j] = SB::read(lb1, wn + j, f, lane);
+                    for (int pa = p ? 0 : PA - 1; pa >= 0; --pa)
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
+                        for (int i = 0; i < 4; ++i)
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) c1[i][j] = E::mma(fb[j], fa[i], c1[i][j]);
-            }
+                            for (int j = 0; j < 2; ++j)
+                                c[i][j] = E::mma(fb[j], fa[pa][i], c[i][j]);
+                }
+            };
+            with(lb0, c0);
+            if constexpr (NB == 2) with(lb1, c1);
         }
     };
     __syncthreads();  // an earlier product's reads
@@ -385,6 +425,25 @@ __device__ __forceinline__ void put(typename E::T* p, int64_t ld, int row, int c
     }
 }
 
+// Four values that are an operand later on: float32 as they are, else two bf16
+// pieces, the second `plane` elements behind the first.
+template <class E>
+__device__ __forceinline__ void put_mid(void* p, int64_t plane, int64_t ld, int row, int col,
+                                        int rows, int cols, f32x4 v) {
+    if constexpr (std::is_same_v<E, F32>) {
+        put<F32>((float*)p, ld, row, col, rows, cols, v);
+    } else {
+        if (row >= rows || col >= cols) return;
+        const float x[4] = {v[0], v[1], v[2], v[3]};
+        uint2 w[2];
+        Second<E>::four(x, w);
+        // whole 16-byte rows: the columns up to the pitch belong to nobody else
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            *(uint2*)((uint16_t*)p + i * plane + (int64_t)row * ld + col) = w[i];
+    }
+}
+
 enum Mode {
     HIDDEN,      // out0 = act(A B0^T) (A B1^T)
     PLAIN,       // out0 = A B0^T
@@ -399,18 +458,39 @@ struct Tile {
     int64_t k, k2;        // depths
     int m, n;             // rows of A, rows of B
     void* out[3];
-    int64_t ldo;
+    int64_t ldo, plane;   // plane: from a first piece of out to its second
     int act;
     int64_t split_k;      // depth of a split (WGRAD*)
     int64_t split_out;    // floats of a split's partial sums; 0: out itself, in E
     bool add;             // to the partial sums that an earlier stretch of rows left
 };
 
+// Pieces of a tiled product's operands: of what was formed on the chip, and of the
+// tensors that it meets (float32 takes the float32 instructions, one piece each).
+template <class E>
+constexpr int kMid = std::is_same_v<E, F32> ? 1 : 2;
+template <class E>
+constexpr int kOther = std::is_same_v<E, F16> ? 2 : 1;
+
+// A product's pieces, and its shared memory: one stage or two.
 template <class E, Mode MODE>
-__global__ __launch_bounds__(kThreads, kExact<E> ? 1 : 2) void k_tile(const Tile q) {
+struct TileShape {
+    static constexpr bool SECOND = MODE != HIDDEN && MODE != BWD_HIDDEN;
+    static constexpr bool GRAD = MODE == WGRAD || MODE == WGRAD2;
+    static constexpr int PA = !SECOND ? 1 : GRAD ? kOther<E> : kMid<E>;
+    static constexpr int PB = !SECOND ? 1 : GRAD ? kMid<E> : kOther<E>;
+    static constexpr int NB = !SECOND || MODE == WGRAD2 ? 2 : 1;
+    static constexpr int STAGE = (PA * kBM + NB * PB * kBN) * 8;
+    static constexpr int BYTES = (2 * STAGE <= kTileSlots<NB, PA, PB> ? 2 : 1) * STAGE * 16;
+    static constexpr int WAVES = kExact<E> || kAlone<NB, PA, PB> ? 1 : 2;  // of a SIMD
+};
+
+template <class E, Mode MODE>
+__global__ __launch_bounds__(kThreads, (TileShape<E, MODE>::WAVES)) void k_tile(const Tile q) {
     using T = typename E::T;
-    constexpr bool dual = MODE == HIDDEN || MODE == BWD_HIDDEN || MODE == WGRAD2;
-    __shared__ u32x4 lds[2 * (kBM + (dual ? 2 : 1) * kBN) * 8];
+    using M = typename Second<E>::M;
+    using S = TileShape<E, MODE>;
+    extern __shared__ u32x4 lds[];
     const int tiles_n = (q.n + kBN - 1) / kBN;
     const uint32_t id = xcd_remap(blockIdx.x, gridDim.x);
     const int m0 = (int)(id / tiles_n) * kBM, n0 = (int)(id % tiles_n) * kBN;
@@ -424,16 +504,16 @@ __global__ __launch_bounds__(kThreads, kExact<E> ? 1 : 2) void k_tile(const Tile
             multiply<E, true, false, 1>(lds, q.a2, q.b2, q.b2, m0, n0, 0, q.k2, c2, c2);
         }
     } else if constexpr (MODE == PLAIN) {
-        multiply<E, true, true, 1>(lds, q.a, q.b0, q.b0, m0, n0, 0, q.k, c0, c0);
+        multiply<M, true, true, 1, S::PA, S::PB>(lds, q.a, q.b0, q.b0, m0, n0, 0, q.k, c0, c0);
     } else if constexpr (MODE == SUM2) {
-        multiply<E, true, false, 1>(lds, q.a, q.b0, q.b0, m0, n0, 0, q.k, c0, c0);
-        multiply<E, true, false, 1>(lds, q.a2, q.b2, q.b2, m0, n0, 0, q.k, c0, c0);
+        multiply<M, true, false, 1, S::PA, S::PB>(lds, q.a, q.b0, q.b0, m0, n0, 0, q.k, c0, c0);
+        multiply<M, true, false, 1, S::PA, S::PB>(lds, q.a2, q.b2, q.b2, m0, n0, 0, q.k, c0, c0);
     } else {
         const int64_t k0 = blockIdx.y * q.split_k;
         const int64_t k1 = k0 + q.split_k < q.k ? k0 + q.split_k : q.k;
         if constexpr (MODE == WGRAD2) clear(c1);
-        multiply<E, false, false, MODE == WGRAD2 ? 2 : 1>(lds, q.a, q.b0, q.b1, m0, n0, k0, k1, c0,
-                                                          c1);
+        multiply<M, false, false, S::NB, S::PA, S::PB>(lds, q.a, q.b0, q.b1, m0, n0, k0, k1, c0,
+                                                       c1);
     }
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const int row0 = m0 + (wave >> 1) * 64 + (lane & 15);
@@ -480,7 +560,7 @@ __global__ __launch_bounds__(kThreads, kExact<E> ? 1 : 2) void k_tile(const Tile
                     float slope;
                     h[e] = activate_any<kExact<E>>(q.act, c0[i][j][e], slope) * c1[i][j][e];
                 }
-                put<E>((T*)q.out[0], q.ldo, row, col, q.m, q.n, h);
+                put_mid<E>(q.out[0], q.plane, q.ldo, row, col, q.m, q.n, h);
             } else if constexpr (MODE == BWD_HIDDEN) {
                 f32x4 dg, du, h;
 #pragma unroll
@@ -492,13 +572,32 @@ __global__ __launch_bounds__(kThreads, kExact<E> ? 1 : 2) void k_tile(const Tile
                     du[e] = dh * a;
                     dg[e] = dh * u * slope;
                 }
-                put<E>((T*)q.out[0], q.ldo, row, col, q.m, q.n, dg);
-                put<E>((T*)q.out[1], q.ldo, row, col, q.m, q.n, du);
-                put<E>((T*)q.out[2], q.ldo, row, col, q.m, q.n, h);
+                put_mid<E>(q.out[0], q.plane, q.ldo, row, col, q.m, q.n, dg);
+                put_mid<E>(q.out[1], q.plane, q.ldo, row, col, q.m, q.n, du);
+                put_mid<E>(q.out[2], q.plane, q.ldo, row, col, q.m, q.n, h);
             } else {
                 put<E>((T*)q.out[0], q.ldo, row, col, q.m, q.n, c0[i][j]);
             }
         }
+}
+
+// The two bf16 pieces of float16 rows, in planes of `pitch` elements a row.  A few
+// us beside the products that read them: splitting in their stages would be done
+// again by every tile.
+__global__ __launch_bounds__(kThreads) void k_pieces(const uint16_t* x, int64_t ld, int64_t rows,
+                                                     int cols, int pitch, uint16_t* out) {
+    const int pairs = (cols + 1) / 2;
+    const int64_t n = rows * pairs, step = (int64_t)gridDim.x * kThreads, plane = rows * pitch;
+    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < n; i += step) {
+        const int64_t row = i / pairs;
+        const int col = (int)(i % pairs) * 2;
+        const uint16_t* at = x + row * ld + col;
+        uint32_t w[2];
+        split_two<false>(F16::up(at[0]), col + 1 < cols ? F16::up(at[1]) : 0.f, &w[0], &w[1]);
+        uint32_t* to = (uint32_t*)(out + row * pitch + col);
+        to[0] = w[0];
+        to[plane / 2] = w[1];
+    }
 }
 
 // Adds up the splits' partial sums in their order.  5 us for 512 x 1365 f16.
@@ -527,8 +626,9 @@ __global__ __launch_bounds__(kThreads) void k_zero_bytes(uint8_t* p, int64_t n) 
 // 921 600 rows of 32 -> 128 -> 64 float32: 177 us, 2.0 TB/s; bound by the matrix
 // units, whose six bf16 products for one float32 run at 1.02 PFLOP/s, 82 % of what
 // a large product reaches (the float32 instructions would take 196 us at best).
-// 2 073 600 rows of 32 -> 96 -> 48 bf16: 104 us, 3.2 TB/s; bound by the vector
-// units (activations, conversions), the copy of its bytes would take 69.
+// 2 073 600 rows of 32 -> 96 -> 48 bf16: 122 us, 2.7 TB/s; bound by the vector
+// units (activations, h's two pieces), the copy of its bytes would take 69; with h
+// rounded to bf16 it took 104.
 //
 // Products run with the weights first, so that a lane holds one row (its column
 // of the product) and consecutive channels: g^T and u^T come out with channels
@@ -551,12 +651,28 @@ struct Narrow {
     int chunks, resident;  // chunks of 32 hidden channels, how many are staged at a time
 };
 
+// A chunk in shared memory: the fragments of Wg and Wu with their pieces, then those
+// of Wd, 64 lanes' 16 bytes each.
+template <class E, int KD, int OB>
+struct FwdShape {
+    static constexpr int PC = Wide<E>::PIECES, PO = Second<E>::OTHER;
+    static constexpr int CHUNK = 4 * KD * PC + OB * PO;
+    static __device__ __forceinline__ int in(int c, int frag, int p) {
+        return (c * CHUNK + frag * PC + p) * 64;
+    }
+    static __device__ __forceinline__ int out(int c, int o, int p) {
+        return (c * CHUNK + 4 * KD * PC + o * PO + p) * 64;
+    }
+};
+
 // Stages `count` chunks from number c0 on: for each chunk, fragments of Wg (two
 // blocks of 16 channels times KD), of Wu, then OB of Wd, each with its pieces.
 template <class E, int KD, int OB>
 __device__ __forceinline__ void stage_weights(const Narrow<E>& q, u32x4* lds, int c0, int count) {
     using Wd = Wide<E>;
-    constexpr int PC = Wd::PIECES, FRAGS = 4 * KD + OB;
+    using S2 = Second<E>;
+    using L = FwdShape<E, KD, OB>;
+    constexpr int FRAGS = 4 * KD + OB;
     for (int i = threadIdx.x; i < count * FRAGS * 64; i += kNarrowThreads) {
         const int lane = i & 63, frag = (i >> 6) % FRAGS, c = (i >> 6) / FRAGS;
         const int r = lane & 15, k8 = (lane >> 4) * 8;
@@ -568,14 +684,18 @@ __device__ __forceinline__ void stage_weights(const Narrow<E>& q, u32x4* lds, in
             if (f < q.hidden && k < q.d_in)
                 raw = load8<E>((which < 2 ? q.wg : q.wu) + (int64_t)f * q.d_in + k, q.d_in - k,
                                q.hidden - 1 - f);
+            const typename Wd::Frag w = Wd::frag(raw);
+#pragma unroll
+            for (int p = 0; p < Wd::PIECES; ++p) lds[L::in(c, frag, p) + lane] = w.p[p];
         } else {
             const int o = (frag - 4 * KD) * 16 + r, k = (c0 + c) * 32 + k8;
             if (o < q.d_out && k < q.hidden)
                 raw = load8<E>(q.wd + (int64_t)o * q.hidden + k, q.hidden - k, q.d_out - 1 - o);
-        }
-        const typename Wd::Frag w = Wd::frag(raw);
+            const typename S2::Other w = S2::other(raw);
 #pragma unroll
-        for (int p = 0; p < PC; ++p) lds[((c * FRAGS + frag) * PC + p) * 64 + lane] = w.p[p];
+            for (int p = 0; p < S2::OTHER; ++p)
+                lds[L::out(c, frag - 4 * KD, p) + lane] = w.p[p];
+        }
     }
 }
 
@@ -583,7 +703,8 @@ template <class E, int KD, int OB, bool GELU>
 __global__ __launch_bounds__(kNarrowThreads) void k_narrow_fwd(const Narrow<E> q) {
     using T = typename E::T;
     using W = Wide<E>;
-    constexpr int PC = W::PIECES, FRAGS = 4 * KD + OB;
+    using S2 = Second<E>;
+    using L = FwdShape<E, KD, OB>;
     constexpr int kWaves = kNarrowThreads / 64, R = kNarrowRows / 16;
     extern __shared__ u32x4 smem[];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
@@ -592,7 +713,7 @@ __global__ __launch_bounds__(kNarrowThreads) void k_narrow_fwd(const Narrow<E> q
     auto weights = [&](int c, int frag) {
         typename W::Frag w;
 #pragma unroll
-        for (int p = 0; p < PC; ++p) w.p[p] = smem[((c * FRAGS + frag) * PC + p) * 64 + lane];
+        for (int p = 0; p < W::PIECES; ++p) w.p[p] = smem[L::in(c, frag, p) + lane];
         return w;
     };
     if (once) {
@@ -643,7 +764,7 @@ __global__ __launch_bounds__(kNarrowThreads) void k_narrow_fwd(const Narrow<E> q
                             u[b][r] = W::mma(wu, x[r][kd], u[b][r]);
                         }
                     }
-                typename W::Frag h[R];
+                typename S2::Mid h[R];
 #pragma unroll
                 for (int r = 0; r < R; ++r) {
                     float v[8], slope;
@@ -651,14 +772,16 @@ __global__ __launch_bounds__(kNarrowThreads) void k_narrow_fwd(const Narrow<E> q
                     for (int i = 0; i < 8; ++i)
                         v[i] = activate<GELU, kExact<E>>(silu, g[i >> 2][r][i & 3], slope) *
                                u[i >> 2][r][i & 3];
-                    h[r] = W::frag(v);
+                    h[r] = S2::mid(v);
                 }
 #pragma unroll
                 for (int o = 0; o < OB; ++o)
                     if (o * 16 < q.d_out) {
-                        const auto wd = weights(c, 4 * KD + o);
+                        typename S2::Other wd;
 #pragma unroll
-                        for (int r = 0; r < R; ++r) y[o][r] = W::mma(wd, h[r], y[o][r]);
+                        for (int p = 0; p < S2::OTHER; ++p) wd.p[p] = smem[L::out(c, o, p) + lane];
+#pragma unroll
+                        for (int r = 0; r < R; ++r) y[o][r] = S2::mma(wd, h[r], y[o][r]);
                     }
             }
         }
@@ -695,11 +818,12 @@ __global__ __launch_bounds__(kNarrowThreads) void k_narrow_fwd(const Narrow<E> q
 // elements) the weight gradients'.  The pairs' parts of dx are added up there
 // too.  Two barriers a tile; the next tile's loads are in flight meanwhile.
 //
-// 921 600 rows of 32 -> 128 -> 64: bf16 158 us, 1.9 TB/s, vector units 68 % busy;
-// float32 430 us (matrix units, the pieces' conversions and shared memory in about
-// equal parts).  One wave for the 32 channels instead of a pair needs twice the
-// registers; with half the waves a SIMD the training step took 414 us instead of
-// 225, float32 870 instead of 656.
+// 921 600 rows of 32 -> 128 -> 64: bf16 240 us, 1.2 TB/s (shared memory, which dg, du
+// and h pass in two pieces, and the vector units in about equal parts; 150 with one
+// piece); float32 490 us (matrix units, the pieces' conversions and shared memory).
+// One wave for the 32 channels instead of a pair needs twice the registers; with half
+// the waves a SIMD the training step took 414 us instead of 225 (in one piece),
+// float32 870 instead of 656.
 //
 // More than 4 x 32 hidden channels run as groups, each with its part of dx;
 // the workgroups' weight gradients and the groups' dx are added up in a fixed
@@ -725,21 +849,25 @@ __device__ __forceinline__ int sum_slot(int row, int slot) {
     return row * SLOTS + (slot ^ (row & (SLOTS - 1)));
 }
 
+// A staged tile's planes: the pieces of the first products' operands, and those of
+// the second ones where they are others (float16, whose bf16 pieces are formed once
+// for all waves).
 template <class E, int KD, int KO>
 struct BwdShape {
-    static constexpr int PC = Wide<E>::PIECES;
-    static constexpr int XS = 4 * KD, YS = 4 * KO;          // slots of a row of x, of dy
-    static constexpr int TILE = kBwdRows * (XS + YS) * PC;  // 16-byte slots of a staged tile
-    static constexpr int GATE = kBwdRows * 4 * PC;          // of a pair's dg, du or h
-    static constexpr int SUM = kBwdRows * 8 * KD;           // of a pair's part of dx
-    static constexpr int SUMS = 16 * KD + 8 * KO;           // weight gradient registers
+    static constexpr int PC = Wide<E>::PIECES, PM = Second<E>::MID, PO = Second<E>::OTHER;
+    static constexpr int AT = std::is_same_v<E, F16> ? 1 : 0, PLANES = AT ? 3 : PC;
+    static constexpr int XS = 4 * KD, YS = 4 * KO;              // slots of a row of x, of dy
+    static constexpr int TILE = kBwdRows * (XS + YS) * PLANES;  // 16-byte slots of a staged tile
+    static constexpr int GATE = kBwdRows * 4 * PM;              // of a pair's dg, du or h
+    static constexpr int SUM = kBwdRows * 8 * KD;               // of a pair's part of dx
+    static constexpr int SUMS = 16 * KD + 8 * KO;               // weight gradient registers
     static int64_t lds(int pairs) { return 16 * (2 * TILE + (int64_t)pairs * (3 * GATE + SUM)); }
 };
 
 // Waves for a SIMD that the registers leave room for: one workgroup or two.
 template <class E, int KD, int KO>
 constexpr int bwd_waves() {
-    return sizeof(typename E::T) == 4 || KD > 1 || KO > 2 ? 2 : 4;
+    return std::is_same_v<E, BF16> && KD == 1 && KO <= 2 ? 4 : 2;
 }
 
 template <class E, int KD, int KO, bool GELU>
@@ -748,8 +876,11 @@ void k_narrow_bwd(const NarrowBwd<E> q) {
     using T = typename E::T;
     using W = Wide<E>;
     using S = BwdShape<E, KD, KO>;
+    using S2 = Second<E>;
     using Frag = typename W::Frag;
-    constexpr int PC = S::PC, R = kBwdRows / 16;
+    using Mid = typename S2::Mid;
+    using Other = typename S2::Other;
+    constexpr int PC = S::PC, PM = S::PM, R = kBwdRows / 16;
     extern __shared__ u32x4 smem[];
     const int threads = blockDim.x, pairs = threads >> 7;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -763,7 +894,8 @@ void k_narrow_bwd(const NarrowBwd<E> q) {
 
     // the wave's weights: its 16 channels' rows (operands of x and of dy), and the
     // pair's 32 channels for every other 16 of dx's
-    Frag wg[KD], wu[KD], wd[KO], wgt[KD], wut[KD];
+    Frag wg[KD], wu[KD], wd[KO];
+    Other wgt[KD], wut[KD];
     {
         auto gather = [&](const T* w, int64_t first, int64_t step, int n) {
             typename W::Raw raw;
@@ -771,7 +903,7 @@ void k_narrow_bwd(const NarrowBwd<E> q) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[i] = i < n ? w[first + i * step] : (T)0;
             __builtin_memcpy(&raw, v, sizeof(raw));
-            return W::frag(raw);
+            return raw;
         };
         const int f = f0 + 16 * half + col;
         const bool there = f < q.hidden;
@@ -790,75 +922,17 @@ void k_narrow_bwd(const NarrowBwd<E> q) {
 #pragma unroll
         for (int ko = 0; ko < KO; ++ko) {
             const int o = ko * 32 + k8;
-            wd[ko] = gather(q.wd, (int64_t)o * q.hidden + f, q.hidden, there ? q.d_out - o : 0);
+            wd[ko] = W::frag(gather(q.wd, (int64_t)o * q.hidden + f, q.hidden,
+                                    there ? q.d_out - o : 0));
         }
 #pragma unroll
         for (int j = 0; j < KD; ++j) {
             const int d = 16 * (2 * j + half) + col, f8 = f0 + k8;
             const int n = d < q.d_in ? q.hidden - f8 : 0;
-            wgt[j] = gather(q.wg, (int64_t)f8 * q.d_in + d, q.d_in, n);
-            wut[j] = gather(q.wu, (int64_t)f8 * q.d_in + d, q.d_in, n);
+            wgt[j] = S2::other(gather(q.wg, (int64_t)f8 * q.d_in + d, q.d_in, n));
+            wut[j] = S2::other(gather(q.wu, (int64_t)f8 * q.d_in + d, q.d_in, n));
         }
     }
-
-    // staging: pieces of eight elements of x's and dy's rows, HELD of them in a
-    // thread's registers one tile ahead
-    constexpr int PIECES = kBwdRows * (S::XS + S::YS);
-    constexpr int HELD = (PIECES + 128 * kBwdPairs - 1) / (128 * kBwdPairs);
-    const int rows = (int)q.rows, step = (int)gridDim.x * kBwdRows;
-    struct Piece {
-        const T* p;    // in the next tile to be read
-        int64_t hop;   // from a tile to the next
-        int row, n;    // its row; how many elements the row has from here on
-        int slot;      // its place in the staged tile
-    };
-    auto piece_of = [&](int n, int row0) {
-        const bool of_x = n < kBwdRows * S::XS;
-        const int i = of_x ? n : n - kBwdRows * S::XS;
-        const int slots = of_x ? S::XS : S::YS, row = i / slots, k = i % slots * 8;
-        const int64_t ld = of_x ? q.ldx : q.lddy;
-        Piece m;
-        m.row = row0 + row;
-        m.p = (of_x ? q.x : q.dy) + (int64_t)m.row * ld + k;
-        m.hop = step * ld;
-        m.n = (of_x ? q.d_in : q.d_out) - k;
-        m.slot = of_x ? tile_slot<S::XS>(row, i % S::XS)
-                      : PC * kBwdRows * S::XS + tile_slot<S::YS>(row, i % S::YS);
-        return m;
-    };
-    auto fetch = [&](const Piece& m) {
-        typename W::Raw raw{};
-        if (m.row < rows && m.n > 0) raw = load8<E>(m.p, m.n, rows - 1 - m.row);
-        return raw;
-    };
-    auto settle = [&](u32x4* tile, const Piece& m, bool of_x, const typename W::Raw& raw) {
-        const Frag f = W::frag(raw);
-        const int pitch = kBwdRows * (of_x ? S::XS : S::YS);
-#pragma unroll
-        for (int p = 0; p < PC; ++p) tile[m.slot + p * pitch] = f.p[p];
-    };
-    Piece mine[HELD];
-    typename W::Raw next[HELD];
-    auto fetch_all = [&] {
-#pragma unroll
-        for (int i = 0; i < HELD; ++i)
-            if (threadIdx.x + i * threads < PIECES) {
-                next[i] = fetch(mine[i]);
-                mine[i].p += mine[i].hop;
-                mine[i].row += step;
-            }
-    };
-    auto settle_all = [&](u32x4* tile, int row0) {
-#pragma unroll
-        for (int i = 0; i < HELD; ++i) {
-            const int n = threadIdx.x + i * threads;
-            if (n < PIECES) settle(tile, mine[i], n < kBwdRows * S::XS, next[i]);
-        }
-        for (int n = threadIdx.x + HELD * threads; n < PIECES; n += threads) {  // fewer pairs
-            const Piece m = piece_of(n, row0);
-            settle(tile, m, n < kBwdRows * S::XS, fetch(m));
-        }
-    };
 
     // no work is moved over these places where the registers hold what is asked for
     constexpr bool EARLY = PC == 3 && KD == 1;
@@ -871,45 +945,121 @@ void k_narrow_bwd(const NarrowBwd<E> q) {
         if constexpr (!EARLY) __builtin_amdgcn_sched_barrier(0);
     };
 
+    // staging: pieces of eight elements of x's and dy's rows, HELD of them in a
+    // thread's registers one tile ahead
+    constexpr int PIECES = kBwdRows * (S::XS + S::YS);
+    constexpr int HELD = (PIECES + 128 * kBwdPairs - 1) / (128 * kBwdPairs);
+    const int rows = (int)q.rows, step = (int)gridDim.x * kBwdRows;
+    struct Piece {  // number n of a tile
+        bool of_x;
+        int row, k;  // in the tile; the first element
+        __device__ __forceinline__ explicit Piece(int n) {
+            of_x = n < kBwdRows * S::XS;
+            const int i = of_x ? n : n - kBwdRows * S::XS, slots = of_x ? S::XS : S::YS;
+            row = i / slots;
+            k = i % slots * 8;
+        }
+    };
+    auto ld_of = [&](const Piece& m) { return m.of_x ? q.ldx : q.lddy; };
+    auto at = [&](const Piece& m, int row) {
+        return (m.of_x ? q.x : q.dy) + row * ld_of(m) + m.k;
+    };
+    auto fetch = [&](const Piece& m, const T* p, int row) {
+        typename W::Raw raw{};
+        const int n = (m.of_x ? q.d_in : q.d_out) - m.k;
+        if (row < rows && n > 0) raw = load8<E>(p, n, rows - 1 - row);
+        return raw;
+    };
+    auto settle = [&](u32x4* tile, const Piece& m, const typename W::Raw& raw) {
+        const Frag f = W::frag(raw);
+        const int pitch = kBwdRows * (m.of_x ? S::XS : S::YS);
+        tile += m.of_x ? tile_slot<S::XS>(m.row, m.k / 8)
+                       : S::PLANES * kBwdRows * S::XS + tile_slot<S::YS>(m.row, m.k / 8);
+#pragma unroll
+        for (int p = 0; p < PC; ++p) tile[p * pitch] = f.p[p];
+        if constexpr (S::AT > 0) {
+            const Other o = S2::other(raw);
+#pragma unroll
+            for (int p = 0; p < S::PO; ++p) tile[(S::AT + p) * pitch] = o.p[p];
+        }
+    };
+    // what a piece's number says is formed again for every tile where registers are
+    // short
+    auto number = [&](int i) {
+        const int n = threadIdx.x + i * threads;
+        return EARLY ? n : here(n);
+    };
+    const T* from[HELD];  // in the next tile to be read
+    int from_row = 0;     // its first row
+    typename W::Raw next[HELD];
+    auto fetch_all = [&] {
+#pragma unroll
+        for (int i = 0; i < HELD; ++i)
+            if (threadIdx.x + i * threads < PIECES) {
+                const Piece m(number(i));
+                next[i] = fetch(m, from[i], from_row + m.row);
+                from[i] += step * ld_of(m);
+            }
+        from_row += step;
+    };
+    auto settle_all = [&](u32x4* tile, int row0) {
+#pragma unroll
+        for (int i = 0; i < HELD; ++i)
+            if (threadIdx.x + i * threads < PIECES) settle(tile, Piece(number(i)), next[i]);
+        for (int n = threadIdx.x + HELD * threads; n < PIECES; n += threads) {  // fewer pairs
+            const Piece m(n);
+            settle(tile, m, fetch(m, at(m, row0 + m.row), row0 + m.row));
+        }
+    };
+
     f32x4 sg[2 * KD], su[2 * KD], sd[2 * KO];  // the weight gradients' sums
 #pragma unroll
     for (int d = 0; d < 2 * KD; ++d) sg[d] = su[d] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int o = 0; o < 2 * KO; ++o) sd[o] = f32x4{0.f, 0.f, 0.f, 0.f};
 
+    // a lane's places in a tile: the row of the first products' operand (its next four
+    // slots: bits flipped), the columns of the second ones'
+    const int x_at = tile_slot<S::XS>(col, quad), y_at = tile_slot<S::YS>(col, quad);
+    const int turned4 = turned_base<4>(lane);
+    const int turned_xs = turned_base<S::XS>(lane), turned_ys = turned_base<S::YS>(lane);
     int row0 = (int)blockIdx.x * kBwdRows;
 #pragma unroll
     for (int i = 0; i < HELD; ++i)
-        if (threadIdx.x + i * threads < PIECES) mine[i] = piece_of(threadIdx.x + i * threads, row0);
+        if (threadIdx.x + i * threads < PIECES) {
+            const Piece m(threadIdx.x + i * threads);
+            from[i] = at(m, row0 + m.row);
+        }
+    from_row = row0;
     fetch_all();
     settle_all(tiles, row0);
     fetch_all();
     __syncthreads();
     for (int turn = 0; row0 < rows; row0 += step, turn ^= 1) {
         const u32x4* xt = tiles + turn * S::TILE;
-        const u32x4* yt = xt + PC * kBwdRows * S::XS;
+        const u32x4* yt = xt + S::PLANES * kBwdRows * S::XS;
         // where the registers allow it, a phase asks shared memory for all that it
         // needs first, and its products begin with the first answer
         Frag fx[R][KD], fy[R][KO];
         auto ask = [&](int r) {
-            const int row = 16 * r + col;
+            const int x0 = EARLY ? x_at : here(x_at), y0 = EARLY ? y_at : here(y_at);
 #pragma unroll
             for (int kd = 0; kd < KD; ++kd)
 #pragma unroll
                 for (int p = 0; p < PC; ++p)
-                    fx[r][kd].p[p] = xt[p * kBwdRows * S::XS + tile_slot<S::XS>(row, kd * 4 + quad)];
+                    fx[r][kd].p[p] = xt[(p * kBwdRows + 16 * r) * S::XS + (x0 ^ 4 * kd)];
 #pragma unroll
             for (int ko = 0; ko < KO; ++ko)
 #pragma unroll
                 for (int p = 0; p < PC; ++p)
-                    fy[r][ko].p[p] = yt[p * kBwdRows * S::YS + tile_slot<S::YS>(row, ko * 4 + quad)];
+                    fy[r][ko].p[p] = yt[(p * kBwdRows + 16 * r) * S::YS + (y0 ^ 4 * ko)];
         };
         if constexpr (EARLY) {
 #pragma unroll
             for (int r = 0; r < R; ++r) ask(r);
             asked();
         }
-        uint2 gate[R][3][PC];
+        uint2 gate[R][3][PM];
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             if constexpr (!EARLY) ask(r);
@@ -931,7 +1081,7 @@ void k_narrow_bwd(const NarrowBwd<E> q) {
                 v[2][i] = a * u[i];
             }
 #pragma unroll
-            for (int j = 0; j < 3; ++j) W::four(v[j], gate[r][j]);
+            for (int j = 0; j < 3; ++j) S2::four(v[j], gate[r][j]);
             pause();
         }
         // lanes of neighbouring quads hold channels 0-3 and 4-7 of the same two
@@ -939,7 +1089,7 @@ void k_narrow_bwd(const NarrowBwd<E> q) {
 #pragma unroll
         for (int j = 0; j < 3; ++j)
 #pragma unroll
-            for (int p = 0; p < PC; ++p) {
+            for (int p = 0; p < PM; ++p) {
                 const auto lo = __builtin_amdgcn_permlane16_swap(gate[0][j][p].x, gate[1][j][p].x,
                                                                  false, false);
                 const auto hi = __builtin_amdgcn_permlane16_swap(gate[0][j][p].y, gate[1][j][p].y,
@@ -951,22 +1101,23 @@ void k_narrow_bwd(const NarrowBwd<E> q) {
         __syncthreads();
         // the pair's part of dx, every other 16 of its channels, and the weight
         // gradients, whose operands lie along the rows
-        Frag fg[R], fu[R], t[3];
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
+        Mid fg[R], fu[R], t[3];
+        auto ask_gates = [&](int r) {
             const int row = 16 * r + col;
 #pragma unroll
-            for (int p = 0; p < PC; ++p) {
+            for (int p = 0; p < PM; ++p) {
                 fg[r].p[p] = gates[p * kBwdRows * 4 + tile_slot<4>(row, quad)];
                 fu[r].p[p] = gates[S::GATE + p * kBwdRows * 4 + tile_slot<4>(row, quad)];
             }
-        }
+        };
         auto turn_gate = [&](int j) {
 #pragma unroll
-            for (int p = 0; p < PC; ++p)
-                t[j].p[p] = read_turned<4>(gates + j * S::GATE + p * kBwdRows * 4, 16 * half, lane);
+            for (int p = 0; p < PM; ++p)
+                t[j].p[p] = read_turned<4>(gates + j * S::GATE + p * kBwdRows * 4, half, turned4);
         };
         if constexpr (EARLY) {
+#pragma unroll
+            for (int r = 0; r < R; ++r) ask_gates(r);
             turn_gate(0);
             turn_gate(1);
             turn_gate(2);
@@ -975,31 +1126,36 @@ void k_narrow_bwd(const NarrowBwd<E> q) {
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             const int row = 16 * r + col;
+            if constexpr (!EARLY) ask_gates(r);
 #pragma unroll
             for (int j = 0; j < KD; ++j) {
                 f32x4 d{0.f, 0.f, 0.f, 0.f};
-                d = W::mma(wgt[j], fg[r], d);
-                d = W::mma(wut[j], fu[r], d);
+                d = S2::mma(wgt[j], fg[r], d);
+                d = S2::mma(wut[j], fu[r], d);
                 sums[pair * S::SUM + sum_slot<8 * KD>(row, (2 * j + half) * 4 + quad)] =
                     __builtin_bit_cast(u32x4, d);
             }
+            pause();
         }
-        pause();
-        auto turned_x = [&](int db) {
-            Frag x;
+        // 16 channels of x or dy along the rows; where registers are short the
+        // places are formed again for every tile, too
+        const int at_x = EARLY ? turned_xs : here(turned_xs);
+        const int at_y = EARLY ? turned_ys : here(turned_ys);
+        auto turned = [&](const u32x4* tile, auto slots, int block, int base) {
+            constexpr int SLOTS = decltype(slots)::value;
+            Other o;
 #pragma unroll
-            for (int p = 0; p < PC; ++p)
-                x.p[p] = read_turned<S::XS>(xt + p * kBwdRows * S::XS, 16 * db, lane);
-            return x;
+            for (int p = 0; p < S::PO; ++p)
+                o.p[p] = read_turned<SLOTS>(tile + (S::AT + p) * kBwdRows * SLOTS, block, base);
+            return o;
+        };
+        auto turned_x = [&](int db) {
+            return turned(xt, std::integral_constant<int, S::XS>{}, db, at_x);
         };
         auto turned_y = [&](int ob) {
-            Frag y;
-#pragma unroll
-            for (int p = 0; p < PC; ++p)
-                y.p[p] = read_turned<S::YS>(yt + p * kBwdRows * S::YS, 16 * ob, lane);
-            return y;
+            return turned(yt, std::integral_constant<int, S::YS>{}, ob, at_y);
         };
-        Frag ahead;  // the next block's operand
+        Other ahead;  // the next block's operand
         if constexpr (EARLY) {
             ahead = turned_x(0);
         } else {
@@ -1009,7 +1165,7 @@ void k_narrow_bwd(const NarrowBwd<E> q) {
         asked();
 #pragma unroll
         for (int db = 0; db < 2 * KD; ++db) {
-            Frag x;
+            Other x;
             if constexpr (EARLY) {
                 x = ahead;
                 ahead = db + 1 < 2 * KD ? turned_x(db + 1) : turned_y(0);
@@ -1017,14 +1173,14 @@ void k_narrow_bwd(const NarrowBwd<E> q) {
             } else {
                 x = turned_x(db);
             }
-            sg[db] = W::mma(x, t[0], sg[db]);
-            su[db] = W::mma(x, t[1], su[db]);
+            sg[db] = S2::mma(x, t[0], sg[db]);
+            su[db] = S2::mma(x, t[1], su[db]);
         }
         pause();
         if constexpr (!EARLY) turn_gate(2);
 #pragma unroll
         for (int ob = 0; ob < 2 * KO; ++ob) {
-            Frag y;
+            Other y;
             if constexpr (EARLY) {
                 y = ahead;
                 if (ob + 1 < 2 * KO) ahead = turned_y(ob + 1);
@@ -1032,7 +1188,7 @@ void k_narrow_bwd(const NarrowBwd<E> q) {
             } else {
                 y = turned_y(ob);
             }
-            sd[ob] = W::mma(y, t[2], sd[ob]);
+            sd[ob] = S2::mma(y, t[2], sd[ob]);
         }
         // the next tile into the other place, then the pairs' parts of dx
         settle_all(tiles + (turn ^ 1) * S::TILE, row0 + step);
@@ -1182,7 +1338,11 @@ template <class E, Mode MODE>
 int launch_tile(const Tile& q, int splits, hipStream_t st) {
     const int64_t n = tiles(q.m, q.n);
     if (n * splits > kMostGroups) return GSX_ERR_TOO_LARGE;
-    hipLaunchKernelGGL((k_tile<E, MODE>), dim3((unsigned)n, (unsigned)splits), dim3(kThreads), 0,
+    constexpr int lds = TileShape<E, MODE>::BYTES;
+    if (hipFuncSetAttribute((const void*)k_tile<E, MODE>,
+                            hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess)
+        return GSX_ERR_HIP;
+    hipLaunchKernelGGL((k_tile<E, MODE>), dim3((unsigned)n, (unsigned)splits), dim3(kThreads), lds,
                        st, q);
     GSX_LAUNCH_CHECK();
     return GSX_OK;
@@ -1206,24 +1366,27 @@ int64_t even_stretch(int64_t rows, int64_t most, int tile) {
     return up_to((rows + count - 1) / count, tile);
 }
 
-// hidden's row pitch in the workspace: whole 16-byte pieces
-int64_t pitch(const Shape& s) { return up_to(s.hidden, 8); }
+// A row's pitch in the workspace: whole 16-byte pieces.  Four bytes an element,
+// float32 or two bf16 pieces.
+int64_t pitch(int width) { return up_to(width, 8); }
+int64_t pitch(const Shape& s) { return pitch(s.hidden); }
+int64_t held_bytes(int64_t rows, int width) { return up_to(rows * pitch(width) * 4, 256); }
 int64_t tiled_stretch(const Shape& s) {
     const int wide = s.hidden > s.d_out ? (s.hidden > s.d_in ? s.hidden : s.d_in)
                                         : (s.d_out > s.d_in ? s.d_out : s.d_in);
-    const int64_t fit = kStretchBytes / (pitch(s) * s.size());
+    // (float16 rows' pieces stand beside the hidden channels)
+    const int64_t fit = kStretchBytes / (4 * (s.dtype == GSX_F16 ? pitch(wide) : pitch(s)));
     const int64_t most = kMostGroups / (up_to(wide, kBN) / kBN) * kBM;
     return even_stretch(s.rows, fit < most ? fit : most, kBM);
 }
-int64_t hidden_bytes(const Shape& s) {
-    return up_to(tiled_stretch(s) * pitch(s) * s.size(), 256);
-}
+int64_t hidden_bytes(const Shape& s) { return held_bytes(tiled_stretch(s), s.hidden); }
 
 // Whether the narrow kernel holds a row's operands and sums in its registers:
 // 8 (KD pieces + OB) of them, beside some 100 others.
 constexpr bool narrow_fits(int pieces, int kd, int ob) { return 8 * (kd * pieces + ob) <= 152; }
 int64_t narrow_chunk_bytes(const Shape& s, int kd, int ob) {
-    return (s.dtype == GSX_F32 ? 3 : 1) * (int64_t)(4 * kd + ob) * 1024;
+    const int in = s.dtype == GSX_F32 ? 3 : 1, out = s.dtype == GSX_BF16 ? 1 : in + 1;
+    return (int64_t)(4 * kd * in + ob * (s.dtype == GSX_F32 ? 3 : out)) * 1024;
 }
 int narrow_kd(const Shape& s) { return s.d_in <= 32 ? 1 : s.d_in <= 64 ? 2 : 4; }
 int narrow_ob(const Shape& s) {
@@ -1232,8 +1395,9 @@ int narrow_ob(const Shape& s) {
 // Weights that shared memory holds whole are staged once; others by every
 // workgroup for every 256 rows, which many rows have to pay for.  Against the
 // tiled path, us a call (131 072, 16 384, 64 rows): 32 -> 128 -> 64 float32, held
-// whole, 32 / 85, 19 / 22, 19 / 22; 128 -> 1024 -> 64 float32 419 / 904, 202 / 144,
-// 191 / 58; 128 -> 512 -> 64 bf16 74 / 113, 34 / 23, 30 / 22.
+// whole, 33 / 84, 17 / 24, 15 / 23; 128 -> 1024 -> 64 float32 431 / 918, 200 / 142,
+// 190 / 58; 128 -> 512 -> 64 bf16 86 / 175, 36 / 29, 33 / 21, f16 93 / 185, 39 / 33,
+// 37 / 24.
 constexpr int64_t kStreamRows = 32768;
 
 bool narrow_fwd(const Shape& s) {
@@ -1245,7 +1409,8 @@ bool narrow_fwd(const Shape& s) {
 }
 
 int64_t fwd_bytes(const Shape& s) {
-    return s.rows == 0 || narrow_fwd(s) ? 0 : hidden_bytes(s);
+    if (s.rows == 0 || narrow_fwd(s)) return 0;
+    return hidden_bytes(s) + (s.dtype == GSX_F16 ? held_bytes(s.d_out, s.hidden) : 0);
 }
 
 template <class E, int KD, int OB>
@@ -1292,6 +1457,13 @@ int narrow_forward(const Shape& s, A... a) {
     }
 }
 
+// The float16 backward's pieces: of a stretch of x and of dy, of both pair weights.
+int64_t pieces_bytes(const Shape& s) {
+    if (s.dtype != GSX_F16) return 0;
+    return held_bytes(tiled_stretch(s), s.d_in) + held_bytes(tiled_stretch(s), s.d_out) +
+           2 * held_bytes(s.hidden, s.d_in);
+}
+
 // One split of one stretch leaves the gradient itself; else each leaves partial
 // sums, kept over the stretches.
 bool direct_grad(const Shape& s, int m) {
@@ -1310,18 +1482,19 @@ int64_t parts_bytes(const Shape& s) {
 
 // The narrow backward: which widths fit its registers (weights in both orders
 // and their gradients' sums), its workgroups and its workspace.
-constexpr bool narrow_bwd_fits(int pieces, int kd, int ko) {
-    return pieces == 3 ? kd + ko <= 3 : kd < 4 || ko <= 2;
+constexpr bool narrow_bwd_fits(int dtype, int kd, int ko) {
+    return dtype == GSX_F32 ? kd + ko <= 3 : kd < 4 || (dtype == GSX_BF16 && ko <= 2);
 }
-// Faster than the tiled path wherever its registers hold the widths, us a call
-// (131 072 and 64 rows): 32 -> 128 -> 64 float32 81 / 586 and 57 / 102 (the host's
-// time), 32 -> 512 -> 64, four groups, 264 / 1592, bf16 108 / 465; hidden widths
-// are bounded by the groups' parts of dx, a float32 array of x's size each.
+// Faster than the tiled path wherever its registers and shared memory hold the
+// widths, us a call (131 072 rows; of few the host's 100 in both): 32 -> 128 -> 64
+// float32 101 / 591, bf16 96 / 350, f16 98 / 441; 32 -> 512 -> 64, four groups,
+// 276 / 1604, 155 / 732, 202 / 857; 128 -> 512 -> 64 bf16 417 / 788.  Hidden widths
+// are bounded by the groups' parts of dx, a float32 array of a stretch of x each.
 constexpr int kNarrowHidden = 2048;
 int narrow_ko(const Shape& s) { return s.d_out <= 32 ? 1 : s.d_out <= 64 ? 2 : 4; }
 bool narrow_bwd(const Shape& s) {
     return s.d_in <= 128 && s.d_out <= 128 && s.hidden <= kNarrowHidden &&
-           narrow_bwd_fits(s.dtype == GSX_F32 ? 3 : 1, narrow_kd(s), narrow_ko(s));
+           narrow_bwd_fits(s.dtype, narrow_kd(s), narrow_ko(s));
 }
 struct BwdPlan {
     int pairs, groups, blocks;
@@ -1337,7 +1510,7 @@ BwdPlan bwd_plan(const Shape& s) {
                               : even_stretch(s.rows, kStretchBytes / (p.groups * s.d_in * 4),
                                              kBwdRows);
     const int64_t tiles = (p.stretch + kBwdRows - 1) / kBwdRows;
-    const int per_unit = (s.dtype == GSX_F32 ? 1 : 2) * kBwdPairs / p.pairs;
+    const int per_unit = (s.dtype == GSX_BF16 ? 2 : 1) * kBwdPairs / p.pairs;
     int64_t want = 256 * per_unit / p.groups;
     if (want > tiles) want = tiles;
     p.blocks = (int)(want < 1 ? 1 : want);
@@ -1349,7 +1522,8 @@ BwdPlan bwd_plan(const Shape& s) {
 
 int64_t bwd_bytes(const Shape& s) {
     if (s.rows == 0) return 0;
-    return narrow_bwd(s) ? bwd_plan(s).bytes : 3 * hidden_bytes(s) + parts_bytes(s);
+    return narrow_bwd(s) ? bwd_plan(s).bytes
+                         : 3 * hidden_bytes(s) + pieces_bytes(s) + parts_bytes(s);
 }
 
 struct BwdArgs {
@@ -1363,7 +1537,10 @@ struct BwdArgs {
 
 template <class E, int KD, int KO>
 int launch_narrow_bwd(const Shape& s, const BwdArgs& a) {
-    if constexpr (!narrow_bwd_fits(Wide<E>::PIECES, KD, KO)) {
+    constexpr int dtype = std::is_same_v<E, F32>    ? GSX_F32
+                          : std::is_same_v<E, BF16> ? GSX_BF16
+                                                    : GSX_F16;
+    if constexpr (!narrow_bwd_fits(dtype, KD, KO)) {
         return GSX_ERR_INVALID;  // narrow_bwd() keeps these out
     } else {
         using T = typename E::T;
@@ -1414,6 +1591,19 @@ int launch_narrow_bwd(const Shape& s, const BwdArgs& a) {
     }
 }
 
+// Launches the split of float16 rows into two planes at `to`, and describes them.
+int pieces(void* to, const void* x, int64_t ld, int64_t rows, int cols, Operand* o,
+           hipStream_t st) {
+    const int wide = (int)pitch(cols);
+    hipLaunchKernelGGL(k_pieces, groups_for(rows * ((cols + 1) / 2)), dim3(kThreads), 0, st,
+                       (const uint16_t*)x, ld, rows, cols, wide, (uint16_t*)to);
+    GSX_LAUNCH_CHECK();
+    o->p = to;
+    o->lo = (uint16_t*)to + rows * wide;
+    o->ld = wide;
+    return GSX_OK;
+}
+
 template <class E>
 int forward(const Shape& s, const void* x, int64_t ldx, const void* wg, const void* wu,
             const void* wd, void* y, void* ws, hipStream_t st) {
@@ -1425,7 +1615,11 @@ int forward(const Shape& s, const void* x, int64_t ldx, const void* wg, const vo
         }
     }
     using T = typename E::T;
-    const int64_t ph = pitch(s), stretch = tiled_stretch(s);
+    const int64_t ph = pitch(s), stretch = tiled_stretch(s), plane = stretch * ph;
+    Operand down{wd, s.hidden, s.d_out};
+    if constexpr (std::is_same_v<E, F16>)
+        if (int e = pieces((char*)ws + hidden_bytes(s), wd, s.hidden, s.d_out, s.hidden, &down, st))
+            return e;
     for (int64_t row0 = 0; row0 < s.rows; row0 += stretch) {
         const int rows = (int)(s.rows - row0 < stretch ? s.rows - row0 : stretch);
         Tile q{};
@@ -1437,11 +1631,12 @@ int forward(const Shape& s, const void* x, int64_t ldx, const void* wg, const vo
         q.n = s.hidden;
         q.out[0] = ws;
         q.ldo = ph;
+        q.plane = plane;
         q.act = s.act;
         if (int e = launch_tile<E, HIDDEN>(q, 1, st)) return e;
         Tile r{};
-        r.a = Operand{ws, ph, rows};
-        r.b0 = Operand{wd, s.hidden, s.d_out};
+        r.a = Operand{ws, ph, rows, (uint16_t*)ws + plane};
+        r.b0 = down;
         r.k = s.hidden;
         r.m = rows;
         r.n = s.d_out;
@@ -1495,12 +1690,27 @@ int backward(const Shape& s, const void* x, int64_t ldx, const void* wg, const v
     }
     using T = typename E::T;
     const int64_t ph = pitch(s), hb = hidden_bytes(s), stretch = tiled_stretch(s);
+    const int64_t plane = stretch * ph;
     void* dg = ws;
     void* du = (char*)ws + hb;
     void* h = (char*)ws + 2 * hb;
+    auto held = [&](const void* p, int n) {
+        return Operand{p, ph, n, (const uint16_t*)p + plane};
+    };
+    // float16: the pieces of x and dy, of the pair's weights
+    char* x_pieces = (char*)ws + 3 * hb;
+    char* dy_pieces = x_pieces + held_bytes(stretch, s.d_in);
+    char* w_pieces = dy_pieces + held_bytes(stretch, s.d_out);
     // the pair's parts, then the down weights'
-    float* pair_parts = (float*)((char*)ws + 3 * hb);
-    float* down_parts = (float*)((char*)ws + 3 * hb + pair_parts_bytes(s));
+    float* pair_parts = (float*)((char*)ws + 3 * hb + pieces_bytes(s));
+    float* down_parts = (float*)((char*)pair_parts + pair_parts_bytes(s));
+    Operand gate{wg, s.d_in, s.d_in}, up{wu, s.d_in, s.d_in};
+    if constexpr (std::is_same_v<E, F16>)
+        if (dx) {
+            const int64_t one = held_bytes(s.hidden, s.d_in);
+            if (int e = pieces(w_pieces, wg, s.d_in, s.hidden, s.d_in, &gate, st)) return e;
+            if (int e = pieces(w_pieces + one, wu, s.d_in, s.hidden, s.d_in, &up, st)) return e;
+        }
     for (int64_t row0 = 0; row0 < s.rows; row0 += stretch) {
         const int rows = (int)(s.rows - row0 < stretch ? s.rows - row0 : stretch);
         const T* xs = (const T*)x + row0 * ldx;
@@ -1519,14 +1729,15 @@ int backward(const Shape& s, const void* x, int64_t ldx, const void* wg, const v
         q.out[1] = du;
         q.out[2] = h;
         q.ldo = ph;
+        q.plane = plane;
         q.act = s.act;
         if (int e = launch_tile<E, BWD_HIDDEN>(q, 1, st)) return e;
         if (dx) {
             Tile r{};
-            r.a = Operand{dg, ph, rows};
-            r.b0 = Operand{wg, s.d_in, s.d_in};
-            r.a2 = Operand{du, ph, rows};
-            r.b2 = Operand{wu, s.d_in, s.d_in};
+            r.a = held(dg, rows);
+            r.b0 = gate;
+            r.a2 = held(du, rows);
+            r.b2 = up;
             r.k = s.hidden;
             r.m = rows;
             r.n = s.d_in;
@@ -1537,8 +1748,10 @@ int backward(const Shape& s, const void* x, int64_t ldx, const void* wg, const v
         if (dwg) {
             Tile r{};
             r.a = Operand{xs, ldx, s.d_in};
-            r.b0 = Operand{dg, ph, s.hidden};
-            r.b1 = Operand{du, ph, s.hidden};
+            if constexpr (std::is_same_v<E, F16>)
+                if (int e = pieces(x_pieces, xs, ldx, rows, s.d_in, &r.a, st)) return e;
+            r.b0 = held(dg, s.hidden);
+            r.b1 = held(du, s.hidden);
             r.m = s.d_in;
             r.n = s.hidden;
             void* outs[2] = {dwg, dwu};
@@ -1547,7 +1760,9 @@ int backward(const Shape& s, const void* x, int64_t ldx, const void* wg, const v
         if (dwd) {
             Tile r{};
             r.a = Operand{dys, lddy, s.d_out};
-            r.b0 = Operand{h, ph, s.hidden};
+            if constexpr (std::is_same_v<E, F16>)
+                if (int e = pieces(dy_pieces, dys, lddy, rows, s.d_out, &r.a, st)) return e;
+            r.b0 = held(h, s.hidden);
             r.m = s.d_out;
             r.n = s.hidden;
             void* outs[1] = {dwd};

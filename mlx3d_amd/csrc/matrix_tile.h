@@ -16,6 +16,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 namespace gsx {
 
 // Keeps the compiler from computing what depends on v ahead of this place (and
@@ -136,16 +138,6 @@ struct Wide {
         u32x4 p[1];
     };
     static __device__ __forceinline__ Frag frag(const Raw& r) { return Frag{{r}}; }
-    static __device__ __forceinline__ Frag frag(const float* x) {
-        Frag f;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) f.p[0][i] = E::pair(x[2 * i], x[2 * i + 1]);
-        return f;
-    }
-    // four elements of each piece
-    static __device__ __forceinline__ void four(const float* x, uint2* w) {
-        w[0] = uint2{E::pair(x[0], x[1]), E::pair(x[2], x[3])};
-    }
     static __device__ __forceinline__ f32x4 mma(const Frag& a, const Frag& b, f32x4 c) {
         return E::mma(a.p[0], b.p[0], c);
     }
@@ -166,7 +158,6 @@ struct Wide<F32> {
     };
     using Frag = Split3;
     static __device__ __forceinline__ Frag frag(const Raw& r) { return split(r.v); }
-    static __device__ __forceinline__ Frag frag(const float* x) { return split(x); }
     static __device__ __forceinline__ void four(const float* x, uint2* w) {
         split_pair(x[0], x[1], &w[0].x, &w[1].x, &w[2].x);
         split_pair(x[2], x[3], &w[0].y, &w[1].y, &w[2].y);
@@ -183,6 +174,96 @@ struct Wide<F32> {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
             if (i >= n) r.v[i] = 0.f;
+    }
+};
+
+// The second products, whose one operand is formed on the chip in float32 (`Mid`:
+// hidden channels and their gradients) and whose other one (`Other`) is the
+// tensors': float32 as above.  In 16 bits Mid is two bf16 pieces, sixteen bits or
+// more in float32's range, so that nothing is rounded to the tensors' type but the
+// outputs; the other operand is itself in bf16, and two bf16 pieces (11 = 8 + 3
+// bits, exact) in float16, where the product of the second pieces, below 2^-16 of
+// one, is left out.  That takes two products for one in bf16 and three in float16.
+struct Split2 {
+    u32x4 p[2];
+};
+// CUT: the first piece is cut off, which no finite number survives as an infinity;
+// else it is rounded, for a smaller second one (float16 products end far below)
+template <bool CUT>
+__device__ __forceinline__ void split_two(float a, float b, uint32_t* p0, uint32_t* p1) {
+    uint32_t ha, hb;
+    if constexpr (CUT) {
+        ha = __float_as_uint(a) & 0xffff0000u;
+        hb = __float_as_uint(b) & 0xffff0000u;
+        *p0 = ha >> 16 | hb;
+    } else {
+        *p0 = BF16::pair(a, b);
+        ha = *p0 << 16;
+        hb = *p0 & 0xffff0000u;
+    }
+    *p1 = BF16::pair(a - __uint_as_float(ha), b - __uint_as_float(hb));
+}
+
+template <class E>
+struct Second {  // BF16, F16
+    static constexpr bool HALF = std::is_same_v<E, F16>;
+    static constexpr int MID = 2, OTHER = HALF ? 2 : 1;
+    using M = BF16;  // the products' type
+    using Mid = Split2;
+    struct Other {
+        u32x4 p[OTHER];
+    };
+    static __device__ __forceinline__ Mid mid(const float* x) {
+        Mid m;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            uint32_t w[2];
+            split_two<!HALF>(x[2 * i], x[2 * i + 1], &w[0], &w[1]);
+            m.p[0][i] = w[0];
+            m.p[1][i] = w[1];
+        }
+        return m;
+    }
+    // four elements of each piece
+    static __device__ __forceinline__ void four(const float* x, uint2* w) {
+        split_two<!HALF>(x[0], x[1], &w[0].x, &w[1].x);
+        split_two<!HALF>(x[2], x[3], &w[0].y, &w[1].y);
+    }
+    static __device__ __forceinline__ Other other(const u32x4& r) {
+        Other o;
+        if constexpr (HALF) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                uint32_t w[2];
+                split_two<false>(E::up((uint16_t)r[i]), E::up((uint16_t)(r[i] >> 16)), &w[0],
+                                 &w[1]);
+                o.p[0][i] = w[0];
+                o.p[1][i] = w[1];
+            }
+        } else {
+            o.p[0] = r;
+        }
+        return o;
+    }
+    static __device__ __forceinline__ f32x4 mma(const Other& o, const Mid& m, f32x4 c) {
+        if constexpr (HALF) c = BF16::mma(o.p[1], m.p[0], c);
+        c = BF16::mma(o.p[0], m.p[1], c);
+        return BF16::mma(o.p[0], m.p[0], c);
+    }
+};
+template <>
+struct Second<F32> {
+    static constexpr int MID = 3, OTHER = 3;
+    using M = F32;  // of the tiled products
+    using Mid = Split3;
+    using Other = Split3;
+    static __device__ __forceinline__ Mid mid(const float* x) { return split(x); }
+    static __device__ __forceinline__ void four(const float* x, uint2* w) {
+        Wide<F32>::four(x, w);
+    }
+    static __device__ __forceinline__ Other other(const Wide<F32>::Raw& r) { return split(r.v); }
+    static __device__ __forceinline__ f32x4 mma(const Other& o, const Mid& m, f32x4 c) {
+        return Wide<F32>::mma(o, m, c);
     }
 };
 

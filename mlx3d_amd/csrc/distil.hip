@@ -926,13 +926,13 @@ Layout layout(int dtype, int64_t rows, int64_t vocab, int64_t top) {
     return l;
 }
 
+// (42 KB of shared memory at most: 4096 columns of 16 bits and 256 entries.)
 template <class E, int G, int N, int KPL, bool LOG_PROBS, int FULL>
 int launch_rows(const Distil& q, hipStream_t st) {
     constexpr int R = 64 / G, kWaves = kThreads / 64;
     const int64_t tiles = (q.rows + R - 1) / R, groups = (tiles + kWaves - 1) / kWaves;
     const int64_t lds = kWaves * (tile_room(R, G * N, q.vocab, sizeof(typename E::T)) +
                                   (int64_t)R * q.top * 8);
-    if (lds > 64 * 1024) return GSX_ERR_TOO_LARGE;
     hipLaunchKernelGGL((k_rows<E, G, N, KPL, LOG_PROBS, FULL>),
                        dim3(q.alone                ? 1u
                             : groups < kRowGroups ? (unsigned)groups
@@ -953,33 +953,44 @@ int launch_rows(const Distil& q, hipStream_t st) {
 }
 
 // The kernel whose lanes hold the row's words and entries with the least room to
-// spare (fewer to choose from where a lane has several entries).  307 039 rows of
-// 21 float16 logits and 5 entries, loss or gradient alone: 20 us with room for two
-// entries and three words, 24 with four and six.
+// spare: a wave works on all the room there is.  Loss and gradient of 300 MB of
+// logits, us with the least room / with the next that would hold them:
+//   words     3 / 6    12 float32 columns 32.0 / 34.4, 21 bf16 33.4 / 38.3
+//             8 / 10   64 float32 89.7 / 93.0, 126 bf16 98.8 / 102.5
+//             8 / 14   64 float32 90.0 / 97.6, 126 bf16 100 / 115
+//            10 / 14   80 float32 107 / 109, 150 bf16 112 / 125
+//            20 / 33   1280 float32 139 / 178, 2558 bf16 154 / 220
+//   entries   1 / 4    128 float32 161 / 212, 150 bf16 112 / 181
+//             2 / 4    80 float32, 15 entries 127 / 137, 150 bf16 141 / 200
+//   four entries with 6 / 14 words  24 float32, 20 entries 83 / 97, 90 bf16, 30
+//                      140 / 197
+//   two entries with 3 / 6 words    21 bf16, 7 entries 41.7 / 44.7
+// Eight lanes and more hold more than seven words each (half of them would do
+// otherwise), or over eight entries for every four lanes.
 template <class E, int G>
 int launch_rows(const Distil& q, int words, hipStream_t st) {
     const int n = (words + G - 1) / G;
-    if (q.top > G && q.top <= 2 * G) {
-        if constexpr (G == 4) {
-            if (n <= 3) return launch_rows<E, G, 3, 2, 0>(q, st);
-        }
-        if (n <= 6) return launch_rows<E, G, 6, 2, 0>(q, st);
-        if constexpr (G == 64) {
-            if (n > 14) return launch_rows<E, G, 33, 2, 15>(q, st);
-        }
-        return launch_rows<E, G, 14, 2, 7>(q, st);
-    }
-    if (q.top > G) {
+    if (q.top > 2 * G) {
         if (n <= 6) return launch_rows<E, G, 6, 4, 0>(q, st);
         if constexpr (G == 64) {
             if (n > 14) return launch_rows<E, G, 33, 4, 15>(q, st);
         }
         return launch_rows<E, G, 14, 4, 7>(q, st);
     }
+    if (q.top > G) {
+        if constexpr (G == 4) {
+            if (n <= 3) return launch_rows<E, G, 3, 2, 0>(q, st);
+            if (n <= 6) return launch_rows<E, G, 6, 2, 0>(q, st);
+        }
+        if constexpr (G == 64) {
+            if (n > 14) return launch_rows<E, G, 33, 2, 15>(q, st);
+        }
+        return launch_rows<E, G, 14, 2, 7>(q, st);
+    }
     if constexpr (G == 4) {
         if (n <= 3) return launch_rows<E, G, 3, 1, 0>(q, st);
+        if (n <= 6) return launch_rows<E, G, 6, 1, 0>(q, st);
     }
-    if (n <= 6) return launch_rows<E, G, 6, 1, 0>(q, st);
     if (n <= 8) return launch_rows<E, G, 8, 1, 7>(q, st);
     if (n <= 10) return launch_rows<E, G, 10, 1, 9>(q, st);
     if constexpr (G == 64) {

@@ -743,9 +743,10 @@ enum gsx_activation { GSX_ACT_SILU = 0, GSX_ACT_GELU = 1, GSX_ACT_SIGMOID = 2 };
  * all, every pointer aligned to it.  The workspace (16-byte aligned; NULL where
  * 0 bytes are asked for) is scratch: it may be freed or reused once the call has
  * returned, in stream order.  Rows are walked in stretches, so it stays below
- * 1 GB forward and, beside the weight gradients' sums, 3 GB backward (or 128 rows'
- * hidden channels).  GSX_ERR_TOO_LARGE above 2^30 rows or widths of 2^20.  The same
- * inputs give the same bits. */
+ * 1 GB forward and 5 GB backward, beside the float16 weights' pieces and the
+ * weight gradients' sums (128 rows' hidden channels at least).
+ * GSX_ERR_TOO_LARGE above 2^30 rows or widths of 2^20.  The same inputs give the
+ * same bits. */
 int64_t gsx_ffn_fwd_workspace_bytes(int32_t dtype, int32_t act, int64_t rows, int32_t d_in,
                                     int32_t hidden, int32_t d_out);
 int gsx_ffn_fwd(int32_t dtype, int32_t act, int64_t rows, int32_t d_in, int32_t hidden,

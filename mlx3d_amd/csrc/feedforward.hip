@@ -818,8 +818,8 @@ __global__ __launch_bounds__(kNarrowThreads) void k_narrow_fwd(const Narrow<E> q
 // elements) the weight gradients'.  The pairs' parts of dx are added up there
 // too.  Two barriers a tile; the next tile's loads are in flight meanwhile.
 //
-// 921 600 rows of 32 -> 128 -> 64: bf16 240 us, 1.2 TB/s (shared memory, which dg, du
-// and h pass in two pieces, and the vector units in about equal parts; 150 with one
+// 921 600 rows of 32 -> 128 -> 64: bf16 213 us, 1.3 TB/s (shared memory, which dg, du
+// and h pass in two pieces, and the vector units, 60 % busy; 150 with one
 // piece); float32 490 us (matrix units, the pieces' conversions and shared memory).
 // One wave for the 32 channels instead of a pair needs twice the registers; with half
 // the waves a SIMD the training step took 414 us instead of 225 (in one piece),
@@ -950,65 +950,63 @@ void k_narrow_bwd(const NarrowBwd<E> q) {
     constexpr int PIECES = kBwdRows * (S::XS + S::YS);
     constexpr int HELD = (PIECES + 128 * kBwdPairs - 1) / (128 * kBwdPairs);
     const int rows = (int)q.rows, step = (int)gridDim.x * kBwdRows;
-    struct Piece {  // number n of a tile
-        bool of_x;
-        int row, k;  // in the tile; the first element
-        __device__ __forceinline__ explicit Piece(int n) {
-            of_x = n < kBwdRows * S::XS;
-            const int i = of_x ? n : n - kBwdRows * S::XS, slots = of_x ? S::XS : S::YS;
-            row = i / slots;
-            k = i % slots * 8;
-        }
+    struct Piece {
+        const T* p;    // in the next tile to be read
+        int row, n;    // its row; how many elements the row has from here on
+        int slot;      // its place in the staged tile
     };
-    auto ld_of = [&](const Piece& m) { return m.of_x ? q.ldx : q.lddy; };
-    auto at = [&](const Piece& m, int row) {
-        return (m.of_x ? q.x : q.dy) + row * ld_of(m) + m.k;
+    const int64_t hop_x = step * q.ldx, hop_y = step * q.lddy;  // from a tile to the next
+    auto of_x = [&](int n) { return n < kBwdRows * S::XS; };
+    auto piece_of = [&](int n, int row0) {
+        const bool x = of_x(n);
+        const int i = x ? n : n - kBwdRows * S::XS;
+        const int slots = x ? S::XS : S::YS, row = i / slots, k = i % slots * 8;
+        Piece m;
+        m.row = row0 + row;
+        m.p = (x ? q.x : q.dy) + (int64_t)m.row * (x ? q.ldx : q.lddy) + k;
+        m.n = (x ? q.d_in : q.d_out) - k;
+        m.slot = x ? tile_slot<S::XS>(row, k / 8)
+                   : S::PLANES * kBwdRows * S::XS + tile_slot<S::YS>(row, k / 8);
+        return m;
     };
-    auto fetch = [&](const Piece& m, const T* p, int row) {
+    auto fetch = [&](const Piece& m) {
         typename W::Raw raw{};
-        const int n = (m.of_x ? q.d_in : q.d_out) - m.k;
-        if (row < rows && n > 0) raw = load8<E>(p, n, rows - 1 - row);
+        if (m.row < rows && m.n > 0) raw = load8<E>(m.p, m.n, rows - 1 - m.row);
         return raw;
     };
-    auto settle = [&](u32x4* tile, const Piece& m, const typename W::Raw& raw) {
+    auto settle = [&](u32x4* tile, const Piece& m, bool x, const typename W::Raw& raw) {
         const Frag f = W::frag(raw);
-        const int pitch = kBwdRows * (m.of_x ? S::XS : S::YS);
-        tile += m.of_x ? tile_slot<S::XS>(m.row, m.k / 8)
-                       : S::PLANES * kBwdRows * S::XS + tile_slot<S::YS>(m.row, m.k / 8);
+        const int pitch = kBwdRows * (x ? S::XS : S::YS);
 #pragma unroll
-        for (int p = 0; p < PC; ++p) tile[p * pitch] = f.p[p];
+        for (int p = 0; p < PC; ++p) tile[m.slot + p * pitch] = f.p[p];
         if constexpr (S::AT > 0) {
             const Other o = S2::other(raw);
 #pragma unroll
-            for (int p = 0; p < S::PO; ++p) tile[(S::AT + p) * pitch] = o.p[p];
+            for (int p = 0; p < S::PO; ++p) tile[m.slot + (S::AT + p) * pitch] = o.p[p];
         }
     };
-    // what a piece's number says is formed again for every tile where registers are
-    // short
-    auto number = [&](int i) {
-        const int n = threadIdx.x + i * threads;
-        return EARLY ? n : here(n);
-    };
-    const T* from[HELD];  // in the next tile to be read
-    int from_row = 0;     // its first row
+    Piece mine[HELD];
     typename W::Raw next[HELD];
     auto fetch_all = [&] {
 #pragma unroll
-        for (int i = 0; i < HELD; ++i)
-            if (threadIdx.x + i * threads < PIECES) {
-                const Piece m(number(i));
-                next[i] = fetch(m, from[i], from_row + m.row);
-                from[i] += step * ld_of(m);
+        for (int i = 0; i < HELD; ++i) {
+            const int n = threadIdx.x + i * threads;
+            if (n < PIECES) {
+                next[i] = fetch(mine[i]);
+                mine[i].p += of_x(n) ? hop_x : hop_y;
+                mine[i].row += step;
             }
-        from_row += step;
+        }
     };
     auto settle_all = [&](u32x4* tile, int row0) {
 #pragma unroll
-        for (int i = 0; i < HELD; ++i)
-            if (threadIdx.x + i * threads < PIECES) settle(tile, Piece(number(i)), next[i]);
+        for (int i = 0; i < HELD; ++i) {
+            const int n = threadIdx.x + i * threads;
+            if (n < PIECES) settle(tile, mine[i], of_x(n), next[i]);
+        }
         for (int n = threadIdx.x + HELD * threads; n < PIECES; n += threads) {  // fewer pairs
-            const Piece m(n);
-            settle(tile, m, fetch(m, at(m, row0 + m.row), row0 + m.row));
+            const Piece m = piece_of(n, row0);
+            settle(tile, m, of_x(n), fetch(m));
         }
     };
 
@@ -1026,11 +1024,7 @@ void k_narrow_bwd(const NarrowBwd<E> q) {
     int row0 = (int)blockIdx.x * kBwdRows;
 #pragma unroll
     for (int i = 0; i < HELD; ++i)
-        if (threadIdx.x + i * threads < PIECES) {
-            const Piece m(threadIdx.x + i * threads);
-            from[i] = at(m, row0 + m.row);
-        }
-    from_row = row0;
+        if (threadIdx.x + i * threads < PIECES) mine[i] = piece_of(threadIdx.x + i * threads, row0);
     fetch_all();
     settle_all(tiles, row0);
     fetch_all();

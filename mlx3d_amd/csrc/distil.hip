@@ -40,8 +40,8 @@ namespace {
 
 constexpr int kThreads = 256;
 // Longest row of the one-launch path: where a wave's registers still hold it.
-// Against segments, us a call (32 768 and 4 rows): float32 512 columns 39 / 130 and
-// 18 / 29, 2048 columns 121 / 225 and 18 / 29, bf16 4096 147 / 255 and 18 / 29.
+// Against segments, us a call (32 768 and 4 rows): float32 512 columns 45 / 138 and
+// 17 / 30, 2048 columns 122 / 237 and 18 / 29, bf16 4096 148 / 260 and 18 / 29.
 constexpr int kRowBytes = 8192;
 constexpr int kSegBytes = 16384;   // a segment of a longer row
 constexpr int kCountParts = 256;   // workgroups of the count of supervised rows
@@ -422,7 +422,7 @@ __host__ __device__ inline int64_t tile_room(int rows, int words, int64_t vocab,
 //
 // FULL: words of a lane that lie in every row that this kernel is launched for.
 //
-// 921 600 rows of 150 bf16 logits and 8 entries, loss and gradient: 165 us,
+// 921 600 rows of 150 bf16 logits and 8 entries, loss and gradient: 166 us,
 // 3.7 TB/s (a large copy: 4.8).  A tile's loads, its arithmetic and its stores
 // follow each other in a wave, and four waves of a SIMD do not cover all of it; six
 // spill.  Stores held back behind the next tile's loads took 7 us more.
@@ -640,8 +640,8 @@ __global__ __launch_bounds__(kThreads, N > 14 ? 2 : KPL > 2 ? 3 : 4) void k_rows
 }
 
 // A segment of a longer row: maximum and sum of its rest (with a teacher of
-// logits, of all of it).  4099 rows of 50 000 float32: 191 us, 4.3 TB/s, bound by
-// memory.
+// logits, of all of it).  4099 rows of 50 000 float32: 195 to 213 us, 4 TB/s, bound by
+// memory and the vector units (busy for 80 %) in about equal parts.
 template <class E>
 __global__ __launch_bounds__(kThreads) void k_seg_sum(const Distil q) {
     using T = typename E::T;
@@ -744,9 +744,9 @@ __global__ __launch_bounds__(64) void k_seg_join(const Distil q) {
         if (lane + i * 64 < q.top) probs[lane + i * 64] = e.value[i];
 }
 
-// A segment's gradient.  4099 rows of 50 000 float32: 278 us, 5.9 TB/s read and
-// written, more than a large copy's 4.8; taking the rows in reverse, so that it
-// began with those that the first pass read last, changed nothing.
+// A segment's gradient.  4099 rows of 50 000 float32: 300 to 329 us, 5 TB/s read and
+// written (a large copy: 4.8); taking the rows in reverse, so that it began with those
+// that the first pass read last, changed nothing.
 template <class E>
 __global__ __launch_bounds__(kThreads) void k_seg_grad(const Distil q) {
     using T = typename E::T;
@@ -908,7 +908,7 @@ int lanes_for(int dtype, int64_t vocab, int64_t top) {
     return g;
 }
 // Workgroups' worth of tiles that one walks alone, with the count and the sum in
-// its one launch: a patch of 64 rows takes 18 us a call instead of 23, whose three
+// its one launch: a patch of 64 rows took 18 us a call instead of 23, whose three
 // launches take longer than their work.
 constexpr int64_t kAlone = 4;
 constexpr int64_t kRowGroups = 2048;  // workgroups that walk the tiles: eight for a unit
@@ -968,16 +968,16 @@ int launch_rows(const Distil& q, hipStream_t st) {
 // The kernel whose lanes hold the row's words and entries with the least room to
 // spare: a wave works on all the room there is.  Loss and gradient of 300 MB of
 // logits, us with the least room / with the next that would hold them:
-//   words     3 / 6    12 float32 columns 32.0 / 34.4, 21 bf16 33.4 / 38.3
-//             8 / 10   64 float32 89.7 / 93.0, 126 bf16 98.8 / 102.5
-//             8 / 14   64 float32 90.0 / 97.6, 126 bf16 100 / 115
-//            10 / 14   80 float32 107 / 109, 150 bf16 112 / 125
-//            20 / 33   1280 float32 139 / 178, 2558 bf16 154 / 220
-//   entries   1 / 4    128 float32 161 / 212, 150 bf16 112 / 181
-//             2 / 4    80 float32, 15 entries 127 / 137, 150 bf16 141 / 200
-//   four entries with 6 / 14 words  24 float32, 20 entries 83 / 97, 90 bf16, 30
-//                      140 / 197
-//   two entries with 3 / 6 words    21 bf16, 7 entries 41.7 / 44.7
+//   words     3 / 6    12 float32 columns 33.4 / 36.6, 21 bf16 35.3 / 40.0
+//             8 / 10   64 float32 93.7 / 95.9, 126 bf16 102 / 104
+//             8 / 14   64 float32 93.7 / 101, 126 bf16 102 / 117
+//            10 / 14   80 float32 108 / 113, 150 bf16 112 / 125
+//            20 / 33   1280 float32 141 / 152, 2558 bf16 154 / 219
+//   entries   1 / 4    128 float32 165 / 224, 150 bf16 112 / 184
+//             2 / 4    80 float32, 15 entries 131 / 147, 150 bf16 143 / 202
+//   four entries with 6 / 14 words  24 float32, 20 entries 90 / 111, 90 bf16, 30
+//                      143 / 208
+//   two entries with 3 / 6 words    21 bf16, 7 entries 40.4 / 44.8
 // Eight lanes and more hold more than seven words each (half of them would do
 // otherwise), or over eight entries for every four lanes.
 template <class E, int G>

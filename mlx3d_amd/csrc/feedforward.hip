@@ -623,7 +623,7 @@ __global__ __launch_bounds__(kThreads) void k_zero_bytes(uint8_t* p, int64_t n) 
 // registers, so x is read and y written once and nothing else moves.  Each wave
 // takes 32 rows through all of it.
 //
-// 921 600 rows of 32 -> 128 -> 64 float32: 177 us, 2.0 TB/s; bound by the matrix
+// 921 600 rows of 32 -> 128 -> 64 float32: 177 to 190 us, 1.9 TB/s; bound by the matrix
 // units, whose six bf16 products for one float32 run at 1.02 PFLOP/s, 82 % of what
 // a large product reaches (the float32 instructions would take 196 us at best).
 // 2 073 600 rows of 32 -> 96 -> 48 bf16: 122 us, 2.7 TB/s; bound by the vector
@@ -820,7 +820,8 @@ __global__ __launch_bounds__(kNarrowThreads) void k_narrow_fwd(const Narrow<E> q
 //
 // 921 600 rows of 32 -> 128 -> 64: bf16 213 us, 1.3 TB/s (shared memory, which dg, du
 // and h pass in two pieces, and the vector units, 60 % busy; 150 with one
-// piece); float32 490 us (matrix units, the pieces' conversions and shared memory).
+// piece); float32 487 to 546 us (matrix units, the pieces' conversions and shared
+// memory; the mean as clocks rise).
 // One wave for the 32 channels instead of a pair needs twice the registers; with half
 // the waves a SIMD the training step took 414 us instead of 225 (in one piece),
 // float32 870 instead of 656.

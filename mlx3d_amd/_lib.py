@@ -294,19 +294,20 @@ class _NoSecondDerivative(torch.autograd.Function):
 
 
 def once_differentiable(what: str):
-    """For a Function's ``backward``: with ``create_graph=True`` its gradients
-    depend on the saved tensors and raise when they are differentiated.  torch's
-    decorator looks at the incoming gradient alone, and hands out constants where
-    that one needs none."""
+    """For a Function's ``backward(ctx, saved, *grads)``, ``saved`` its saved tensors
+    (read once, as checkpointing asks): with ``create_graph=True`` its gradients
+    depend on them and raise when they are differentiated.  torch's decorator looks
+    at the incoming gradient alone, and hands out constants where that one needs
+    none."""
     def wrap(backward):
         @functools.wraps(backward)
         def run(ctx, *grads):
+            saved = ctx.saved_tensors
             if not torch.is_grad_enabled():
-                return backward(ctx, *grads)
+                return backward(ctx, saved, *grads)
             with torch.no_grad():
-                out = backward(ctx, *grads)
-            return tuple(g if g is None else
-                         _NoSecondDerivative.apply(what, g, *grads, *ctx.saved_tensors)
+                out = backward(ctx, saved, *grads)
+            return tuple(g if g is None else _NoSecondDerivative.apply(what, g, *grads, *saved)
                          for g in out)
         return run
     return wrap

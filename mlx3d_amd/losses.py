@@ -262,9 +262,9 @@ class _DistillationFn(torch.autograd.Function):
 
     @staticmethod
     @_lib.once_differentiable("distillation_loss")
-    def backward(ctx, g_loss):
+    def backward(ctx, saved, g_loss):
         # saved with the rest so that an entry changed in place since is noticed
-        logits, ws, _, _ = ctx.saved_tensors
+        logits, ws, _, _ = saved
         call = ctx.call
         rows, stride = _lib.rows_of(logits)
         g = _lib.f32c(g_loss)

@@ -45,8 +45,8 @@ class _GatedFeedForward(torch.autograd.Function):
 
     @staticmethod
     @_lib.once_differentiable("gated_feed_forward")
-    def backward(ctx, g_y):
-        x, *weights = ctx.saved_tensors
+    def backward(ctx, saved, g_y):
+        x, *weights = saved
         L = _lib.load()
         rows, stride = _lib.rows_of(x)
         g_rows, g_stride = _lib.rows_of(g_y)

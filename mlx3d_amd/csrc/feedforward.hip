@@ -852,11 +852,13 @@ __device__ __forceinline__ int sum_slot(int row, int slot) {
 
 // A staged tile's planes: the pieces of the first products' operands, and those of
 // the second ones where they are others (float16, whose bf16 pieces are formed once
-// for all waves).
+// for all waves).  LATE: of 128 float16 inputs neither shared memory nor registers
+// hold the pieces; each wave forms them where it uses them.
 template <class E, int KD, int KO>
 struct BwdShape {
     static constexpr int PC = Wide<E>::PIECES, PM = Second<E>::MID, PO = Second<E>::OTHER;
-    static constexpr int AT = std::is_same_v<E, F16> ? 1 : 0, PLANES = AT ? 3 : PC;
+    static constexpr bool HALF = std::is_same_v<E, F16>, LATE = HALF && KD == 4;
+    static constexpr int AT = HALF && !LATE ? 1 : 0, PLANES = AT ? 3 : PC;
     static constexpr int XS = 4 * KD, YS = 4 * KO;              // slots of a row of x, of dy
     static constexpr int TILE = kBwdRows * (XS + YS) * PLANES;  // 16-byte slots of a staged tile
     static constexpr int GATE = kBwdRows * 4 * PM;              // of a pair's dg, du or h
@@ -896,7 +898,8 @@ void k_narrow_bwd(const NarrowBwd<E> q) {
     // the wave's weights: its 16 channels' rows (operands of x and of dy), and the
     // pair's 32 channels for every other 16 of dx's
     Frag wg[KD], wu[KD], wd[KO];
-    Other wgt[KD], wut[KD];
+    using Kept = std::conditional_t<S::LATE, typename W::Raw, Other>;
+    Kept wgt[KD], wut[KD];
     {
         auto gather = [&](const T* w, int64_t first, int64_t step, int n) {
             typename W::Raw raw;
@@ -930,8 +933,15 @@ void k_narrow_bwd(const NarrowBwd<E> q) {
         for (int j = 0; j < KD; ++j) {
             const int d = 16 * (2 * j + half) + col, f8 = f0 + k8;
             const int n = d < q.d_in ? q.hidden - f8 : 0;
-            wgt[j] = S2::other(gather(q.wg, (int64_t)f8 * q.d_in + d, q.d_in, n));
-            wut[j] = S2::other(gather(q.wu, (int64_t)f8 * q.d_in + d, q.d_in, n));
+            const auto a = gather(q.wg, (int64_t)f8 * q.d_in + d, q.d_in, n);
+            const auto c = gather(q.wu, (int64_t)f8 * q.d_in + d, q.d_in, n);
+            if constexpr (S::LATE) {
+                wgt[j] = a;
+                wut[j] = c;
+            } else {
+                wgt[j] = S2::other(a);
+                wut[j] = S2::other(c);
+            }
         }
     }
 
@@ -1118,19 +1128,31 @@ void k_narrow_bwd(const NarrowBwd<E> q) {
             turn_gate(2);
         }
         asked();
+        auto dx_part = [&](int r, int j, const Other& g, const Other& u) {
+            f32x4 d{0.f, 0.f, 0.f, 0.f};
+            d = S2::mma(g, fg[r], d);
+            d = S2::mma(u, fu[r], d);
+            sums[pair * S::SUM + sum_slot<8 * KD>(16 * r + col, (2 * j + half) * 4 + quad)] =
+                __builtin_bit_cast(u32x4, d);
+        };
+        if constexpr (S::LATE) {
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-            const int row = 16 * r + col;
-            if constexpr (!EARLY) ask_gates(r);
+            for (int r = 0; r < R; ++r) ask_gates(r);
 #pragma unroll
             for (int j = 0; j < KD; ++j) {
-                f32x4 d{0.f, 0.f, 0.f, 0.f};
-                d = S2::mma(wgt[j], fg[r], d);
-                d = S2::mma(wut[j], fu[r], d);
-                sums[pair * S::SUM + sum_slot<8 * KD>(row, (2 * j + half) * 4 + quad)] =
-                    __builtin_bit_cast(u32x4, d);
+                const Other g = S2::other(here(wgt[j])), u = S2::other(here(wut[j]));
+#pragma unroll
+                for (int r = 0; r < R; ++r) dx_part(r, j, g, u);
+                pause();
             }
-            pause();
+        } else {
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                if constexpr (!EARLY) ask_gates(r);
+#pragma unroll
+                for (int j = 0; j < KD; ++j) dx_part(r, j, wgt[j], wut[j]);
+                pause();
+            }
         }
         // 16 channels of x or dy along the rows; where registers are short the
         // places are formed again for every tile, too
@@ -1138,6 +1160,7 @@ void k_narrow_bwd(const NarrowBwd<E> q) {
         const int at_y = EARLY ? turned_ys : here(turned_ys);
         auto turned = [&](const u32x4* tile, auto slots, int block, int base) {
             constexpr int SLOTS = decltype(slots)::value;
+            if constexpr (S::LATE) return S2::other(read_turned<SLOTS>(tile, block, base));
             Other o;
 #pragma unroll
             for (int p = 0; p < S::PO; ++p)
@@ -1478,13 +1501,14 @@ int64_t parts_bytes(const Shape& s) {
 // The narrow backward: which widths fit its registers (weights in both orders
 // and their gradients' sums), its workgroups and its workspace.
 constexpr bool narrow_bwd_fits(int dtype, int kd, int ko) {
-    return dtype == GSX_F32 ? kd + ko <= 3 : kd < 4 || (dtype == GSX_BF16 && ko <= 2);
+    return dtype == GSX_F32 ? kd + ko <= 3 : kd < 4 || ko <= 2;
 }
 // Faster than the tiled path wherever its registers and shared memory hold the
 // widths, us a call (131 072 rows; of few the host's 100 in both): 32 -> 128 -> 64
 // float32 101 / 591, bf16 96 / 350, f16 98 / 441; 32 -> 512 -> 64, four groups,
-// 276 / 1604, 155 / 732, 202 / 857; 128 -> 512 -> 64 bf16 417 / 788.  Hidden widths
-// are bounded by the groups' parts of dx, a float32 array of a stretch of x each.
+// 276 / 1604, 155 / 732, 202 / 857; 128 -> 512 -> 64 bf16 395 / 788, f16 503 / 927.
+// Hidden widths are bounded by the groups' parts of dx, a float32 array of a stretch of
+// x each.
 constexpr int kNarrowHidden = 2048;
 int narrow_ko(const Shape& s) { return s.d_out <= 32 ? 1 : s.d_out <= 64 ? 2 : 4; }
 bool narrow_bwd(const Shape& s) {

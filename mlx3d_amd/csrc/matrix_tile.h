@@ -31,6 +31,10 @@ using f32x4 = __attribute__((ext_vector_type(4))) float;
 using f16x8 = __attribute__((ext_vector_type(8))) _Float16;
 using bf16x8 = __attribute__((ext_vector_type(8))) __bf16;
 using u32x4 = __attribute__((ext_vector_type(4))) uint32_t;
+__device__ __forceinline__ u32x4 here(u32x4 v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
 
 // The three element types of the decoder's tensors (gsx_dtype).  Sums are
 // float32 in all of them.

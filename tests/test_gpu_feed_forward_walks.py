@@ -16,7 +16,8 @@ pytestmark = pytest.mark.gpu
 # workgroups: 2048 / pairs of them for one group, 512 / groups for more
 BACKWARD = [(330_013, 32, 20, 64), (164_005, 27, 40, 21), (110_003, 16, 70, 33),
             (82_017, 32, 128, 64), (28_001, 32, 300, 64), (164_001, 64, 33, 32),
-            (82_003, 40, 128, 16), (82_001, 8, 100, 100), (20_009, 128, 600, 30)]
+            (82_003, 40, 128, 16), (82_001, 8, 100, 100), (20_009, 128, 600, 30),
+            (20_011, 100, 130, 50), (82_011, 128, 90, 64)]
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)

@@ -188,6 +188,7 @@ struct Wide<F32> {
 // outputs; the other operand is itself in bf16, and two bf16 pieces (11 = 8 + 3
 // bits, exact) in float16, where the product of the second pieces, below 2^-16 of
 // one, is left out.  That takes two products for one in bf16 and three in float16.
+// An infinity has no second piece here either: it gives NaN.
 struct Split2 {
     u32x4 p[2];
 };

@@ -79,7 +79,8 @@ def gated_feed_forward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor
 
     Products are summed in float32.  In 16 bits the hidden channels and their
     gradients are held to sixteen bits in float32's range (two bfloat16 pieces),
-    so only the outputs are rounded to the type."""
+    so only the outputs are rounded to the type.  A row with an infinite or NaN
+    input comes out infinite or NaN, and no other row does."""
     if activation not in _ACTIVATIONS:
         raise ValueError("activation must be 'silu', 'gelu' or 'sigmoid'.")
     if x.ndim < 1 or x.dtype not in _lib.DTYPES:

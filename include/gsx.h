@@ -809,6 +809,58 @@ int gsx_distil_fwd_bwd(int32_t dtype, int64_t rows, int32_t vocab, int32_t top, 
                        float scale, float* loss, void* g_logits, void* workspace,
                        int64_t workspace_bytes, void* stream);
 
+/* ------------------------------------ feature field: around the decoder --
+ * Tensors are of a type of gsx_dtype, sums float32 in all of them; every pointer
+ * is aligned to its elements, rows of any width and stride (in elements) are
+ * taken.  A workspace (16-byte aligned) is scratch: it may be freed or reused
+ * once the call has returned, in stream order.  The same inputs give the same
+ * bits. */
+
+/* Rows of a table: y (count, width) = scale * table[indices], 0 where an index
+ * lies outside [0, rows).  indices int32 or (index64 = 1) int64, contiguous;
+ * table with a row stride; y contiguous.  GSX_ERR_TOO_LARGE above 2^30 indices
+ * or rows, or 2^20 columns. */
+int gsx_embed_fwd(int32_t dtype, int64_t count, int64_t rows, int32_t width, const void* indices,
+                  int32_t index64, const void* table, int64_t table_stride, float scale, void* y,
+                  void* stream);
+
+/* Its gradient: g_table (rows, width), contiguous and written whole, row v the
+ * sum of scale * g_y over the indices that are v, in their order by tiles of the
+ * sorted indices; g_y (count, width) with a row stride. */
+int64_t gsx_embed_bwd_workspace_bytes(int32_t dtype, int64_t count, int64_t rows, int32_t width);
+int gsx_embed_bwd(int32_t dtype, int64_t count, int64_t rows, int32_t width, const void* indices,
+                  int32_t index64, const void* g_y, int64_t g_y_stride, float scale, void* g_table,
+                  void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Layer norm: y = (x - mean) / sqrt(var + eps) * weight + bias over the rows of
+ * x (rows, width) with a row stride; weight and bias (width) may each be NULL (1
+ * and 0); y contiguous.  1.2e-38 <= eps <= 3e38.  GSX_ERR_TOO_LARGE above 2^30
+ * rows or 2^20 columns. */
+int gsx_layer_norm_fwd(int32_t dtype, int64_t rows, int32_t width, const void* x, int64_t x_stride,
+                       const void* weight, const void* bias, float eps, void* y, void* stream);
+
+/* Its gradient from g_y (rows, width, a row stride): g_x (rows, width), g_weight
+ * and g_bias (width), contiguous; each may be NULL.  Needs nothing of the
+ * forward call.  rows = 0 clears g_weight and g_bias. */
+int64_t gsx_layer_norm_bwd_workspace_bytes(int32_t dtype, int64_t rows, int32_t width);
+int gsx_layer_norm_bwd(int32_t dtype, int64_t rows, int32_t width, const void* x, int64_t x_stride,
+                       const void* weight, const void* g_y, int64_t g_y_stride, float eps,
+                       void* g_x, void* g_weight, void* g_bias, void* workspace,
+                       int64_t workspace_bytes, void* stream);
+
+/* Dropout without a stored mask: y[i] = residual[i] + x[i] / (1 - p) where element
+ * i is kept, else residual[i] (residual NULL: 0); all of n contiguous elements.
+ * Element i has a 32-bit number of the counter-based generator Philox4x32-10 with
+ * the key `seed` and the counter (i / 8, offset): its upper half is half-word
+ * i % 8 of that block, its lower half that of the counter (2^63 + i / 8, offset);
+ * it is kept where the number is at least p 2^32 to the nearest.  offset >= 0 is
+ * the argument, or read from offset_at (one int64 on the device) if that is not
+ * NULL.  The gradient of x is the same call on y's.  0 <= p <= 1.
+ * GSX_ERR_TOO_LARGE above 2^34 elements. */
+int gsx_dropout(int32_t dtype, int64_t n, double p, uint64_t seed, int64_t offset,
+                const int64_t* offset_at, const void* x, const void* residual, void* y,
+                void* stream);
+
 /* ---------------------------------------------------------- diagnostics --
  * Evaluates the device exp used by the rasterizer (the stand-in for
  * metal::exp at rasterize.py:80,171,274) on n inputs; tests check it

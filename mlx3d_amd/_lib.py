@@ -7,6 +7,7 @@ device, the call raises instead of silently computing something else.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import functools
 import os
@@ -208,6 +209,16 @@ SIGNATURES = {
                                       _I32, _P, _P, _P, _I64, _P]),
     "gsx_distil_fwd_bwd": (ctypes.c_int, [_I32, _I64, _I32, _I32, _P, _I64, _P, _P, _I32, _F,
                                           _I32, _I32, _F, _P, _P, _P, _I64, _P]),
+    "gsx_embed_fwd": (ctypes.c_int, [_I32, _I64, _I64, _I32, _P, _I32, _P, _I64, _F, _P, _P]),
+    "gsx_embed_bwd_workspace_bytes": (_I64, [_I32, _I64, _I64, _I32]),
+    "gsx_embed_bwd": (ctypes.c_int, [_I32, _I64, _I64, _I32, _P, _I32, _P, _I64, _F, _P, _P, _I64,
+                                     _P]),
+    "gsx_layer_norm_fwd": (ctypes.c_int, [_I32, _I64, _I32, _P, _I64, _P, _P, _F, _P, _P]),
+    "gsx_layer_norm_bwd_workspace_bytes": (_I64, [_I32, _I64, _I32]),
+    "gsx_layer_norm_bwd": (ctypes.c_int, [_I32, _I64, _I32, _P, _I64, _P, _P, _I64, _F, _P, _P,
+                                          _P, _P, _I64, _P]),
+    "gsx_dropout": (ctypes.c_int, [_I32, _I64, ctypes.c_double, ctypes.c_uint64, _I64, _P, _P, _P,
+                                   _P, _P]),
     "gsx_debug_expf": (ctypes.c_int, [_I64, _P, _P, _P]),
     "gsx_debug_atanf": (ctypes.c_int, [_I64, _P, _P, _P]),
 }
@@ -259,6 +270,16 @@ def stream_handle(device: torch.device):
     if index is None:
         index = torch.cuda.current_device()
     return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(index))
+
+
+_HERE_ALREADY = contextlib.nullcontext()
+
+
+def on_device(device: torch.device):
+    """A context in which `device` is the current one, as a launch on its stream needs."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return _HERE_ALREADY
+    return torch.cuda.device(device)
 
 
 def require_device(*tensors: torch.Tensor | None) -> torch.device:

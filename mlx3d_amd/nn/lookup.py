@@ -1,0 +1,92 @@
+"""Rows of a table by their indices (``gsx_embed_fwd`` / ``gsx_embed_bwd``).
+
+Gaussians that share a codebook, pixels that take their view's appearance, tokens
+of a text: each names a row of a table, and the table's gradient is the sum over
+those that named a row.  No counterpart in the reference.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from .. import _lib
+from ..profiling import stage
+
+__all__ = ["Embedding", "embedding"]
+
+
+class _Embedding(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, indices, table, scale):
+        held = indices.contiguous()
+        rows, stride = _lib.rows_of(table)
+        width = table.shape[1]
+        y = torch.empty((*indices.shape, width), dtype=table.dtype, device=table.device)
+        head = (_lib.DTYPES[table.dtype], indices.numel(), table.shape[0], width)
+        with _lib.on_device(table.device), stage("embed_fwd"):
+            _lib.check(_lib.load().gsx_embed_fwd(
+                *head, _lib.ptr(held), int(indices.dtype == torch.int64), _lib.ptr(rows), stride,
+                scale, _lib.ptr(y), _lib.stream_handle(table.device)), "gsx_embed_fwd")
+        ctx.save_for_backward(indices)
+        ctx.head, ctx.scale = head, scale
+        return y
+
+    @staticmethod
+    @_lib.once_differentiable("embedding")
+    def backward(ctx, saved, g_y):
+        (indices,) = saved
+        L = _lib.load()
+        held = indices.contiguous()
+        rows, stride = _lib.rows_of(g_y)
+        g_table = torch.empty(ctx.head[2:], dtype=g_y.dtype, device=g_y.device)
+        n = _lib.check(int(L.gsx_embed_bwd_workspace_bytes(*ctx.head)),
+                       "gsx_embed_bwd_workspace_bytes")
+        ws = torch.empty((n,), dtype=torch.uint8, device=g_y.device)
+        with _lib.on_device(g_y.device), stage("embed_bwd"):
+            _lib.check(L.gsx_embed_bwd(
+                *ctx.head, _lib.ptr(held), int(indices.dtype == torch.int64), _lib.ptr(rows),
+                stride, ctx.scale, _lib.ptr(g_table), _lib.ptr(ws), n,
+                _lib.stream_handle(g_y.device)), "gsx_embed_bwd")
+        return None, g_table, None
+
+
+def embedding(indices: torch.Tensor, table: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
+    """(..., C) = ``scale`` times the rows of ``table`` (V, C) that ``indices``
+    (..., int32 or int64) name; zeros where an index lies outside [0, V), so -1 stands
+    for no row.  ``table`` is float32, bfloat16 or float16; differentiable with respect
+    to it, once (its gradient has none and says so).
+
+    The gradient is dense, summed in float32 in an order that the indices fix, so the
+    same inputs give the same bits.  Rows that no index names have zeros."""
+    if indices.dtype not in (torch.int32, torch.int64):
+        raise ValueError("indices must be int32 or int64.")
+    if table.ndim != 2 or table.dtype not in _lib.DTYPES:
+        raise ValueError("table must be (V, C) in float32, bfloat16 or float16.")
+    if min(table.shape) < 1:
+        raise ValueError("the table must have at least 1 row and 1 column.")
+    scale = float(scale)
+    if not abs(scale) < 3.4e38:
+        raise ValueError("scale must be finite in float32.")
+    _lib.require_device(indices, table)
+    return _Embedding.apply(indices, table, scale)
+
+
+class Embedding:
+    """A table with its scale: ``table(indices)`` looks rows up.
+
+    ``params`` holds the leaf tensor ``table`` (normal with variance 1 / scale^2, so
+    that what is looked up has variance 1), as :class:`mlx3d_amd.optim.Adam` takes it."""
+
+    def __init__(self, rows: int, width: int, scale: float = 1.0,
+                 dtype: torch.dtype = torch.float32, device="cuda", seed: int = 0):
+        if min(rows, width) < 1:
+            raise ValueError("the table must have at least 1 row and 1 column.")
+        if not 0.0 < abs(float(scale)) < 3.4e38:
+            raise ValueError("scale must be finite in float32, and not 0.")
+        self.scale = float(scale)
+        g = torch.Generator().manual_seed(seed)
+        table = torch.randn((rows, width), generator=g) / self.scale
+        self.params = {"table": table.to(device=device, dtype=dtype).requires_grad_(True)}
+
+    def __call__(self, indices: torch.Tensor) -> torch.Tensor:
+        return embedding(indices, self.params["table"], self.scale)

@@ -16,6 +16,7 @@
 #include "gsx.h"
 #include "gsx_device.h"
 #include "matrix_tile.h"
+#include "row_pieces.h"
 
 using namespace gsx;
 
@@ -32,57 +33,105 @@ struct Drop {
     int64_t offset;
     const int64_t* offset_at;  // on the device, in place of offset; or NULL
     uint32_t upper, lower;     // the threshold's halves; upper may be 2^16: none is kept
+    uint32_t limit;            // what a half-word has to reach
     float scale;
 };
 
+__device__ __forceinline__ uint32_t xor3(uint32_t a, uint32_t b, uint32_t c) {
+    return __builtin_amdgcn_bitop3_b32(a, b, c, 0x96);
+}
 __device__ __forceinline__ void philox(uint32_t* c, uint32_t k0, uint32_t k1) {
 #pragma unroll
     for (int r = 0; r < 10; ++r) {
         const uint64_t p = (uint64_t)c[0] * 0xD2511F53u, q = (uint64_t)c[2] * 0xCD9E8D57u;
-        c[0] = (uint32_t)(q >> 32) ^ c[1] ^ k0;
+        c[0] = xor3((uint32_t)(q >> 32), c[1], k0);
         c[1] = (uint32_t)q;
-        c[2] = (uint32_t)(p >> 32) ^ c[3] ^ k1;
+        c[2] = xor3((uint32_t)(p >> 32), c[3], k1);
         c[3] = (uint32_t)p;
         k0 += 0x9E3779B9u;
         k1 += 0xBB67AE85u;
     }
 }
 
-// Which of the block's eight elements are kept, a bit each.
-__device__ __forceinline__ uint32_t kept(const Drop& q, uint64_t block, int64_t offset) {
-    const uint32_t o0 = (uint32_t)offset, o1 = (uint32_t)((uint64_t)offset >> 32);
-    uint32_t hi[4] = {(uint32_t)block, (uint32_t)(block >> 32), o0, o1};
-    uint32_t lo[4] = {(uint32_t)block, (uint32_t)(block >> 32) | 0x80000000u, o0, o1};
-    philox(hi, q.key0, q.key1);
-    philox(lo, q.key0, q.key1);
-    uint32_t bits = 0;
+// The block's eight half-words, two a word, of which element e is kept where its own is
+// at least q.limit.  Half-words equal to the threshold's upper half, if a lower half
+// matters, are replaced by what the lower one decides; a wave gets there once in 128
+// times.
+__device__ __forceinline__ void halves(const Drop& q, uint64_t block, int64_t offset,
+                                       uint32_t* hi) {
+    const uint32_t c[4] = {(uint32_t)block, (uint32_t)(block >> 32), (uint32_t)offset,
+                           (uint32_t)((uint64_t)offset >> 32)};
 #pragma unroll
-    for (int e = 0; e < kBlock; ++e) {
-        const uint32_t a = (hi[e / 2] >> (16 * (e % 2))) & 0xffffu;
-        const uint32_t b = (lo[e / 2] >> (16 * (e % 2))) & 0xffffu;
-        bits |= (uint32_t)(a > q.upper || (a == q.upper && b >= q.lower)) << e;
+    for (int i = 0; i < 4; ++i) hi[i] = c[i];
+    philox(hi, q.key0, q.key1);
+    if (q.lower == 0) return;
+    // a half of t that is zero sets its top bit in `equal` (and so may halves above it)
+    uint32_t equal = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t t = hi[i] ^ (q.upper | q.upper << 16);
+        equal |= (t - 0x00010001u) & ~t & 0x80008000u;
     }
-    return bits;
+    if (equal) {
+        uint32_t lo[4] = {c[0], c[1] | 0x80000000u, c[2], c[3]};
+        philox(lo, q.key0, q.key1);
+#pragma unroll
+        for (int e = 0; e < kBlock; ++e) {
+            const int shift = 16 * (e % 2);
+            const uint32_t part = 0xffffu << shift;
+            if ((hi[e / 2] & part) == q.upper << shift)
+                hi[e / 2] = (lo[e / 2] >> shift & 0xffffu) >= q.lower ? hi[e / 2] | part
+                                                                      : hi[e / 2] & ~part;
+        }
+    }
+}
+__device__ __forceinline__ bool kept(const Drop& q, const uint32_t* hi, int e) {
+    return (e % 2 ? hi[e / 2] >> 16 : hi[e / 2] & 0xffffu) >= q.limit;
 }
 
+// One generator block a thread: eight elements.
 template <class E, bool RES>
 __global__ __launch_bounds__(kThreads) void k_dropout(const Drop q) {
     using T = typename E::T;
+    using P = Piece<E, E::VEC>;
+    constexpr int N = kBlock / E::VEC;  // vectors of a block
     const int64_t block = (int64_t)blockIdx.x * kThreads + threadIdx.x;
     const int64_t first = block * kBlock;
     if (first >= q.n) return;
-    const int64_t offset = q.offset_at ? *q.offset_at : q.offset;
-    const uint32_t bits = kept(q, (uint64_t)block, offset);
-    const int left = (int)min<int64_t>(kBlock, q.n - first);
     const T* x = (const T*)q.x + first;
     const T* r = (const T*)q.residual + first;
     T* y = (T*)q.y + first;
+    const bool whole = first + kBlock <= q.n;
+    typename P::Raw rx[N], rr[N];
+    if (whole) {
 #pragma unroll
-    for (int e = 0; e < kBlock; ++e)
-        if (e < left) {
-            const float base = RES ? E::up(r[e]) : 0.f;
-            y[e] = E::down(bits >> e & 1 ? fmaf(E::up(x[e]), q.scale, base) : base);
+        for (int k = 0; k < N; ++k) {
+            rx[k] = P::load(x + k * E::VEC);
+            if (RES) rr[k] = P::load(r + k * E::VEC);
         }
+    }
+    uint32_t hi[4];
+    halves(q, (uint64_t)block, q.offset_at ? *q.offset_at : q.offset, hi);
+    if (whole) {
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            float v[E::VEC], base[E::VEC] = {};
+            P::up(rx[k], v);
+            if (RES) P::up(rr[k], base);
+#pragma unroll
+            for (int e = 0; e < E::VEC; ++e)
+                v[e] = kept(q, hi, k * E::VEC + e) ? fmaf(v[e], q.scale, base[e]) : base[e];
+            P::store(y + k * E::VEC, P::down(v));
+        }
+    } else {
+        const int left = (int)(q.n - first);
+#pragma unroll
+        for (int e = 0; e < kBlock - 1; ++e)
+            if (e < left) {
+                const float base = RES ? E::up(r[e]) : 0.f;
+                y[e] = E::down(kept(q, hi, e) ? fmaf(E::up(x[e]), q.scale, base) : base);
+            }
+    }
 }
 
 template <class E>
@@ -124,6 +173,9 @@ extern "C" int gsx_dropout(int32_t dtype, int64_t n, double p, uint64_t seed, in
     q.offset_at = offset_at;
     q.upper = (uint32_t)(threshold >> 16);
     q.lower = (uint32_t)(threshold & 0xffffu);
+    // kept: above the upper half, and at it where nothing is below; replaced half-words
+    // are 0 or 2^16 - 1, so the limit lies between them
+    q.limit = q.lower == 0 ? q.upper : q.upper > 1 ? q.upper : 1;
     q.scale = p < 1.0 ? (float)(1.0 / (1.0 - p)) : 0.f;
     hipStream_t st = (hipStream_t)stream;
     if (dtype == GSX_F32) return run<F32>(q, st);

@@ -33,7 +33,10 @@ constexpr int kThreads = 256;
 constexpr int kBits = 8, kRadix = 1 << kBits;
 constexpr int kSortThreads = 512, kItems = 8, kChunk = kSortThreads * kItems;
 constexpr int kScanGroups = 16;  // of chunks, in the prefix
-constexpr int kTile = 64;        // sorted tokens that a group of lanes adds up
+constexpr int kMostTile = 64;    // sorted tokens that a team of lanes adds up, at most
+constexpr int kBatch = 8;        // rows that a team asks for at a time
+constexpr int kSpan = 32;        // tiles of a row that a single team joins, at most
+constexpr int kJoinThreads = 1024;
 
 struct Embed {
     const void *table, *g_y, *indices;
@@ -233,6 +236,7 @@ struct Sum {
     Embed q;
     const uint2* pairs;
     const uint32_t* live;
+    int tile;      // sorted tokens of a tile
     float* parts;  // (tiles, 2, width): what a tile shares with the one before, and behind
 };
 
@@ -242,14 +246,14 @@ __global__ __launch_bounds__(kThreads) void k_zero(T* p, int64_t n) {
     for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < n; i += step) p[i] = 0;
 }
 
-// One tile, V columns of it.
+// One tile, V columns of it.  A batch of rows is asked for before the first is added.
 template <class E, int V>
 __device__ __forceinline__ void tile_sum(const Sum& s, int64_t tile, int64_t live, int c) {
     using P = Piece<E, V>;
     using T = typename E::T;
     const Embed& q = s.q;
-    const int64_t first = tile * kTile;
-    const int n = (int)min<int64_t>(kTile, live - first);
+    const int64_t first = tile * s.tile;
+    const int n = (int)min<int64_t>(s.tile, live - first);
     const uint2* pairs = s.pairs + first;
     uint32_t key = pairs[0].x;
     bool open = first > 0 && pairs[-1].x == key;  // the tile before has some of this row
@@ -265,19 +269,29 @@ __device__ __forceinline__ void tile_sum(const Sum& s, int64_t tile, int64_t liv
             P::store((T*)q.g_table + (int64_t)key * q.width + c, P::down(acc));
         }
     };
-    for (int j = 0; j < n; ++j) {
-        const uint2 p = pairs[j];
-        float v[V];
-        P::up(P::load((const T*)q.g_y + (int64_t)p.y * q.stride + c), v);
-        if (p.x != key) {
-            write();
-            key = p.x;
-            open = false;
+    for (int j = 0; j < n; j += kBatch) {
+        uint2 p[kBatch];
+        typename P::Raw raw[kBatch];
 #pragma unroll
-            for (int e = 0; e < V; ++e) acc[e] = 0.f;
+        for (int u = 0; u < kBatch; ++u) p[u] = pairs[min(j + u, n - 1)];
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u)
+            raw[u] = P::load((const T*)q.g_y + (int64_t)p[u].y * q.stride + c);
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+            if (j + u >= n) break;
+            if (p[u].x != key) {
+                write();
+                key = p[u].x;
+                open = false;
+#pragma unroll
+                for (int e = 0; e < V; ++e) acc[e] = 0.f;
+            }
+            float v[V];
+            P::up(raw[u], v);
+#pragma unroll
+            for (int e = 0; e < V; ++e) acc[e] += v[e];
         }
-#pragma unroll
-        for (int e = 0; e < V; ++e) acc[e] += v[e];
     }
     if (!more) write();
     else store_floats<V>(open ? part : part + q.width, acc);
@@ -290,49 +304,107 @@ __global__ __launch_bounds__(kThreads) void k_tile_sums(const Sum s) {
     if (at >= s.q.width) return;
     const int64_t live = *s.live, step = (int64_t)gridDim.x * (kThreads / G);
     for (int64_t tile = (int64_t)blockIdx.x * (kThreads / G) + threadIdx.x / G;
-         tile * kTile < live; tile += step)
+         tile * s.tile < live; tile += step)
         tile_sum<E, V>(s, tile, live, min(at, s.q.width - V));
 }
 
-// The row over several tiles that begins in this one, if there is one.
-template <class E, int V>
-__device__ __forceinline__ void join(const Sum& s, int64_t tile, int64_t live, int c) {
-    using P = Piece<E, V>;
-    using T = typename E::T;
-    const Embed& q = s.q;
-    const int64_t first = tile * kTile;
-    const uint32_t key = s.pairs[first + kTile - 1].x;
-    if (s.pairs[first + kTile].x != key) return;
-    // begins in an earlier tile
-    if (first > 0 && s.pairs[first].x == key && s.pairs[first - 1].x == key) return;
-    float acc[V], v[V];
-    load_floats<V>(s.parts + (tile * 2 + 1) * q.width + c, acc);
-    for (int64_t t = tile + 1; t * kTile < live && s.pairs[t * kTile].x == key; ++t) {
-        load_floats<V>(s.parts + t * 2 * q.width + c, v);
-#pragma unroll
-        for (int e = 0; e < V; ++e) acc[e] += v[e];
+// How many tiles after `tile` share the row that it leaves open and that begins in
+// it; 0 if there is none.
+__device__ __forceinline__ int64_t span_of(const Sum& s, int64_t tile, int64_t live) {
+    const int64_t first = tile * s.tile, next = first + s.tile;
+    if (next >= live) return 0;
+    const uint32_t key = s.pairs[next - 1].x;
+    if (s.pairs[next].x != key) return 0;
+    if (first > 0 && s.pairs[first].x == key && s.pairs[first - 1].x == key) return 0;
+    // tiles' first keys do not fall: double the reach, then halve it
+    const int64_t tiles = (live + s.tile - 1) / s.tile;
+    int64_t in = tile + 1, reach = 1;
+    while (in + reach < tiles && s.pairs[(in + reach) * s.tile].x == key) {
+        in += reach;
+        reach *= 2;
     }
-#pragma unroll
-    for (int e = 0; e < V; ++e) acc[e] *= q.scale;
-    P::store((T*)q.g_table + (int64_t)key * q.width + c, P::down(acc));
+    for (; reach > 0; reach /= 2)
+        if (in + reach < tiles && s.pairs[(in + reach) * s.tile].x == key) in += reach;
+    return in - tile;
 }
 
+// Adds up a row's parts in tiles first, first + step, ... below end.
+template <int V>
+__device__ __forceinline__ void add_parts(const Sum& s, int64_t first, int64_t end, int64_t step,
+                                          int c, float* acc) {
+    for (int64_t t = first; t < end; t += kBatch * step) {
+        float v[kBatch][V];
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u)
+            load_floats<V>(s.parts + min(t + u * step, end - 1) * 2 * s.q.width + c, v[u]);
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u)
+            if (t + u * step < end) {
+#pragma unroll
+                for (int e = 0; e < V; ++e) acc[e] += v[u][e];
+            }
+    }
+}
+
+// Rows over several tiles, each by the team of lanes of the tile in which it begins;
+// over more than kSpan, by all teams of the workgroup together.
 template <class E, int V, int G>
-__global__ __launch_bounds__(kThreads) void k_join(const Sum s) {
-    const int at = (blockIdx.y * G + threadIdx.x % G) * V;
-    if (at >= s.q.width) return;
-    const int64_t live = *s.live, step = (int64_t)gridDim.x * (kThreads / G);
-    for (int64_t tile = (int64_t)blockIdx.x * (kThreads / G) + threadIdx.x / G;
-         tile * kTile + kTile < live; tile += step)
-        join<E, V>(s, tile, live, min(at, s.q.width - V));
+__global__ __launch_bounds__(kJoinThreads) void k_join(const Sum s) {
+    using P = Piece<E, V>;
+    using T = typename E::T;
+    constexpr int kTeams = kJoinThreads / G;
+    __shared__ float room[kJoinThreads][V + 1];
+    __shared__ int64_t spans[kTeams];
+    const Embed& q = s.q;
+    const int team = threadIdx.x / G, at = (blockIdx.y * G + threadIdx.x % G) * V;
+    const int c = min(at, q.width - V);
+    const int64_t live = *s.live, step = (int64_t)gridDim.x * kTeams;
+    auto write = [&](int64_t tile, float* acc) {
+        const uint32_t key = s.pairs[tile * s.tile + s.tile - 1].x;
+#pragma unroll
+        for (int e = 0; e < V; ++e) acc[e] *= q.scale;
+        if (at < q.width) P::store((T*)q.g_table + (int64_t)key * q.width + c, P::down(acc));
+    };
+    for (int64_t base = (int64_t)blockIdx.x * kTeams; base * s.tile < live; base += step) {
+        const int64_t tile = base + team, span = span_of(s, tile, live);
+        if (span > 0 && span <= kSpan) {
+            float acc[V];
+            load_floats<V>(s.parts + (tile * 2 + 1) * q.width + c, acc);
+            add_parts<V>(s, tile + 1, tile + 1 + span, 1, c, acc);
+            write(tile, acc);
+        }
+        if (threadIdx.x % G == 0) spans[team] = span;
+        if (!__syncthreads_or(span > kSpan)) continue;
+        for (int t = 0; t < kTeams; ++t) {
+            const int64_t far = spans[t], own = base + t;
+            if (far <= kSpan) continue;
+            float acc[V] = {};
+            if (team == 0) load_floats<V>(s.parts + (own * 2 + 1) * q.width + c, acc);
+            add_parts<V>(s, own + 1 + team, own + 1 + far, kTeams, c, acc);
+#pragma unroll
+            for (int e = 0; e < V; ++e) room[threadIdx.x][e] = acc[e];
+            for (int n = kTeams / 2; n > 0; n /= 2) {
+                __syncthreads();
+                if (team < n) {
+#pragma unroll
+                    for (int e = 0; e < V; ++e) {
+                        acc[e] += room[threadIdx.x + n * G][e];
+                        room[threadIdx.x][e] = acc[e];
+                    }
+                }
+            }
+            if (team == 0) write(own, acc);
+            __syncthreads();
+        }
+    }
 }
 
 // ----------------------------------------------------------------- host --
 
-// A launch holds fewer than 2^32 threads: at most 2^23 workgroups here, a power of
-// two below the limit, whose threads walk on.
+// A launch holds fewer than 2^32 threads: at most 2^21 workgroups of 1024 and
+// fewer here, whose threads walk on.
 dim3 grid_for(int64_t n, int per_group, int times) {
-    const int64_t groups = (n + per_group - 1) / per_group, most = ((int64_t)1 << 23) / times;
+    const int64_t groups = (n + per_group - 1) / per_group, most = ((int64_t)1 << 21) / times;
     return dim3((unsigned)(groups < most ? groups : most), (unsigned)times);
 }
 
@@ -357,7 +429,7 @@ int check_args(int dtype, int64_t count, int64_t rows, int32_t width, const void
 }
 
 struct Layout {
-    int chunks, passes, bits;
+    int chunks, passes, bits, tile;
     int64_t tiles, counts, totals, live, pairs[2], parts, total;
 };
 
@@ -367,7 +439,8 @@ Layout layout(int64_t count, int64_t rows, int32_t width) {
     l.bits = 1;
     while (((int64_t)1 << l.bits) < rows) ++l.bits;
     l.passes = (l.bits + kBits - 1) / kBits;
-    l.tiles = (count + kTile - 1) / kTile;
+    l.tile = kMostTile;
+    l.tiles = (count + l.tile - 1) / l.tile;
     l.counts = 0;
     l.totals = up_to((int64_t)l.chunks * kRadix * 4, 256);
     l.live = l.totals + kRadix * 4;
@@ -443,13 +516,15 @@ int gradient(const Embed& q, char* ws, hipStream_t st) {
     u.q = q;
     u.pairs = s.to;
     u.live = s.live;
+    u.tile = l.tile;
     u.parts = (float*)(ws + l.parts);
     return for_width<E>(q.width, [&](auto v, auto g, int times) -> int {
         constexpr int V = decltype(v)::value, G = decltype(g)::value;
         const dim3 grid = grid_for(l.tiles, kThreads / G, times);
         hipLaunchKernelGGL((k_tile_sums<E, V, G>), grid, dim3(kThreads), 0, st, u);
         GSX_LAUNCH_CHECK();
-        hipLaunchKernelGGL((k_join<E, V, G>), grid, dim3(kThreads), 0, st, u);
+        hipLaunchKernelGGL((k_join<E, V, G>), grid_for(l.tiles, kJoinThreads / G, times),
+                           dim3(kJoinThreads), 0, st, u);
         GSX_LAUNCH_CHECK();
         return GSX_OK;
     });

@@ -30,10 +30,11 @@ using namespace gsx;
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kBits = 8, kRadix = 1 << kBits;
 constexpr int kSortThreads = 512, kItems = 8, kChunk = kSortThreads * kItems;
 constexpr int kScanGroups = 16;  // of chunks, in the prefix
+constexpr int kFewItems = 16;    // tokens of a thread, where one workgroup sorts them all
 constexpr int kMostTile = 64;    // sorted tokens that a team of lanes adds up, at most
+constexpr int kLook = 4;         // tokens that a team looks up at a time
 constexpr int kBatch = 8;        // rows that a team asks for at a time
 constexpr int kSpan = 32;        // tiles of a row that a single team joins, at most
 constexpr int kJoinThreads = 1024;
@@ -48,29 +49,40 @@ struct Embed {
 
 // Token i's row, or -1.
 __device__ __forceinline__ int64_t row_of(const Embed& q, int64_t i) {
-    const int64_t k = q.index64 ? ((const int64_t*)q.indices)[i] : ((const int32_t*)q.indices)[i];
+    const int64_t k =
+        q.index64 ? ((const int64_t*)q.indices)[i] : (int64_t)((const int32_t*)q.indices)[i];
     return k >= 0 && k < q.rows ? k : -1;
 }
 
-// G lanes a token, a piece of V elements each; blockIdx.y: pieces from 64 on.
+// G lanes a token, a piece of V elements each; blockIdx.y: pieces from 64 on.  A team
+// takes kLook tokens at a time, whose indices are asked for together, and then the rows.
 template <class E, int V, int G>
 __global__ __launch_bounds__(kThreads) void k_lookup(const Embed q) {
     using P = Piece<E, V>;
     using T = typename E::T;
+    constexpr int kTeams = kThreads / G;
     const int at = (blockIdx.y * G + threadIdx.x % G) * V;
     if (at >= q.width) return;
     const int c = min(at, q.width - V);
-    const int64_t step = (int64_t)gridDim.x * (kThreads / G);
-    for (int64_t i = (int64_t)blockIdx.x * (kThreads / G) + threadIdx.x / G; i < q.count;
+    const int64_t step = (int64_t)gridDim.x * (kTeams * kLook);
+    for (int64_t i = (int64_t)blockIdx.x * (kTeams * kLook) + threadIdx.x / G; i < q.count;
          i += step) {
-        const int64_t k = row_of(q, i);
-        float v[V] = {};
-        if (k >= 0) {
-            P::up(P::load((const T*)q.table + k * q.stride + c), v);
+        int64_t k[kLook];
+        typename P::Raw raw[kLook];
 #pragma unroll
-            for (int e = 0; e < V; ++e) v[e] *= q.scale;
+        for (int u = 0; u < kLook; ++u) k[u] = row_of(q, min(i + u * kTeams, q.count - 1));
+#pragma unroll
+        for (int u = 0; u < kLook; ++u)
+            raw[u] = P::load((const T*)q.table + max(k[u], (int64_t)0) * q.stride + c);
+#pragma unroll
+        for (int u = 0; u < kLook; ++u) {
+            if (i + u * kTeams >= q.count) break;
+            float v[V];
+            P::up(raw[u], v);
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[e] = k[u] >= 0 ? v[e] * q.scale : 0.f;
+            P::store((T*)q.y + (i + u * kTeams) * q.width + c, P::down(v));
         }
-        P::store((T*)q.y + i * q.width + c, P::down(v));
     }
 }
 
@@ -80,37 +92,89 @@ struct Sort {
     Embed q;
     const uint2* from;  // (key, token), or NULL: the indices
     uint2* to;
-    uint32_t* counts;   // (chunks, kRadix)
-    uint32_t* totals;   // kRadix
+    uint32_t* counts;   // (chunks, 2^BITS)
+    uint32_t* totals;   // 2^BITS
     uint32_t* live;     // how many tokens name a row
     int chunks, shift, bits;
+    int64_t zeros;      // bytes of the table's gradient, cleared beside the first counts
 };
 
-__device__ __forceinline__ int64_t live_tokens(const Sort& s) {
-    return s.from ? (int64_t)*s.live : s.q.count;
-}
-// The pair at place i of the pass, if there is one.
-__device__ __forceinline__ bool pair_at(const Sort& s, int64_t i, int64_t n, uint2* p) {
-    if (i >= n) return false;
-    if (s.from) {
-        *p = s.from[i];
-        return true;
-    }
-    const int64_t k = row_of(s.q, i);
-    *p = make_uint2((uint32_t)k, (uint32_t)i);
-    return k >= 0;
+// Clears the table's gradient: workgroup `at` of `of`.
+template <int THREADS>
+__device__ __forceinline__ void clear(const Sort& s, int64_t at, int64_t of) {
+    // whole vectors from the first aligned address on, single bytes before and behind
+    uint8_t* p = (uint8_t*)s.q.g_table;
+    const int64_t head = min<int64_t>((16 - (uintptr_t)p % 16) % 16, s.zeros);
+    const int64_t vectors = (s.zeros - head) / 16, tail = s.zeros - head - vectors * 16;
+    u32x4* v = (u32x4*)(p + head);
+    for (int64_t i = at * THREADS + threadIdx.x; i < vectors; i += of * THREADS)
+        v[i] = u32x4{0, 0, 0, 0};
+    if (at == 0 && (int)threadIdx.x < head) p[threadIdx.x] = 0;
+    if (at == 0 && (int)threadIdx.x < tail) p[head + vectors * 16 + threadIdx.x] = 0;
 }
 
+constexpr uint32_t kNone = ~0u;  // the key of a place without a pair; rows lie below 2^30
+
+// Keys and tokens at places base + own, base + own + step, ... of the pass's n; all are
+// asked for before the first is looked at.  base, the same in the whole workgroup, lies
+// below the number of tokens.
+template <int ITEMS>
+__device__ __forceinline__ void load_indices(const Sort& s, int64_t base, int own, int step,
+                                             uint32_t* key, uint32_t* token) {
+    const int left = (int)min<int64_t>(s.q.count - base, 1 << 20);
+    uint32_t high[ITEMS];
+#pragma unroll
+    for (int r = 0; r < ITEMS; ++r) {
+        const uint32_t at = (uint32_t)min(own + r * step, left - 1);
+        if (s.q.index64) {
+            const uint2 v = ((const uint2*)s.q.indices + base)[at];
+            key[r] = v.x;
+            high[r] = v.y;
+        } else {
+            key[r] = ((const uint32_t*)s.q.indices + base)[at];
+            high[r] = 0;
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < ITEMS; ++r) {
+        // an index of 32 bits that is negative is not below 2^30
+        const bool there = own + r * step < left && high[r] == 0 && key[r] < (uint32_t)s.q.rows;
+        key[r] = there ? key[r] : kNone;
+        token[r] = (uint32_t)base + (uint32_t)(own + r * step);
+    }
+}
+template <int ITEMS>
+__device__ __forceinline__ void load_pairs(const Sort& s, int64_t base, int own, int step,
+                                           uint32_t* key, uint32_t* token) {
+    if (!s.from) return load_indices<ITEMS>(s, base, own, step, key, token);
+    const int left = (int)min<int64_t>(max<int64_t>((int64_t)*s.live - base, 0), 1 << 20);
+    const uint2* from = s.from + base;
+#pragma unroll
+    for (int r = 0; r < ITEMS; ++r) {
+        const uint2 v = from[max(min(own + r * step, left - 1), 0)];
+        key[r] = v.x;
+        token[r] = v.y;
+    }
+#pragma unroll
+    for (int r = 0; r < ITEMS; ++r) key[r] = own + r * step < left ? key[r] : kNone;
+}
+
+// The first s.chunks workgroups count; those behind clear the gradient.
+template <int BITS>
 __global__ __launch_bounds__(kSortThreads) void k_count(const Sort s) {
+    constexpr int kRadix = 1 << BITS;
     __shared__ uint32_t hist[kRadix];
+    if ((int)blockIdx.x >= s.chunks) {
+        clear<kSortThreads>(s, blockIdx.x - s.chunks, gridDim.x - s.chunks);
+        return;
+    }
     for (int d = threadIdx.x; d < kRadix; d += kSortThreads) hist[d] = 0;
     __syncthreads();
-    const int64_t n = live_tokens(s), first = (int64_t)blockIdx.x * kChunk;
-    for (int r = 0; r < kItems; ++r) {
-        uint2 p;
-        if (pair_at(s, first + r * kSortThreads + threadIdx.x, n, &p))
-            atomicAdd(&hist[(p.x >> s.shift) & (kRadix - 1)], 1u);
-    }
+    uint32_t key[kItems], token[kItems];
+    load_pairs<kItems>(s, (int64_t)blockIdx.x * kChunk, threadIdx.x, kSortThreads, key, token);
+#pragma unroll
+    for (int r = 0; r < kItems; ++r)
+        if (key[r] != kNone) atomicAdd(&hist[key[r] >> s.shift & (kRadix - 1)], 1u);
     __syncthreads();
     for (int d = threadIdx.x; d < kRadix; d += kSortThreads)
         s.counts[(int64_t)blockIdx.x * kRadix + d] = hist[d];
@@ -118,14 +182,23 @@ __global__ __launch_bounds__(kSortThreads) void k_count(const Sort s) {
 
 // Each digit's prefix over the chunks, in place, and its total: 64 digits a
 // workgroup, the chunks in kScanGroups stretches.
+template <int BITS>
 __global__ __launch_bounds__(64 * kScanGroups) void k_prefix(const Sort s) {
+    constexpr int kRadix = 1 << BITS, kHeld = 16;
     __shared__ uint32_t sums[kScanGroups][64];
     const int lane = threadIdx.x & 63, g = threadIdx.x >> 6;
     const int d = blockIdx.x * 64 + lane;
     const int per = (s.chunks + kScanGroups - 1) / kScanGroups;
     const int first = min(g * per, s.chunks), end = min(first + per, s.chunks);
-    uint32_t sum = 0;
-    for (int c = first; c < end; ++c) sum += s.counts[(int64_t)c * kRadix + d];
+    // the first kHeld counts stay in registers
+    uint32_t v[kHeld], sum = 0;
+#pragma unroll
+    for (int k = 0; k < kHeld; ++k)
+        v[k] = first + k < end ? s.counts[(int64_t)(first + k) * kRadix + d] : 0;
+#pragma unroll
+    for (int k = 0; k < kHeld; ++k) sum += v[k];
+#pragma unroll 8
+    for (int c = first + kHeld; c < end; ++c) sum += s.counts[(int64_t)c * kRadix + d];
     sums[g][lane] = sum;
     __syncthreads();
     uint32_t run = 0, total = 0;
@@ -134,100 +207,206 @@ __global__ __launch_bounds__(64 * kScanGroups) void k_prefix(const Sort s) {
         if (k < g) run += sums[k][lane];
         total += sums[k][lane];
     }
-    for (int c = first; c < end; ++c) {
+#pragma unroll
+    for (int k = 0; k < kHeld; ++k) {
+        if (first + k < end) s.counts[(int64_t)(first + k) * kRadix + d] = run;
+        run += v[k];
+    }
+#pragma unroll 8
+    for (int c = first + kHeld; c < end; ++c) {
         uint32_t* at = s.counts + (int64_t)c * kRadix + d;
-        const uint32_t v = *at;
+        const uint32_t t = *at;
         *at = run;
-        run += v;
+        run += t;
     }
     if (g == 0) s.totals[d] = total;
 }
 
-// Lanes of the wave, among the valid ones, with the same digit.
+// Lanes of the wave, among the valid ones, with the same digit: those that differ in no
+// bit.  A bit's ballot, against this lane's bit in all places, gives those that do.
 __device__ __forceinline__ uint64_t same_digit(uint32_t d, bool valid, int bits) {
-    uint64_t differ = 0;
+    uint32_t lo = 0, hi = 0;
     for (int b = 0; b < bits; ++b) {
-        const uint64_t set = __ballot(d >> b & 1);
-        differ |= set ^ (d >> b & 1 ? ~0ull : 0ull);
+        const uint32_t own = (uint32_t)((int)(d << (31 - b)) >> 31);
+        const uint64_t set = __ballot(own);
+        lo = __builtin_amdgcn_bitop3_b32(lo, (uint32_t)set, own, 0xf6);  // a | b ^ c
+        hi = __builtin_amdgcn_bitop3_b32(hi, (uint32_t)(set >> 32), own, 0xf6);
     }
-    return ~differ & __ballot(valid);
+    return ~((uint64_t)hi << 32 | lo) & __ballot(valid);
 }
 
-__global__ __launch_bounds__(kSortThreads) void k_place(const Sort s) {
-    constexpr int kWaves = kSortThreads / 64;
-    __shared__ uint32_t cnt[kWaves][kRadix];
-    __shared__ uint32_t in_chunk[kRadix], base[kRadix];
-    __shared__ uint32_t sums[2][kRadix / 64];
-    __shared__ uint2 pairs[kChunk];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    for (int k = tid; k < kWaves * kRadix; k += kSortThreads) (&cnt[0][0])[k] = 0;
-    const int64_t n = live_tokens(s);
-    const int64_t first = (int64_t)blockIdx.x * kChunk + wave * (64 * kItems);
-    uint2 p[kItems];
-    bool valid[kItems];
-    uint32_t rank[kItems];
+// The rank of each of a wave's items among those of its digit, in their order, with
+// cnt[d] (zero before) left as the digit's count.
+template <int ITEMS, int RADIX>
+__device__ __forceinline__ void wave_ranks(const uint32_t* key, int shift, int bits,
+                                           uint16_t* cnt, uint32_t* rank) {
+    const int lane = threadIdx.x & 63;
 #pragma unroll
-    for (int r = 0; r < kItems; ++r) {
-        p[r] = make_uint2(0, 0);
-        valid[r] = pair_at(s, first + r * 64 + lane, n, &p[r]);
-    }
-    __syncthreads();
-    // a wave's tokens in their order: each digit's count so far, and the lanes before
-#pragma unroll
-    for (int r = 0; r < kItems; ++r) {
-        const uint32_t d = (p[r].x >> s.shift) & (kRadix - 1);
-        const uint64_t same = same_digit(d, valid[r], s.bits);
+    for (int r = 0; r < ITEMS; ++r) {
+        const uint32_t d = key[r] >> shift & (RADIX - 1);
+        const uint64_t same = same_digit(d, key[r] != kNone, bits);
         const uint64_t before = same & ((1ull << lane) - 1);
-        const uint32_t c = cnt[wave][d];
+        const uint32_t c = cnt[d];
         rank[r] = c + (uint32_t)__popcll(before);
         wave_fence();
-        if (valid[r] && before == 0) cnt[wave][d] = c + (uint32_t)__popcll(same);
+        if (key[r] != kNone && before == 0) cnt[d] = (uint16_t)(c + (uint32_t)__popcll(same));
         wave_fence();
     }
+}
+
+// Exclusive sums over a workgroup of THREADS, with the total.  `room`: THREADS / 64
+// words, free again after the next barrier.
+template <int THREADS>
+__device__ __forceinline__ uint32_t prefix_sum(uint32_t v, uint32_t* room, uint32_t* total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const uint32_t incl = wave_incl_scan(v);
+    if (lane == 63) room[wave] = incl;
     __syncthreads();
-    // digits' places: in the chunk by the chunk's counts, in the whole by the totals
-    uint32_t mine = 0, total = 0, mine_incl = 0, total_incl = 0;
-    if (tid < kRadix) {
+    uint32_t before = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < THREADS / 64; ++w) {
+        if (w < wave) before += room[w];
+        all += room[w];
+    }
+    *total = all;
+    return before + incl - v;
+}
+
+// Up to 8 bits the chunk is regrouped by digit first, so that stores are runs; with
+// more digits than a chunk has tokens there are none.  A wave's counts are 16 bits, two
+// digits a word, which are added up as words: a chunk's 4096 tokens do not carry.
+template <int BITS>
+__global__ __launch_bounds__(kSortThreads) void k_place(const Sort s) {
+    constexpr int kRadix = 1 << BITS, kWaves = kSortThreads / 64, kWords = kRadix / 2;
+    constexpr int kEach = kWords > kSortThreads ? kWords / kSortThreads : 1;  // words a thread
+    constexpr bool kRegroup = BITS <= 8;
+    using Words = __attribute__((ext_vector_type(kEach))) uint32_t;
+    using Bases = __attribute__((ext_vector_type(2 * kEach))) uint32_t;
+    static_assert(kChunk < 1 << 16, "counts of 16 bits");
+    __shared__ alignas(16) uint16_t cnt[kWaves][kRadix];
+    __shared__ alignas(16) uint32_t base[kRadix];
+    __shared__ uint32_t room[2][kWaves];
+    __shared__ uint32_t in_chunk[kRegroup ? kRadix : 1];
+    __shared__ uint2 pairs[kRegroup ? kChunk : 1];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    for (int k = tid; k < kWaves * kRadix / 8; k += kSortThreads)
+        ((u32x4*)cnt)[k] = u32x4{0, 0, 0, 0};
+    uint32_t key[kItems], token[kItems], rank[kItems];
+    load_pairs<kItems>(s, (int64_t)blockIdx.x * kChunk, wave * (64 * kItems) + lane, 64, key,
+                       token);
+    Bases before = 0, total = 0;
+    const bool mine = tid * kEach < kWords;
+    if (mine) {
+        total = ((const Bases*)s.totals)[tid];
+        before = ((const Bases*)(s.counts + (int64_t)blockIdx.x * kRadix))[tid];
+    }
+    uint32_t sum = 0, live, held = 0;
+#pragma unroll
+    for (int k = 0; k < 2 * kEach; ++k) sum += total[k];
+    uint32_t at = prefix_sum<kSortThreads>(sum, room[0], &live);  // its barrier: cnt is clear
+    wave_ranks<kItems, kRadix>(key, s.shift, s.bits, cnt[wave], rank);
+    // the first pass counts the tokens that name a row
+    if (!s.from && blockIdx.x == 0 && tid == 0) *s.live = live;
+    __syncthreads();
+    Words own = 0;
+    if (mine) {
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) {
-            const uint32_t c = cnt[w][tid];
-            cnt[w][tid] = mine;
-            mine += c;
+            Words* c = (Words*)cnt[w] + tid;
+            const Words v = *c;
+            *c = own;
+            own += v;
         }
-        total = s.totals[tid];
-        mine_incl = wave_incl_scan(mine);
-        total_incl = wave_incl_scan(total);
-        if (lane == 63) {
-            sums[0][wave] = mine_incl;
-            sums[1][wave] = total_incl;
+#pragma unroll
+        for (int k = 0; k < 2 * kEach; ++k) {
+            before[k] += at;
+            at += total[k];
+        }
+        ((Bases*)base)[tid] = before;
+    }
+    if constexpr (kRegroup) {
+        static_assert(kEach == 1, "two digits a thread");
+        const uint32_t first = own[0] & 0xffffu, second = own[0] >> 16;
+        const uint32_t start = prefix_sum<kSortThreads>(first + second, room[1], &held);
+        if (mine) {
+            in_chunk[2 * tid] = start;
+            in_chunk[2 * tid + 1] = start + first;
         }
     }
     __syncthreads();
-    if (tid < kRadix) {
-        for (int w = 0; w < wave; ++w) {
-            mine_incl += sums[0][w];
-            total_incl += sums[1][w];
-        }
-        in_chunk[tid] = mine_incl - mine;
-        base[tid] = total_incl - total + s.counts[(int64_t)blockIdx.x * kRadix + tid];
-        // the first pass counts the tokens that name a row
-        if (!s.from && blockIdx.x == 0 && tid == kRadix - 1) *s.live = total_incl;
-    }
-    __syncthreads();
-    // regrouped by digit, so that stores are runs
 #pragma unroll
     for (int r = 0; r < kItems; ++r)
-        if (valid[r]) {
-            const uint32_t d = (p[r].x >> s.shift) & (kRadix - 1);
-            pairs[in_chunk[d] + cnt[wave][d] + rank[r]] = p[r];
+        if (key[r] != kNone) {
+            const uint32_t d = key[r] >> s.shift & (kRadix - 1), k = cnt[wave][d] + rank[r];
+            if constexpr (kRegroup) pairs[in_chunk[d] + k] = make_uint2(key[r], token[r]);
+            else s.to[base[d] + k] = make_uint2(key[r], token[r]);
         }
-    __syncthreads();
-    const int held = (int)(sums[0][0] + sums[0][1] + sums[0][2] + sums[0][3]);
-    for (int j = tid; j < held; j += kSortThreads) {
-        const uint2 e = pairs[j];
-        const uint32_t d = (e.x >> s.shift) & (kRadix - 1);
-        s.to[base[d] + (uint32_t)j - in_chunk[d]] = e;
+    if constexpr (kRegroup) {
+        __syncthreads();
+        for (int j = tid; j < (int)held; j += kSortThreads) {
+            const uint2 e = pairs[j];
+            const uint32_t d = (e.x >> s.shift) & (kRadix - 1);
+            s.to[base[d] + (uint32_t)j - in_chunk[d]] = e;
+        }
     }
+}
+
+// All passes over few tokens by one workgroup, in shared memory; the others clear the
+// gradient.
+constexpr int kFewThreads = 1024;
+template <int ITEMS>
+__global__ __launch_bounds__(kFewThreads) void k_sort_few(const Sort s) {
+    constexpr int kWaves = kFewThreads / 64, kRadix = 256;
+    __shared__ uint2 pairs[kFewThreads * ITEMS];
+    __shared__ uint16_t cnt[kWaves][kRadix];
+    __shared__ uint32_t start[kRadix], room[kWaves];
+    if (blockIdx.x > 0) {
+        clear<kFewThreads>(s, blockIdx.x - 1, gridDim.x - 1);
+        return;
+    }
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    uint32_t key[ITEMS], token[ITEMS];
+    load_indices<ITEMS>(s, 0, wave * (64 * ITEMS) + lane, 64, key, token);
+    uint32_t live = 0;
+    for (int shift = 0; shift < s.bits; shift += 8) {
+        for (int k = tid; k < kWaves * kRadix / 2; k += kFewThreads) ((uint32_t*)cnt)[k] = 0;
+        __syncthreads();
+        uint32_t rank[ITEMS];
+        wave_ranks<ITEMS, kRadix>(key, shift, min(s.bits - shift, 8), cnt[wave], rank);
+        __syncthreads();
+        uint32_t mine = 0;
+        if (tid < kRadix) {
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) {
+                const uint32_t c = cnt[w][tid];
+                cnt[w][tid] = (uint16_t)mine;
+                mine += c;
+            }
+        }
+        const uint32_t at = prefix_sum<kFewThreads>(mine, room, &live);
+        if (tid < kRadix) start[tid] = at;
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < ITEMS; ++r)
+            if (key[r] != kNone) {
+                // (formed again: kept, the places of 16 digits take too many registers)
+                const uint32_t d = (uint32_t)here((int)key[r]) >> shift & (kRadix - 1);
+                pairs[start[d] + cnt[wave][d] + rank[r]] = make_uint2(key[r], token[r]);
+            }
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < ITEMS; ++r) {
+            const uint32_t i = wave * (64 * ITEMS) + r * 64 + lane;
+            const uint2 e = pairs[i];  // from `live` on: whatever is there
+            key[r] = i < live ? e.x : kNone;
+            token[r] = e.y;
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < ITEMS; ++r)
+        if (key[r] != kNone)
+            s.to[wave * (64 * ITEMS) + r * 64 + lane] = make_uint2(key[r], token[r]);
+    if (tid == 0) *s.live = live;
 }
 
 // ------------------------------------------------------------------ sum --
@@ -236,15 +415,10 @@ struct Sum {
     Embed q;
     const uint2* pairs;
     const uint32_t* live;
-    int tile;      // sorted tokens of a tile
+    int tile;          // sorted tokens of a tile
+    uint32_t* begins;  // of a row that spans tiles, the first; others' are not set
     float* parts;  // (tiles, 2, width): what a tile shares with the one before, and behind
 };
-
-template <class T>
-__global__ __launch_bounds__(kThreads) void k_zero(T* p, int64_t n) {
-    const int64_t step = (int64_t)gridDim.x * kThreads;
-    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < n; i += step) p[i] = 0;
-}
 
 // One tile, V columns of it.  A batch of rows is asked for before the first is added.
 template <class E, int V>
@@ -293,8 +467,14 @@ __device__ __forceinline__ void tile_sum(const Sum& s, int64_t tile, int64_t liv
             for (int e = 0; e < V; ++e) acc[e] += v[e];
         }
     }
-    if (!more) write();
-    else store_floats<V>(open ? part : part + q.width, acc);
+    if (!more) {
+        write();
+    } else if (open) {
+        store_floats<V>(part, acc);
+    } else {
+        store_floats<V>(part + q.width, acc);
+        s.begins[key] = (uint32_t)tile;
+    }
 }
 
 // G lanes a tile, a piece of V columns each.
@@ -308,37 +488,28 @@ __global__ __launch_bounds__(kThreads) void k_tile_sums(const Sum s) {
         tile_sum<E, V>(s, tile, live, min(at, s.q.width - V));
 }
 
-// How many tiles after `tile` share the row that it leaves open and that begins in
+// How many tiles before this one share the row that is open at its begin and ends in
 // it; 0 if there is none.
 __device__ __forceinline__ int64_t span_of(const Sum& s, int64_t tile, int64_t live) {
     const int64_t first = tile * s.tile, next = first + s.tile;
-    if (next >= live) return 0;
-    const uint32_t key = s.pairs[next - 1].x;
-    if (s.pairs[next].x != key) return 0;
-    if (first > 0 && s.pairs[first].x == key && s.pairs[first - 1].x == key) return 0;
-    // tiles' first keys do not fall: double the reach, then halve it
-    const int64_t tiles = (live + s.tile - 1) / s.tile;
-    int64_t in = tile + 1, reach = 1;
-    while (in + reach < tiles && s.pairs[(in + reach) * s.tile].x == key) {
-        in += reach;
-        reach *= 2;
-    }
-    for (; reach > 0; reach /= 2)
-        if (in + reach < tiles && s.pairs[(in + reach) * s.tile].x == key) in += reach;
-    return in - tile;
+    if (first == 0 || first >= live) return 0;
+    const uint32_t key = s.pairs[first].x;
+    if (s.pairs[first - 1].x != key || (next < live && s.pairs[next].x == key)) return 0;
+    return tile - (int64_t)s.begins[key];
 }
 
 // Adds up a row's parts in tiles first, first + step, ... below end.
 template <int V>
 __device__ __forceinline__ void add_parts(const Sum& s, int64_t first, int64_t end, int64_t step,
                                           int c, float* acc) {
-    for (int64_t t = first; t < end; t += kBatch * step) {
-        float v[kBatch][V];
+    constexpr int kParts = V == 8 ? kBatch / 2 : kBatch;
+    for (int64_t t = first; t < end; t += kParts * step) {
+        float v[kParts][V];
 #pragma unroll
-        for (int u = 0; u < kBatch; ++u)
+        for (int u = 0; u < kParts; ++u)
             load_floats<V>(s.parts + min(t + u * step, end - 1) * 2 * s.q.width + c, v[u]);
 #pragma unroll
-        for (int u = 0; u < kBatch; ++u)
+        for (int u = 0; u < kParts; ++u)
             if (t + u * step < end) {
 #pragma unroll
                 for (int e = 0; e < V; ++e) acc[e] += v[u][e];
@@ -346,7 +517,7 @@ __device__ __forceinline__ void add_parts(const Sum& s, int64_t first, int64_t e
     }
 }
 
-// Rows over several tiles, each by the team of lanes of the tile in which it begins;
+// Rows over several tiles, each by the team of lanes of the tile in which it ends;
 // over more than kSpan, by all teams of the workgroup together.
 template <class E, int V, int G>
 __global__ __launch_bounds__(kJoinThreads) void k_join(const Sum s) {
@@ -354,13 +525,14 @@ __global__ __launch_bounds__(kJoinThreads) void k_join(const Sum s) {
     using T = typename E::T;
     constexpr int kTeams = kJoinThreads / G;
     __shared__ float room[kJoinThreads][V + 1];
-    __shared__ int64_t spans[kTeams];
+    __shared__ int64_t spans[kTeams];  // the long ones
+    __shared__ int teams[kTeams], found;
     const Embed& q = s.q;
     const int team = threadIdx.x / G, at = (blockIdx.y * G + threadIdx.x % G) * V;
     const int c = min(at, q.width - V);
     const int64_t live = *s.live, step = (int64_t)gridDim.x * kTeams;
     auto write = [&](int64_t tile, float* acc) {
-        const uint32_t key = s.pairs[tile * s.tile + s.tile - 1].x;
+        const uint32_t key = s.pairs[tile * s.tile].x;
 #pragma unroll
         for (int e = 0; e < V; ++e) acc[e] *= q.scale;
         if (at < q.width) P::store((T*)q.g_table + (int64_t)key * q.width + c, P::down(acc));
@@ -369,18 +541,26 @@ __global__ __launch_bounds__(kJoinThreads) void k_join(const Sum s) {
         const int64_t tile = base + team, span = span_of(s, tile, live);
         if (span > 0 && span <= kSpan) {
             float acc[V];
-            load_floats<V>(s.parts + (tile * 2 + 1) * q.width + c, acc);
-            add_parts<V>(s, tile + 1, tile + 1 + span, 1, c, acc);
+            load_floats<V>(s.parts + ((tile - span) * 2 + 1) * q.width + c, acc);
+            add_parts<V>(s, tile - span + 1, tile + 1, 1, c, acc);
             write(tile, acc);
         }
-        if (threadIdx.x % G == 0) spans[team] = span;
         if (!__syncthreads_or(span > kSpan)) continue;
-        for (int t = 0; t < kTeams; ++t) {
-            const int64_t far = spans[t], own = base + t;
-            if (far <= kSpan) continue;
+        if (threadIdx.x == 0) found = 0;
+        __syncthreads();
+        if (threadIdx.x % G == 0 && span > kSpan) {
+            // in any order: each is a sum of its own
+            const int k = atomicAdd(&found, 1);
+            spans[k] = span;
+            teams[k] = team;
+        }
+        __syncthreads();
+        const int n_long = found;
+        for (int k = 0; k < n_long; ++k) {
+            const int64_t far = spans[k], own = base + teams[k];
             float acc[V] = {};
-            if (team == 0) load_floats<V>(s.parts + (own * 2 + 1) * q.width + c, acc);
-            add_parts<V>(s, own + 1 + team, own + 1 + far, kTeams, c, acc);
+            if (team == 0) load_floats<V>(s.parts + ((own - far) * 2 + 1) * q.width + c, acc);
+            add_parts<V>(s, own - far + 1 + team, own + 1, kTeams, c, acc);
 #pragma unroll
             for (int e = 0; e < V; ++e) room[threadIdx.x][e] = acc[e];
             for (int n = kTeams / 2; n > 0; n /= 2) {
@@ -429,24 +609,34 @@ int check_args(int dtype, int64_t count, int64_t rows, int32_t width, const void
 }
 
 struct Layout {
-    int chunks, passes, bits, tile;
-    int64_t tiles, counts, totals, live, pairs[2], parts, total;
+    int chunks, passes, bits, digit, tile;
+    bool few;
+    int64_t tiles, counts, totals, live, pairs[2], begins, parts, total;
 };
 
-Layout layout(int64_t count, int64_t rows, int32_t width) {
+Layout layout(int dtype, int64_t count, int64_t rows, int32_t width) {
     Layout l{};
     l.chunks = (int)((count + kChunk - 1) / kChunk);
     l.bits = 1;
     while (((int64_t)1 << l.bits) < rows) ++l.bits;
-    l.passes = (l.bits + kBits - 1) / kBits;
+    l.few = count <= kFewThreads * kFewItems;
+    l.digit = l.bits <= 8 || (l.bits > 12 && l.bits <= 16) ? 8 : 12;
+    l.passes = l.few ? 1 : (l.bits + l.digit - 1) / l.digit;
+    // lanes of a team, and teams beside each other, as for_width has them: about 2^16
+    // lanes fill the chip, in tiles of at least a batch
+    const int vec = dtype == GSX_F32 ? F32::VEC : BF16::VEC;
+    const int64_t pieces = width < vec ? width : (width + vec - 1) / vec;
     l.tile = kMostTile;
+    while (l.tile > kBatch && count * pieces < ((int64_t)1 << 16) * l.tile) l.tile /= 2;
     l.tiles = (count + l.tile - 1) / l.tile;
-    l.counts = 0;
-    l.totals = up_to((int64_t)l.chunks * kRadix * 4, 256);
-    l.live = l.totals + kRadix * 4;
-    l.pairs[0] = l.live + 256;
+    const int64_t radix = l.few ? 0 : 1 << l.digit;
+    l.live = 0;
+    l.totals = 256;
+    l.counts = l.totals + radix * 4;
+    l.pairs[0] = up_to(l.counts + l.chunks * radix * 4, 256);
     l.pairs[1] = up_to(l.pairs[0] + count * 8, 256);
-    l.parts = up_to(l.pairs[1] + (l.passes > 1 ? count * 8 : 0), 256);
+    l.begins = up_to(l.pairs[1] + (l.passes > 1 ? count * 8 : 0), 256);
+    l.parts = up_to(l.begins + (l.tiles > 1 ? rows * 4 : 0), 256);
     l.total = up_to(l.parts + l.tiles * 2 * width * 4, 256);
     return l;
 }
@@ -478,43 +668,69 @@ template <class E>
 int lookup(const Embed& q, hipStream_t st) {
     return for_width<E>(q.width, [&](auto v, auto g, int times) -> int {
         constexpr int V = decltype(v)::value, G = decltype(g)::value;
-        hipLaunchKernelGGL((k_lookup<E, V, G>), grid_for(q.count, kThreads / G, times),
+        hipLaunchKernelGGL((k_lookup<E, V, G>), grid_for(q.count, kThreads / G * kLook, times),
                            dim3(kThreads), 0, st, q);
         GSX_LAUNCH_CHECK();
         return GSX_OK;
     });
 }
 
+template <int BITS>
+int passes(Sort s, const Layout& l, char* ws, unsigned fill, hipStream_t st) {
+    for (int p = 0; p < l.passes; ++p) {
+        s.from = p ? (const uint2*)(ws + l.pairs[(p - 1) % 2]) : nullptr;
+        s.to = (uint2*)(ws + l.pairs[p % 2]);
+        s.shift = p * BITS;
+        s.bits = l.bits - s.shift < BITS ? l.bits - s.shift : BITS;
+        hipLaunchKernelGGL((k_count<BITS>), dim3((unsigned)l.chunks + (p ? 0 : fill)),
+                           dim3(kSortThreads), 0, st, s);
+        GSX_LAUNCH_CHECK();
+        hipLaunchKernelGGL((k_prefix<BITS>), dim3((1 << BITS) / 64), dim3(64 * kScanGroups), 0, st,
+                           s);
+        GSX_LAUNCH_CHECK();
+        hipLaunchKernelGGL((k_place<BITS>), dim3((unsigned)l.chunks), dim3(kSortThreads), 0, st, s);
+        GSX_LAUNCH_CHECK();
+    }
+    return GSX_OK;
+}
+
 template <class E>
-int gradient(const Embed& q, char* ws, hipStream_t st) {
-    const Layout l = layout(q.count, q.rows, q.width);
-    const int64_t table = q.rows * q.width;
-    const int64_t fill = (table + kThreads - 1) / kThreads;
-    hipLaunchKernelGGL((k_zero<typename E::T>), dim3((unsigned)(fill < 8192 ? fill : 8192)),
-                       dim3(kThreads), 0, st, (typename E::T*)q.g_table, table);
-    GSX_LAUNCH_CHECK();
-    if (q.count == 0) return GSX_OK;
+int gradient(int dtype, const Embed& q, char* ws, hipStream_t st) {
+    const Layout l = layout(dtype, q.count, q.rows, q.width);
     Sort s{};
     s.q = q;
     s.counts = (uint32_t*)(ws + l.counts);
     s.totals = (uint32_t*)(ws + l.totals);
     s.live = (uint32_t*)(ws + l.live);
     s.chunks = l.chunks;
-    for (int p = 0; p < l.passes; ++p) {
-        s.from = p ? (const uint2*)(ws + l.pairs[(p - 1) % 2]) : nullptr;
-        s.to = (uint2*)(ws + l.pairs[p % 2]);
-        s.shift = p * kBits;
-        s.bits = l.bits - s.shift < kBits ? l.bits - s.shift : kBits;
-        hipLaunchKernelGGL(k_count, dim3((unsigned)l.chunks), dim3(kSortThreads), 0, st, s);
+    s.zeros = q.rows * q.width * (int64_t)sizeof(typename E::T);
+    const int64_t fill = (s.zeros + (1 << 15) - 1) >> 15;
+    const unsigned fillers = (unsigned)(fill < 2048 ? fill : 2048);
+    if (q.count == 0) {
+        s.chunks = 0;
+        hipLaunchKernelGGL((k_count<8>), dim3(fillers), dim3(kSortThreads), 0, st, s);
         GSX_LAUNCH_CHECK();
-        hipLaunchKernelGGL(k_prefix, dim3(kRadix / 64), dim3(64 * kScanGroups), 0, st, s);
+        return GSX_OK;
+    }
+    if (l.few) {
+        s.to = (uint2*)(ws + l.pairs[0]);
+        s.bits = l.bits;
+        const dim3 grid(1 + fillers);
+        if (q.count <= kFewThreads)
+            hipLaunchKernelGGL((k_sort_few<1>), grid, dim3(kFewThreads), 0, st, s);
+        else if (q.count <= kFewThreads * 4)
+            hipLaunchKernelGGL((k_sort_few<4>), grid, dim3(kFewThreads), 0, st, s);
+        else
+            hipLaunchKernelGGL((k_sort_few<kFewItems>), grid, dim3(kFewThreads), 0, st, s);
         GSX_LAUNCH_CHECK();
-        hipLaunchKernelGGL(k_place, dim3((unsigned)l.chunks), dim3(kSortThreads), 0, st, s);
-        GSX_LAUNCH_CHECK();
+    } else if (int e = l.digit == 8 ? passes<8>(s, l, ws, fillers, st)
+                                    : passes<12>(s, l, ws, fillers, st)) {
+        return e;
     }
     Sum u{};
     u.q = q;
-    u.pairs = s.to;
+    u.pairs = (const uint2*)(ws + l.pairs[(l.passes - 1) % 2]);
+    u.begins = (uint32_t*)(ws + l.begins);
     u.live = s.live;
     u.tile = l.tile;
     u.parts = (float*)(ws + l.parts);
@@ -523,6 +739,7 @@ int gradient(const Embed& q, char* ws, hipStream_t st) {
         const dim3 grid = grid_for(l.tiles, kThreads / G, times);
         hipLaunchKernelGGL((k_tile_sums<E, V, G>), grid, dim3(kThreads), 0, st, u);
         GSX_LAUNCH_CHECK();
+        if (l.tiles == 1) return GSX_OK;
         hipLaunchKernelGGL((k_join<E, V, G>), grid_for(l.tiles, kJoinThreads / G, times),
                            dim3(kJoinThreads), 0, st, u);
         GSX_LAUNCH_CHECK();
@@ -560,7 +777,7 @@ int gsx_embed_fwd(int32_t dtype, int64_t count, int64_t rows, int32_t width, con
 
 int64_t gsx_embed_bwd_workspace_bytes(int32_t dtype, int64_t count, int64_t rows, int32_t width) {
     if (int e = check_shape(dtype, count, rows, width)) return e;
-    return layout(count, rows, width).total;
+    return layout(dtype, count, rows, width).total;
 }
 
 int gsx_embed_bwd(int32_t dtype, int64_t count, int64_t rows, int32_t width, const void* indices,
@@ -570,7 +787,7 @@ int gsx_embed_bwd(int32_t dtype, int64_t count, int64_t rows, int32_t width, con
         return e;
     if (!g_table || (uintptr_t)g_table % (dtype == GSX_F32 ? 4 : 2)) return GSX_ERR_INVALID;
     if ((uintptr_t)workspace % 16) return GSX_ERR_INVALID;
-    if (!workspace || workspace_bytes < layout(count, rows, width).total) return GSX_ERR_WORKSPACE;
+    if (!workspace || workspace_bytes < layout(dtype, count, rows, width).total) return GSX_ERR_WORKSPACE;
     Embed q{};
     q.g_y = g_y;
     q.indices = indices;
@@ -582,9 +799,9 @@ int gsx_embed_bwd(int32_t dtype, int64_t count, int64_t rows, int32_t width, con
     q.index64 = index64;
     q.scale = scale;
     hipStream_t st = (hipStream_t)stream;
-    if (dtype == GSX_F32) return gradient<F32>(q, (char*)workspace, st);
-    if (dtype == GSX_BF16) return gradient<BF16>(q, (char*)workspace, st);
-    return gradient<F16>(q, (char*)workspace, st);
+    if (dtype == GSX_F32) return gradient<F32>(dtype, q, (char*)workspace, st);
+    if (dtype == GSX_BF16) return gradient<BF16>(dtype, q, (char*)workspace, st);
+    return gradient<F16>(dtype, q, (char*)workspace, st);
 }
 
 }  // extern "C"

@@ -7,13 +7,14 @@ device, the call raises instead of silently computing something else.
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import functools
 import os
 import threading
 
 import torch
+
+from . import profiling
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libgsx.so")
@@ -272,14 +273,37 @@ def stream_handle(device: torch.device):
     return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(index))
 
 
-_HERE_ALREADY = contextlib.nullcontext()
+def launch(name: str, label: str, device: torch.device, *args) -> None:
+    """Calls an entry point that enqueues work, with torch's current stream on `device`
+    as its last argument and that device the current one; `label` is its stage.  (The
+    usual case, no timer and one device, takes no context: each costs a microsecond,
+    three on autograd's thread.)"""
+    index = device.index
+    entry = getattr(load(), name)
+    if profiling._active is None and index == torch._C._cuda_getDevice():
+        status = entry(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(device), profiling.stage(label):
+            status = entry(*args, stream_handle(device))
+    if status < 0:
+        check(status, name)
 
 
-def on_device(device: torch.device):
-    """A context in which `device` is the current one, as a launch on its stream needs."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return _HERE_ALREADY
-    return torch.cuda.device(device)
+@functools.lru_cache(maxsize=4096)
+def workspace_bytes(name: str, *shape: int) -> int:
+    """What a ``*_workspace_bytes`` entry point says of a shape."""
+    return check(int(getattr(load(), name)(*shape)), name)
+
+
+def scratch(n: int, device: torch.device) -> torch.Tensor:
+    return torch.empty(n, dtype=torch.uint8, device=device)
+
+
+def contiguous_like(t: torch.Tensor) -> torch.Tensor:
+    """An uninitialised tensor of t's shape and type in row-major order."""
+    if t.is_contiguous():
+        return torch.empty_like(t)  # half the time of the call below
+    return torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 
 def require_device(*tensors: torch.Tensor | None) -> torch.device:

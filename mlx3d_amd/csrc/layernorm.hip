@@ -510,8 +510,10 @@ int gsx_layer_norm_bwd(int32_t dtype, int64_t rows, int32_t width, const void* x
     if ((uintptr_t)g_y % size || (uintptr_t)g_x % size || (uintptr_t)g_weight % size ||
         (uintptr_t)g_bias % size || (uintptr_t)workspace % 16)
         return GSX_ERR_INVALID;
-    if (!g_weight && !g_bias && (!g_x || rows == 0)) return GSX_OK;
-    if (!workspace || workspace_bytes < gsx_layer_norm_bwd_workspace_bytes(dtype, rows, width))
+    const bool params = g_weight || g_bias;
+    if (!params && (!g_x || rows == 0)) return GSX_OK;
+    if (params &&
+        (!workspace || workspace_bytes < gsx_layer_norm_bwd_workspace_bytes(dtype, rows, width)))
         return GSX_ERR_WORKSPACE;
     const int64_t most = rows < kMostGroups ? rows : kMostGroups;
     Norm q{};
@@ -525,7 +527,7 @@ int gsx_layer_norm_bwd(int32_t dtype, int64_t rows, int32_t width, const void* x
     q.inv_width = 1.0f / (float)width;
     q.eps = eps;
     q.g_x = g_x;
-    q.parts = g_weight || g_bias ? (float*)workspace : nullptr;
+    q.parts = params ? (float*)workspace : nullptr;
     q.stats = (float*)((char*)workspace + up_to(most * 2 * width * 4, 256));
     hipStream_t st = (hipStream_t)stream;
     if (dtype == GSX_F32) return backward<F32>(q, g_weight, g_bias, st);

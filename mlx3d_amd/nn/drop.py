@@ -9,40 +9,34 @@ from __future__ import annotations
 import torch
 
 from .. import _lib
-from ..profiling import stage
 
 __all__ = ["Dropout", "dropout"]
 
 
-def _drop(x, residual, p, seed, offset):
+def _drop(x, residual, p, seed, offset, at):
+    """The values, with the counter `offset`, or what `at` on the device holds."""
     held = x.contiguous()
     base = None if residual is None else residual.contiguous()
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    at = offset if isinstance(offset, torch.Tensor) else None
-    with _lib.on_device(x.device), stage("dropout"):
-        _lib.check(_lib.load().gsx_dropout(
-            _lib.DTYPES[x.dtype], x.numel(), p, seed, 0 if at is not None else offset,
-            _lib.ptr(at), _lib.ptr(held), _lib.ptr(base), _lib.ptr(y),
-            _lib.stream_handle(x.device)), "gsx_dropout")
+    y = torch.empty_like(held)
+    _lib.launch("gsx_dropout", "dropout", x.device, _lib.DTYPES[x.dtype], held.numel(), p, seed,
+                offset, _lib.ptr(at), held.data_ptr(), _lib.ptr(base), y.data_ptr())
     return y
 
 
 class _Dropout(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, residual, p, seed, offset):
-        y = _drop(x, residual, p, seed, offset)
+    def forward(ctx, x, residual, p, seed, offset, at):
+        ctx.how = (p, seed, offset)
         # saved, so that a counter that moves on before the gradient is noticed
-        ctx.save_for_backward(*([offset] if isinstance(offset, torch.Tensor) else []))
-        ctx.how = (p, seed, offset if isinstance(offset, int) else None)
-        return y
+        ctx.save_for_backward(at)
+        return _drop(x, residual, p, seed, offset, at)
 
     @staticmethod
     @_lib.once_differentiable("dropout")
     def backward(ctx, saved, g_y):
-        p, seed, offset = ctx.how
-        need = ctx.needs_input_grad
-        g_x = _drop(g_y, None, p, seed, saved[0] if saved else offset) if need[0] else None
-        return g_x, g_y if need[1] else None, None, None, None
+        need_x, need_residual = ctx.needs_input_grad[:2]
+        g_x = _drop(g_y, None, *ctx.how, saved[0]) if need_x else None
+        return g_x, g_y if need_residual else None, None, None, None, None
 
 
 def dropout(x: torch.Tensor, p: float, seed: int, offset: int | torch.Tensor = 0,
@@ -72,12 +66,13 @@ def dropout(x: torch.Tensor, p: float, seed: int, offset: int | torch.Tensor = 0
     if isinstance(offset, torch.Tensor):
         if offset.dtype != torch.int64 or offset.numel() != 1:
             raise ValueError("an offset on the device must be one int64.")
-        _lib.require_device(x, residual, offset)
+        offset, at = 0, offset
     else:
         if not isinstance(offset, int) or not 0 <= offset < 1 << 63:
             raise ValueError("offset must be a whole number from 0 to 2^63 - 1.")
-        _lib.require_device(x, residual)
-    return _Dropout.apply(x, residual, p, seed, offset)
+        at = None
+    _lib.require_device(x, residual, at)
+    return _Dropout.apply(x, residual, p, seed, offset, at)
 
 
 class Dropout:

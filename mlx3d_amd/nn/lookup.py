@@ -10,7 +10,6 @@ from __future__ import annotations
 import torch
 
 from .. import _lib
-from ..profiling import stage
 
 __all__ = ["Embedding", "embedding"]
 
@@ -20,33 +19,26 @@ class _Embedding(torch.autograd.Function):
     def forward(ctx, indices, table, scale):
         held = indices.contiguous()
         rows, stride = _lib.rows_of(table)
-        width = table.shape[1]
-        y = torch.empty((*indices.shape, width), dtype=table.dtype, device=table.device)
-        head = (_lib.DTYPES[table.dtype], indices.numel(), table.shape[0], width)
-        with _lib.on_device(table.device), stage("embed_fwd"):
-            _lib.check(_lib.load().gsx_embed_fwd(
-                *head, _lib.ptr(held), int(indices.dtype == torch.int64), _lib.ptr(rows), stride,
-                scale, _lib.ptr(y), _lib.stream_handle(table.device)), "gsx_embed_fwd")
+        count, device = held.numel(), table.device
+        y = torch.empty((*held.shape, table.shape[1]), dtype=table.dtype, device=device)
+        ctx.head = head = (_lib.DTYPES[table.dtype], count, *table.shape)
+        ctx.how = how = (int(indices.dtype == torch.int64), scale)
+        _lib.launch("gsx_embed_fwd", "embed_fwd", device, *head, held.data_ptr(), how[0],
+                    rows.data_ptr(), stride, scale, y.data_ptr())
         ctx.save_for_backward(indices)
-        ctx.head, ctx.scale = head, scale
         return y
 
     @staticmethod
     @_lib.once_differentiable("embedding")
     def backward(ctx, saved, g_y):
-        (indices,) = saved
-        L = _lib.load()
-        held = indices.contiguous()
+        held = saved[0].contiguous()
+        head, (index64, scale), device = ctx.head, ctx.how, g_y.device
         rows, stride = _lib.rows_of(g_y)
-        g_table = torch.empty(ctx.head[2:], dtype=g_y.dtype, device=g_y.device)
-        n = _lib.check(int(L.gsx_embed_bwd_workspace_bytes(*ctx.head)),
-                       "gsx_embed_bwd_workspace_bytes")
-        ws = torch.empty((n,), dtype=torch.uint8, device=g_y.device)
-        with _lib.on_device(g_y.device), stage("embed_bwd"):
-            _lib.check(L.gsx_embed_bwd(
-                *ctx.head, _lib.ptr(held), int(indices.dtype == torch.int64), _lib.ptr(rows),
-                stride, ctx.scale, _lib.ptr(g_table), _lib.ptr(ws), n,
-                _lib.stream_handle(g_y.device)), "gsx_embed_bwd")
+        g_table = torch.empty(head[2:], dtype=g_y.dtype, device=device)
+        n = _lib.workspace_bytes("gsx_embed_bwd_workspace_bytes", *head)
+        ws = _lib.scratch(n, device)
+        _lib.launch("gsx_embed_bwd", "embed_bwd", device, *head, held.data_ptr(), index64,
+                    rows.data_ptr(), stride, scale, g_table.data_ptr(), ws.data_ptr(), n)
         return None, g_table, None
 
 

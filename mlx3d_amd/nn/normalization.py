@@ -9,7 +9,6 @@ from __future__ import annotations
 import torch
 
 from .. import _lib
-from ..profiling import stage
 
 __all__ = ["LayerNorm", "layer_norm"]
 
@@ -18,37 +17,33 @@ class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
         rows, stride = _lib.rows_of(x)
-        w, b = (None if t is None else t.contiguous() for t in (weight, bias))
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        head = (_lib.DTYPES[x.dtype], rows.shape[0], x.shape[-1])
-        with _lib.on_device(x.device), stage("layer_norm_fwd"):
-            _lib.check(_lib.load().gsx_layer_norm_fwd(
-                *head, _lib.ptr(rows), stride, _lib.ptr(w), _lib.ptr(b), eps, _lib.ptr(y),
-                _lib.stream_handle(x.device)), "gsx_layer_norm_fwd")
+        w = None if weight is None else weight.contiguous()
+        b = None if bias is None else bias.contiguous()
+        y = _lib.contiguous_like(x)
+        ctx.head = head = (_lib.DTYPES[x.dtype], rows.shape[0], rows.shape[1])
+        _lib.launch("gsx_layer_norm_fwd", "layer_norm_fwd", x.device, *head, rows.data_ptr(), stride,
+                    _lib.ptr(w), _lib.ptr(b), eps, y.data_ptr())
         ctx.save_for_backward(x, weight)
-        ctx.head, ctx.eps = head, eps
+        ctx.eps = eps
         return y
 
     @staticmethod
     @_lib.once_differentiable("layer_norm")
     def backward(ctx, saved, g_y):
         x, weight = saved
-        L = _lib.load()
+        head, device = ctx.head, x.device
         rows, stride = _lib.rows_of(x)
         g_rows, g_stride = _lib.rows_of(g_y)
         w = None if weight is None else weight.contiguous()
-        need = ctx.needs_input_grad
-        g_x = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need[0] else None
-        g_w, g_b = (torch.empty(x.shape[-1:], dtype=x.dtype, device=x.device) if k else None
-                    for k in need[1:3])
-        n = _lib.check(int(L.gsx_layer_norm_bwd_workspace_bytes(*ctx.head)),
-                       "gsx_layer_norm_bwd_workspace_bytes")
-        ws = torch.empty((n,), dtype=torch.uint8, device=x.device)
-        with _lib.on_device(x.device), stage("layer_norm_bwd"):
-            _lib.check(L.gsx_layer_norm_bwd(
-                *ctx.head, _lib.ptr(rows), stride, _lib.ptr(w), _lib.ptr(g_rows), g_stride,
-                ctx.eps, _lib.ptr(g_x), _lib.ptr(g_w), _lib.ptr(g_b), _lib.ptr(ws), n,
-                _lib.stream_handle(x.device)), "gsx_layer_norm_bwd")
+        need_x, need_w, need_b, _ = ctx.needs_input_grad
+        g_x = _lib.contiguous_like(x) if need_x else None
+        g_w = torch.empty(head[2], dtype=x.dtype, device=device) if need_w else None
+        g_b = torch.empty(head[2], dtype=x.dtype, device=device) if need_b else None
+        n = _lib.workspace_bytes("gsx_layer_norm_bwd_workspace_bytes", *head)
+        ws = _lib.scratch(n, device) if need_w or need_b else None
+        _lib.launch("gsx_layer_norm_bwd", "layer_norm_bwd", device, *head, rows.data_ptr(), stride,
+                    _lib.ptr(w), g_rows.data_ptr(), g_stride, ctx.eps, _lib.ptr(g_x), _lib.ptr(g_w),
+                    _lib.ptr(g_b), _lib.ptr(ws), n)
         return g_x, g_w, g_b, None
 
 

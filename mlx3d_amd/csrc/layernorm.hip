@@ -32,9 +32,10 @@ using namespace gsx;
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kWaves = kThreads / 64;
 constexpr int kMostGroups = 1024;  // workgroups of a gradient, whose partial rows are joined
-constexpr int kPieces = 4;         // of a row on a lane at most
+constexpr int kWideGroups = 512;   // where a row takes a workgroup: two a compute unit
+constexpr int kFwdGroups = 8192;    // workgroups of a forward pass at most
+constexpr int kMostWidth = 8192;    // of a row that a workgroup holds
 
 struct Norm {
     const void *x, *weight, *bias, *g_y;
@@ -46,15 +47,19 @@ struct Norm {
     float* stats;  // longer rows: (rows, 3)
 };
 
+// The threads of a workgroup whose teams have G lanes.
+template <int G>
+constexpr int threads_of = G > kThreads ? G : kThreads;
+
 // Sums of K values over a team of G lanes; every lane gets them.  A workgroup's team
 // goes through shared memory, `turn` telling two rooms apart so that one barrier a sum
 // is enough.
 template <int G, int K>
 __device__ __forceinline__ void team_sum(float* v, int turn) {
-    constexpr int L = G < 64 ? G : 64;
+    constexpr int L = G < 64 ? G : 64, kWaves = G / L;
 #pragma unroll
     for (int k = 0; k < K; ++k) v[k] = group_sum<L>(v[k]);
-    if constexpr (G > 64) {
+    if constexpr (kWaves > 1) {
         __shared__ float room[2][K][kWaves];
         const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
@@ -70,142 +75,177 @@ __device__ __forceinline__ void team_sum(float* v, int turn) {
     }
 }
 
-// The places of a lane's N pieces in a row: where each begins, and how many of its
-// elements belong to the piece before (all of them: the lane has no such piece).
-template <int V, int G, int N>
+// (var + eps)^(-1/2): the hardware's root (a unit in the last place) and a Newton step;
+// 0 where the variance overflows.
+__device__ __forceinline__ float inverse_root(float v) {
+    const float r = __builtin_amdgcn_rsqf(v);
+    const float e = fmaf(-v * r, r, 1.f);
+    return r == 0.f ? 0.f : fmaf(0.5f * r, e, r);
+}
+
+// The places of a lane's N pieces in a row.  The team's lanes hold the pieces in turn,
+// so all of them but the last of each lane lie inside the row (the choice of G and N
+// sees to that) and are a piece's length apart; the last ends with the row.  Its first
+// `skip` elements belong to the piece before, or all of them to another lane (skip = V):
+// `in` is 0 there and 1 elsewhere, and sums take them times that.  Outputs are formed
+// for them, too: what two lanes write to one place is the same.
+template <class E, int V, int G, int N>
 struct Places {
-    int at[N], skip[N];
+    using P = Piece<E, V>;
+    using T = typename E::T;
+    int first, last, skip;
+    float in[V];
     __device__ __forceinline__ Places(int width) {
         const int lane = threadIdx.x % G;
+        first = lane * V;
+        const int p = ((N - 1) * G + lane) * V;
+        last = min(p, width - V);
+        skip = min(p - last, V);
+#pragma unroll
+        for (int e = 0; e < V; ++e) in[e] = e >= skip ? 1.f : 0.f;
+    }
+    __device__ __forceinline__ int at(int k) const {
+        return k < N - 1 ? first + k * G * V : last;
+    }
+    // element i of the lane's N V, as sums take it
+    __device__ __forceinline__ float inside(int i, float v) const {
+        return V == 1 || i < (N - 1) * V ? v : v * in[i - (N - 1) * V];
+    }
+    __device__ __forceinline__ void load(const void* rows, int64_t row, typename P::Raw* r) const {
+#pragma unroll
+        for (int k = 0; k < N; ++k) r[k] = P::load((const T*)rows + row + at(k));
+    }
+    __device__ __forceinline__ void up(const typename P::Raw* r, float* v) const {
+#pragma unroll
+        for (int k = 0; k < N; ++k) P::up(r[k], v + k * V);
+    }
+    // weights of the pieces, or `other` where there are none
+    __device__ __forceinline__ void weights(const void* w, float other, float* v) const {
 #pragma unroll
         for (int k = 0; k < N; ++k) {
-            const int p = (k * G + lane) * V;
-            at[k] = min(p, width - V);
-            skip[k] = min(p - at[k], V);
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[k * V + e] = other;
+            if (w) P::up(P::load((const T*)w + at(k)), v + k * V);
         }
+    }
+    // whether element e of piece k is this lane's
+    __device__ __forceinline__ bool own(int k, int e) const { return k < N - 1 || e >= skip; }
+    __device__ __forceinline__ void store(void* rows, int64_t row, int k, const float* v) const {
+        if (k < N - 1 || skip < V) P::store((T*)rows + row + at(k), P::down(v));
     }
 };
 
-// Differences to the rounded mean, zero outside the row.
-template <int V, int G, int N>
-__device__ __forceinline__ void center(const Norm& q, const Places<V, G, N>& at, float* v,
-                                       int turn) {
+// Differences to the rounded mean.
+template <class At, int V, int G, int N>
+__device__ __forceinline__ void center(const Norm& q, const At& at, float* v, int turn) {
     float s = 0.f;
 #pragma unroll
-    for (int k = 0; k < N; ++k)
-#pragma unroll
-        for (int e = 0; e < V; ++e) s += e >= at.skip[k] ? v[k * V + e] : 0.f;
+    for (int i = 0; i < N * V; ++i)
+        s = V == 1 || i < (N - 1) * V ? s + v[i] : fmaf(v[i], at.in[i - (N - 1) * V], s);
     team_sum<G, 1>(&s, turn);
     const float m = s * q.inv_width;
 #pragma unroll
-    for (int k = 0; k < N; ++k)
-#pragma unroll
-        for (int e = 0; e < V; ++e) v[k * V + e] -= m;
+    for (int i = 0; i < N * V; ++i) v[i] -= m;
 }
 
+// The next row is asked for before this one's sums.
 template <class E, int V, int G, int N>
-__global__ __launch_bounds__(kThreads) void k_norm_fwd(const Norm q) {
-    using P = Piece<E, V>;
-    using T = typename E::T;
-    constexpr int kTeams = kThreads / G;
-    const Places<V, G, N> at(q.width);
+__global__ __launch_bounds__(threads_of<G>) void k_norm_fwd(const Norm q) {
+    using At = Places<E, V, G, N>;
+    constexpr int kTeams = threads_of<G> / G;
+    const At at(q.width);
     float w[N * V], b[N * V];
-#pragma unroll
-    for (int i = 0; i < N * V; ++i) w[i] = 1.f, b[i] = 0.f;
-#pragma unroll
-    for (int k = 0; k < N; ++k) {
-        if (q.weight) P::up(P::load((const T*)q.weight + at.at[k]), w + k * V);
-        if (q.bias) P::up(P::load((const T*)q.bias + at.at[k]), b + k * V);
-    }
+    at.weights(q.weight, 1.f, w);
+    at.weights(q.bias, 0.f, b);
     const int64_t step = (int64_t)gridDim.x * kTeams;
+    int64_t own = (int64_t)blockIdx.x * kTeams + threadIdx.x / G;
+    typename At::P::Raw raw[N];
+    at.load(q.x, min(own, q.rows - 1) * q.x_stride, raw);
     int turn = 0;
     // whole waves stay together, as their lanes' sums need
-    for (int64_t base = (int64_t)blockIdx.x * kTeams; base < q.rows; base += step, turn ^= 1) {
-        const int64_t own = base + threadIdx.x / G, row = min(own, q.rows - 1);
+    for (int64_t base = (int64_t)blockIdx.x * kTeams; base < q.rows;
+         base += step, own += step, turn ^= 1) {
         float v[N * V];
-#pragma unroll
-        for (int k = 0; k < N; ++k)
-            P::up(P::load((const T*)q.x + row * q.x_stride + at.at[k]), v + k * V);
-        center<V, G, N>(q, at, v, turn);
+        at.up(raw, v);
+        at.load(q.x, min(own + step, q.rows - 1) * q.x_stride, raw);
+        center<At, V, G, N>(q, at, v, turn);
         float s[2] = {0.f, 0.f};
 #pragma unroll
-        for (int k = 0; k < N; ++k)
-#pragma unroll
-            for (int e = 0; e < V; ++e) {
-                const float d = e >= at.skip[k] ? v[k * V + e] : 0.f;
-                s[0] += d;
-                s[1] = fmaf(d, d, s[1]);
-            }
+        for (int i = 0; i < N * V; ++i) {
+            const float d = at.inside(i, v[i]);
+            s[0] += d;
+            s[1] = fmaf(d, v[i], s[1]);
+        }
         team_sum<G, 2>(s, turn);
         const float off = s[0] * q.inv_width;
-        const float r = 1.0f / sqrtf(fmaxf(fmaf(-off, off, s[1] * q.inv_width), 0.f) + q.eps);
+        const float r = inverse_root(fmaxf(fmaf(-off, off, s[1] * q.inv_width), 0.f) + q.eps);
+        const float c = -off * r;
 #pragma unroll
-        for (int k = 0; k < N; ++k) {
+        for (int i = 0; i < N * V; ++i) v[i] = fmaf(fmaf(v[i], r, c), w[i], b[i]);
+        if (own < q.rows) {
 #pragma unroll
-            for (int e = 0; e < V; ++e)
-                v[k * V + e] = fmaf((v[k * V + e] - off) * r, w[k * V + e], b[k * V + e]);
-            if (own < q.rows && at.skip[k] < V)
-                P::store((T*)q.y + row * q.width + at.at[k], P::down(v + k * V));
+            for (int k = 0; k < N; ++k) at.store(q.y, own * q.width, k, v + k * V);
         }
     }
 }
 
+// dx = g r + d B + A with B = -r^2 mean(g h) and A what the means leave: two products an
+// element, and one more for h, which dw needs.
 template <class E, int V, int G, int N>
-__global__ __launch_bounds__(kThreads) void k_norm_bwd(const Norm q) {
-    using P = Piece<E, V>;
-    using T = typename E::T;
-    constexpr int kTeams = kThreads / G;
-    const Places<V, G, N> at(q.width);
+__global__ __launch_bounds__(threads_of<G>) void k_norm_bwd(const Norm q) {
+    using At = Places<E, V, G, N>;
+    using Raw = typename At::P::Raw;
+    constexpr int kTeams = threads_of<G> / G;
+    const At at(q.width);
     float w[N * V], dw[N * V], db[N * V];
+    at.weights(q.weight, 1.f, w);
 #pragma unroll
-    for (int i = 0; i < N * V; ++i) w[i] = 1.f, dw[i] = db[i] = 0.f;
-#pragma unroll
-    for (int k = 0; k < N; ++k)
-        if (q.weight) P::up(P::load((const T*)q.weight + at.at[k]), w + k * V);
+    for (int i = 0; i < N * V; ++i) dw[i] = db[i] = 0.f;
     const int64_t step = (int64_t)gridDim.x * kTeams;
+    int64_t own = (int64_t)blockIdx.x * kTeams + threadIdx.x / G;
+    Raw raw_x[N], raw_g[N];
+    at.load(q.x, min(own, q.rows - 1) * q.x_stride, raw_x);
+    at.load(q.g_y, min(own, q.rows - 1) * q.g_stride, raw_g);
     int turn = 0;
-    for (int64_t base = (int64_t)blockIdx.x * kTeams; base < q.rows; base += step, turn ^= 1) {
-        const int64_t own = base + threadIdx.x / G, row = min(own, q.rows - 1);
+    for (int64_t base = (int64_t)blockIdx.x * kTeams; base < q.rows;
+         base += step, own += step, turn ^= 1) {
+        const bool there = own < q.rows;
         float v[N * V], g[N * V];
+        at.up(raw_x, v);
 #pragma unroll
         for (int k = 0; k < N; ++k) {
-            P::up(P::load((const T*)q.x + row * q.x_stride + at.at[k]), v + k * V);
-            P::up(P::load((const T*)q.g_y + row * q.g_stride + at.at[k]), g + k * V);
+            if (!there) raw_g[k] = Raw{};  // a row past the end adds nothing
+            At::P::up(raw_g[k], g + k * V);
         }
-        center<V, G, N>(q, at, v, turn);
+        at.load(q.x, min(own + step, q.rows - 1) * q.x_stride, raw_x);
+        at.load(q.g_y, min(own + step, q.rows - 1) * q.g_stride, raw_g);
+        center<At, V, G, N>(q, at, v, turn);
         float s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int k = 0; k < N; ++k)
-#pragma unroll
-            for (int e = 0; e < V; ++e) {
-                const int i = k * V + e;
-                const bool in = e >= at.skip[k];
-                const float d = in ? v[i] : 0.f, gw = in ? g[i] * w[i] : 0.f;
-                s[0] += d;
-                s[1] = fmaf(d, d, s[1]);
-                s[2] += gw;
-                s[3] = fmaf(gw, d, s[3]);
-            }
+        for (int i = 0; i < N * V; ++i) {
+            const float d = at.inside(i, v[i]), gw = at.inside(i, g[i] * w[i]);
+            s[0] += d;
+            s[1] = fmaf(d, v[i], s[1]);
+            s[2] += gw;
+            s[3] = fmaf(gw, v[i], s[3]);
+        }
         team_sum<G, 4>(s, turn);
         const float off = s[0] * q.inv_width;
-        const float r = 1.0f / sqrtf(fmaxf(fmaf(-off, off, s[1] * q.inv_width), 0.f) + q.eps);
-        const float mean_g = s[2] * q.inv_width;
+        const float r = inverse_root(fmaxf(fmaf(-off, off, s[1] * q.inv_width), 0.f) + q.eps);
+        const float c = -off * r;
         const float mean_gh = fmaf(-off, s[2], s[3]) * r * q.inv_width;
+        const float B = -r * mean_gh * r, A = fmaf(-off, B, -r * (s[2] * q.inv_width));
 #pragma unroll
         for (int k = 0; k < N; ++k) {
             float dx[V];
 #pragma unroll
             for (int e = 0; e < V; ++e) {
                 const int i = k * V + e;
-                const float h = (v[i] - off) * r;
-                dx[e] = (g[i] * w[i] - mean_g - h * mean_gh) * r;
-                if (own < q.rows && e >= at.skip[k]) {
-                    dw[i] = fmaf(g[i], h, dw[i]);
-                    db[i] += g[i];
-                }
+                dx[e] = fmaf(g[i] * w[i], r, fmaf(v[i], B, A));
+                dw[i] = fmaf(g[i], fmaf(v[i], r, c), dw[i]);
+                db[i] += g[i];
             }
-            if (q.g_x && own < q.rows && at.skip[k] < V)
-                P::store((T*)q.g_x + row * q.width + at.at[k], P::down(dx));
+            if (q.g_x && there) at.store(q.g_x, own * q.width, k, dx);
         }
     }
     if (!q.parts) return;
@@ -215,9 +255,9 @@ __global__ __launch_bounds__(kThreads) void k_norm_bwd(const Norm q) {
         for (int k = 0; k < N; ++k)
 #pragma unroll
             for (int e = 0; e < V; ++e)
-                if (e >= at.skip[k]) {
-                    to[at.at[k] + e] = dw[k * V + e];
-                    to[q.width + at.at[k] + e] = db[k * V + e];
+                if (at.own(k, e)) {
+                    to[at.at(k) + e] = dw[k * V + e];
+                    to[q.width + at.at(k) + e] = db[k * V + e];
                 }
     } else {
         // a wave's teams, then the waves one after another
@@ -230,61 +270,103 @@ __global__ __launch_bounds__(kThreads) void k_norm_bwd(const Norm q) {
                 db[i] += __shfl_xor(db[i], o, 64);
             }
         const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-        for (int t = 0; t < kWaves; ++t) {
+        for (int t = 0; t < kThreads / 64; ++t) {
             if (wave == t && lane < G) {
 #pragma unroll
                 for (int k = 0; k < N; ++k)
 #pragma unroll
                     for (int e = 0; e < V; ++e)
-                        if (e >= at.skip[k]) {
-                            float* c = cols + at.at[k] + e;
-                            c[0] = t ? c[0] + dw[k * V + e] : dw[k * V + e];
-                            c[q.width] = t ? c[q.width] + db[k * V + e] : db[k * V + e];
+                        if (at.own(k, e)) {
+                            float* col = cols + at.at(k) + e;
+                            col[0] = t ? col[0] + dw[k * V + e] : dw[k * V + e];
+                            col[q.width] = t ? col[q.width] + db[k * V + e] : db[k * V + e];
                         }
             }
             __syncthreads();
         }
-        for (int c = threadIdx.x; c < 2 * q.width; c += kThreads) to[c] = cols[c];
+        for (int i = threadIdx.x; i < 2 * q.width; i += kThreads) to[i] = cols[i];
     }
 }
 
-// ---- longer rows: a workgroup each, element by element ----
+// ---- longer rows: a workgroup each, which reads them again for each sum ----
+
+// Calls f with the place of each piece of a row that this thread takes, and with its
+// elements' shares in sums (0 for those of the piece before).
+constexpr int kLongThreads = 512;
+template <int V, class F>
+__device__ __forceinline__ void long_pieces(const Norm& q, F f) {
+    for (int p = threadIdx.x * V; p < q.width; p += kLongThreads * V) {
+        const int at = min(p, q.width - V);
+        float in[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) in[e] = e >= p - at ? 1.f : 0.f;
+        f(at, in);
+    }
+}
 
 template <class E>
 __device__ __forceinline__ float3 long_stats(const Norm& q, const typename E::T* x) {
+    constexpr int V = E::VEC;
+    using P = Piece<E, V>;
     float s = 0.f;
-    for (int c = threadIdx.x; c < q.width; c += kThreads) s += E::up(x[c]);
-    team_sum<kThreads, 1>(&s, 0);
+    long_pieces<V>(q, [&](int at, const float* in) {
+        float v[V];
+        P::up(P::load(x + at), v);
+#pragma unroll
+        for (int e = 0; e < V; ++e) s = fmaf(v[e], in[e], s);
+    });
+    team_sum<kLongThreads, 1>(&s, 0);
     const float m = s * q.inv_width;
     float t[2] = {0.f, 0.f};
-    for (int c = threadIdx.x; c < q.width; c += kThreads) {
-        const float d = E::up(x[c]) - m;
-        t[0] += d;
-        t[1] = fmaf(d, d, t[1]);
-    }
-    team_sum<kThreads, 2>(t, 0);
+    long_pieces<V>(q, [&](int at, const float* in) {
+        float v[V];
+        P::up(P::load(x + at), v);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            const float d = (v[e] - m) * in[e];
+            t[0] += d;
+            t[1] = fmaf(d, d, t[1]);
+        }
+    });
+    team_sum<kLongThreads, 2>(t, 0);
     const float off = t[0] * q.inv_width;
     const float var = fmaxf(fmaf(-off, off, t[1] * q.inv_width), 0.f);
-    return make_float3(m, off, 1.0f / sqrtf(var + q.eps));
+    return make_float3(m, off, inverse_root(var + q.eps));
+}
+
+// V columns of weights, or 1 or 0 where there are none.
+template <class E, int V>
+__device__ __forceinline__ void long_weights(const void* w, int at, float other, float* v) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] = other;
+    if (w) Piece<E, V>::up(Piece<E, V>::load((const typename E::T*)w + at), v);
 }
 
 template <class E>
-__global__ __launch_bounds__(kThreads) void k_long_fwd(const Norm q) {
+__global__ __launch_bounds__(kLongThreads) void k_long_fwd(const Norm q) {
+    constexpr int V = E::VEC;
+    using P = Piece<E, V>;
     using T = typename E::T;
     for (int64_t row = blockIdx.x; row < q.rows; row += gridDim.x) {
         const T* x = (const T*)q.x + row * q.x_stride;
         T* y = (T*)q.y + row * q.width;
         const float3 st = long_stats<E>(q, x);
-        for (int c = threadIdx.x; c < q.width; c += kThreads) {
-            const float w = q.weight ? E::up(((const T*)q.weight)[c]) : 1.f;
-            const float b = q.bias ? E::up(((const T*)q.bias)[c]) : 0.f;
-            y[c] = E::down(fmaf((E::up(x[c]) - st.x - st.y) * st.z, w, b));
-        }
+        long_pieces<V>(q, [&](int at, const float*) {
+            float v[V], w[V], b[V];
+            P::up(P::load(x + at), v);
+            long_weights<E, V>(q.weight, at, 1.f, w);
+            long_weights<E, V>(q.bias, at, 0.f, b);
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[e] = fmaf((v[e] - st.x - st.y) * st.z, w[e], b[e]);
+            P::store(y + at, P::down(v));
+        });
     }
 }
 
 template <class E>
-__global__ __launch_bounds__(kThreads) void k_long_bwd(const Norm q) {
+__global__ __launch_bounds__(kLongThreads) void k_long_bwd(const Norm q) {
+    constexpr int V = E::VEC;
+    using P = Piece<E, V>;
     using T = typename E::T;
     for (int64_t row = blockIdx.x; row < q.rows; row += gridDim.x) {
         const T* x = (const T*)q.x + row * q.x_stride;
@@ -297,20 +379,38 @@ __global__ __launch_bounds__(kThreads) void k_long_bwd(const Norm q) {
             to[2] = st.z;
         }
         if (!q.g_x) continue;
+        auto values = [&](int at, float* h, float* g) {
+            float w[V];
+            P::up(P::load(x + at), h);
+            P::up(P::load(dy + at), g);
+            long_weights<E, V>(q.weight, at, 1.f, w);
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                h[e] = (h[e] - st.x - st.y) * st.z;
+                g[e] *= w[e];
+            }
+        };
         float s[2] = {0.f, 0.f};
-        for (int c = threadIdx.x; c < q.width; c += kThreads) {
-            const float g = E::up(dy[c]) * (q.weight ? E::up(((const T*)q.weight)[c]) : 1.f);
-            s[0] += g;
-            s[1] = fmaf(g, (E::up(x[c]) - st.x - st.y) * st.z, s[1]);
-        }
-        team_sum<kThreads, 2>(s, 1);
+        long_pieces<V>(q, [&](int at, const float* in) {
+            float h[V], g[V];
+            values(at, h, g);
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                const float t = g[e] * in[e];
+                s[0] += t;
+                s[1] = fmaf(t, h[e], s[1]);
+            }
+        });
+        team_sum<kLongThreads, 2>(s, 1);
         const float mean_g = s[0] * q.inv_width, mean_gh = s[1] * q.inv_width;
         T* dx = (T*)q.g_x + row * q.width;
-        for (int c = threadIdx.x; c < q.width; c += kThreads) {
-            const float g = E::up(dy[c]) * (q.weight ? E::up(((const T*)q.weight)[c]) : 1.f);
-            const float h = (E::up(x[c]) - st.x - st.y) * st.z;
-            dx[c] = E::down((g - mean_g - h * mean_gh) * st.z);
-        }
+        long_pieces<V>(q, [&](int at, const float*) {
+            float h[V], g[V];
+            values(at, h, g);
+#pragma unroll
+            for (int e = 0; e < V; ++e) g[e] = (g[e] - mean_g - h[e] * mean_gh) * st.z;
+            P::store(dx + at, P::down(g));
+        });
     }
 }
 
@@ -377,9 +477,6 @@ int check_args(int dtype, int64_t rows, int32_t width, const void* x, int64_t st
     return GSX_OK;
 }
 
-bool is_long(int dtype, int width) {
-    return width > kThreads * kPieces * (dtype == GSX_F32 ? F32::VEC : BF16::VEC);
-}
 
 // Workgroups that walk the rows, as many rows a workgroup as it has teams.
 int64_t groups_for(int64_t rows, int teams, int64_t most) {
@@ -388,32 +485,56 @@ int64_t groups_for(int64_t rows, int teams, int64_t most) {
 }
 
 // Calls f with the elements of a piece, the lanes of a team and the pieces of a lane
-// that hold a row of `width`, or returns false.
+// that hold a row of `width`, or returns false.  n pieces take the first pair with
+// G N >= n; the list goes by rising G N, so that n > G (N - 1).
 template <class E, class F>
 bool for_width(int width, F f) {
     auto with = [&](auto v, auto g, auto n) { f(v, g, n); };
+    if (width > kMostWidth) return false;
     auto lanes = [&](auto v) {
         constexpr int V = decltype(v)::value;
         const int n = (width + V - 1) / V;
 #define GSX_TEAM(G, N)                                                  \
     if (n <= G * N)                                                     \
         return with(v, std::integral_constant<int, G>{}, std::integral_constant<int, N>{})
-        GSX_TEAM(1, 1);
-        GSX_TEAM(2, 1);
-        GSX_TEAM(4, 1);
-        GSX_TEAM(8, 1);
-        if constexpr (V > 1) {
-            GSX_TEAM(16, 1);
-            GSX_TEAM(32, 1);
-            GSX_TEAM(64, 1);
+        if constexpr (V == 1) {
+            // a row a lane
+            GSX_TEAM(1, 1);
+            GSX_TEAM(1, 2);
+            GSX_TEAM(1, 3);
+            if constexpr (E::VEC > 4) {
+                GSX_TEAM(1, 4);
+                GSX_TEAM(1, 5);
+                GSX_TEAM(1, 6);
+                GSX_TEAM(1, 7);
+            }
+        } else {
+            GSX_TEAM(1, 1);
+            GSX_TEAM(2, 1);
+            GSX_TEAM(4, 1);
+            GSX_TEAM(4, 2);
+            GSX_TEAM(4, 3);
+            GSX_TEAM(8, 2);
+            GSX_TEAM(8, 3);
+            GSX_TEAM(16, 2);
+            GSX_TEAM(16, 3);
+            GSX_TEAM(32, 2);
+            GSX_TEAM(32, 3);
             GSX_TEAM(64, 2);
-            GSX_TEAM(64, 4);
+            GSX_TEAM(64, 3);
+            GSX_TEAM(256, 1);
             GSX_TEAM(256, 2);
-            GSX_TEAM(256, 4);
+            GSX_TEAM(256, 3);
+            if constexpr (V == 4) {
+                GSX_TEAM(256, 4);
+                GSX_TEAM(512, 3);
+                GSX_TEAM(512, 4);
+            } else {
+                GSX_TEAM(512, 2);
+            }
         }
 #undef GSX_TEAM
     };
-    if (width > kThreads * kPieces * E::VEC) return false;
     if (width < E::VEC) lanes(std::integral_constant<int, 1>{});
     else lanes(std::integral_constant<int, E::VEC>{});
     return true;
@@ -423,13 +544,13 @@ template <class E>
 int forward(const Norm& q, hipStream_t st) {
     const bool held = for_width<E>(q.width, [&](auto v, auto g, auto n) {
         constexpr int V = decltype(v)::value, G = decltype(g)::value, N = decltype(n)::value;
-        const int64_t groups = groups_for(q.rows, kThreads / G, 1 << 16);
-        hipLaunchKernelGGL((k_norm_fwd<E, V, G, N>), dim3((unsigned)groups), dim3(kThreads), 0, st,
-                           q);
+        const int64_t groups = groups_for(q.rows, threads_of<G> / G, kFwdGroups);
+        hipLaunchKernelGGL((k_norm_fwd<E, V, G, N>), dim3((unsigned)groups), dim3(threads_of<G>),
+                           0, st, q);
     });
     if (!held)
         hipLaunchKernelGGL((k_long_fwd<E>), dim3((unsigned)groups_for(q.rows, 1, 1 << 16)),
-                           dim3(kThreads), 0, st, q);
+                           dim3(kLongThreads), 0, st, q);
     GSX_LAUNCH_CHECK();
     return GSX_OK;
 }
@@ -440,13 +561,13 @@ int backward(const Norm& q, void* g_w, void* g_b, hipStream_t st) {
     if (q.rows > 0) {
         const bool held = for_width<E>(q.width, [&](auto v, auto g, auto n) {
             constexpr int V = decltype(v)::value, G = decltype(g)::value, N = decltype(n)::value;
-            groups = groups_for(q.rows, kThreads / G, kMostGroups);
-            hipLaunchKernelGGL((k_norm_bwd<E, V, G, N>), dim3((unsigned)groups), dim3(kThreads),
+            groups = groups_for(q.rows, threads_of<G> / G, G > 64 ? kWideGroups : kMostGroups);
+            hipLaunchKernelGGL((k_norm_bwd<E, V, G, N>), dim3((unsigned)groups), dim3(threads_of<G>),
                                (unsigned)(q.parts && G <= 64 ? 2 * q.width * 4 : 0), st, q);
         });
         if (!held) {
             hipLaunchKernelGGL((k_long_bwd<E>), dim3((unsigned)groups_for(q.rows, 1, 1 << 16)),
-                               dim3(kThreads), 0, st, q);
+                               dim3(kLongThreads), 0, st, q);
             GSX_LAUNCH_CHECK();
             groups = groups_for(q.rows, 1, kMostGroups);
             if (q.parts)
@@ -497,7 +618,7 @@ int gsx_layer_norm_fwd(int32_t dtype, int64_t rows, int32_t width, const void* x
 int64_t gsx_layer_norm_bwd_workspace_bytes(int32_t dtype, int64_t rows, int32_t width) {
     if (int e = check_shape(dtype, rows, width)) return e;
     const int64_t most = rows < kMostGroups ? rows : kMostGroups;
-    return 256 + up_to(most * 2 * width * 4, 256) + (is_long(dtype, width) ? rows * 12 : 0);
+    return 256 + up_to(most * 2 * width * 4, 256) + (width > kMostWidth ? rows * 12 : 0);
 }
 
 int gsx_layer_norm_bwd(int32_t dtype, int64_t rows, int32_t width, const void* x, int64_t x_stride,

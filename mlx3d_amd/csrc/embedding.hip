@@ -235,22 +235,25 @@ __device__ __forceinline__ uint64_t same_digit(uint32_t d, bool valid, int bits)
     return ~((uint64_t)hi << 32 | lo) & __ballot(valid);
 }
 
-// The rank of each of a wave's items among those of its digit, in their order, with
-// cnt[d] (zero before) left as the digit's count.
+// The rank of each of a wave's first `rounds` items a lane among those of its digit, in
+// their order, with cnt[d] (zero before) left as the digit's count.
 template <int ITEMS, int RADIX>
-__device__ __forceinline__ void wave_ranks(const uint32_t* key, int shift, int bits,
+__device__ __forceinline__ void wave_ranks(const uint32_t* key, int shift, int bits, int rounds,
                                            uint16_t* cnt, uint32_t* rank) {
     const int lane = threadIdx.x & 63;
 #pragma unroll
     for (int r = 0; r < ITEMS; ++r) {
-        const uint32_t d = key[r] >> shift & (RADIX - 1);
-        const uint64_t same = same_digit(d, key[r] != kNone, bits);
-        const uint64_t before = same & ((1ull << lane) - 1);
-        const uint32_t c = cnt[d];
-        rank[r] = c + (uint32_t)__popcll(before);
-        wave_fence();
-        if (key[r] != kNone && before == 0) cnt[d] = (uint16_t)(c + (uint32_t)__popcll(same));
-        wave_fence();
+        rank[r] = 0;
+        if (r < rounds) {
+            const uint32_t d = key[r] >> shift & (RADIX - 1);
+            const uint64_t same = same_digit(d, key[r] != kNone, bits);
+            const uint64_t before = same & ((1ull << lane) - 1);
+            const uint32_t c = cnt[d];
+            rank[r] = c + (uint32_t)__popcll(before);
+            wave_fence();
+            if (key[r] != kNone && before == 0) cnt[d] = (uint16_t)(c + (uint32_t)__popcll(same));
+            wave_fence();
+        }
     }
 }
 
@@ -304,7 +307,7 @@ __global__ __launch_bounds__(kSortThreads) void k_place(const Sort s) {
 #pragma unroll
     for (int k = 0; k < 2 * kEach; ++k) sum += total[k];
     uint32_t at = prefix_sum<kSortThreads>(sum, room[0], &live);  // its barrier: cnt is clear
-    wave_ranks<kItems, kRadix>(key, s.shift, s.bits, cnt[wave], rank);
+    wave_ranks<kItems, kRadix>(key, s.shift, s.bits, kItems, cnt[wave], rank);
     // the first pass counts the tokens that name a row
     if (!s.from && blockIdx.x == 0 && tid == 0) *s.live = live;
     __syncthreads();
@@ -352,27 +355,33 @@ __global__ __launch_bounds__(kSortThreads) void k_place(const Sort s) {
 }
 
 // All passes over few tokens by one workgroup, in shared memory; the others clear the
-// gradient.
+// gradient.  The waves share the tokens evenly, `rounds` times 64 each.
 constexpr int kFewThreads = 1024;
 template <int ITEMS>
 __global__ __launch_bounds__(kFewThreads) void k_sort_few(const Sort s) {
     constexpr int kWaves = kFewThreads / 64, kRadix = 256;
     __shared__ uint2 pairs[kFewThreads * ITEMS];
-    __shared__ uint16_t cnt[kWaves][kRadix];
+    __shared__ alignas(16) uint16_t cnt[kWaves][kRadix];
     __shared__ uint32_t start[kRadix], room[kWaves];
     if (blockIdx.x > 0) {
         clear<kFewThreads>(s, blockIdx.x - 1, gridDim.x - 1);
         return;
     }
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x, wave = tid >> 6;
+    const int rounds = ((int)s.q.count + kFewThreads - 1) / kFewThreads;  // ITEMS at most
+    const int first = wave * 64 * rounds + (tid & 63);
     uint32_t key[ITEMS], token[ITEMS];
-    load_indices<ITEMS>(s, 0, wave * (64 * ITEMS) + lane, 64, key, token);
+    load_indices<ITEMS>(s, 0, first, 64, key, token);
+#pragma unroll
+    for (int r = 0; r < ITEMS; ++r)
+        if (r >= rounds) key[r] = kNone;  // another wave's
     uint32_t live = 0;
     for (int shift = 0; shift < s.bits; shift += 8) {
-        for (int k = tid; k < kWaves * kRadix / 2; k += kFewThreads) ((uint32_t*)cnt)[k] = 0;
+        for (int k = tid; k < kWaves * kRadix / 8; k += kFewThreads)
+            ((u32x4*)cnt)[k] = u32x4{0, 0, 0, 0};
         __syncthreads();
         uint32_t rank[ITEMS];
-        wave_ranks<ITEMS, kRadix>(key, shift, min(s.bits - shift, 8), cnt[wave], rank);
+        wave_ranks<ITEMS, kRadix>(key, shift, min(s.bits - shift, 8), rounds, cnt[wave], rank);
         __syncthreads();
         uint32_t mine = 0;
         if (tid < kRadix) {
@@ -396,16 +405,16 @@ __global__ __launch_bounds__(kFewThreads) void k_sort_few(const Sort s) {
         __syncthreads();
 #pragma unroll
         for (int r = 0; r < ITEMS; ++r) {
-            const uint32_t i = wave * (64 * ITEMS) + r * 64 + lane;
-            const uint2 e = pairs[i];  // from `live` on: whatever is there
-            key[r] = i < live ? e.x : kNone;
+            const uint32_t i = (uint32_t)(first + r * 64);
+            const bool there = r < rounds && i < live;
+            const uint2 e = pairs[there ? i : 0];
+            key[r] = there ? e.x : kNone;
             token[r] = e.y;
         }
     }
 #pragma unroll
     for (int r = 0; r < ITEMS; ++r)
-        if (key[r] != kNone)
-            s.to[wave * (64 * ITEMS) + r * 64 + lane] = make_uint2(key[r], token[r]);
+        if (key[r] != kNone) s.to[first + r * 64] = make_uint2(key[r], token[r]);
     if (tid == 0) *s.live = live;
 }
 

@@ -435,7 +435,7 @@ __global__ __launch_bounds__(kThreads) void k_long_columns(const Norm q) {
 
 // ---- the workgroups' partial rows: 16 columns a workgroup, in 64 stretches ----
 
-constexpr int kJoinColumns = 16, kJoinParts = 64;
+constexpr int kJoinColumns = 16, kJoinParts = 64, kJoinBatch = 16;
 template <class E>
 __global__ __launch_bounds__(kJoinColumns * kJoinParts) void k_norm_join(const float* parts,
                                                                          int groups, int width,
@@ -444,12 +444,25 @@ __global__ __launch_bounds__(kJoinColumns * kJoinParts) void k_norm_join(const f
     const int col = threadIdx.x % kJoinColumns, part = threadIdx.x / kJoinColumns;
     const int c = blockIdx.x * kJoinColumns + col;
     float s = 0.f;
-    if (c < 2 * width)
-        for (int k = part; k < groups; k += kJoinParts) s += parts[(int64_t)k * 2 * width + c];
-    room[part][col] = s;
-    __syncthreads();
+    if (c < 2 * width) {
+        // a stretch's rows are asked for together
+        for (int k = part; k < groups; k += kJoinBatch * kJoinParts) {
+            float v[kJoinBatch];
+#pragma unroll
+            for (int u = 0; u < kJoinBatch; ++u)
+                v[u] = parts[(int64_t)min(k + u * kJoinParts, groups - 1) * 2 * width + c];
+#pragma unroll
+            for (int u = 0; u < kJoinBatch; ++u)
+                s += k + u * kJoinParts < groups ? v[u] : 0.f;
+        }
+    }
+    for (int n = kJoinParts / 2; n > 0; n /= 2) {
+        room[part][col] = s;
+        __syncthreads();
+        if (part < n) s += room[part + n][col];
+        __syncthreads();
+    }
     if (part != 0 || c >= 2 * width) return;
-    for (int k = 1; k < kJoinParts; ++k) s += room[k][col];
     typename E::T* to = (typename E::T*)(c < width ? g_w : g_b);
     if (to) to[c < width ? c : c - width] = E::down(s);
 }
@@ -512,8 +525,12 @@ bool for_width(int width, F f) {
             GSX_TEAM(1, 1);
             GSX_TEAM(2, 1);
             GSX_TEAM(4, 1);
-            GSX_TEAM(4, 2);
-            GSX_TEAM(4, 3);
+            if constexpr (V == 4) {
+                GSX_TEAM(8, 1);
+            } else {
+                GSX_TEAM(4, 2);
+                GSX_TEAM(4, 3);
+            }
             GSX_TEAM(8, 2);
             GSX_TEAM(8, 3);
             GSX_TEAM(16, 2);

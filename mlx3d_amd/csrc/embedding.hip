@@ -30,14 +30,14 @@ using namespace gsx;
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kSortThreads = 512, kItems = 8, kChunk = kSortThreads * kItems;
+constexpr int kSortThreads = 1024, kItems = 4, kChunk = kSortThreads * kItems;
 constexpr int kScanGroups = 16;  // of chunks, in the prefix
 constexpr int kFewItems = 16;    // tokens of a thread, where one workgroup sorts them all
 constexpr int kMostTile = 64;    // sorted tokens that a team of lanes adds up, at most
 constexpr int kLook = 4;         // tokens that a team looks up at a time
 constexpr int kBatch = 8;        // rows that a team asks for at a time
 constexpr int kSpan = 32;        // tiles of a row that a single team joins, at most
-constexpr int kJoinThreads = 1024;
+constexpr int kJoinThreads = 512;
 
 struct Embed {
     const void *table, *g_y, *indices;
@@ -511,7 +511,7 @@ __device__ __forceinline__ int64_t span_of(const Sum& s, int64_t tile, int64_t l
 template <int V>
 __device__ __forceinline__ void add_parts(const Sum& s, int64_t first, int64_t end, int64_t step,
                                           int c, float* acc) {
-    constexpr int kParts = V == 8 ? kBatch / 2 : kBatch;
+    constexpr int kParts = V == 8 ? 12 : 16;  // in flight, as registers allow
     for (int64_t t = first; t < end; t += kParts * step) {
         float v[kParts][V];
 #pragma unroll
@@ -533,7 +533,7 @@ __global__ __launch_bounds__(kJoinThreads) void k_join(const Sum s) {
     using P = Piece<E, V>;
     using T = typename E::T;
     constexpr int kTeams = kJoinThreads / G;
-    __shared__ float room[kJoinThreads][V + 1];
+    __shared__ float room[kJoinThreads / 64][G][V + 1];
     __shared__ int64_t spans[kTeams];  // the long ones
     __shared__ int teams[kTeams], found;
     const Embed& q = s.q;
@@ -570,17 +570,23 @@ __global__ __launch_bounds__(kJoinThreads) void k_join(const Sum s) {
             float acc[V] = {};
             if (team == 0) load_floats<V>(s.parts + ((own - far) * 2 + 1) * q.width + c, acc);
             add_parts<V>(s, own - far + 1 + team, own + 1, kTeams, c, acc);
+            // a wave's teams, then the waves
 #pragma unroll
-            for (int e = 0; e < V; ++e) room[threadIdx.x][e] = acc[e];
-            for (int n = kTeams / 2; n > 0; n /= 2) {
-                __syncthreads();
-                if (team < n) {
+            for (int e = 0; e < V; ++e)
 #pragma unroll
-                    for (int e = 0; e < V; ++e) {
-                        acc[e] += room[threadIdx.x + n * G][e];
-                        room[threadIdx.x][e] = acc[e];
-                    }
-                }
+                for (int o = G; o < 64; o <<= 1) acc[e] += __shfl_xor(acc[e], o, 64);
+            const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+            if (lane < G) {
+#pragma unroll
+                for (int e = 0; e < V; ++e) room[wave][lane][e] = acc[e];
+            }
+            __syncthreads();
+            if (team == 0) {
+#pragma unroll
+                for (int e = 0; e < V; ++e) acc[e] = 0.f;
+                for (int w = 0; w < kJoinThreads / 64; ++w)
+#pragma unroll
+                    for (int e = 0; e < V; ++e) acc[e] += room[w][lane][e];
             }
             if (team == 0) write(own, acc);
             __syncthreads();

@@ -30,10 +30,11 @@ using namespace gsx;
 namespace {
 
 constexpr int kThreads = 256;
+// a chunk of the sort: 16 waves of 4 rounds place it 10 % sooner than 8 of 8
 constexpr int kSortThreads = 1024, kItems = 4, kChunk = kSortThreads * kItems;
 constexpr int kScanGroups = 16;  // of chunks, in the prefix
 constexpr int kFewItems = 16;    // tokens of a thread, where one workgroup sorts them all
-constexpr int kMostTile = 64;    // sorted tokens that a team of lanes adds up, at most
+constexpr int kMostTile = 256;   // sorted tokens that a team of lanes adds up, at most
 constexpr int kLook = 4;         // tokens that a team looks up at a time
 constexpr int kBatch = 8;        // rows that a team asks for at a time
 constexpr int kSpan = 32;        // tiles of a row that a single team joins, at most

@@ -33,6 +33,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMostGroups = 1024;  // workgroups of a gradient, whose partial rows are joined
+constexpr int kLongStrips = 256;   // of rows, whose columns are added up apart from the rows' sums
 constexpr int kWideGroups = 512;   // where a row takes a workgroup: two a compute unit
 constexpr int kFwdGroups = 8192;    // workgroups of a forward pass at most
 constexpr int kMostWidth = 8192;    // of a row that a workgroup holds
@@ -586,7 +587,7 @@ int backward(const Norm& q, void* g_w, void* g_b, hipStream_t st) {
             hipLaunchKernelGGL((k_long_bwd<E>), dim3((unsigned)groups_for(q.rows, 1, 1 << 16)),
                                dim3(kLongThreads), 0, st, q);
             GSX_LAUNCH_CHECK();
-            groups = groups_for(q.rows, 1, kMostGroups);
+            groups = groups_for(q.rows, 1, kLongStrips);
             if (q.parts)
                 hipLaunchKernelGGL((k_long_columns<E>),
                                    dim3((unsigned)groups,

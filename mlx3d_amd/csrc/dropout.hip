@@ -8,7 +8,13 @@
 // the key `seed` and the counter (block, offset): the eight half-words of the block
 // i / 8 are the upper halves of eight elements' numbers, those of the block
 // 2^63 + i / 8 the lower ones.  A lower half matters only where the upper one equals
-// the threshold's, once in 65 536 elements.
+// the threshold's, once in 65 536 elements: a block's ten rounds serve eight elements
+// and not four.
+//
+// Bound by memory: 118 million bfloat16 79 us (6.0 TB/s, 4 bytes an element), 59 million
+// float32 80 us, 124 on top of a residual (5.7).  The rounds take about two thirds of
+// that in the vector units, beside it; with both blocks formed for all elements, and
+// elements loaded one by one, the first took 238.
 #include <hip/hip_runtime.h>
 
 #include <cmath>

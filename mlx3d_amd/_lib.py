@@ -273,37 +273,25 @@ def stream_handle(device: torch.device):
     return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(index))
 
 
-def launch(name: str, label: str, device: torch.device, *args) -> None:
-    """Calls an entry point that enqueues work, with torch's current stream on `device`
-    as its last argument and that device the current one; `label` is its stage.  (The
-    usual case, no timer and one device, takes no context: each costs a microsecond,
-    three on autograd's thread.)"""
-    index = device.index
-    entry = getattr(load(), name)
-    if profiling._active is None and index == torch._C._cuda_getDevice():
-        status = entry(*args, torch._C._cuda_getCurrentRawStream(index))
-    else:
-        with torch.cuda.device(device), profiling.stage(label):
-            status = entry(*args, stream_handle(device))
-    if status < 0:
-        check(status, name)
+_autograd = None
 
 
-@functools.lru_cache(maxsize=4096)
-def workspace_bytes(name: str, *shape: int) -> int:
-    """What a ``*_workspace_bytes`` entry point says of a shape."""
-    return check(int(getattr(load(), name)(*shape)), name)
-
-
-def scratch(n: int, device: torch.device) -> torch.Tensor:
-    return torch.empty(n, dtype=torch.uint8, device=device)
-
-
-def contiguous_like(t: torch.Tensor) -> torch.Tensor:
-    """An uninitialised tensor of t's shape and type in row-major order."""
-    if t.is_contiguous():
-        return torch.empty_like(t)  # half the time of the call below
-    return torch.empty(t.shape, dtype=t.dtype, device=t.device)
+def autograd():
+    """The native autograd nodes (csrc/autograd.cpp), loaded once; raise if they have not
+    been built."""
+    global _autograd
+    if _autograd is None:
+        load()
+        try:
+            from . import _autograd as module
+        except ImportError as e:
+            raise ImportError(
+                "mlx3d_amd: _autograd.so is missing or does not load. Build it with "
+                "`python mlx3d_amd/csrc/build.py` (or __graft_entry__.build()); there is no "
+                f"fallback. ({e})") from e
+        profiling.watch(module.set_timed)
+        _autograd = module
+    return _autograd
 
 
 def require_device(*tensors: torch.Tensor | None) -> torch.device:

@@ -7,6 +7,8 @@ the source tree).  Flags:
                              radii, tile rectangles, contributor counts)
   -munsafe-fp-atomics        hardware global_atomic_add_f32 in the backward
   -packed-fp32-ops disabled  no v_pk_*_f32 generated
+Beside it goes mlx3d_amd/_autograd.so, the field layers' autograd nodes: host code
+against torch's headers, linked to libgsx.so.
 The compiler's per-kernel resource usage (VGPRs, scratch, occupancy) is
 written to _build/resource_usage.json, and the build fails if any kernel
 spills registers to scratch memory.
@@ -20,6 +22,7 @@ import os
 import re
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 PKG = os.path.dirname(HERE)
@@ -28,6 +31,7 @@ SOURCES = ["capi.hip", "preprocess.hip", "binning.hip", "raster.hip", "train.hip
            "density.hip", "geometry.hip", "feedforward.hip", "distil.hip",
            "embedding.hip", "layernorm.hip", "dropout.hip"]
 LIB = os.path.join(PKG, "libgsx.so")
+AUTOGRAD = os.path.join(PKG, "_autograd.so")
 ARCH = os.environ.get("GSX_OFFLOAD_ARCH", "gfx950")
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
@@ -80,12 +84,41 @@ def _compile(src: str, obj: str) -> dict:
     return _resources(r.stderr)
 
 
+def _compile_autograd(obj: str) -> None:
+    from torch.utils import cpp_extension
+
+    includes = [*cpp_extension.include_paths(), sysconfig.get_paths()["include"],
+                "/opt/rocm/include", os.path.join(ROOT, "include")]
+    # (the last two name the runtime that torch's own headers are to declare)
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-Wall", "-Wno-unknown-pragmas",
+           *(f"-I{d}" for d in includes), "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+           "-c", os.path.join(HERE, "autograd.cpp"), "-o", obj]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed for autograd.cpp:\n{r.stdout}\n{r.stderr}")
+
+
+def _link_autograd(obj: str) -> None:
+    from torch.utils import cpp_extension
+
+    libs = [f"-L{d}" for d in cpp_extension.library_paths()]
+    cmd = ["g++", "-shared", "-o", AUTOGRAD + ".tmp", obj, *libs, "-lc10", "-lc10_hip",
+           "-ltorch_cpu", "-ltorch_python", f"-L{PKG}", "-l:libgsx.so", "-Wl,-rpath,$ORIGIN"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"link failed for {AUTOGRAD}:\n{r.stdout}\n{r.stderr}")
+    os.replace(AUTOGRAD + ".tmp", AUTOGRAD)
+
+
 def build(verbose: bool = False) -> str:
     objdir = os.path.join(PKG, "_build")
     os.makedirs(objdir, exist_ok=True)
     objs = [os.path.join(objdir, s.replace(".hip", ".o")) for s in SOURCES]
-    with concurrent.futures.ThreadPoolExecutor(max_workers=min(4, len(SOURCES))) as ex:
+    nodes = os.path.join(objdir, "autograd.o")
+    with concurrent.futures.ThreadPoolExecutor(max_workers=min(8, len(SOURCES))) as ex:
+        host = ex.submit(_compile_autograd, nodes)
         usage = list(ex.map(lambda a: _compile(*a), zip(SOURCES, objs)))
+        host.result()
     kernels = {k: v for u in usage for k, v in u.items()}
     with open(os.path.join(objdir, "resource_usage.json"), "w") as f:
         json.dump(kernels, f, indent=1, sort_keys=True)
@@ -99,6 +132,7 @@ def build(verbose: bool = False) -> str:
     if r.returncode != 0:
         raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
     os.replace(tmp, LIB)
+    _link_autograd(nodes)
     if verbose:
         print(f"built {LIB}")
     return LIB

@@ -13,32 +13,6 @@ from .. import _lib
 __all__ = ["Dropout", "dropout"]
 
 
-def _drop(x, residual, p, seed, offset, at):
-    """The values, with the counter `offset`, or what `at` on the device holds."""
-    held = x.contiguous()
-    base = None if residual is None else residual.contiguous()
-    y = torch.empty_like(held)
-    _lib.launch("gsx_dropout", "dropout", x.device, _lib.DTYPES[x.dtype], held.numel(), p, seed,
-                offset, _lib.ptr(at), held.data_ptr(), _lib.ptr(base), y.data_ptr())
-    return y
-
-
-class _Dropout(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, residual, p, seed, offset, at):
-        ctx.how = (p, seed, offset)
-        # saved, so that a counter that moves on before the gradient is noticed
-        ctx.save_for_backward(at)
-        return _drop(x, residual, p, seed, offset, at)
-
-    @staticmethod
-    @_lib.once_differentiable("dropout")
-    def backward(ctx, saved, g_y):
-        need_x, need_residual = ctx.needs_input_grad[:2]
-        g_x = _drop(g_y, None, *ctx.how, saved[0]) if need_x else None
-        return g_x, g_y if need_residual else None, None, None, None, None
-
-
 def dropout(x: torch.Tensor, p: float, seed: int, offset: int | torch.Tensor = 0,
             residual: torch.Tensor | None = None) -> torch.Tensor:
     """Each element of ``x`` with probability 1 - ``p`` divided by 1 - p, else 0; with a
@@ -72,7 +46,7 @@ def dropout(x: torch.Tensor, p: float, seed: int, offset: int | torch.Tensor = 0
             raise ValueError("offset must be a whole number from 0 to 2^63 - 1.")
         at = None
     _lib.require_device(x, residual, at)
-    return _Dropout.apply(x, residual, p, seed, offset, at)
+    return _lib.autograd().dropout(x, residual, p, seed, offset, at)
 
 
 class Dropout:

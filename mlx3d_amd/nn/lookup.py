@@ -14,34 +14,6 @@ from .. import _lib
 __all__ = ["Embedding", "embedding"]
 
 
-class _Embedding(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, indices, table, scale):
-        held = indices.contiguous()
-        rows, stride = _lib.rows_of(table)
-        count, device = held.numel(), table.device
-        y = torch.empty((*held.shape, table.shape[1]), dtype=table.dtype, device=device)
-        ctx.head = head = (_lib.DTYPES[table.dtype], count, *table.shape)
-        ctx.how = how = (int(indices.dtype == torch.int64), scale)
-        _lib.launch("gsx_embed_fwd", "embed_fwd", device, *head, held.data_ptr(), how[0],
-                    rows.data_ptr(), stride, scale, y.data_ptr())
-        ctx.save_for_backward(indices)
-        return y
-
-    @staticmethod
-    @_lib.once_differentiable("embedding")
-    def backward(ctx, saved, g_y):
-        held = saved[0].contiguous()
-        head, (index64, scale), device = ctx.head, ctx.how, g_y.device
-        rows, stride = _lib.rows_of(g_y)
-        g_table = torch.empty(head[2:], dtype=g_y.dtype, device=device)
-        n = _lib.workspace_bytes("gsx_embed_bwd_workspace_bytes", *head)
-        ws = _lib.scratch(n, device)
-        _lib.launch("gsx_embed_bwd", "embed_bwd", device, *head, held.data_ptr(), index64,
-                    rows.data_ptr(), stride, scale, g_table.data_ptr(), ws.data_ptr(), n)
-        return None, g_table, None
-
-
 def embedding(indices: torch.Tensor, table: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
     """(..., C) = ``scale`` times the rows of ``table`` (V, C) that ``indices``
     (..., int32 or int64) name; zeros where an index lies outside [0, V), so -1 stands
@@ -60,7 +32,7 @@ def embedding(indices: torch.Tensor, table: torch.Tensor, scale: float = 1.0) ->
     if not abs(scale) < 3.4e38:
         raise ValueError("scale must be finite in float32.")
     _lib.require_device(indices, table)
-    return _Embedding.apply(indices, table, scale)
+    return _lib.autograd().embedding(indices, table, scale)
 
 
 class Embedding:

@@ -13,40 +13,6 @@ from .. import _lib
 __all__ = ["LayerNorm", "layer_norm"]
 
 
-class _LayerNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, eps):
-        rows, stride = _lib.rows_of(x)
-        w = None if weight is None else weight.contiguous()
-        b = None if bias is None else bias.contiguous()
-        y = _lib.contiguous_like(x)
-        ctx.head = head = (_lib.DTYPES[x.dtype], rows.shape[0], rows.shape[1])
-        _lib.launch("gsx_layer_norm_fwd", "layer_norm_fwd", x.device, *head, rows.data_ptr(), stride,
-                    _lib.ptr(w), _lib.ptr(b), eps, y.data_ptr())
-        ctx.save_for_backward(x, weight)
-        ctx.eps = eps
-        return y
-
-    @staticmethod
-    @_lib.once_differentiable("layer_norm")
-    def backward(ctx, saved, g_y):
-        x, weight = saved
-        head, device = ctx.head, x.device
-        rows, stride = _lib.rows_of(x)
-        g_rows, g_stride = _lib.rows_of(g_y)
-        w = None if weight is None else weight.contiguous()
-        need_x, need_w, need_b, _ = ctx.needs_input_grad
-        g_x = _lib.contiguous_like(x) if need_x else None
-        g_w = torch.empty(head[2], dtype=x.dtype, device=device) if need_w else None
-        g_b = torch.empty(head[2], dtype=x.dtype, device=device) if need_b else None
-        n = _lib.workspace_bytes("gsx_layer_norm_bwd_workspace_bytes", *head)
-        ws = _lib.scratch(n, device) if need_w or need_b else None
-        _lib.launch("gsx_layer_norm_bwd", "layer_norm_bwd", device, *head, rows.data_ptr(), stride,
-                    _lib.ptr(w), g_rows.data_ptr(), g_stride, ctx.eps, _lib.ptr(g_x), _lib.ptr(g_w),
-                    _lib.ptr(g_b), _lib.ptr(ws), n)
-        return g_x, g_w, g_b, None
-
-
 def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None,
                bias: torch.Tensor | None = None, eps: float = 1e-5) -> torch.Tensor:
     """(x - mean) / sqrt(var + eps) * weight + bias over the last dimension of ``x``
@@ -68,7 +34,7 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None,
     if not 1.2e-38 <= eps <= 3.0e38:
         raise ValueError("eps must be positive, finite and normal in float32 (from 1.2e-38 on).")
     _lib.require_device(x, weight, bias)
-    return _LayerNorm.apply(x, weight, bias, eps)
+    return _lib.autograd().layer_norm(x, weight, bias, eps)
 
 
 class LayerNorm:

@@ -15,6 +15,20 @@ from collections import defaultdict
 import torch
 
 _active: "StageTimer | None" = None
+_watchers: list = []  # told whether a timer is active
+
+
+def watch(tell) -> None:
+    """Calls tell(whether a timer is active) now and whenever that changes."""
+    _watchers.append(tell)
+    tell(_active is not None)
+
+
+def _activate(timer: "StageTimer | None") -> None:
+    global _active
+    _active = timer
+    for tell in _watchers:
+        tell(timer is not None)
 
 
 class StageTimer:
@@ -24,14 +38,12 @@ class StageTimer:
         self.counters: dict[str, list[float]] = defaultdict(list)
 
     def __enter__(self):
-        global _active
         self._prev = _active
-        _active = self
+        _activate(self)
         return self
 
     def __exit__(self, *exc):
-        global _active
-        _active = self._prev
+        _activate(self._prev)
         self.collect()
         return False
 

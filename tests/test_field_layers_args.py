@@ -2,6 +2,7 @@
 any launch (no GPU needed)."""
 
 import ctypes
+import sys
 
 import pytest
 import torch
@@ -104,6 +105,30 @@ def test_modules_refuse():
         Dropout(0.5, seed=1, device="cpu")(torch.zeros(3, 4))
     a, b = (Embedding(3, 4, device="cpu", seed=5).params["table"] for _ in range(2))
     assert torch.equal(a, b)
+
+
+def test_missing_nodes_are_named(monkeypatch):
+    """Without the native nodes the layers raise; there is no other path."""
+    monkeypatch.setattr(_lib, "_autograd", None)
+    monkeypatch.setitem(sys.modules, "mlx3d_amd._autograd", None)
+    monkeypatch.delattr("mlx3d_amd._autograd", raising=False)
+    with pytest.raises(ImportError, match="_autograd.so is missing"):
+        _lib.autograd()
+
+
+def test_the_nodes_hear_of_timers():
+    from mlx3d_amd import profiling
+
+    heard = []
+    profiling.watch(heard.append)
+    try:
+        with profiling.StageTimer():
+            with profiling.StageTimer():
+                pass
+    finally:
+        profiling._watchers.remove(heard.append)
+    assert heard == [False, True, True, True, False]
+    assert _lib.autograd() is _lib.autograd()
 
 
 BUF = (ctypes.c_char * 4096)()

@@ -309,5 +309,6 @@ def test_a_timer_sees_the_stages():
 def test_errors_of_the_entry_points_reach_the_caller():
     x = torch.zeros((4, 4), device=DEV)
     with pytest.raises(_lib.GsxError, match="gsx_dropout failed"):
-        _lib.launch("gsx_dropout", "dropout", x.device, 7, 16, 0.5, 1, 0, None, x.data_ptr(), None,
-                    x.data_ptr())
+        _lib.autograd().dropout(x, None, 1.5, 1, 0, None)
+    with pytest.raises(_lib.GsxError, match="gsx_layer_norm_fwd failed"):
+        _lib.autograd().layer_norm(x, None, None, 0.0)

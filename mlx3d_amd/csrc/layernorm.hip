@@ -18,14 +18,14 @@
 // dw and db in registers over all its rows; a workgroup leaves one partial row of
 // each, and a second launch adds those up.
 //
-// Memory bounds both directions: 118 MB of 32 float32 columns take 39 us forward (6.0
-// TB/s) and 68 backward (5.2), 199 million bfloat16 in rows of 96 143 us forward (5.6).
+// Memory bounds both directions: 118 MB of 32 float32 columns take 39 us forward (6.1
+// TB/s) and 65 backward (5.5), 199 million bfloat16 in rows of 96 145 us forward (5.5).
 // In 16 bits the vector units come close behind, so what a row costs beside its elements
 // counts: teams are as small as whole lines allow, with two or three pieces a lane, so
 // that a sum takes few steps and few lanes are idle (120 MB of bfloat16, forward and
 // backward: 300 columns 53 and 83 us, on 64 lanes with one piece each 83 and 120; 48
 // columns 51 and 84 for 67 and 91), and the next row is asked for before this one's sums.
-// Odd widths cost up to a third more in 16 bits: their vectors straddle lines.
+// Odd widths cost up to a quarter more in 16 bits: their vectors straddle lines.
 #include <hip/hip_runtime.h>
 
 #include <type_traits>
@@ -41,10 +41,16 @@ using namespace gsx;
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kMostGroups = 1024;  // workgroups of a gradient, whose partial rows are joined
+// Workgroups of a gradient, whose partial rows are joined: two to four a compute unit, no
+// more than its registers hold at once (a second generation waits for the first).  120 MB,
+// gradient and join, us, with 512 / 768 / 1024: a row a lane, 5 bfloat16 columns 128 / 114 /
+// 113; one piece a lane, 32 float32 70 / 69 / 72, 32 bfloat16 80 / 75 / 75; more, 64
+// bfloat16 74 / 77 / 85, 512 float32 75 / 75 / 76.
+constexpr int kMostGroups = 1024;
+template <int V, int G, int N>
+constexpr int groups_of = V == 1 ? kMostGroups : N == 1 && G <= 64 ? 768 : 512;
 constexpr int kLongStrips = 256;   // of rows, whose columns are added up apart from the rows' sums
-constexpr int kWideGroups = 512;   // where a row takes a workgroup: two a compute unit
-constexpr int kFwdGroups = 8192;    // workgroups of a forward pass at most
+constexpr int kFwdGroups = 8192;   // workgroups of a forward pass at most
 constexpr int kMostWidth = 8192;    // of a row that a workgroup holds
 
 struct Norm {
@@ -509,6 +515,20 @@ int64_t groups_for(int64_t rows, int teams, int64_t most) {
     return n < most ? n : most;
 }
 
+// For the forward pass: about four rounds each, the same for all, so that what a workgroup
+// begins with (its weights) is paid for; one where there are few, more where there are
+// many.  118 million bfloat16 in rows of 127, 14.8 thousand rounds in all, us: one round
+// a workgroup 67, one or two 55, four 50; 400 MB in rows of 512, 49 thousand: one 172, six
+// 152, twelve 158.
+int64_t forward_groups(int64_t rows, int teams) {
+    const int64_t rounds = (rows + teams - 1) / teams;
+    int64_t groups = (rounds + 3) / 4;
+    if (groups < kFwdGroups / 4) groups = kFwdGroups / 4;
+    if (groups > kFwdGroups) groups = kFwdGroups;
+    const int64_t each = (rounds + groups - 1) / groups;
+    return (rounds + each - 1) / each;
+}
+
 // Calls f with the elements of a piece, the lanes of a team and the pieces of a lane
 // that hold a row of `width`, or returns false.  n pieces take the first pair with
 // G N >= n; the list goes by rising G N, so that n > G (N - 1).  (Float32 rows of 17 to 32
@@ -575,7 +595,7 @@ template <class E>
 int forward(const Norm& q, hipStream_t st) {
     const bool held = for_width<E>(q.width, [&](auto v, auto g, auto n) {
         constexpr int V = decltype(v)::value, G = decltype(g)::value, N = decltype(n)::value;
-        const int64_t groups = groups_for(q.rows, threads_of<G> / G, kFwdGroups);
+        const int64_t groups = forward_groups(q.rows, threads_of<G> / G);
         hipLaunchKernelGGL((k_norm_fwd<E, V, G, N>), dim3((unsigned)groups), dim3(threads_of<G>),
                            0, st, q);
     });
@@ -592,7 +612,7 @@ int backward(const Norm& q, void* g_w, void* g_b, hipStream_t st) {
     if (q.rows > 0) {
         const bool held = for_width<E>(q.width, [&](auto v, auto g, auto n) {
             constexpr int V = decltype(v)::value, G = decltype(g)::value, N = decltype(n)::value;
-            groups = groups_for(q.rows, threads_of<G> / G, G > 64 ? kWideGroups : kMostGroups);
+            groups = groups_for(q.rows, threads_of<G> / G, groups_of<V, G, N>);
             hipLaunchKernelGGL((k_norm_bwd<E, V, G, N>), dim3((unsigned)groups), dim3(threads_of<G>),
                                (unsigned)(q.parts && G <= 64 ? 2 * q.width * 4 : 0), st, q);
         });

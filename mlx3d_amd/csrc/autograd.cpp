@@ -276,12 +276,14 @@ struct Dropout : Function<Dropout> {
 }  // namespace
 
 PYBIND11_MODULE(_autograd, m) {
-    static py::object error = py::module_::import("mlx3d_amd._lib").attr("GsxError");
+    // never let go: the interpreter may have ended before statics do
+    static const auto* error =
+        new py::object(py::module_::import("mlx3d_amd._lib").attr("GsxError"));
     py::register_exception_translator([](std::exception_ptr p) {
         try {
             if (p) std::rethrow_exception(p);
         } catch (const Failure& e) {
-            PyErr_SetString(error.ptr(), e.what());
+            PyErr_SetString(error->ptr(), e.what());
         }
     });
     using Release = py::call_guard<py::gil_scoped_release>;

@@ -285,8 +285,8 @@ __device__ __forceinline__ uint32_t prefix_sum(uint32_t v, uint32_t* room, uint3
 // Up to 8 bits the chunk is regrouped by digit first, so that stores are runs; with
 // more digits than a chunk has tokens there are none.  A wave's counts are 16 bits, two
 // digits a word, which are added up as words: a chunk's 4096 tokens do not carry.
-// 17 us with 12 bits, most of it scattered stores of 8 bytes (digit by digit, not in
-// words, 25); 10 with 8 bits.
+// 16 us with 12 bits, most of it scattered stores of 8 bytes, which write 27 MB of lines
+// for 8 (counts digit by digit, not in words, 25 us); 10 us and 8 MB with 8 bits.
 template <int BITS>
 __global__ __launch_bounds__(kSortThreads) void k_place(const Sort s) {
     constexpr int kRadix = 1 << BITS, kWaves = kSortThreads / 64, kWords = kRadix / 2;
@@ -650,7 +650,7 @@ Layout layout(int dtype, int64_t count, int64_t rows, int32_t width) {
     l.bits = 1;
     while (((int64_t)1 << l.bits) < rows) ++l.bits;
     l.few = count <= kFewThreads * kFewItems;
-    // One pass of 12 bits instead of two of 8: 26 us for 34; two of 12 for two of 8 lose
+    // One pass of 12 bits instead of two of 8: 25 us for 34; two of 12 for two of 8 lose
     // (200 000 tokens 39 us for 29), whose stores are runs.
     l.digit = l.bits <= 8 || (l.bits > 12 && l.bits <= 16) ? 8 : 12;
     l.passes = l.few ? 1 : (l.bits + l.digit - 1) / l.digit;

@@ -226,3 +226,28 @@ def test_more_elements_than_32_bits_count():
     assert torch.equal(y.detach()[picks], table.detach()[k[picks]])
     assert torch.equal(grad[k[picks]], table.detach()[k[picks]])
     assert torch.equal(grad[k[5]], (2 * table.detach()[k[5]].float()).to(torch.bfloat16))
+
+
+def test_rows_of_a_million_columns():
+    """More column blocks and tokens than a launch holds: workgroups walk on."""
+    if torch.cuda.mem_get_info()[0] < 60 << 30:
+        pytest.skip("takes 60 GB of device memory")
+    width, count = 1 << 20, 16_500
+    g = torch.Generator(device=DEV).manual_seed(3)
+    table = torch.randn((7, width), generator=g, device=DEV).to(torch.bfloat16)
+    k = torch.randint(-1, 7, (count,), generator=g, device=DEV)
+    y = embedding(k, table)
+    for i in (0, 1, 16_383, 16_384, 16_385, count - 1):
+        want = table[k[i]] if int(k[i]) >= 0 else torch.zeros_like(table[0])
+        assert torch.equal(y[i], want)
+    named = (k >= 0).sum()
+    assert int((y[:, 0] != 0).sum()) == int(named) and int((y[:, -1] != 0).sum()) == int(named)
+
+
+@pytest.mark.parametrize("mode", (torch.no_grad, torch.inference_mode))
+def test_without_a_graph(mode):
+    k, table, _ = inputs(40, 9, 12, torch.float32)
+    want = embedding(k, table)
+    with mode():
+        y = embedding(k, table.requires_grad_(True) if mode is torch.no_grad else table)
+        assert not y.requires_grad and torch.equal(y, want)

@@ -4,6 +4,7 @@ not depend on how many others there are."""
 
 import importlib.util
 import os
+import threading
 
 import pytest
 import torch
@@ -279,6 +280,41 @@ def test_gradients_through_a_checkpoint(which, create_graph):
                               create_graph=create_graph)
     for a, b in zip(got, want):
         assert torch.equal(a.detach(), b)
+
+
+@pytest.mark.parametrize("which", range(5))
+@pytest.mark.parametrize("mode", (torch.no_grad, torch.inference_mode))
+def test_without_a_graph(which, mode):
+    call, leaves = ops()[which]
+    want = call(*leaves).detach()
+    with mode():
+        y = call(*(t.detach() for t in leaves))
+        assert not y.requires_grad and torch.equal(y, want)
+
+
+def test_threads_at_once():
+    """Forward and gradient from four threads, each on a stream of its own."""
+    call, leaves = ops()[0]
+    dy = torch.randn((50, 8), generator=torch.Generator().manual_seed(1)).to(DEV)
+    want = torch.autograd.grad(call(*leaves), leaves, dy)
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work():
+        mine = [t.detach().clone().requires_grad_(True) for t in leaves]
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(50):
+                got = torch.autograd.grad(call(*mine), mine, dy)
+            torch.cuda.current_stream().synchronize()
+            if not all(torch.equal(a, b) for a, b in zip(got, want)):
+                wrong.append(threading.get_ident())
+
+    threads = [threading.Thread(target=work) for _ in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
 
 
 def test_inputs_changed_before_the_gradient_are_noticed():

@@ -100,6 +100,15 @@ def test_against_64_bits(size, dtype):
     check(outputs(*t), *formulas(*t, 1e-5), dtype)
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("size", [(5000, 1030), (1700, 2100), (1300, 4300), (700, 8100),
+                                  (600, 8200), (9000, 520), (70_000, 96), (150_000, 3)], ids=str)
+def test_workgroups_that_walk_many_rows(size, dtype):
+    """More rows than teams at once, in each kind of team: several rounds a workgroup."""
+    t = inputs(*size, dtype, seed=sum(size))
+    check(outputs(*t), *formulas(*t, 1e-5), dtype)
+
+
 @pytest.mark.parametrize("width", (27, 96, 700, 5000))
 def test_far_from_zero(width):
     """Rows whose mean is a thousand times their spread keep the spread's digits."""

@@ -4,12 +4,13 @@
 //   dT[v] = s sum over i with k_i = v of dy_i
 //
 // The gradient sorts the tokens (stably, so that a row's sum has one order) and
-// walks them in tiles: a group of lanes adds up a tile's rows of dy as long as the
-// key stays the same.  What begins and ends inside a tile is written at once; what a
-// tile shares with its neighbours goes into two partial rows, which a last launch
+// walks them in tiles: a team of lanes adds up a tile's rows of dy as long as the
+// key stays the same.  What begins and ends inside a tile is written at once; what
+// tiles of a workgroup share is put together in shared memory, and what its block of
+// tiles shares with its neighbours goes into two partial rows, which a last launch
 // joins.  So a row that every token names is spread over as many lanes as rows that
 // one token names, no sum depends on the order of arrival, and sums stay short: a
-// tile's, then the tiles'.
+// tile's, a block's, then the blocks'.
 //
 // The sort is a stable radix sort by digits of 8 or 12 bits, three launches a pass: a
 // chunk's counts of each digit, their prefix over the chunks, and the placement.  No
@@ -41,7 +42,7 @@ constexpr int kFewItems = 16;    // tokens of a thread, where one workgroup sort
 constexpr int kMostTile = 256;   // sorted tokens that a team of lanes adds up, at most
 constexpr int kLook = 4;         // tokens that a team looks up at a time
 constexpr int kBatch = 8;        // rows that a team asks for at a time
-constexpr int kSpan = 32;        // tiles of a row that a single team joins, at most
+constexpr int kSpan = 32;        // blocks of a row that a single team joins, at most
 constexpr int kJoinThreads = 512;
 
 struct Embed {
@@ -436,32 +437,53 @@ struct Sum {
     const uint2* pairs;
     const uint32_t* live;
     int tile;          // sorted tokens of a tile
-    uint32_t* begins;  // of a row that spans tiles, the first; others' are not set
-    float* parts;      // (tiles, 2, width): what a tile shares with the one before, and behind
+    int block;         // and of the tiles of one workgroup
+    uint32_t* begins;  // of a row that spans blocks, the first; others' are not set
+    float* parts;      // (blocks, 2, width): what a block shares with the one before, and behind
 };
 
-// One tile, V columns of it.  A batch of rows is asked for before the first is added:
-// 30 us, 4.3 TB/s of gathered rows (row by row 62).
+// What a tile leaves to others: of the row that was open at its begin, and of the row
+// that is open at its end.  A tile within one row (whole) has the first alone.
+struct Edges {
+    bool open, more, whole;
+    uint32_t first_key, last_key;
+};
+
 template <class E, int V>
-__device__ __forceinline__ void tile_sum(const Sum& s, int64_t tile, int64_t live, int c) {
+__device__ __forceinline__ void write_row(const Embed& q, uint32_t key, int c, const float* acc) {
+    using P = Piece<E, V>;
+    float v[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] = acc[e] * q.scale;
+    P::store((typename E::T*)q.g_table + (int64_t)key * q.width + c, P::down(v));
+}
+
+// One tile, V columns of it: rows that begin and end in it are written, the others go to
+// head and tail.  A batch of rows is asked for before the first is added: 30 us, 4.3 TB/s
+// of gathered rows (row by row 62).
+template <class E, int V>
+__device__ __forceinline__ Edges tile_sum(const Sum& s, int64_t tile, int64_t live, int c,
+                                          float* head, float* tail) {
     using P = Piece<E, V>;
     using T = typename E::T;
     const Embed& q = s.q;
     const int64_t first = tile * s.tile;
+    if (first >= live) return Edges{false, false, false, 0, 0};
     const int n = (int)min<int64_t>(s.tile, live - first);
     const uint2* pairs = s.pairs + first;
     uint32_t key = pairs[0].x;
-    bool open = first > 0 && pairs[-1].x == key;  // the tile before has some of this row
-    const bool more = first + n < live && pairs[n].x == pairs[n - 1].x;
+    Edges edges;
+    edges.first_key = key;
+    edges.open = first > 0 && pairs[-1].x == key;
+    edges.more = first + n < live && pairs[n].x == pairs[n - 1].x;
+    bool open = edges.open;
     float acc[V] = {};
-    float* part = s.parts + tile * 2 * q.width + c;
-    auto write = [&]() {
+    auto close = [&]() {
         if (open) {
-            store_floats<V>(part, acc);
-        } else {
 #pragma unroll
-            for (int e = 0; e < V; ++e) acc[e] *= q.scale;
-            P::store((T*)q.g_table + (int64_t)key * q.width + c, P::down(acc));
+            for (int e = 0; e < V; ++e) head[e] = acc[e];
+        } else {
+            write_row<E, V>(q, key, c, acc);
         }
     };
     for (int j = 0; j < n; j += kBatch) {
@@ -476,7 +498,7 @@ __device__ __forceinline__ void tile_sum(const Sum& s, int64_t tile, int64_t liv
         for (int u = 0; u < kBatch; ++u) {
             if (j + u >= n) break;
             if (p[u].x != key) {
-                write();
+                close();
                 key = p[u].x;
                 open = false;
 #pragma unroll
@@ -488,38 +510,100 @@ __device__ __forceinline__ void tile_sum(const Sum& s, int64_t tile, int64_t liv
             for (int e = 0; e < V; ++e) acc[e] += v[e];
         }
     }
-    if (!more) {
-        write();
-    } else if (open) {
-        store_floats<V>(part, acc);
+    edges.last_key = key;
+    edges.whole = edges.more && open;
+    if (!edges.more || open) {
+        close();
     } else {
-        store_floats<V>(part + q.width, acc);
-        s.begins[key] = (uint32_t)tile;
+#pragma unroll
+        for (int e = 0; e < V; ++e) tail[e] = acc[e];
+    }
+    return edges;
+}
+
+// G lanes a tile, a piece of V columns each.  Rows that span tiles of one workgroup are
+// put together in shared memory, each by the team in whose tile it ends; what leaves the
+// workgroup's block of tiles goes to its parts.
+template <class E, int V, int G>
+__global__ __launch_bounds__(kThreads) void k_tile_sums(const Sum s) {
+    constexpr int kTeams = kThreads / G;
+    constexpr int kBack = V == 8 ? 4 : 8;  // tiles that are looked at together
+    __shared__ float heads[kTeams][G][V], tails[kTeams][G][V];
+    __shared__ bool whole[kTeams];
+    const Embed& q = s.q;
+    const int team = threadIdx.x / G, lane = threadIdx.x % G;
+    const int at = (blockIdx.y * G + lane) * V;
+    const bool here = at < q.width;
+    const int c = min(at, q.width - V);
+    const int64_t live = *s.live;
+    for (int64_t block = blockIdx.x; block * s.block < live; block += gridDim.x) {
+        const Edges mine = tile_sum<E, V>(s, block * kTeams + team, live, c, heads[team][lane],
+                                    tails[team][lane]);
+        if (lane == 0) whole[team] = mine.whole;
+        __syncthreads();
+        // Adds the tiles before `team`, last first, to where the row begins; true if it
+        // begins before this block.
+        auto reach_back = [&](float* acc) {
+            int begin = team - 1;  // the tile whose tail it is, or -1
+            for (bool on = true; on; ) {
+                bool within[kBack];
+                float v[kBack][V];
+#pragma unroll
+                for (int u = 0; u < kBack; ++u) {
+                    const int t = max(begin - u, 0);
+                    within[u] = begin - u >= 0 && whole[t];
+#pragma unroll
+                    for (int e = 0; e < V; ++e) v[u][e] = heads[t][lane][e];
+                }
+                int passed = 0;
+#pragma unroll
+                for (int u = 0; u < kBack; ++u) {
+                    on = on && within[u];
+                    passed += on;
+#pragma unroll
+                    for (int e = 0; e < V; ++e) acc[e] += on ? v[u][e] : 0.f;
+                }
+                begin -= passed;
+            }
+            if (begin < 0) return true;
+#pragma unroll
+            for (int e = 0; e < V; ++e) acc[e] += tails[begin][lane][e];
+            return false;
+        };
+        float* part = s.parts + block * 2 * q.width + c;
+        if (here && mine.open && !mine.whole) {
+            float acc[V];
+#pragma unroll
+            for (int e = 0; e < V; ++e) acc[e] = heads[team][lane][e];
+            if (reach_back(acc)) store_floats<V>(part, acc);
+            else write_row<E, V>(q, mine.first_key, c, acc);
+        }
+        // the row that goes on behind the block
+        if (here && team == kTeams - 1 && mine.more) {
+            float acc[V];
+            bool before = false;
+#pragma unroll
+            for (int e = 0; e < V; ++e)
+                acc[e] = mine.whole ? heads[team][lane][e] : tails[team][lane][e];
+            if (mine.whole) before = reach_back(acc);
+            store_floats<V>(before ? part : part + q.width, acc);
+            if (!before) s.begins[mine.last_key] = (uint32_t)block;
+        }
+        __syncthreads();
     }
 }
 
-// G lanes a tile, a piece of V columns each.
-template <class E, int V, int G>
-__global__ __launch_bounds__(kThreads) void k_tile_sums(const Sum s) {
-    const int at = (blockIdx.y * G + threadIdx.x % G) * V;
-    if (at >= s.q.width) return;
-    const int64_t live = *s.live, step = (int64_t)gridDim.x * (kThreads / G);
-    for (int64_t tile = (int64_t)blockIdx.x * (kThreads / G) + threadIdx.x / G;
-         tile * s.tile < live; tile += step)
-        tile_sum<E, V>(s, tile, live, min(at, s.q.width - V));
-}
-
-// How many tiles before this one share the row that is open at its begin and ends in
+// How many blocks before this one share the row that is open at its begin and ends in
 // it; 0 if there is none.
-__device__ __forceinline__ int64_t span_of(const Sum& s, int64_t tile, int64_t live) {
-    const int64_t first = tile * s.tile, next = first + s.tile;
+__device__ __forceinline__ int64_t span_of(const Sum& s, int64_t block, int64_t live) {
+    const int64_t first = block * s.block, next = first + s.block;
     if (first == 0 || first >= live) return 0;
     const uint32_t key = s.pairs[first].x;
     if (s.pairs[first - 1].x != key || (next < live && s.pairs[next].x == key)) return 0;
-    return tile - (int64_t)s.begins[key];
+    return block - (int64_t)s.begins[key];
 }
 
-// Adds up a row's parts in tiles first, first + step, ... below end.
+// Adds up a row's parts in blocks first, first + step, ... below end.
 template <int V>
 __device__ __forceinline__ void add_parts(const Sum& s, int64_t first, int64_t end, int64_t step,
                                           int c, float* acc) {
@@ -538,15 +622,13 @@ __device__ __forceinline__ void add_parts(const Sum& s, int64_t first, int64_t e
     }
 }
 
-// Rows over several tiles, each by the team of lanes of the tile in which it ends;
-// over more than kSpan, by all teams of the workgroup together.  7 us; by single teams,
-// however many tiles, 431, as the most popular row has 62 000 tokens.  921 600 tokens of
-// 201 rows, 48 bfloat16: 16 us (1198), bound by one compute unit reading the parts of a
-// sixth of all tokens.
+// Rows over several blocks, each by a team of lanes for the block in which it ends;
+// over more than kSpan, by all teams of the workgroup together.  5 us, most of it four
+// loads one after another; 7 for 921 600 tokens of 201 rows, 48 bfloat16.  (Parts by the
+// tile, not by the block: 7 and 16, and by single teams, however many, 431 and 1198: the
+// most popular rows have 62 000 and 157 000 tokens.)
 template <class E, int V, int G>
 __global__ __launch_bounds__(kJoinThreads) void k_join(const Sum s) {
-    using P = Piece<E, V>;
-    using T = typename E::T;
     constexpr int kTeams = kJoinThreads / G;
     __shared__ float room[kJoinThreads / 64][G][V + 1];
     __shared__ int64_t spans[kTeams];  // the long ones
@@ -555,19 +637,16 @@ __global__ __launch_bounds__(kJoinThreads) void k_join(const Sum s) {
     const int team = threadIdx.x / G, at = (blockIdx.y * G + threadIdx.x % G) * V;
     const int c = min(at, q.width - V);
     const int64_t live = *s.live, step = (int64_t)gridDim.x * kTeams;
-    auto write = [&](int64_t tile, float* acc) {
-        const uint32_t key = s.pairs[tile * s.tile].x;
-#pragma unroll
-        for (int e = 0; e < V; ++e) acc[e] *= q.scale;
-        if (at < q.width) P::store((T*)q.g_table + (int64_t)key * q.width + c, P::down(acc));
+    auto write = [&](int64_t block, const float* acc) {
+        if (at < q.width) write_row<E, V>(q, s.pairs[block * s.block].x, c, acc);
     };
-    for (int64_t base = (int64_t)blockIdx.x * kTeams; base * s.tile < live; base += step) {
-        const int64_t tile = base + team, span = span_of(s, tile, live);
+    for (int64_t base = (int64_t)blockIdx.x * kTeams; base * s.block < live; base += step) {
+        const int64_t block = base + team, span = span_of(s, block, live);
         if (span > 0 && span <= kSpan) {
             float acc[V];
-            load_floats<V>(s.parts + ((tile - span) * 2 + 1) * q.width + c, acc);
-            add_parts<V>(s, tile - span + 1, tile + 1, 1, c, acc);
-            write(tile, acc);
+            load_floats<V>(s.parts + ((block - span) * 2 + 1) * q.width + c, acc);
+            add_parts<V>(s, block - span + 1, block + 1, 1, c, acc);
+            write(block, acc);
         }
         if (!__syncthreads_or(span > kSpan)) continue;
         if (threadIdx.x == 0) found = 0;
@@ -639,9 +718,9 @@ int check_args(int dtype, int64_t count, int64_t rows, int32_t width, const void
 }
 
 struct Layout {
-    int chunks, passes, bits, digit, tile;
+    int chunks, passes, bits, digit, tile, block;
     bool few;
-    int64_t tiles, counts, totals, live, pairs[2], begins, parts, total;
+    int64_t blocks, counts, totals, live, pairs[2], begins, parts, total;
 };
 
 Layout layout(int dtype, int64_t count, int64_t rows, int32_t width) {
@@ -656,14 +735,16 @@ Layout layout(int dtype, int64_t count, int64_t rows, int32_t width) {
     l.passes = l.few ? 1 : (l.bits + l.digit - 1) / l.digit;
     // Lanes of a team, and teams beside each other, as for_width has them: about 2^16
     // lanes are enough for the sums, in tiles of at least a batch.  8205 x 512 float16 in
-    // tiles of 8: 7 us, of 64: 20; more lanes leave more parts to join (2^18: 921 600 x 48
-    // bfloat16, 16 -> 47 us in the join).  4 000 000 x 16 float32 in tiles of 256 and of
-    // 64: joins of 12 and 17 us.
+    // tiles of 8: 7 us, of 64: 20; more lanes leave more parts to put together (with parts
+    // by the tile, 2^18 took 47 us for 16 in the join of 921 600 x 48 bfloat16).
     const int vec = dtype == GSX_F32 ? F32::VEC : BF16::VEC;
     const int64_t pieces = width < vec ? width : (width + vec - 1) / vec;
     l.tile = kMostTile;
     while (l.tile > kBatch && count * pieces < ((int64_t)1 << 16) * l.tile) l.tile /= 2;
-    l.tiles = (count + l.tile - 1) / l.tile;
+    int lanes = 1;
+    while (lanes < 64 && lanes < pieces) lanes *= 2;
+    l.block = l.tile * (kThreads / lanes);
+    l.blocks = (count + l.block - 1) / l.block;
     const int64_t radix = l.few ? 0 : 1 << l.digit;
     l.live = 0;
     l.totals = 256;
@@ -671,8 +752,8 @@ Layout layout(int dtype, int64_t count, int64_t rows, int32_t width) {
     l.pairs[0] = up_to(l.counts + l.chunks * radix * 4, 256);
     l.pairs[1] = up_to(l.pairs[0] + count * 8, 256);
     l.begins = up_to(l.pairs[1] + (l.passes > 1 ? count * 8 : 0), 256);
-    l.parts = up_to(l.begins + (l.tiles > 1 ? rows * 4 : 0), 256);
-    l.total = up_to(l.parts + l.tiles * 2 * width * 4, 256);
+    l.parts = up_to(l.begins + (l.blocks > 1 ? rows * 4 : 0), 256);
+    l.total = up_to(l.parts + l.blocks * 2 * width * 4, 256);
     return l;
 }
 
@@ -768,14 +849,15 @@ int gradient(int dtype, const Embed& q, char* ws, hipStream_t st) {
     u.begins = (uint32_t*)(ws + l.begins);
     u.live = s.live;
     u.tile = l.tile;
+    u.block = l.block;
     u.parts = (float*)(ws + l.parts);
     return for_width<E>(q.width, [&](auto v, auto g, int times) -> int {
         constexpr int V = decltype(v)::value, G = decltype(g)::value;
-        const dim3 grid = grid_for(l.tiles, kThreads / G, times);
+        const dim3 grid = grid_for(l.blocks, 1, times);
         hipLaunchKernelGGL((k_tile_sums<E, V, G>), grid, dim3(kThreads), 0, st, u);
         GSX_LAUNCH_CHECK();
-        if (l.tiles == 1) return GSX_OK;
-        hipLaunchKernelGGL((k_join<E, V, G>), grid_for(l.tiles, kJoinThreads / G, times),
+        if (l.blocks == 1) return GSX_OK;
+        hipLaunchKernelGGL((k_join<E, V, G>), grid_for(l.blocks, kJoinThreads / G, times),
                            dim3(kJoinThreads), 0, st, u);
         GSX_LAUNCH_CHECK();
         return GSX_OK;

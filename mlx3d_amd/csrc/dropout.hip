@@ -13,7 +13,7 @@
 //
 // Bound by memory: 118 million bfloat16 79 us (6.0 TB/s, 4 bytes an element), 59 million
 // float32 80 us, 124 on top of a residual (5.7).  Beside it the rounds keep the vector
-// units busy for 56 % of the first; with both blocks formed for all elements, and
+// units busy for 61 % of the first; with both blocks formed for all elements, and
 // elements loaded one by one, it took 238.
 #include <hip/hip_runtime.h>
 

@@ -20,7 +20,7 @@
 //
 // Memory bounds both directions: 118 MB of 32 float32 columns take 39 us forward (6.1
 // TB/s) and 65 backward (5.5), 199 million bfloat16 in rows of 96 145 us forward (5.5).
-// The vector units are busy for 43 to 45 % of that, and waves wait in between, so what a
+// The vector units are busy for 45 to 51 % of that, and waves wait in between, so what a
 // row costs beside its elements counts, in 16 bits the more: teams are as small as whole lines allow, with two or three pieces a lane, so
 // that a sum takes few steps and few lanes are idle (120 MB of bfloat16, forward and
 // backward: 300 columns 53 and 83 us, on 64 lanes with one piece each 83 and 120; 48

@@ -18,8 +18,10 @@
 
 #include <atomic>
 #include <optional>
+#include <stdexcept>
 #include <string>
-#include <tuple>
+#include <utility>
+#include <vector>
 
 #include "gsx.h"
 
@@ -43,12 +45,15 @@ class Stage {
         stage_ = new py::object(py::module_::import("mlx3d_amd.profiling").attr("stage")(label));
         stage_->attr("__enter__")();
     }
-    ~Stage() noexcept(false) {
+    ~Stage() {
         if (!stage_) return;
         py::gil_scoped_acquire gil;
-        const py::object held = std::move(*stage_);
+        try {
+            stage_->attr("__exit__")(py::none(), py::none(), py::none());
+        } catch (py::error_already_set& e) {
+            e.discard_as_unraisable("mlx3d_amd.profiling.stage");
+        }
         delete stage_;
-        held.attr("__exit__")(py::none(), py::none(), py::none());
     }
     Stage(const Stage&) = delete;
 

@@ -21,10 +21,11 @@
 // Memory bounds both directions: 118 MB of 32 float32 columns take 39 us forward (6.1
 // TB/s) and 65 backward (5.5), 199 million bfloat16 in rows of 96 145 us forward (5.5).
 // The vector units are busy for 45 to 51 % of that, and waves wait in between, so what a
-// row costs beside its elements counts, in 16 bits the more: teams are as small as whole lines allow, with two or three pieces a lane, so
-// that a sum takes few steps and few lanes are idle (120 MB of bfloat16, forward and
-// backward: 300 columns 53 and 83 us, on 64 lanes with one piece each 83 and 120; 48
-// columns 51 and 84 for 67 and 91), and the next row is asked for before this one's sums.
+// row costs beside its elements counts, in 16 bits the more: teams are as small as whole
+// lines allow, with two or three pieces a lane, so that a sum takes few steps and few
+// lanes are idle (120 MB of bfloat16, forward and backward: 300 columns 53 and 83 us, on
+// 64 lanes with one piece each 83 and 120; 48 columns 51 and 84 for 67 and 91), and the
+// next row is asked for before this one's sums.
 // Odd widths cost up to a quarter more in 16 bits: their vectors straddle lines.
 #include <hip/hip_runtime.h>
 
@@ -49,9 +50,9 @@ constexpr int kThreads = 256;
 constexpr int kMostGroups = 1024;
 template <int V, int G, int N>
 constexpr int groups_of = V == 1 ? kMostGroups : N == 1 && G <= 64 ? 768 : 512;
-constexpr int kLongStrips = 256;   // of rows, whose columns are added up apart from the rows' sums
-constexpr int kFwdGroups = 8192;   // workgroups of a forward pass at most
-constexpr int kMostWidth = 8192;    // of a row that a workgroup holds
+constexpr int kLongStrips = 256;  // of long rows, in the sums of their columns
+constexpr int kFwdGroups = 8192;  // workgroups of a forward pass at most
+constexpr int kMostWidth = 8192;  // of a row that a workgroup holds
 
 struct Norm {
     const void *x, *weight, *bias, *g_y;

@@ -251,6 +251,25 @@ def test_a_row_that_is_not_finite_stays_alone(width, dtype):
     assert torch.equal(got["db"], clean["db"])
 
 
+@pytest.mark.parametrize("dtype", (torch.float32, torch.bfloat16), ids=str)
+@pytest.mark.parametrize("width", (6, 27, 32, 500, 1365, 9000))
+def test_rows_beyond_the_range_of_squares(width, dtype):
+    """Finite rows whose squares or whose sum float32 does not hold."""
+    x, w, b, dy = inputs(40, width, dtype, seed=4)
+    clean = outputs(x, w, b, dy)
+    x[17] = (x[17].float() * 1e30).to(dtype)
+    x[20] = (x[20].float() * 1e20).to(dtype)
+    x[39] = 3e38
+    got = outputs(x, w, b, dy)
+    assert torch.equal(got["y"][17], b) and torch.equal(got["y"][20], b)
+    assert not bool(got["dx"][[17, 20]].any())
+    assert bool(got["y"][39].isnan().all()) and bool(got["dx"][39].isnan().all())
+    rest = [i for i in range(39) if i not in (17, 20)]
+    for name in ("y", "dx"):
+        assert torch.equal(got[name][rest], clean[name][rest])
+    assert torch.equal(got["db"], clean["db"])
+
+
 def test_same_bits_every_time_and_on_another_stream():
     t = inputs(5000, 48, torch.float32, seed=1)
     first = outputs(*t)

@@ -17,6 +17,7 @@
 #include <c10/hip/HIPStream.h>
 
 #include <atomic>
+#include <limits>
 #include <optional>
 #include <stdexcept>
 #include <string>
@@ -71,6 +72,14 @@ int64_t check(int64_t status, const char* what) {
         throw Failure(std::string(what) + " failed: " + gsx_strerror((int)status) + " (status " +
                       std::to_string(status) + ")");
     return status;
+}
+
+// t's last dimension as the entry points take it.  What 32 bits do not hold is refused here,
+// as the entry points refuse what is too large, and before anything is copied or divided.
+int width_of(const Tensor& t, const char* what) {
+    const int64_t width = t.size(-1);
+    if (width > std::numeric_limits<int32_t>::max()) check(GSX_ERR_TOO_LARGE, what);
+    return (int)width;
 }
 
 int dtype_of(const Tensor& t) {
@@ -138,16 +147,17 @@ variable_list once(const char* what, variable_list grads, const variable_list& i
 struct Embedding : Function<Embedding> {
     static Tensor forward(AutogradContext* ctx, const Tensor& indices, const Tensor& table,
                           double scale) {
+        const int width = width_of(table, "gsx_embed_fwd");
         const Tensor held = indices.contiguous();
         const auto [rows, stride] = rows_of(table);
         std::vector<int64_t> shape = held.sizes().vec();
-        shape.push_back(table.size(1));
+        shape.push_back(width);
         Tensor y = at::empty(shape, table.options());
         {
             const Launch on(table, "embed_fwd");
-            check(gsx_embed_fwd(dtype_of(table), held.numel(), table.size(0), (int)table.size(1),
-                                ptr(held), held.scalar_type() == at::kLong, ptr(rows), stride,
-                                (float)scale, ptr(y), on.stream),
+            check(gsx_embed_fwd(dtype_of(table), held.numel(), table.size(0), width, ptr(held),
+                                held.scalar_type() == at::kLong, ptr(rows), stride, (float)scale,
+                                ptr(y), on.stream),
                   "gsx_embed_fwd");
         }
         ctx->save_for_backward({indices});
@@ -160,10 +170,10 @@ struct Embedding : Function<Embedding> {
         Tensor g_table;
         {
             const at::NoGradGuard no_grad;
-            const Tensor held = saved[0].contiguous();
             const Tensor& g_y = incoming[0];
+            const int dtype = dtype_of(g_y), width = width_of(g_y, "gsx_embed_bwd");
+            const Tensor held = saved[0].contiguous();
             const auto [g_rows, stride] = rows_of(g_y);
-            const int dtype = dtype_of(g_y), width = (int)g_y.size(-1);
             const int64_t rows = ctx->saved_data["rows"].toInt(), count = held.numel();
             g_table = at::empty({rows, width}, g_y.options());
             const int64_t n = check(gsx_embed_bwd_workspace_bytes(dtype, count, rows, width),
@@ -185,9 +195,9 @@ struct Embedding : Function<Embedding> {
 struct LayerNorm : Function<LayerNorm> {
     static Tensor forward(AutogradContext* ctx, const Tensor& x, const OptTensor& weight,
                           const OptTensor& bias, double eps) {
+        const int width = width_of(x, "gsx_layer_norm_fwd");
         const auto [rows, stride] = rows_of(x);
         const OptTensor w = contiguous(weight), b = contiguous(bias);
-        const int width = (int)x.size(-1);
         Tensor y = contiguous_like(x);
         {
             const Launch on(x, "layer_norm_fwd");
@@ -210,10 +220,10 @@ struct LayerNorm : Function<LayerNorm> {
         Tensor g_x, g_w, g_b;
         {
             const at::NoGradGuard no_grad;
+            const int dtype = dtype_of(x), width = width_of(x, "gsx_layer_norm_bwd");
             const auto [rows, stride] = rows_of(x);
             const auto [g_rows, g_stride] = rows_of(g_y);
             const Tensor w = has_w ? weight.contiguous() : weight;
-            const int dtype = dtype_of(x), width = (int)x.size(-1);
             const int64_t count = x.numel() / width;
             if (ctx->needs_input_grad(0)) g_x = contiguous_like(x);
             if (need_w) g_w = at::empty({width}, x.options());

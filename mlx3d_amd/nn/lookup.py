@@ -21,7 +21,8 @@ def embedding(indices: torch.Tensor, table: torch.Tensor, scale: float = 1.0) ->
     to it, once (its gradient has none and says so).
 
     The gradient is dense, summed in float32 in an order that the indices fix, so the
-    same inputs give the same bits.  Rows that no index names have zeros."""
+    same inputs give the same bits.  Rows that no index names have zeros.  At most 2^30
+    indices and rows and 2^20 columns; more is refused (``GsxError``)."""
     if indices.dtype not in (torch.int32, torch.int64):
         raise ValueError("indices must be int32 or int64.")
     if table.ndim != 2 or table.dtype not in _lib.DTYPES:

@@ -23,7 +23,8 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None,
     Statistics and sums are float32, the variance is that of the differences to the
     mean; outputs are rounded once.  A row with an infinite or NaN input, or whose float32
     sum overflows, comes out NaN, and no other row does; one whose float32 variance
-    alone overflows (differences from about 1e19) is normalised to zeros."""
+    alone overflows (differences from about 1e19) is normalised to zeros.  At most 2^20
+    columns and 2^30 rows; more is refused (``GsxError``)."""
     if x.ndim < 1 or x.dtype not in _lib.DTYPES:
         raise ValueError("x must be (..., C) in float32, bfloat16 or float16.")
     if x.shape[-1] < 1:

@@ -20,6 +20,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libgsx.so")
 
 GSX_OK = 0
+GSX_ERR_TOO_LARGE = -4
 LOG_SCALES = 1
 LOGIT_OPACITY = 2
 ANTIALIAS = 4
@@ -257,6 +258,13 @@ def check(status: int, what: str) -> int:
     if status < 0:
         raise GsxError(f"{what} failed: {strerror(status)} (status {status})")
     return status
+
+
+def check_widths(what: str, *widths: int) -> None:
+    """Refuses widths that 32 bits do not hold, as ``what`` refuses what is too large:
+    ctypes would hand their lower bits on."""
+    if max(widths) >= 1 << 31:
+        check(GSX_ERR_TOO_LARGE, what)
 
 
 def ptr(t: torch.Tensor | None):

@@ -93,6 +93,7 @@ def gated_feed_forward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor
         raise ValueError("w_down must have shape (d_out, hidden).")
     if min(*w_gate.shape, *w_down.shape) < 1:
         raise ValueError("the block's widths must be at least 1.")
+    _lib.check_widths("gsx_ffn_fwd", *w_gate.shape, w_down.shape[0])
     _lib.require_device(x, w_gate, w_up, w_down)
     return _GatedFeedForward.apply(x, w_gate, w_up, w_down, _ACTIVATIONS[activation])
 

@@ -226,6 +226,7 @@ class _Distillation:
             raise ValueError("teacher must be 'logits' or 'log_probs'.")
         if reduction not in _REDUCTIONS:
             raise ValueError("reduction must be 'none', 'sum' or 'mean'.")
+        _lib.check_widths("gsx_distil_fwd", vocab)
         self.device = _lib.require_device(logits, values, indices)
         self.shape = logits.shape
         self.reduction = reduction

@@ -9,6 +9,7 @@
 // and 11 / 6, 7 and 6.
 //
 // Arguments are checked by the Python functions in front of these.
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/utils/pybind.h>
 
@@ -66,6 +67,8 @@ class Stage {
 struct Failure : std::runtime_error {
     using std::runtime_error::runtime_error;
 };
+// mlx3d_amd._lib.GsxError; never let go: the interpreter may have ended before statics do.
+const py::object* gsx_error = nullptr;
 
 int64_t check(int64_t status, const char* what) {
     if (status < 0)
@@ -142,9 +145,26 @@ variable_list once(const char* what, variable_list grads, const variable_list& i
     return grads;
 }
 
+// A node whose gradient is Op::gradient.  The engine, which calls backward, hands a Python
+// error on as it is, and makes a RuntimeError of any other exception.
+template <class Op>
+struct Layer : Function<Op> {
+    static variable_list backward(AutogradContext* ctx, const variable_list& incoming) {
+        try {
+            return Op::gradient(ctx, incoming);
+        } catch (const Failure& e) {
+            py::gil_scoped_acquire gil;
+            PyErr_SetString(gsx_error->ptr(), e.what());
+            python_error raised;
+            raised.persist();
+            throw raised;
+        }
+    }
+};
+
 // ---- embedding ----
 
-struct Embedding : Function<Embedding> {
+struct Embedding : Layer<Embedding> {
     static Tensor forward(AutogradContext* ctx, const Tensor& indices, const Tensor& table,
                           double scale) {
         const int width = width_of(table, "gsx_embed_fwd");
@@ -165,7 +185,7 @@ struct Embedding : Function<Embedding> {
         ctx->saved_data["rows"] = table.size(0);
         return y;
     }
-    static variable_list backward(AutogradContext* ctx, const variable_list& incoming) {
+    static variable_list gradient(AutogradContext* ctx, const variable_list& incoming) {
         const variable_list saved = ctx->get_saved_variables();
         Tensor g_table;
         {
@@ -192,7 +212,7 @@ struct Embedding : Function<Embedding> {
 
 // ---- layer norm ----
 
-struct LayerNorm : Function<LayerNorm> {
+struct LayerNorm : Layer<LayerNorm> {
     static Tensor forward(AutogradContext* ctx, const Tensor& x, const OptTensor& weight,
                           const OptTensor& bias, double eps) {
         const int width = width_of(x, "gsx_layer_norm_fwd");
@@ -210,7 +230,7 @@ struct LayerNorm : Function<LayerNorm> {
         ctx->saved_data["bias"] = bias.has_value();
         return y;
     }
-    static variable_list backward(AutogradContext* ctx, const variable_list& incoming) {
+    static variable_list gradient(AutogradContext* ctx, const variable_list& incoming) {
         const variable_list saved = ctx->get_saved_variables();
         const Tensor &x = saved[0], &weight = saved[1], &g_y = incoming[0];
         // inputs that are tensors are counted, absent ones are not
@@ -259,7 +279,7 @@ Tensor drop(const Tensor& x, const OptTensor& residual, double p, int64_t seed, 
     return y;
 }
 
-struct Dropout : Function<Dropout> {
+struct Dropout : Layer<Dropout> {
     static Tensor forward(AutogradContext* ctx, const Tensor& x, const OptTensor& residual,
                           double p, int64_t seed, int64_t offset, const OptTensor& at_device) {
         const Tensor at = at_device ? *at_device : Tensor();
@@ -271,7 +291,7 @@ struct Dropout : Function<Dropout> {
         ctx->saved_data["residual"] = residual.has_value();
         return drop(x, residual, p, seed, offset, at);
     }
-    static variable_list backward(AutogradContext* ctx, const variable_list& incoming) {
+    static variable_list gradient(AutogradContext* ctx, const variable_list& incoming) {
         const variable_list saved = ctx->get_saved_variables();
         Tensor g_x, g_residual;
         {
@@ -291,14 +311,12 @@ struct Dropout : Function<Dropout> {
 }  // namespace
 
 PYBIND11_MODULE(_autograd, m) {
-    // never let go: the interpreter may have ended before statics do
-    static const auto* error =
-        new py::object(py::module_::import("mlx3d_amd._lib").attr("GsxError"));
+    gsx_error = new py::object(py::module_::import("mlx3d_amd._lib").attr("GsxError"));
     py::register_exception_translator([](std::exception_ptr p) {
         try {
             if (p) std::rethrow_exception(p);
         } catch (const Failure& e) {
-            PyErr_SetString(error->ptr(), e.what());
+            PyErr_SetString(gsx_error->ptr(), e.what());
         }
     });
     using Release = py::call_guard<py::gil_scoped_release>;

@@ -842,7 +842,8 @@ int gsx_layer_norm_fwd(int32_t dtype, int64_t rows, int32_t width, const void* x
 /* Its gradient from g_y (rows, width, a row stride): g_x (rows, width), g_weight
  * and g_bias (width), contiguous; each may be NULL, and without the last two
  * the workspace.  Needs nothing of the forward call.  rows = 0 clears g_weight
- * and g_bias. */
+ * and g_bias.  The workspace holds a partial row of both for each workgroup, of
+ * which wider rows have fewer: ask for the very sizes of the call. */
 int64_t gsx_layer_norm_bwd_workspace_bytes(int32_t dtype, int64_t rows, int32_t width);
 int gsx_layer_norm_bwd(int32_t dtype, int64_t rows, int32_t width, const void* x, int64_t x_stride,
                        const void* weight, const void* g_y, int64_t g_y_stride, float eps,

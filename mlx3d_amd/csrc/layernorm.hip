@@ -607,13 +607,36 @@ int forward(const Norm& q, hipStream_t st) {
     return GSX_OK;
 }
 
+// Partial rows of a gradient: the workgroups that leave one, or the strips of long rows.
+template <class E>
+int64_t partial_rows(int64_t rows, int width) {
+    int64_t groups = groups_for(rows, 1, kLongStrips);
+    for_width<E>(width, [&](auto v, auto g, auto n) {
+        constexpr int V = decltype(v)::value, G = decltype(g)::value, N = decltype(n)::value;
+        groups = groups_for(rows, threads_of<G> / G, groups_of<V, G, N>);
+    });
+    return groups;
+}
+
+// A gradient's workspace: the partial rows, then a long row's statistics.
+struct Layout {
+    int64_t stats, total;
+};
+
+Layout layout(int dtype, int64_t rows, int width) {
+    const int64_t parts = dtype == GSX_F32    ? partial_rows<F32>(rows, width)
+                          : dtype == GSX_BF16 ? partial_rows<BF16>(rows, width)
+                                              : partial_rows<F16>(rows, width);
+    const int64_t stats = up_to(parts * 2 * width * 4, 256);
+    return {stats, 256 + stats + (width > kMostWidth ? rows * 12 : 0)};
+}
+
 template <class E>
 int backward(const Norm& q, void* g_w, void* g_b, hipStream_t st) {
-    int64_t groups = 0;
+    const int64_t groups = partial_rows<E>(q.rows, q.width);
     if (q.rows > 0) {
         const bool held = for_width<E>(q.width, [&](auto v, auto g, auto n) {
             constexpr int V = decltype(v)::value, G = decltype(g)::value, N = decltype(n)::value;
-            groups = groups_for(q.rows, threads_of<G> / G, groups_of<V, G, N>);
             hipLaunchKernelGGL((k_norm_bwd<E, V, G, N>), dim3((unsigned)groups), dim3(threads_of<G>),
                                (unsigned)(q.parts && G <= 64 ? 2 * q.width * 4 : 0), st, q);
         });
@@ -621,7 +644,6 @@ int backward(const Norm& q, void* g_w, void* g_b, hipStream_t st) {
             hipLaunchKernelGGL((k_long_bwd<E>), dim3((unsigned)groups_for(q.rows, 1, 1 << 16)),
                                dim3(kLongThreads), 0, st, q);
             GSX_LAUNCH_CHECK();
-            groups = groups_for(q.rows, 1, kLongStrips);
             if (q.parts)
                 hipLaunchKernelGGL((k_long_columns<E>),
                                    dim3((unsigned)groups,
@@ -669,8 +691,7 @@ int gsx_layer_norm_fwd(int32_t dtype, int64_t rows, int32_t width, const void* x
 
 int64_t gsx_layer_norm_bwd_workspace_bytes(int32_t dtype, int64_t rows, int32_t width) {
     if (int e = check_shape(dtype, rows, width)) return e;
-    const int64_t most = rows < kMostGroups ? rows : kMostGroups;
-    return 256 + up_to(most * 2 * width * 4, 256) + (width > kMostWidth ? rows * 12 : 0);
+    return layout(dtype, rows, width).total;
 }
 
 int gsx_layer_norm_bwd(int32_t dtype, int64_t rows, int32_t width, const void* x, int64_t x_stride,
@@ -685,10 +706,8 @@ int gsx_layer_norm_bwd(int32_t dtype, int64_t rows, int32_t width, const void* x
         return GSX_ERR_INVALID;
     const bool params = g_weight || g_bias;
     if (!params && (!g_x || rows == 0)) return GSX_OK;
-    if (params &&
-        (!workspace || workspace_bytes < gsx_layer_norm_bwd_workspace_bytes(dtype, rows, width)))
-        return GSX_ERR_WORKSPACE;
-    const int64_t most = rows < kMostGroups ? rows : kMostGroups;
+    const Layout l = layout(dtype, rows, width);
+    if (params && (!workspace || workspace_bytes < l.total)) return GSX_ERR_WORKSPACE;
     Norm q{};
     q.x = x;
     q.x_stride = x_stride;
@@ -701,7 +720,7 @@ int gsx_layer_norm_bwd(int32_t dtype, int64_t rows, int32_t width, const void* x
     q.eps = eps;
     q.g_x = g_x;
     q.parts = params ? (float*)workspace : nullptr;
-    q.stats = (float*)((char*)workspace + up_to(most * 2 * width * 4, 256));
+    q.stats = (float*)((char*)workspace + l.stats);
     hipStream_t st = (hipStream_t)stream;
     if (dtype == GSX_F32) return backward<F32>(q, g_weight, g_bias, st);
     if (dtype == GSX_BF16) return backward<BF16>(q, g_weight, g_bias, st);

@@ -1,5 +1,7 @@
 """Sizes at the ends of what the embedding and the layer norm take, through their public
-calls: what is too large is refused before anything is copied, allocated or launched."""
+calls: what is too large is refused before any launch."""
+
+import contextlib
 
 import pytest
 import torch
@@ -14,25 +16,31 @@ DEV = "cuda"
 WIDTHS = ((1 << 20) + 1, 1 << 31, 1 << 32, (1 << 32) + 64)
 
 
+@contextlib.contextmanager
+def refused(entry):
+    """A ``GsxError`` before more than a copy of three rows of 2^20 + 1 is allocated (these
+    are copied first, being one element repeated)."""
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    with pytest.raises(_lib.GsxError, match=entry + r" failed: .*\(status -4\)"):
+        yield
+    assert torch.cuda.max_memory_allocated() < before + (1 << 26)
+
+
 @pytest.mark.parametrize("rows", (0, 1, 3))
 @pytest.mark.parametrize("width", WIDTHS)
 def test_a_norm_that_is_too_wide_is_refused(width, rows):
-    """(Rows of 2^20 + 1 are copied first, since these are one element repeated.)"""
     x = torch.zeros((1, 1), dtype=torch.bfloat16, device=DEV).expand(rows or 1, width)[:rows]
-    before = torch.cuda.memory_allocated()
-    with pytest.raises(_lib.GsxError, match=r"gsx_layer_norm_fwd failed: .*\(status -4\)"):
+    with refused("gsx_layer_norm_fwd"):
         layer_norm(x)
-    assert torch.cuda.memory_allocated() == before
 
 
 @pytest.mark.parametrize("count", (0, 3))
 @pytest.mark.parametrize("width", WIDTHS)
 def test_a_table_that_is_too_wide_is_refused(width, count):
     table = torch.zeros((1, 1), dtype=torch.bfloat16, device=DEV).expand(2, width)
-    before = torch.cuda.memory_allocated()
-    with pytest.raises(_lib.GsxError, match=r"gsx_embed_fwd failed: .*\(status -4\)"):
+    with refused("gsx_embed_fwd"):
         embedding(torch.zeros((count,), dtype=torch.int64, device=DEV), table)
-    assert torch.cuda.memory_allocated() == before
 
 
 def test_the_widest_rows_are_taken():

@@ -366,8 +366,8 @@ __global__ __launch_bounds__(kSortThreads) void k_place(const Sort s) {
 
 // All passes over few tokens by one workgroup, in shared memory; the others clear the
 // gradient.  The waves share the tokens evenly, `rounds` times 64 each.  8205 tokens of
-// 50 000 rows 25 us, bound by one compute unit's ranking; the seven launches of two
-// passes take 30 and some 20 of the host's.
+// 50 000 rows 23 to 25 us, bound by one compute unit's ranking; the six launches of two
+// passes take 31 (a gradient of 512 float16 columns 34 us a call, with those 41).
 constexpr int kFewThreads = 1024;
 template <int ITEMS>
 __global__ __launch_bounds__(kFewThreads) void k_sort_few(const Sort s) {
